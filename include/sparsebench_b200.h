@@ -396,6 +396,56 @@ int sb_ep_sdd_dispatch(const void* recv_rows, const void* w1, const int32_t* row
                        const uint32_t* epoch_word, int32_t my_rank, int32_t num_ranks, int32_t experts_local,
                        int32_t capacity, int32_t push_warps, int32_t* dev_status, sb_stream_t stream);
 
+/*
+ * The gated expert block and its backward pass, on the layout of sb_route at block size 128 (no counterpart in the
+ * reference, whose experts have one up projection). bf16 in and out, fp32 accumulation. d_model and ffn_dim are
+ * multiples of 128; w_gate and w_up are [E, D, F], w_down is [E, F, D]; every buffer 16-byte aligned.
+ *
+ * sb_sdd_gated: h_blocks = act(x[row_token] . w_gate[e]) * (x[row_token] . w_up[e]) in one kernel, laid out like
+ * sb_sdd's blocks; the down projection is sb_dsd. g_blocks / u_blocks (both or neither NULL): the two projections
+ * before the activation, for the backward pass; every row of a 64-row half that holds real rows is then written
+ * (padding rows as zeros). Without them skip_padding_rows works as in sb_sdd.
+ *
+ * The backward pass, in this order, from grad_out [T, D]:
+ *   sb_gated_gather        x_rows[r] = x[token], grad_rows[r] = gate * grad_out[token], row_gate[r] = gate of the row's
+ *                          copy; zeros for padding rows. [num_row_blocks * 128] rows; those past the real end stay as
+ *                          they are. gate_dtype: 0 = bf16, 1 = fp32.
+ *   sb_gated_grad_hidden   dg_blocks, du_blocks: gradients of the two projections; gate_partial
+ *                          [num_row_blocks * 128, F / 128] fp32: each row's share of its gate's gradient per 128 hidden
+ *                          columns (rows of real copies only).
+ *   sb_gated_grad_weights  dw_gate, dw_up [E, D, F], dw_down [E, F, D]; zeros for an expert without rows.
+ *   sb_gated_grad_rows     dx_rows[r] = dG w_gate^T + dU w_up^T; 32-row groups of padding are not written. May write over
+ *                          x_rows once the weight gradients are done.
+ *   sb_gated_join          dx[t] = sum of the token's rows, dgate[t, j] = sum of the copy's partials, in a fixed order.
+ * A copy whose expert id was rejected contributes nothing and its gate's gradient is 0.
+ */
+enum sb_activation { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* erf form */ };
+int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
+                 const int32_t* row_block_expert, const int32_t* row_offsets, void* h_blocks, void* g_blocks,
+                 void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                 int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
+                 sb_stream_t stream);
+int sb_gated_gather(const void* x, const void* grad_out, const void* gate, int gate_dtype, const int32_t* row_token,
+                    const int32_t* copy_row, const int32_t* padded_offsets, int32_t num_experts, void* x_rows,
+                    void* grad_rows, float* row_gate, int64_t num_tokens, int32_t k, int32_t d_model,
+                    int32_t num_row_blocks, sb_stream_t stream);
+int sb_gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_blocks, const void* u_blocks,
+                         const float* row_gate, const int32_t* row_token, const int32_t* row_block_expert,
+                         const int32_t* row_offsets, void* dg_blocks, void* du_blocks, float* gate_partial,
+                         int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                         int32_t num_row_blocks, int32_t activation, int32_t* dev_status, sb_stream_t stream);
+int sb_gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_blocks, const void* dg_blocks,
+                          const void* du_blocks, const int32_t* padded_offsets, const int32_t* tokens_per_expert,
+                          const int32_t* row_offsets, void* dw_gate, void* dw_up, void* dw_down, int32_t d_model,
+                          int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status,
+                          sb_stream_t stream);
+int sb_gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up,
+                       const int32_t* row_token, const int32_t* row_block_expert, const int32_t* row_offsets,
+                       void* dx_rows, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
+                       int32_t* dev_status, sb_stream_t stream);
+int sb_gated_join(const void* dx_rows, const float* gate_partial, const int32_t* copy_row, void* dx, void* dgate,
+                  int gate_dtype, int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, sb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -323,6 +323,115 @@ def token_rounding_cuda(scores: torch.Tensor, k: int, tile: int):
     return token, expert, weight, count
 
 
+# ---- the gated expert block and its backward pass (no counterpart in the reference) ---------------------
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _check_activation(activation: str) -> int:
+    _check(activation in ACTIVATIONS, f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    return ACTIVATIONS[activation]
+
+
+def _check_bf16(device: torch.device, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+        _check(t.device == device, f"all inputs must be on the same GPU: {name} is on {t.device}, not {device}")
+        _check(t.dtype == torch.bfloat16, f"{name} must be bfloat16, got {t.dtype}")
+        _check(t.is_contiguous(), f"{name} must be contiguous")
+
+
+def _check_gated_weights(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor) -> None:
+    _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
+    _check_bf16(x.device, x=x, w_gate=w_gate, w_up=w_up)
+    _check(x.dim() == 2 and w_gate.dim() == 3 and w_gate.shape[1] == x.shape[1] and w_up.shape == w_gate.shape,
+           f"x must be [T, D] and w_gate, w_up [E, D, F], got {tuple(x.shape)}, {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    _check(x.shape[1] > 0 and x.shape[1] % BLOCK == 0, f"D ({x.shape[1]}) must be a positive multiple of 128")
+    _check(w_gate.shape[2] > 0 and w_gate.shape[2] % BLOCK == 0, f"F ({w_gate.shape[2]}) must be a positive multiple of 128")
+
+
+def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, row_token: torch.Tensor,
+                   row_block_expert: torch.Tensor, row_offsets: torch.Tensor, num_nnz: int, activation: str,
+                   skip_padding_rows: bool = False, keep: bool = False
+                   ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """(H, G, U), blocks [num_nnz, 128, 128] each: G = x[row_token] @ w_gate[expert], U the same with w_up,
+    H = act(G) * U, in one kernel. G and U are None unless keep: then all three have every row the backward pass
+    reads (padding rows of a 64-row half that holds real rows as zeros). Dead row blocks are left unwritten."""
+    lib = _lib.load()
+    _check_gated_weights(x, w_gate, w_up)
+    code = _check_activation(activation)
+    for t, name in ((row_token, "row_token"), (row_block_expert, "row_block_expert"), (row_offsets, "row_offsets")):
+        _check_index(t, name)
+        _check(t.device == x.device, f"{name} must be on x's GPU")
+    num_experts, d_model, ffn_dim = w_gate.shape
+    num_row_blocks = row_offsets.numel() - 1
+    _check(row_token.numel() == num_row_blocks * BLOCK and row_block_expert.numel() == num_row_blocks,
+           "the layout does not match block size 128")
+    _check(num_nnz == num_row_blocks * (ffn_dim // BLOCK),
+           f"expected {num_row_blocks * (ffn_dim // BLOCK)} blocks (row blocks x F/128), got {num_nnz}")
+    with torch.cuda.device(x.device):
+        h = torch.empty((num_nnz, BLOCK, BLOCK), dtype=torch.bfloat16, device=x.device)
+        g, u = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
+        if num_row_blocks > 0:
+            _lib.check(lib.sb_sdd_gated(_ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(row_token), _ptr(row_block_expert),
+                                        _ptr(row_offsets), _ptr(h), _ptr(g), _ptr(u), x.shape[0], d_model, ffn_dim,
+                                        num_experts, num_row_blocks, code, int(bool(skip_padding_rows)),
+                                        _ptr(device_status(x.device)), _stream()))
+    return h, g, u
+
+
+def gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
+                        w_up: torch.Tensor, w_down: torch.Tensor, h: torch.Tensor, g: torch.Tensor, u: torch.Tensor,
+                        layout: list[torch.Tensor], activation: str) -> tuple[torch.Tensor, ...]:
+    """(dx, dexpert_weight, dw_gate, dw_up, dw_down) of the gated layer from grad_out [T, D]. h, g, u: what
+    sdd_gated_cuda kept; layout: build_topology_cuda's eight arrays for the same routing. Six launches."""
+    lib = _lib.load()
+    _check_gated_weights(x, w_gate, w_up)
+    _check_bf16(x.device, grad_out=grad_out, w_down=w_down, h=h, g=g, u=u)
+    code = _check_activation(activation)
+    num_experts, d_model, ffn_dim = w_gate.shape
+    num_tokens, k = expert_weight.shape
+    tokens_per_expert, padded_offsets, row_token, copy_row, row_block_expert, row_offsets = layout[:6]
+    num_row_blocks = row_offsets.numel() - 1
+    _check(grad_out.shape == x.shape, f"grad_out must be {tuple(x.shape)}, got {tuple(grad_out.shape)}")
+    _check(w_down.shape == (num_experts, ffn_dim, d_model), f"w_down must be {(num_experts, ffn_dim, d_model)}")
+    _check(expert_weight.dtype in (torch.bfloat16, torch.float32), "expert_weight must be bfloat16 or float32")
+    _check(expert_weight.is_contiguous() and expert_weight.device == x.device, "expert_weight must be contiguous, on x's GPU")
+    _check(num_tokens == x.shape[0] and copy_row.numel() == num_tokens * k, "the layout is of another batch")
+    _check(row_token.numel() == num_row_blocks * BLOCK and padded_offsets.numel() == num_experts + 1,
+           "the layout does not match block size 128 and the number of experts")
+    for t in (h, g, u):
+        _check(t.shape == (num_row_blocks * (ffn_dim // BLOCK), BLOCK, BLOCK), "the kept blocks are of another layout")
+    gate_dtype = int(expert_weight.dtype == torch.float32)
+    rows = num_row_blocks * BLOCK
+    with torch.cuda.device(x.device):
+        status, stream = _ptr(device_status(x.device)), _stream()
+        x_rows, grad_rows = (torch.empty((rows, d_model), dtype=torch.bfloat16, device=x.device) for _ in range(2))
+        row_gate = torch.empty(rows, dtype=torch.float32, device=x.device)
+        gate_partial = torch.empty((rows, ffn_dim // BLOCK), dtype=torch.float32, device=x.device)
+        dg, du = torch.empty_like(g), torch.empty_like(u)
+        dx, dgate = torch.empty_like(x), torch.empty_like(expert_weight)
+        dw_gate, dw_up, dw_down = (torch.empty_like(w) for w in (w_gate, w_up, w_down))
+        _lib.check(lib.sb_gated_gather(_ptr(x), _ptr(grad_out), _ptr(expert_weight), gate_dtype, _ptr(row_token),
+                                       _ptr(copy_row), _ptr(padded_offsets), num_experts, _ptr(x_rows), _ptr(grad_rows),
+                                       _ptr(row_gate), num_tokens, k, d_model, num_row_blocks, stream))
+        _lib.check(lib.sb_gated_grad_hidden(_ptr(grad_out), _ptr(w_down), _ptr(g), _ptr(u), _ptr(row_gate),
+                                            _ptr(row_token), _ptr(row_block_expert), _ptr(row_offsets), _ptr(dg),
+                                            _ptr(du), _ptr(gate_partial), num_tokens, d_model, ffn_dim, num_experts,
+                                            num_row_blocks, code, status, stream))
+        _lib.check(lib.sb_gated_grad_weights(_ptr(x_rows), _ptr(grad_rows), _ptr(h), _ptr(dg), _ptr(du),
+                                             _ptr(padded_offsets), _ptr(tokens_per_expert), _ptr(row_offsets),
+                                             _ptr(dw_gate), _ptr(dw_up), _ptr(dw_down), d_model, ffn_dim, num_experts,
+                                             num_row_blocks, status, stream))
+        # The rows of dx take the place of the gathered rows of x, which the weight gradients were the last to read.
+        _lib.check(lib.sb_gated_grad_rows(_ptr(dg), _ptr(du), _ptr(w_gate), _ptr(w_up), _ptr(row_token),
+                                          _ptr(row_block_expert), _ptr(row_offsets), _ptr(x_rows), d_model, ffn_dim,
+                                          num_experts, num_row_blocks, status, stream))
+        _lib.check(lib.sb_gated_join(_ptr(x_rows), _ptr(gate_partial), _ptr(copy_row), _ptr(dx), _ptr(dgate), gate_dtype,
+                                     num_tokens, k, d_model, ffn_dim, stream))
+    return dx, dgate, dw_gate, dw_up, dw_down
+
+
 # ---- expert-parallel plumbing (no counterpart in the reference's extension) ----------------------
 
 def sort_copies_cuda(expert_idx: torch.Tensor, num_experts: int) -> list[torch.Tensor]:

@@ -56,6 +56,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                    c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P]),
     "sb_ep_dsd_push": (c_int, [_P, c_int64, _P, c_int64, c_int32, _P, _P, c_int32, _P, _P, c_int32, c_int32, c_int32,
                                _P, _P]),
+    "sb_sdd_gated": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+                             c_int, _P, _P]),
+    "sb_gated_gather": (c_int, [_P, _P, _P, c_int, _P, _P, _P, c_int32, _P, _P, _P, c_int64, c_int32, c_int32, c_int32,
+                                _P]),
+    "sb_gated_grad_hidden": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32,
+                                     c_int32, c_int32, _P, _P]),
+    "sb_gated_grad_weights": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32,
+                                      _P, _P]),
+    "sb_gated_grad_rows": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, _P, _P]),
+    "sb_gated_join": (c_int, [_P, _P, _P, _P, _P, c_int, c_int64, c_int32, c_int32, c_int32, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,756 @@
+// The gated expert block of the MoE layer and its backward pass, on the block-sparse layout of sb_route.
+//
+//   forward    G = X Wg[e], U = X Wu[e], H = act(G) * U            (GatedUp; the product H Wd[e] is sb_dsd)
+//   backward   S = dO Wd[e]^T (dO = grad_out of the row's token, before the gate w of its copy is applied)
+//              dgate = sum_f H S, dH = w S, dU = dH act(G), dG = dH U act'(G)                      (GradHidden)
+//              dWd = H^T (w dO), dWg = X^T dG, dWu = X^T dU                                         (GradWeights)
+//              dx[t] = sum over the token's copies of dG Wg^T + dU Wu^T                             (GradRows, join)
+//
+// dgate comes from S and H, not from Y, so the forward has to keep only G, U and H (bf16); the gate multiplies S in
+// fp32, so dH is not rounded. Roundings to bf16: G, U, H, w dO, dG, dU, the rows of dx before their sum, the results.
+//
+// act is SiLU, v / (1 + exp(-v)), or the erf form of GELU.
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "tile_gemm.cuh"
+
+namespace sb {
+namespace {
+
+constexpr float kInvSqrt2Pi = 0.3989422804014327f;
+
+__device__ __forceinline__ float fast_rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// exp(-v) overflows to inf below v = -88: the reciprocal is then 0, the limit.
+__device__ __forceinline__ float sigmoid(float v) { return fast_rcp(1.0f + __expf(-v)); }
+
+__device__ __forceinline__ float act_value(float v, int32_t activation) {
+  return activation == 0 ? v * sigmoid(v) : gelu_erf(v);
+}
+
+// act(v) and its derivative.
+__device__ __forceinline__ void act_and_slope(float v, int32_t activation, float* value, float* slope) {
+  if (activation == 0) {
+    const float s = sigmoid(v);
+    *value = v * s;
+    *slope = s * fmaf(v, 1.0f - s, 1.0f);
+  } else {
+    // Phi(v) = (1 + erf(v / sqrt 2)) / 2 by Abramowitz-Stegun 7.1.26 (absolute error below 1.5e-7), whose exponential
+    // exp(-v^2 / 2) is also the one of the density in the derivative Phi(v) + v phi(v).
+    const float a = fabsf(v) * 0.70710678118654752f;
+    const float t = fast_rcp(fmaf(0.3275911f, a, 1.0f));
+    float poly = fmaf(1.061405429f, t, -1.453152027f);
+    poly = fmaf(poly, t, 1.421413741f);
+    poly = fmaf(poly, t, -0.284496736f);
+    poly = fmaf(poly, t, 0.254829592f);
+    const float e = __expf(-a * a);
+    const float phi_abs = 1.0f - 0.5f * poly * t * e;  // Phi(|v|)
+    const float cdf = v >= 0.0f ? phi_abs : 1.0f - phi_abs;
+    *value = v * cdf;
+    *slope = fmaf(v * kInvSqrt2Pi, e, cdf);
+  }
+}
+
+// The 64-row half of the row block that a warp's 32 rows lie in holds real rows (padding sits at the end of a row
+// block). The weight gradients read the rows of an expert in steps of 64: halves without real rows are never read.
+__device__ __forceinline__ bool half_has_rows(const int32_t* row_token, int32_t row_block, int quarter) {
+  return __ldg(row_token + static_cast<int64_t>(row_block) * kTileRows + (quarter & 2) * 32) >= 0;
+}
+
+// ---- forward: both projections, the activation and the product ----------------------------------------------------
+// The tile's 256 accumulator columns are 128 columns of G next to the same 128 of U, so a thread that drains column c
+// finds its partner 128 columns on and H leaves the chip as the only result (plus G and U for training).
+struct GatedUp {
+  struct Params {
+    BandOrder order;
+    const int32_t* row_offsets;
+    const int32_t* row_token;
+    const int32_t* row_block_expert;
+    const __nv_bfloat16* x;
+    int32_t d_model;
+    int32_t activation;
+    int32_t skip_padding;  // 32-row groups of padding are not stored
+    int32_t keep;          // G and U are stored too, and every row that the backward pass reads
+  };
+  struct Tile {
+    int32_t k_steps, row_block, n0, expert, first_block;
+    bool live;
+  };
+  struct Early { bool store; };
+  static constexpr bool kGather = true, kAMnMajor = false, kBMnMajor = true;
+
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
+  static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
+    Tile t;
+    int32_t slice;
+    p.order.at(index, &t.row_block, &slice);
+    t.n0 = slice * 128;
+    t.first_block = __ldg(p.row_offsets + t.row_block);
+    t.live = __ldg(p.row_offsets + t.row_block + 1) != t.first_block;
+    t.k_steps = t.live ? p.d_model / kTileStep : 0;
+    t.expert = __ldg(p.row_block_expert + t.row_block);
+    return t;
+  }
+  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t,
+                                              uint32_t b, uint32_t bar) {
+    const uint64_t once = ptx::policy_evict_first();
+    const int32_t row = t.expert * p.d_model + ks * kTileStep;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      ptx::tma_load_2d_hint(b + j * TileSmem::kSlabBytes, &maps.m[j >> 1], t.n0 + (j & 1) * 64, row, bar, once);
+  }
+  static __device__ __forceinline__ const __nv_bfloat16* any_row(const Params& p) { return p.x; }
+  static __device__ __forceinline__ const __nv_bfloat16* gather_row(const Params& p, const Tile& t, int row) {
+    const int32_t token = __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + row);
+    return token >= 0 ? p.x + static_cast<int64_t>(token) * p.d_model : nullptr;
+  }
+  static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
+    if (p.keep) return {half_has_rows(p.row_token, t.row_block, w.quarter)};
+    return {!p.skip_padding || __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32) >= 0};
+  }
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+                                                  const Early& early) {
+    if (!early.store) return;
+    const int32_t col = w.half * 64;
+    const int32_t row = (t.first_block + (t.n0 >> 7)) * kTileRows + w.quarter * 32;
+    const uint32_t gate = w.taddr + w.half * 64;
+    const uint32_t up = gate + 128;
+    uint32_t packed[32];
+    if (p.keep) {
+      load_packed_x64(gate, packed);
+      store_rows_x64(w, &maps.m[3], packed, col, row);
+      load_packed_x64(up, packed);
+      store_rows_x64(w, &maps.m[4], packed, col, row);
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      uint32_t g[32], u[32];
+      ptx::tmem_ld_32x32b_x32(gate + part * 32, g);
+      ptx::tmem_ld_32x32b_x32(up + part * 32, u);
+      ptx::tmem_ld_wait();
+#pragma unroll
+      for (int h = 0; h < 16; ++h)
+        packed[part * 16 + h] =
+            pack_bf16(act_value(__uint_as_float(g[2 * h]), p.activation) * __uint_as_float(u[2 * h]),
+                      act_value(__uint_as_float(g[2 * h + 1]), p.activation) * __uint_as_float(u[2 * h + 1]));
+    }
+    store_rows_x64(w, &maps.m[2], packed, col, row);
+  }
+};
+
+// ---- backward: gradients of G, U and of the gates -----------------------------------------------------------------
+// S = dO Wd^T over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. The epilogue reads G and U of
+// its own row (32 columns at a time, the next 32 on their way while the current ones are worked on) and leaves dG, dU
+// and, per row and 128 columns, its share of dgate, summed in a fixed order by the join kernel.
+struct GradHidden {
+  struct Params {
+    BandOrder order;
+    const int32_t* row_offsets;
+    const int32_t* row_token;
+    const int32_t* row_block_expert;
+    const __nv_bfloat16* grad_out;
+    const __nv_bfloat16* g;
+    const __nv_bfloat16* u;
+    const float* row_gate;
+    float* gate_partial;  // [rows, F / 128]
+    int32_t d_model, ffn_dim;
+    int32_t activation;
+  };
+  struct Tile {
+    int32_t k_steps, row_block, n0, expert, first_block;
+    bool live;
+  };
+  struct Early {
+    bool store, real;
+    float gate;
+    const uint4* g;  // this row's 128 columns
+    const uint4* u;
+    uint4 g0[4], u0[4];
+  };
+  static constexpr bool kGather = true, kAMnMajor = false, kBMnMajor = false;
+
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
+  static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
+    Tile t;
+    int32_t slice;
+    p.order.at(index, &t.row_block, &slice);
+    t.n0 = slice * kTileCols;
+    t.first_block = __ldg(p.row_offsets + t.row_block);
+    t.live = __ldg(p.row_offsets + t.row_block + 1) != t.first_block;
+    t.k_steps = t.live ? p.d_model / kTileStep : 0;
+    t.expert = __ldg(p.row_block_expert + t.row_block);
+    return t;
+  }
+  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t,
+                                              uint32_t b, uint32_t bar) {
+    // With F an odd multiple of 128 the last tile's upper 128 columns are rows of the next expert (or zeros past the
+    // end): computed, never stored.
+    ptx::tma_load_2d_hint(b, &maps.m[0], ks * kTileStep, t.expert * p.ffn_dim + t.n0, bar, ptx::policy_evict_first());
+  }
+  static __device__ __forceinline__ const __nv_bfloat16* any_row(const Params& p) { return p.grad_out; }
+  static __device__ __forceinline__ const __nv_bfloat16* gather_row(const Params& p, const Tile& t, int row) {
+    const int32_t token = __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + row);
+    return token >= 0 ? p.grad_out + static_cast<int64_t>(token) * p.d_model : nullptr;
+  }
+  static __device__ __forceinline__ void fetch(const Early& e, int part, uint4 (&g)[4], uint4 (&u)[4]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      g[c] = __ldg(e.g + part * 4 + c);
+      u[c] = __ldg(e.u + part * 4 + c);
+    }
+  }
+  static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
+    Early e;
+    const int32_t n = t.n0 + w.half * 128;
+    e.store = n < p.ffn_dim && half_has_rows(p.row_token, t.row_block, w.quarter);
+    e.real = false;
+    e.gate = 0.0f;
+    if (!e.store) return e;
+    const int64_t row = static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane;
+    e.real = __ldg(p.row_token + row) >= 0;
+    e.gate = __ldg(p.row_gate + row);
+    const int64_t at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128;
+    e.g = reinterpret_cast<const uint4*>(p.g + at);
+    e.u = reinterpret_cast<const uint4*>(p.u + at);
+    fetch(e, 0, e.g0, e.u0);
+    return e;
+  }
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+                                                  const Early& early) {
+    if (!early.store) return;
+    const int32_t n = t.n0 + w.half * 128;
+    const int32_t out_row = (t.first_block + (n >> 7)) * kTileRows + w.quarter * 32;
+    // Two 32 x 32 pieces of 64-byte rows share the staging tile: dG in front, dU behind (64-byte swizzle).
+    const uint32_t swz = static_cast<uint32_t>((w.lane >> 1) & 3);
+    const uint32_t dst = w.staging + static_cast<uint32_t>(w.lane) * 64u;
+    uint4 gq[4], uq[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) { gq[c] = early.g0[c]; uq[c] = early.u0[c]; }
+    float dgate = 0.0f;
+#pragma unroll
+    for (int part = 0; part < 4; ++part) {
+      uint32_t s[32];
+      ptx::tmem_ld_32x32b_x32(w.taddr + w.half * 128 + part * 32, s);
+      uint4 gn[4], un[4];
+      if (part < 3) fetch(early, part + 1, gn, un);
+      ptx::tmem_ld_wait();
+      uint32_t dg[16], du[16];
+#pragma unroll
+      for (int h = 0; h < 16; ++h) {
+        const uint32_t graw = reinterpret_cast<const uint32_t*>(gq)[h];
+        const uint32_t uraw = reinterpret_cast<const uint32_t*>(uq)[h];
+        const float2 gf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&graw));
+        const float2 uf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uraw));
+        float a0, a1, d0, d1;
+        act_and_slope(gf.x, p.activation, &a0, &d0);
+        act_and_slope(gf.y, p.activation, &a1, &d1);
+        const float s0 = __uint_as_float(s[2 * h]);
+        const float s1 = __uint_as_float(s[2 * h + 1]);
+        dgate = fmaf(a0 * uf.x, s0, dgate);
+        dgate = fmaf(a1 * uf.y, s1, dgate);
+        const float h0 = s0 * early.gate;
+        const float h1 = s1 * early.gate;
+        dg[h] = early.real ? pack_bf16(h0 * uf.x * d0, h1 * uf.y * d1) : 0u;
+        du[h] = early.real ? pack_bf16(h0 * a0, h1 * a1) : 0u;
+      }
+      if (w.lane == 0) ptx::bulk_wait_read();
+      __syncwarp();
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) {
+        ptx::st_shared_v4(dst + ((c ^ swz) << 4), dg[4 * c], dg[4 * c + 1], dg[4 * c + 2], dg[4 * c + 3]);
+        ptx::st_shared_v4(dst + 2048u + ((c ^ swz) << 4), du[4 * c], du[4 * c + 1], du[4 * c + 2], du[4 * c + 3]);
+      }
+      ptx::fence_proxy_async_shared();
+      __syncwarp();
+      if (w.lane == 0) {
+        ptx::tma_store_2d(&maps.m[1], w.staging, part * 32, out_row);
+        ptx::tma_store_2d(&maps.m[2], w.staging + 2048u, part * 32, out_row);
+        ptx::bulk_commit();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) { gq[c] = gn[c]; uq[c] = un[c]; }
+    }
+    if (early.real)
+      p.gate_partial[(static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane) * (p.ffn_dim / 128) + (n >> 7)] = dgate;
+  }
+};
+
+// ---- backward: the rows of dx -------------------------------------------------------------------------------------
+// dG Wg^T + dU Wu^T as one product with 2 F inner columns. Wg and Wu [D, F] are K-major operands as they lie.
+struct GradRows {
+  struct Params {
+    BandOrder order;
+    const int32_t* row_offsets;
+    const int32_t* row_token;
+    const int32_t* row_block_expert;
+    int32_t d_model, ffn_dim;
+  };
+  struct Tile {
+    int32_t k_steps, row_block, n0, expert, first_block;
+    bool live;
+  };
+  struct Early { bool store; };
+  static constexpr bool kGather = false, kAMnMajor = false, kBMnMajor = false;
+
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
+  static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
+    Tile t;
+    int32_t slice;
+    p.order.at(index, &t.row_block, &slice);
+    t.n0 = slice * kTileCols;
+    t.first_block = __ldg(p.row_offsets + t.row_block);
+    t.live = __ldg(p.row_offsets + t.row_block + 1) != t.first_block;
+    t.k_steps = t.live ? 2 * (p.ffn_dim / kTileStep) : 0;
+    t.expert = __ldg(p.row_block_expert + t.row_block);
+    return t;
+  }
+  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
+                                              uint32_t b, uint32_t bar) {
+    const uint64_t once = ptx::policy_evict_first();
+    const int32_t steps = p.ffn_dim / kTileStep;
+    const int which = ks < steps ? 0 : 1;
+    const int32_t k = (ks - which * steps) * kTileStep;
+    ptx::tma_load_2d_hint(a, &maps.m[which], k & 127, (t.first_block + (k >> 7)) * kTileRows, bar, once);
+    ptx::tma_load_2d_hint(b, &maps.m[2 + which], k, t.expert * p.d_model + t.n0, bar, once);
+  }
+  static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
+    return {__ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32) >= 0};
+  }
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+                                                  const Early& early) {
+    if (!early.store) return;
+#pragma unroll 1
+    for (int g = 0; g < 2; ++g) {
+      const int32_t col = t.n0 + w.half * 128 + g * 64;
+      if (col >= p.d_model) break;
+      uint32_t packed[32];
+      load_packed_x64(w.taddr + w.half * 128 + g * 64, packed);
+      store_rows_x64(w, &maps.m[4], packed, col, t.row_block * kTileRows + w.quarter * 32);
+    }
+  }
+};
+
+// ---- backward: the three weight gradients -------------------------------------------------------------------------
+// The rows of an expert are the inner dimension, so both operands are MN-major: X, w dO, H, dG and dU as they lie.
+// An expert's rows end inside a step of 64; the rest of that step is zero rows in X and w dO (written by the gather
+// kernel) against finite ones (zeros) in H, dG and dU. An expert without rows gets zeros.
+struct GradWeights {
+  struct Params {
+    const int32_t* padded_offsets;
+    const int32_t* tokens_per_expert;
+    const int32_t* row_offsets;
+    int32_t num_experts, d_model, ffn_dim;
+    int32_t down_cols, down_tiles;  // column tiles of dWd [F, D], its tiles per expert
+    int32_t up_cols, up_tiles;      // the same of dWg and dWu [D, F]
+  };
+  struct Tile {
+    int32_t k_steps, which, expert, m0, n0, row0, block0;  // which: 0 dWd, 1 dWg, 2 dWu
+    bool live;
+  };
+  struct Early {};
+  static constexpr bool kGather = false, kAMnMajor = true, kBMnMajor = true;
+
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) {
+    return p.num_experts * (p.down_tiles + 2 * p.up_tiles);
+  }
+  static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
+    Tile t;
+    const int32_t per_expert = p.down_tiles + 2 * p.up_tiles;
+    t.expert = index / per_expert;
+    int32_t i = index - t.expert * per_expert;
+    t.which = 0;
+    int32_t cols = p.down_cols;
+    if (i >= p.down_tiles) {
+      i -= p.down_tiles;
+      t.which = i >= p.up_tiles ? 2 : 1;
+      i -= (t.which - 1) * p.up_tiles;
+      cols = p.up_cols;
+    }
+    const int32_t m = i / cols;
+    t.m0 = m * kTileRows;
+    t.n0 = (i - m * cols) * kTileCols;
+    t.live = true;
+    t.k_steps = (__ldg(p.tokens_per_expert + t.expert) + kTileStep - 1) / kTileStep;
+    t.row0 = __ldg(p.padded_offsets + t.expert);
+    t.block0 = __ldg(p.row_offsets + t.row0 / kTileRows);
+    return t;
+  }
+  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
+                                              uint32_t b, uint32_t bar) {
+    const int32_t row = t.row0 + ks * kTileStep;                        // of X and w dO
+    const int32_t block = t.block0 + (ks >> 1) * (p.ffn_dim >> 7);      // first of the row block's blocks
+    const int32_t inside = (ks & 1) * kTileStep;
+    const int32_t slab = TileSmem::kSlabBytes;
+    if (t.which == 0) {
+      const int32_t h_row = (block + (t.m0 >> 7)) * kTileRows + inside;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) ptx::tma_load_2d(a + j * slab, &maps.m[2], j * 64, h_row, bar);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ptx::tma_load_2d(b + j * slab, &maps.m[1], t.n0 + j * 64, row, bar);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) ptx::tma_load_2d(a + j * slab, &maps.m[0], t.m0 + j * 64, row, bar);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // With F an odd multiple of 128 the last tile's upper blocks are the next row block's: never stored.
+        const int32_t n = t.n0 + j * 64;
+        ptx::tma_load_2d(b + j * slab, &maps.m[2 + t.which], n & 127, (block + (n >> 7)) * kTileRows + inside, bar);
+      }
+    }
+  }
+  static __device__ __forceinline__ Early prefetch(const Params&, const Tile&, const EpilogueWarp&) { return {}; }
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+                                                  const Early&) {
+    const int32_t width = t.which == 0 ? p.d_model : p.ffn_dim;
+    const int32_t row = t.expert * (t.which == 0 ? p.ffn_dim : p.d_model) + t.m0 + w.quarter * 32;
+#pragma unroll 1
+    for (int g = 0; g < 2; ++g) {
+      const int32_t col = t.n0 + w.half * 128 + g * 64;
+      if (col >= width) break;
+      uint32_t packed[32];
+      if (t.k_steps > 0) {
+        load_packed_x64(w.taddr + w.half * 128 + g * 64, packed);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 32; ++h) packed[h] = 0u;
+      }
+      store_rows_x64(w, &maps.m[5 + t.which], packed, col, row);
+    }
+  }
+};
+
+// ---- small kernels ------------------------------------------------------------------------------------------------
+
+constexpr int kSmallThreads = 256;
+
+__device__ __forceinline__ float gate_at(const void* gate, int gate_dtype, int64_t i) {
+  return gate_dtype == 1 ? __ldg(static_cast<const float*>(gate) + i)
+                         : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(gate) + i));
+}
+
+// One warp per row of the layout: X[r] = x[token], (w dO)[r] = w * grad_out[token], row_gate[r] = w; zeros for padding.
+__global__ void __launch_bounds__(kSmallThreads)
+gated_gather_kernel(const uint4* __restrict__ x, const uint4* __restrict__ grad_out, const void* __restrict__ gate,
+                    int gate_dtype, const int32_t* __restrict__ row_token, const int32_t* __restrict__ copy_row,
+                    const int32_t* __restrict__ num_rows, uint4* __restrict__ x_rows, uint4* __restrict__ grad_rows,
+                    float* __restrict__ row_gate, int32_t k, int32_t vecs) {
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int32_t rows = __ldg(num_rows);
+  const int32_t warps = static_cast<int32_t>(gridDim.x * (kSmallThreads / 32));
+  for (int32_t r = static_cast<int32_t>(blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)); r < rows; r += warps) {
+    const int32_t token = __ldg(row_token + r);
+    uint4* xr = x_rows + static_cast<int64_t>(r) * vecs;
+    uint4* gr = grad_rows + static_cast<int64_t>(r) * vecs;
+    if (token < 0) {
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      for (int32_t v = lane; v < vecs; v += 32) { xr[v] = zero; gr[v] = zero; }
+      if (lane == 0) row_gate[r] = 0.0f;
+      continue;
+    }
+    // The copy of the token that this row is: the one whose row it is (rows are unique).
+    float w = 0.0f;
+    for (int32_t j0 = 0; j0 < k; j0 += 32) {
+      const int32_t j = j0 + lane;
+      const bool mine = j < k && __ldg(copy_row + static_cast<int64_t>(token) * k + j) == r;
+      const unsigned who = __ballot_sync(0xffffffffu, mine);
+      if (who != 0u) {
+        w = gate_at(gate, gate_dtype, static_cast<int64_t>(token) * k + j0 + __ffs(who) - 1);
+        break;
+      }
+    }
+    if (lane == 0) row_gate[r] = w;
+    const uint4* xs = x + static_cast<int64_t>(token) * vecs;
+    const uint4* gs = grad_out + static_cast<int64_t>(token) * vecs;
+    for (int32_t v = lane; v < vecs; v += 32) {
+      xr[v] = __ldg(xs + v);
+      uint4 raw = __ldg(gs + v);
+      uint32_t* q = reinterpret_cast<uint32_t*>(&raw);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[c]));
+        q[c] = pack_bf16(f.x * w, f.y * w);
+      }
+      gr[v] = raw;
+    }
+  }
+}
+
+// dx[t] = sum over the token's copies of their rows, in copy order in fp32; dgate[t, j] = sum of the row's partial
+// sums in column order. One warp per token.
+__global__ void __launch_bounds__(kSmallThreads)
+gated_join_kernel(const uint4* __restrict__ dx_rows, const float* __restrict__ gate_partial,
+                  const int32_t* __restrict__ copy_row, uint4* __restrict__ dx, void* __restrict__ dgate, int gate_dtype,
+                  int64_t num_tokens, int32_t k, int32_t vecs, int32_t partials) {
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kSmallThreads / 32);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kSmallThreads / 32) + (threadIdx.x >> 5); t < num_tokens; t += warps) {
+    for (int32_t v = lane; v < vecs; v += 32) {
+      float acc[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
+      for (int32_t j = 0; j < k; ++j) {
+        const int32_t row = __ldg(copy_row + t * k + j);
+        if (row < 0) continue;
+        const uint4 raw = __ldg(dx_rows + static_cast<int64_t>(row) * vecs + v);
+        const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 f = __bfloat1622float2(pairs[q]);
+          acc[2 * q] += f.x;
+          acc[2 * q + 1] += f.y;
+        }
+      }
+      uint4 packed;
+      uint32_t* o = reinterpret_cast<uint32_t*>(&packed);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = pack_bf16(acc[2 * q], acc[2 * q + 1]);
+      dx[t * vecs + v] = packed;
+    }
+    for (int32_t j = 0; j < k; ++j) {
+      const int32_t row = __ldg(copy_row + t * k + j);
+      float sum = 0.0f;
+      if (row >= 0)
+        for (int32_t b = lane; b < partials; b += 32) sum += __ldg(gate_partial + static_cast<int64_t>(row) * partials + b);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) {
+        if (gate_dtype == 1) static_cast<float*>(dgate)[t * k + j] = sum;
+        else static_cast<__nv_bfloat16*>(dgate)[t * k + j] = __float2bfloat16_rn(sum);
+      }
+    }
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------
+
+// Size rules all the products of the gated layer share. Sets *ffn_blocks.
+int check_gated(const char* what, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
+                int32_t activation) {
+  if (d_model <= 0 || d_model % 128 != 0) return fail(SB_ERR_INVALID_ARGUMENT, "%s: D (%d) must be a positive multiple of 128", what, d_model);
+  if (ffn_dim <= 0 || ffn_dim % 128 != 0) return fail(SB_ERR_INVALID_ARGUMENT, "%s: F (%d) must be a positive multiple of 128", what, ffn_dim);
+  if (num_experts <= 0 || num_row_blocks < 0) return fail(SB_ERR_INVALID_ARGUMENT, "%s: bad sizes", what);
+  if (activation != SB_ACT_SILU && activation != SB_ACT_GELU)
+    return fail(SB_ERR_INVALID_ARGUMENT, "%s: activation must be 0 (SiLU) or 1 (GELU), got %d", what, activation);
+  const int64_t most = static_cast<int64_t>(num_row_blocks) * ffn_dim;  // rows of the block arrays seen as [nnz * 128, 128]
+  if (most > INT32_MAX - 4 * kTileRows || static_cast<int64_t>(num_experts) * d_model > INT32_MAX - kTileCols ||
+      static_cast<int64_t>(num_experts) * ffn_dim > INT32_MAX - kTileCols ||
+      static_cast<int64_t>(num_row_blocks) * kTileRows > INT32_MAX)
+    return fail(SB_ERR_INVALID_ARGUMENT, "%s: problem too large", what);
+  return SB_OK;
+}
+
+// Row blocks per band of the tile walk, for products that stream an expert's weights in column slices.
+int32_t band_for(int32_t num_row_blocks, int32_t num_experts) {
+  return num_row_blocks >= 4 * static_cast<int64_t>(num_experts) ? 8 : 1;
+}
+
+bool any_misaligned(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return true;
+  return false;
+}
+bool any_null(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (p == nullptr) return true;
+  return false;
+}
+
+}  // namespace
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
+                            const int32_t* row_block_expert, const int32_t* row_offsets, void* h_blocks, void* g_blocks,
+                            void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                            int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
+                            sb_stream_t stream) {
+  clear_error();
+  if (int rc = check_gated("sdd_gated", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
+  if (num_row_blocks == 0) return SB_OK;
+  if (any_null({x, w_gate, w_up, row_token, row_block_expert, row_offsets, h_blocks}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: NULL buffer");
+  if ((g_blocks == nullptr) != (u_blocks == nullptr))
+    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: pass both kept arrays or neither");
+  if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: T must be positive");
+  if (any_misaligned({x, w_gate, w_up, h_blocks, g_blocks, u_blocks}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: x, the weights and the blocks must be 16-byte aligned");
+  const uint64_t w_rows = static_cast<uint64_t>(num_experts) * d_model;
+  const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;  // nnz * 128
+  TileMaps maps{};
+  if (int rc = encode_2d_map(&maps.m[0], w_gate, w_rows, ffn_dim, 64, 64, 2, "sdd_gated (w_gate)")) return rc;
+  if (int rc = encode_2d_map(&maps.m[1], w_up, w_rows, ffn_dim, 64, 64, 2, "sdd_gated (w_up)")) return rc;
+  if (int rc = encode_2d_map(&maps.m[2], h_blocks, b_rows, 128, 32, 64, 2, "sdd_gated (blocks)")) return rc;
+  if (g_blocks != nullptr) {
+    if (int rc = encode_2d_map(&maps.m[3], g_blocks, b_rows, 128, 32, 64, 2, "sdd_gated (kept gate)")) return rc;
+    if (int rc = encode_2d_map(&maps.m[4], u_blocks, b_rows, 128, 32, 64, 2, "sdd_gated (kept up)")) return rc;
+  }
+  GatedUp::Params p{};
+  p.order = {num_row_blocks, ffn_dim / 128, band_for(num_row_blocks, num_experts)};
+  p.row_offsets = row_offsets;
+  p.row_token = row_token;
+  p.row_block_expert = row_block_expert;
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.d_model = d_model;
+  p.activation = activation;
+  p.skip_padding = skip_padding_rows ? 1 : 0;
+  p.keep = g_blocks != nullptr ? 1 : 0;
+  return launch_tile_gemm<GatedUp>(maps, p, static_cast<int64_t>(num_row_blocks) * (ffn_dim / 128), dev_status,
+                                   as_stream(stream), "sdd_gated");
+}
+
+extern "C" int sb_gated_gather(const void* x, const void* grad_out, const void* gate, int gate_dtype,
+                               const int32_t* row_token, const int32_t* copy_row, const int32_t* padded_offsets,
+                               int32_t num_experts, void* x_rows, void* grad_rows, float* row_gate, int64_t num_tokens,
+                               int32_t k, int32_t d_model, int32_t num_row_blocks, sb_stream_t stream) {
+  clear_error();
+  if (int rc = check_gated("gated_gather", d_model, 128, num_experts, num_row_blocks, 0)) return rc;
+  if (num_row_blocks == 0) return SB_OK;
+  if (any_null({x, grad_out, gate, row_token, copy_row, padded_offsets, x_rows, grad_rows, row_gate}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: NULL buffer");
+  if (num_tokens <= 0 || k <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: T and k must be positive");
+  if (gate_dtype != 0 && gate_dtype != 1) return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: gate_dtype must be 0 (bf16) or 1 (fp32)");
+  if (any_misaligned({x, grad_out, x_rows, grad_rows}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: rows must be 16-byte aligned");
+  const DeviceInfo* info = current_device_info();
+  if (info == nullptr) return SB_ERR_CUDA;
+  const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
+  gated_gather_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, as_stream(stream)>>>(
+      static_cast<const uint4*>(x), static_cast<const uint4*>(grad_out), gate, gate_dtype, row_token, copy_row,
+      padded_offsets + num_experts, static_cast<uint4*>(x_rows), static_cast<uint4*>(grad_rows), row_gate, k, d_model / 8);
+  return check_launch("gated_gather");
+}
+
+extern "C" int sb_gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_blocks, const void* u_blocks,
+                                    const float* row_gate, const int32_t* row_token, const int32_t* row_block_expert,
+                                    const int32_t* row_offsets, void* dg_blocks, void* du_blocks, float* gate_partial,
+                                    int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                                    int32_t num_row_blocks, int32_t activation, int32_t* dev_status, sb_stream_t stream) {
+  clear_error();
+  if (int rc = check_gated("gated_grad_hidden", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
+  if (num_row_blocks == 0) return SB_OK;
+  if (any_null({grad_out, w_down, g_blocks, u_blocks, row_gate, row_token, row_block_expert, row_offsets, dg_blocks,
+                du_blocks, gate_partial}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: NULL buffer");
+  if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: T must be positive");
+  if (any_misaligned({grad_out, w_down, g_blocks, u_blocks, dg_blocks, du_blocks}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: buffers must be 16-byte aligned");
+  const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
+  TileMaps maps{};
+  if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, 256, 64, 2, "gated_grad_hidden (w_down)")) return rc;
+  if (int rc = encode_2d_map(&maps.m[1], dg_blocks, b_rows, 128, 32, 32, 2, "gated_grad_hidden (dG)")) return rc;
+  if (int rc = encode_2d_map(&maps.m[2], du_blocks, b_rows, 128, 32, 32, 2, "gated_grad_hidden (dU)")) return rc;
+  GradHidden::Params p{};
+  const int32_t slices = (ffn_dim + kTileCols - 1) / kTileCols;
+  p.order = {num_row_blocks, slices, band_for(num_row_blocks, num_experts)};
+  p.row_offsets = row_offsets;
+  p.row_token = row_token;
+  p.row_block_expert = row_block_expert;
+  p.grad_out = static_cast<const __nv_bfloat16*>(grad_out);
+  p.g = static_cast<const __nv_bfloat16*>(g_blocks);
+  p.u = static_cast<const __nv_bfloat16*>(u_blocks);
+  p.row_gate = row_gate;
+  p.gate_partial = gate_partial;
+  p.d_model = d_model;
+  p.ffn_dim = ffn_dim;
+  p.activation = activation;
+  return launch_tile_gemm<GradHidden>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, as_stream(stream),
+                                      "gated_grad_hidden");
+}
+
+extern "C" int sb_gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_blocks, const void* dg_blocks,
+                                     const void* du_blocks, const int32_t* padded_offsets, const int32_t* tokens_per_expert,
+                                     const int32_t* row_offsets, void* dw_gate, void* dw_up, void* dw_down, int32_t d_model,
+                                     int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status,
+                                     sb_stream_t stream) {
+  clear_error();
+  if (int rc = check_gated("gated_grad_weights", d_model, ffn_dim, num_experts, num_row_blocks, 0)) return rc;
+  if (num_row_blocks <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_weights: the layout has no row blocks");
+  if (any_null({x_rows, grad_rows, h_blocks, dg_blocks, du_blocks, padded_offsets, tokens_per_expert, row_offsets, dw_gate,
+                dw_up, dw_down}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_weights: NULL buffer");
+  if (any_misaligned({x_rows, grad_rows, h_blocks, dg_blocks, du_blocks, dw_gate, dw_up, dw_down}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_weights: buffers must be 16-byte aligned");
+  const char* what = "gated_grad_weights";
+  const uint64_t rows = static_cast<uint64_t>(num_row_blocks) * kTileRows;
+  const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
+  const uint64_t up_rows = static_cast<uint64_t>(num_experts) * d_model;
+  const uint64_t down_rows = static_cast<uint64_t>(num_experts) * ffn_dim;
+  TileMaps maps{};
+  if (int rc = encode_2d_map(&maps.m[0], x_rows, rows, d_model, 64, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[1], grad_rows, rows, d_model, 64, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[2], h_blocks, b_rows, 128, 64, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[3], dg_blocks, b_rows, 128, 64, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[4], du_blocks, b_rows, 128, 64, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[5], dw_down, down_rows, d_model, 32, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[6], dw_gate, up_rows, ffn_dim, 32, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[7], dw_up, up_rows, ffn_dim, 32, 64, 2, what)) return rc;
+  GradWeights::Params p{};
+  p.padded_offsets = padded_offsets;
+  p.tokens_per_expert = tokens_per_expert;
+  p.row_offsets = row_offsets;
+  p.num_experts = num_experts;
+  p.d_model = d_model;
+  p.ffn_dim = ffn_dim;
+  p.down_cols = (d_model + kTileCols - 1) / kTileCols;
+  p.down_tiles = ffn_dim / kTileRows * p.down_cols;
+  p.up_cols = (ffn_dim + kTileCols - 1) / kTileCols;
+  p.up_tiles = d_model / kTileRows * p.up_cols;
+  const int64_t tiles = static_cast<int64_t>(num_experts) * (p.down_tiles + 2ll * p.up_tiles);
+  return launch_tile_gemm<GradWeights>(maps, p, tiles, dev_status, as_stream(stream), what);
+}
+
+extern "C" int sb_gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up,
+                                  const int32_t* row_token, const int32_t* row_block_expert, const int32_t* row_offsets,
+                                  void* dx_rows, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                                  int32_t num_row_blocks, int32_t* dev_status, sb_stream_t stream) {
+  clear_error();
+  if (int rc = check_gated("gated_grad_rows", d_model, ffn_dim, num_experts, num_row_blocks, 0)) return rc;
+  if (num_row_blocks == 0) return SB_OK;
+  if (any_null({dg_blocks, du_blocks, w_gate, w_up, row_token, row_block_expert, row_offsets, dx_rows}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_rows: NULL buffer");
+  if (any_misaligned({dg_blocks, du_blocks, w_gate, w_up, dx_rows}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_rows: buffers must be 16-byte aligned");
+  const char* what = "gated_grad_rows";
+  const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
+  const uint64_t w_rows = static_cast<uint64_t>(num_experts) * d_model;
+  TileMaps maps{};
+  if (int rc = encode_2d_map(&maps.m[0], dg_blocks, b_rows, 128, 128, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[1], du_blocks, b_rows, 128, 128, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[2], w_gate, w_rows, ffn_dim, 256, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[3], w_up, w_rows, ffn_dim, 256, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[4], dx_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, what)) return rc;
+  GradRows::Params p{};
+  const int32_t slices = (d_model + kTileCols - 1) / kTileCols;
+  p.order = {num_row_blocks, slices, 1};
+  p.row_offsets = row_offsets;
+  p.row_token = row_token;
+  p.row_block_expert = row_block_expert;
+  p.d_model = d_model;
+  p.ffn_dim = ffn_dim;
+  return launch_tile_gemm<GradRows>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, as_stream(stream), what);
+}
+
+extern "C" int sb_gated_join(const void* dx_rows, const float* gate_partial, const int32_t* copy_row, void* dx, void* dgate,
+                             int gate_dtype, int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim,
+                             sb_stream_t stream) {
+  clear_error();
+  if (int rc = check_gated("gated_join", d_model, ffn_dim, 1, 0, 0)) return rc;
+  if (any_null({dx_rows, gate_partial, copy_row, dx, dgate})) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: NULL buffer");
+  if (num_tokens <= 0 || k <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: T and k must be positive");
+  if (gate_dtype != 0 && gate_dtype != 1) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: gate_dtype must be 0 (bf16) or 1 (fp32)");
+  if (any_misaligned({dx_rows, dx})) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: rows must be 16-byte aligned");
+  const DeviceInfo* info = current_device_info();
+  if (info == nullptr) return SB_ERR_CUDA;
+  const int64_t blocks = std::min<int64_t>((num_tokens + 7) / 8, static_cast<int64_t>(info->sm_count) * 8);
+  gated_join_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, as_stream(stream)>>>(
+      static_cast<const uint4*>(dx_rows), gate_partial, copy_row, static_cast<uint4*>(dx), dgate, gate_dtype, num_tokens, k,
+      d_model / 8, ffn_dim / 128);
+  return check_launch("gated_join");
+}

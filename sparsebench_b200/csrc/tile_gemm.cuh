@@ -1,0 +1,353 @@
+// A persistent tcgen05 matmul kernel whose tiles, operand loads and epilogue come from a policy class; the matmuls
+// of the gated expert layer and of its backward pass (gated.cu) are policies of it.
+//
+// One output tile = 128 rows x 256 columns, accumulated in fp32 in TMEM (two accumulators, so the epilogue of one
+// tile runs while the tensor cores fill the other). K steps of 64. Warp roles, with nothing but mbarriers between
+// them: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue, warps 10-13 row gather (policies that gather).
+//
+// A stage of the shared-memory ring holds A (16 KB) and B (32 KB) with the 128-byte swizzle, each in one of two forms:
+//   K-major   rows of the M (N) dimension, 64 K elements = 128 bytes per row
+//   MN-major  slabs of 64 K rows x 64 M (N) elements, 8 KB per slab
+// so weights, activations and their gradients are all consumed as they lie in memory; nothing is transposed or copied.
+//
+// Every wait is bounded; on expiry the role sets a bit in *dev_status, raises the block's abort flag and all roles
+// drain to the common exit, where TMEM is released.
+#pragma once
+
+#include "bsr_gemm.cuh"
+
+namespace sb {
+
+constexpr int kTileRows = 128;
+constexpr int kTileCols = 256;
+constexpr int kTileStep = 64;
+
+struct alignas(64) TileMaps {
+  CUtensorMap m[8];
+};
+
+struct TileSmem {
+  static constexpr int kStages = 4;
+  static constexpr int kABytes = kTileRows * kTileStep * 2;
+  static constexpr int kBBytes = kTileCols * kTileStep * 2;
+  static constexpr int kSlabBytes = kTileStep * 128;
+  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kStagingBytes = 32 * 128;  // per epilogue warp: 32 rows x 64 bf16
+  static constexpr int kBarrierBytes = 256;
+  static constexpr int kBytes = 1024 + kStages * (kABytes + kBBytes) + kEpilogueWarps * kStagingBytes + kBarrierBytes;
+  static_assert(kBytes <= 227 * 1024, "shared memory budget");
+};
+
+// What an epilogue warp works with.
+struct EpilogueWarp {
+  int quarter;       // rows quarter * 32 .. + 31 of the tile (TMEM lanes this warp may read)
+  int half;          // 0 or 1: which half of the tile's columns is this warp's
+  int lane;
+  uint32_t staging;  // this warp's 4 KB in shared memory
+  uint32_t taddr;    // TMEM address of (lane quarter, column 0) of the finished accumulator
+};
+
+// bf16 pairs of 64 columns of this lane's row -> the warp's staging tile -> one TMA store of 32 rows x 64 columns.
+__device__ __forceinline__ void store_rows_x64(const EpilogueWarp& w, const CUtensorMap* map, const uint32_t (&packed)[32],
+                                               int32_t col, int32_t row) {
+  if (w.lane == 0) ptx::bulk_wait_read();  // the store before has read the staging tile
+  __syncwarp();
+  const uint32_t swz = static_cast<uint32_t>(w.lane & 7);
+  const uint32_t dst = w.staging + static_cast<uint32_t>(w.lane) * 128u;
+#pragma unroll
+  for (uint32_t c = 0; c < 8; ++c)
+    ptx::st_shared_v4(dst + ((c ^ swz) << 4), packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+  ptx::fence_proxy_async_shared();
+  __syncwarp();
+  if (w.lane == 0) {
+    ptx::tma_store_2d(map, w.staging, col, row);
+    ptx::bulk_commit();
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 pair = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&pair);
+}
+
+// 64 accumulator columns as they are, rounded to bf16.
+__device__ __forceinline__ void load_packed_x64(uint32_t taddr, uint32_t (&packed)[32]) {
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    uint32_t v[32];
+    ptx::tmem_ld_32x32b_x32(taddr + part * 32, v);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int h = 0; h < 16; ++h)
+      packed[part * 16 + h] = pack_bf16(__uint_as_float(v[2 * h]), __uint_as_float(v[2 * h + 1]));
+  }
+}
+
+// Tile order over (row block, column slice): bands of `band` row blocks, inside a band the row block changes fastest.
+// A band of 1 is row-block-major. Taller bands let the row blocks of one expert that run at the same time share a
+// weight tile through L2 where an expert has many row blocks.
+struct BandOrder {
+  int32_t num_row_blocks, num_slices, band;
+  __device__ __forceinline__ void at(int32_t tile, int32_t* row_block, int32_t* slice) const {
+    const int32_t per_band = band * num_slices;
+    const int32_t b = tile / per_band;
+    const int32_t first = b * band;
+    const int32_t height = min(band, num_row_blocks - first);
+    const int32_t inside = tile - b * per_band;
+    *slice = inside / height;
+    *row_block = first + inside - *slice * height;
+  }
+};
+
+// A policy Op has
+//   Params, Tile (with int32_t k_steps: 0 = nothing to multiply; bool live: the epilogue has something to do)
+//   static constexpr bool kGather, kAMnMajor, kBMnMajor
+//   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar), tx_bytes
+//   gather_row(p, tile, row) -> source row of A or nullptr (zeros), for kGather
+//   prefetch(p, tile, w) -> Early (global loads that can start before the accumulator is ready)
+//   epilogue(maps, p, tile, w, early)
+template <class Op>
+struct TileConfig {
+  static constexpr int kGatherWarps = Op::kGather ? 4 : 0;
+  static constexpr int kFirstGatherWarp = 2 + TileSmem::kEpilogueWarps;
+  static constexpr int kThreads = 32 * (kFirstGatherWarp + kGatherWarps);
+  static constexpr uint32_t kFullArrivals = 1 + 32 * kGatherWarps;
+};
+
+template <class Op>
+__global__ void __launch_bounds__(TileConfig<Op>::kThreads, 1)
+tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ typename Op::Params p, int32_t* dev_status) {
+  using Cfg = TileConfig<Op>;
+  using S = TileSmem;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t a_base = smem_base;
+  const uint32_t b_base = a_base + S::kStages * S::kABytes;
+  const uint32_t staging_base = b_base + S::kStages * S::kBBytes;
+  const uint32_t full_bar = staging_base + S::kEpilogueWarps * S::kStagingBytes;  // [kStages]
+  const uint32_t empty_bar = full_bar + 8 * S::kStages;                           // [kStages]
+  const uint32_t acc_full_bar = empty_bar + 8 * S::kStages;                       // [2]
+  const uint32_t acc_empty_bar = acc_full_bar + 16;                               // [2]
+  const uint32_t tmem_slot = acc_empty_bar + 16;
+  const uint32_t abort_slot = tmem_slot + 4;
+  uint8_t* smem_aligned = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
+  volatile uint32_t* tmem_word = reinterpret_cast<volatile uint32_t*>(smem_aligned + (tmem_slot - smem_base));
+  volatile uint32_t* abort_word = reinterpret_cast<volatile uint32_t*>(smem_aligned + (abort_slot - smem_base));
+
+  const int warp = static_cast<int>(threadIdx.x >> 5);
+  const int lane = static_cast<int>(threadIdx.x & 31);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      ptx::mbar_init(full_bar + 8 * s, Cfg::kFullArrivals);
+      ptx::mbar_init(empty_bar + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(acc_full_bar + 8 * a, 1);
+      ptx::mbar_init(acc_empty_bar + 8 * a, 32 * S::kEpilogueWarps);
+    }
+    *abort_word = 0u;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, 2 * kTileCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  ptx::tcgen05_fence_after_sync();
+  const uint32_t tmem_base = *tmem_word;
+
+  const int32_t total = Op::total_tiles(p);
+  const int32_t step = static_cast<int32_t>(gridDim.x);
+  auto give_up = [&](int bit) {
+    *abort_word = 1u;
+    if (dev_status != nullptr) atomicOr(dev_status, bit);
+  };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      int32_t index = blockIdx.x;
+      typename Op::Tile next{};
+      if (index < total) next = Op::tile(p, index);
+      for (; ok && index < total; index += step) {
+        const typename Op::Tile tile = next;
+        if (index + step < total) next = Op::tile(p, index + step);
+        for (int32_t ks = 0; ks < tile.k_steps; ++ks) {
+          if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
+            give_up(SB_DEV_TIMEOUT_PRODUCER);
+            ok = false;
+            break;
+          }
+          const uint32_t bar = full_bar + 8 * stage;
+          ptx::mbar_arrive_expect_tx(bar, S::kBBytes + (Op::kGather ? 0 : S::kABytes));
+          Op::load(maps, p, tile, ks, a_base + stage * S::kABytes, b_base + stage * S::kBBytes, bar);
+          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = ptx::make_idesc_bf16(kTileRows, kTileCols, Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      int32_t index = blockIdx.x;
+      typename Op::Tile next{};
+      if (index < total) next = Op::tile(p, index);
+      for (; ok && index < total; index += step) {
+        const int32_t k_steps = next.k_steps;
+        if (index + step < total) next = Op::tile(p, index + step);
+        if (k_steps == 0) continue;
+        if (!ptx::mbar_wait_bounded(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_word)) {
+          give_up(SB_DEV_TIMEOUT_MMA);
+          break;
+        }
+        ptx::tcgen05_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + acc * kTileCols;
+        for (int32_t ks = 0; ks < k_steps; ++ks) {
+          if (!ptx::mbar_wait_bounded(full_bar + 8 * stage, phase, abort_word)) {
+            give_up(SB_DEV_TIMEOUT_MMA);
+            ok = false;
+            break;
+          }
+          if (Op::kGather) ptx::fence_proxy_async_shared();  // rows written by cp.async, read by the tensor core
+          ptx::tcgen05_fence_after_sync();
+          const uint32_t a_addr = a_base + stage * S::kABytes;
+          const uint32_t b_addr = b_base + stage * S::kBBytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint64_t desc_a = Op::kAMnMajor ? ptx::make_smem_desc(a_addr + kk * 2048, S::kSlabBytes, 1024)
+                                                  : ptx::make_smem_desc(a_addr + kk * 32, 16, 1024);
+            const uint64_t desc_b = Op::kBMnMajor ? ptx::make_smem_desc(b_addr + kk * 2048, S::kSlabBytes, 1024)
+                                                  : ptx::make_smem_desc(b_addr + kk * 32, 16, 1024);
+            ptx::umma_bf16(d_tmem, desc_a, desc_b, kIdesc, (ks | kk) != 0);
+          }
+          ptx::umma_commit(empty_bar + 8 * stage);
+          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        ptx::umma_commit(acc_full_bar + 8 * acc);
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+  } else if (warp < Cfg::kFirstGatherWarp) {
+    // ---------------------------------------------------------------- epilogue
+    EpilogueWarp w;
+    w.quarter = warp & 3;
+    w.half = (warp - 2) >> 2;
+    w.lane = lane;
+    w.staging = staging_base + static_cast<uint32_t>(warp - 2) * S::kStagingBytes;
+    uint32_t acc = 0, acc_phase = 0;
+    for (int32_t index = blockIdx.x; index < total; index += step) {
+      const typename Op::Tile tile = Op::tile(p, index);
+      if (!tile.live) continue;
+      const typename Op::Early early = Op::prefetch(p, tile, w);
+      if (tile.k_steps > 0) {
+        if (!ptx::mbar_wait_bounded(acc_full_bar + 8 * acc, acc_phase, abort_word)) {
+          give_up(SB_DEV_TIMEOUT_EPILOGUE);
+          break;
+        }
+        ptx::tcgen05_fence_after_sync();
+      }
+      w.taddr = tmem_base + (static_cast<uint32_t>(w.quarter * 32) << 16) + acc * kTileCols;
+      Op::epilogue(maps, p, tile, w, early);
+      if (tile.k_steps > 0) {
+        ptx::tcgen05_fence_before_sync();
+        ptx::mbar_arrive(acc_empty_bar + 8 * acc);
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+    if (lane == 0) ptx::bulk_wait_all();
+  } else {
+    // ---------------------------------------------------------------- row gather
+    if constexpr (Op::kGather) {
+      // Eight lanes share a row (its 128 bytes of the K step), a warp instruction moves four rows; warp gw covers
+      // rows j * 16 + gw * 4 + lane / 8. Rows without a source use the zero-fill form, which reads nothing.
+      const int gw = warp - Cfg::kFirstGatherWarp;
+      const int row0 = gw * 4 + (lane >> 3);
+      const uint32_t chunk = static_cast<uint32_t>(lane & 7);
+      const uint32_t dst_off = static_cast<uint32_t>(row0) * 128u + ((chunk ^ static_cast<uint32_t>(row0 & 7)) << 4);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      int32_t index = blockIdx.x;
+      typename Op::Tile next{};
+      const __nv_bfloat16* next_src[8];
+      auto fetch = [&](int32_t at) {
+        next = Op::tile(p, at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) next_src[j] = next.k_steps > 0 ? Op::gather_row(p, next, row0 + j * 16) : nullptr;
+      };
+      if (index < total) fetch(index);
+      for (; ok && index < total; index += step) {
+        const int32_t k_steps = next.k_steps;
+        const __nv_bfloat16* src[8];
+        bool real[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          real[j] = next_src[j] != nullptr;
+          src[j] = (real[j] ? next_src[j] : Op::any_row(p)) + chunk * 8;  // padding still passes a valid address
+        }
+        if (index + step < total) fetch(index + step);
+        for (int32_t ks = 0; ks < k_steps; ++ks) {
+          if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
+            give_up(SB_DEV_TIMEOUT_PRODUCER);
+            ok = false;
+            break;
+          }
+          const uint32_t dst = a_base + stage * S::kABytes + dst_off;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ptx::cp_async_16_zfill(dst + j * 2048, src[j] + ks * kTileStep, real[j]);
+          ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
+          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      ptx::cp_async_wait_all();
+    }
+  }
+
+  if (*abort_word != 0u) {
+    // Gave up mid-pipeline: leave copies still in flight time to land before the shared memory is handed back.
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tcgen05_fence_after_sync();
+    ptx::tmem_dealloc(tmem_base, 2 * kTileCols);
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------
+
+// A row-major [rows, cols] map of 2-byte (bf16) or 4-byte (fp32) elements whose boxes are 128 bytes wide (128-byte
+// swizzle) or 64 bytes wide (64-byte swizzle).
+int encode_2d_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
+                  uint32_t element_bytes, const char* what);
+
+template <class Op>
+int launch_tile_gemm(const TileMaps& maps, const typename Op::Params& p, int64_t tiles, int32_t* dev_status,
+                     cudaStream_t stream, const char* what) {
+  int device = 0;
+  const DeviceInfo* info = current_device_info(&device);
+  if (info == nullptr) return SB_ERR_CUDA;
+  static std::atomic<bool> done[kMaxDevices] = {};
+  if (!done[device].load(std::memory_order_acquire)) {
+    const cudaError_t err = cudaFuncSetAttribute(tile_gemm_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem::kBytes);
+    if (err != cudaSuccess) return fail(SB_ERR_CUDA, "%s: shared memory opt-in: %s", what, cudaGetErrorString(err));
+    done[device].store(true, std::memory_order_release);
+  }
+  if (tiles <= 0) return SB_OK;
+  if (tiles > INT32_MAX - info->sm_count) return fail(SB_ERR_INVALID_ARGUMENT, "%s: problem too large", what);
+  const unsigned grid = static_cast<unsigned>(tiles < info->sm_count ? tiles : info->sm_count);
+  tile_gemm_kernel<Op><<<grid, TileConfig<Op>::kThreads, TileSmem::kBytes, stream>>>(maps, p, dev_status);
+  return check_launch(what);
+}
+
+}  // namespace sb

@@ -1,0 +1,158 @@
+"""The MoE layer with gated experts, for serving and for training.
+
+    out[t] = sum over the token's picks of gate * (act(x w_gate[e]) * (x w_up[e])) w_down[e]
+
+Forward: routing -> sdd_gated -> DSD -> combine, like moe_forward. The backward pass is a call of its own
+(moe_backward_gated), so that a training step can be captured into a CUDA graph as it is; moe_gated() wraps the two
+for torch.autograd. No host sync anywhere.
+"""
+
+from __future__ import annotations
+
+from collections.abc import Callable
+from dataclasses import dataclass
+from typing import NamedTuple
+
+import torch
+
+from sparsebench_b200 import _C
+from sparsebench_b200.moe import BLOCK_SIZE, _no_mark
+from sparsebench_b200.routing import DeviceTopology, route_device
+from sparsebench_b200.spmm import combine, dsd
+
+
+@dataclass(frozen=True)
+class GatedSaved:
+    """What moe_forward_gated_saved keeps for moe_backward_gated: the inputs by reference (they must still hold the
+    same values then), the layout, and the blocks of H, G and U (3 * rows * F bf16). topo is None for an empty batch."""
+
+    x: torch.Tensor
+    expert_weight: torch.Tensor
+    w_gate: torch.Tensor
+    w_up: torch.Tensor
+    w_down: torch.Tensor
+    activation: str
+    topo: DeviceTopology | None
+    h: torch.Tensor | None
+    g: torch.Tensor | None
+    u: torch.Tensor | None
+
+
+class GatedGrads(NamedTuple):
+    x: torch.Tensor  # [T, D]
+    expert_weight: torch.Tensor  # [T, k], in expert_weight's type
+    w_gate: torch.Tensor  # [E, D, F]
+    w_up: torch.Tensor  # [E, D, F]
+    w_down: torch.Tensor  # [E, F, D]
+
+
+def _check_shapes(x, expert_idx, expert_weight, w_gate, w_up, w_down) -> None:
+    if w_gate.dim() != 3 or w_up.shape != w_gate.shape:
+        raise ValueError(f"w_gate and w_up must be [E, D, F], got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    num_experts, d_model, ffn_dim = w_gate.shape
+    if w_down.shape != (num_experts, ffn_dim, d_model):
+        raise ValueError(f"w_down must be {(num_experts, ffn_dim, d_model)}, got {tuple(w_down.shape)}")
+    if (x.dim() != 2 or x.shape[1] != d_model or expert_idx.dim() != 2 or expert_idx.shape != expert_weight.shape
+            or expert_idx.shape[0] != x.shape[0]):
+        raise ValueError("x must be [T, D] and expert_idx / expert_weight [T, k]")
+
+
+def _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, keep, mark):
+    _check_shapes(x, expert_idx, expert_weight, w_gate, w_up, w_down)
+    _C._check_gated_weights(x, w_gate, w_up)
+    _C._check_bf16(x.device, w_down=w_down)
+    _C._check_activation(activation)
+    for t, name in ((expert_idx, "expert_idx"), (expert_weight, "expert_weight")):
+        _C._check(t.device == x.device, f"all inputs must be on the same GPU: {name} is on {t.device}, not {x.device}")
+    num_experts, d_model, ffn_dim = w_gate.shape
+    if expert_idx.numel() == 0:  # host-known size: nothing routed anywhere
+        return torch.zeros_like(x), None, None, None, None
+    topo = route_device(expert_idx, num_experts, ffn_dim, BLOCK_SIZE)
+    mark("routing")
+    h, g, u = _C.sdd_gated_cuda(x, w_gate, w_up, topo.row_token, topo.row_block_expert, topo.row_offsets,
+                                topo.col_indices.numel(), activation, skip_padding_rows=True, keep=keep)
+    mark("gated SDD")
+    y = dsd(h, w_down.view(num_experts * ffn_dim, d_model), topo, version=4, skip_padding_rows=True,
+            layout_from_routing=True)
+    mark("DSD")
+    out = combine(y, expert_weight, topo)
+    mark("combine")
+    return out, topo, h, g, u
+
+
+def moe_forward_gated(
+    x: torch.Tensor,
+    expert_idx: torch.Tensor,
+    expert_weight: torch.Tensor,
+    w_gate: torch.Tensor,
+    w_up: torch.Tensor,
+    w_down: torch.Tensor,
+    activation: str = "silu",
+    mark: Callable[[str], None] = _no_mark,
+) -> torch.Tensor:
+    """x [T, D], expert_idx / expert_weight [T, k], w_gate and w_up [E, D, F], w_down [E, F, D] -> [T, D]; bf16 (gates
+    bf16 or fp32), fp32 accumulation inside the kernels, D and F multiples of 128. activation: "silu" (SwiGLU experts)
+    or "gelu" (erf form). An expert id outside [0, E) is skipped, as in moe_forward. mark as in moe_forward, with
+    "gated SDD" for the second stage."""
+    return _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, False, mark)[0]
+
+
+def moe_forward_gated_saved(
+    x: torch.Tensor,
+    expert_idx: torch.Tensor,
+    expert_weight: torch.Tensor,
+    w_gate: torch.Tensor,
+    w_up: torch.Tensor,
+    w_down: torch.Tensor,
+    activation: str = "silu",
+) -> tuple[torch.Tensor, GatedSaved]:
+    """moe_forward_gated that also returns what moe_backward_gated needs."""
+    out, topo, h, g, u = _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, True, _no_mark)
+    return out, GatedSaved(x, expert_weight, w_gate, w_up, w_down, activation, topo, h, g, u)
+
+
+def moe_backward_gated(grad_out: torch.Tensor, saved: GatedSaved) -> GatedGrads:
+    """The gradients of everything moe_forward_gated_saved took, from the gradient of its output [T, D] (bf16). May be
+    called more than once. Sums over rows are in a fixed order: the same inputs give the same bits."""
+    s = saved
+    if grad_out.shape != s.x.shape:
+        raise ValueError(f"grad_out must be {tuple(s.x.shape)}, got {tuple(grad_out.shape)}")
+    if s.topo is None:
+        return GatedGrads(*(torch.zeros_like(t) for t in (s.x, s.expert_weight, s.w_gate, s.w_up, s.w_down)))
+    t = s.topo
+    layout = [t.tokens_per_expert, t.padded_offsets, t.row_token, t.copy_row, t.row_block_expert, t.row_offsets]
+    return GatedGrads(*_C.gated_backward_cuda(grad_out, s.x, s.expert_weight, s.w_gate, s.w_up, s.w_down, s.h, s.g, s.u,
+                                              layout, s.activation))
+
+
+class _GatedMoE(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, expert_idx, expert_weight, w_gate, w_up, w_down, activation):
+        out, saved = moe_forward_gated_saved(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
+        ctx.save_for_backward(x, expert_weight, w_gate, w_up, w_down)  # autograd checks them for in-place changes
+        ctx.rest = (activation, saved.topo, saved.h, saved.g, saved.u)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the autograd form of the gated layer cannot be captured into a CUDA graph: "
+                               "capture moe_forward_gated_saved and moe_backward_gated")
+        activation, topo, h, g, u = ctx.rest
+        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*ctx.saved_tensors, activation, topo, h, g, u))
+        return grads.x, None, grads.expert_weight, grads.w_gate, grads.w_up, grads.w_down, None
+
+
+def moe_gated(
+    x: torch.Tensor,
+    expert_idx: torch.Tensor,
+    expert_weight: torch.Tensor,
+    w_gate: torch.Tensor,
+    w_up: torch.Tensor,
+    w_down: torch.Tensor,
+    activation: str = "silu",
+) -> torch.Tensor:
+    """moe_forward_gated for torch.autograd: differentiable in x, expert_weight and the three weights (once). Its
+    backward pass refuses to run under CUDA graph capture: capture the two explicit calls instead."""
+    return _GatedMoE.apply(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)

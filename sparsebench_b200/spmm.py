@@ -55,6 +55,17 @@ def sdd(x: torch.Tensor, w1: torch.Tensor, topo: Topology | DeviceTopology, gelu
                        skip_padding_rows, topo.padded_offsets if layout_from_routing else None)
 
 
+def sdd_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, topo: Topology | DeviceTopology,
+              activation: str = "silu", skip_padding_rows: bool = False) -> torch.Tensor:
+    """H = act(x_grouped @ w_gate[e]) * (x_grouped @ w_up[e]) on topo's blocks: sdd() of a gated expert, both
+    projections, the activation ("silu" or "gelu", the erf form) and the product in one kernel. w_gate, w_up
+    [E, D, F] -> [nnz, 128, 128]. skip_padding_rows as in sdd()."""
+    if topo.block_size != 128:
+        raise ValueError(f"sdd_gated needs block size 128, got {topo.block_size}")
+    return _C.sdd_gated_cuda(x, w_gate, w_up, topo.row_token, topo.row_block_expert, topo.row_offsets,
+                             topo.col_indices.numel(), activation, skip_padding_rows)[0]
+
+
 def combine(y: torch.Tensor, expert_weight: torch.Tensor, topo: Topology | DeviceTopology) -> torch.Tensor:
     """[P, D] expert outputs -> [T, D]: each token's k rows, gate-weighted and summed in fp32
     (reference: sparsebench/moe.py:51-55), as one bandwidth-bound kernel."""

@@ -1,0 +1,279 @@
+"""The gated MoE layer and its backward pass against their definitions in 64 bits (oracle/gated.py).
+
+Two tolerances. Element by element: the bound that oracle/gated.py carries along (every rounding half a step, every
+fp32 sum n 2^-24 of its magnitudes), with 1 % for products of two errors and the last rounding on top. Over a whole
+output: roundings are independent and each is uniform within half a step, 2^-8 / sqrt(3) of the value in the root mean
+square at most; a path has at most seven of them (G, U, w dO, dG or dU, row, result and one in H), each passed on with a
+factor of at most 1.13 (the largest slope of the activations), which makes sqrt(7) 1.13 2^-8 / sqrt(3) = 6.8e-3.
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle.gated import gated_layer, gated_reference
+from tests.cases import routing_case
+
+pytestmark = pytest.mark.gpu
+
+NORM_TOL = math.sqrt(7) * 1.13 * 2.0**-8 / math.sqrt(3)
+NAMES = ("dx", "dgate", "dw_gate", "dw_up", "dw_down")
+
+
+def make(num_tokens, d_model, ffn_dim, num_experts, k, seed=0, gate_dtype=torch.bfloat16, idx=None):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(num_tokens, d_model, generator=g).bfloat16()
+    if idx is None:
+        idx = torch.rand(num_tokens, num_experts, generator=g).topk(k, dim=-1).indices
+    gate = torch.softmax(torch.randn(num_tokens, k, generator=g), dim=-1).to(gate_dtype)
+    wg, wu = ((torch.randn(num_experts, d_model, ffn_dim, generator=g) / d_model**0.5).bfloat16() for _ in range(2))
+    wd = (torch.randn(num_experts, ffn_dim, d_model, generator=g) / ffn_dim**0.5).bfloat16()
+    go = torch.randn(num_tokens, d_model, generator=g).bfloat16()
+    return [t.cuda() for t in (x, idx, gate, wg, wu, wd, go)]
+
+
+def close(name, got, want, bound):
+    assert torch.isfinite(got).all(), name
+    last = (2.0**-8 if got.dtype == torch.bfloat16 else 2.0**-24)
+    err = (got.double() - want).abs()
+    # 2^-133 is half the smallest bf16 step: values that small round to it or to 0.
+    allowed = 1.01 * (bound + last * (want.abs() + bound)) + 2.0**-133
+    assert bool((err <= allowed).all()), f"{name}: {float((err / allowed).max()):.3g} times the bound"
+    norm = float(want.norm())
+    if norm > 0 and want.numel() >= 64:
+        assert float(err.norm()) <= NORM_TOL * norm, f"{name}: {float(err.norm()) / norm:.3g} of the norm"
+
+
+def step(x, idx, gate, wg, wu, wd, go, act):
+    from sparsebench_b200 import moe_backward_gated, moe_forward_gated_saved
+
+    out, saved = moe_forward_gated_saved(x, idx, gate, wg, wu, wd, activation=act)
+    return dict(zip(("out", *NAMES), (out, *moe_backward_gated(go, saved))))
+
+
+def check(x, idx, gate, wg, wu, wd, go, act="silu"):
+    from sparsebench_b200 import moe_forward_gated
+
+    want = gated_reference(x, idx, gate, wg, wu, wd, act, go)
+    got = step(x, idx, gate, wg, wu, wd, go, act)
+    assert torch.equal(got["out"], moe_forward_gated(x, idx, gate, wg, wu, wd, activation=act)) or len(x) <= 64
+    for name, (value, bound) in want.items():
+        assert got[name].dtype == (gate.dtype if name == "dgate" else torch.bfloat16)
+        close(name, got[name], value, bound)
+    return got
+
+
+@pytest.mark.parametrize(("num_tokens", "d_model", "ffn_dim", "num_experts", "k", "act"), [
+    (1, 128, 128, 1, 1, "silu"),
+    (1, 256, 384, 8, 2, "gelu"),
+    (2, 128, 640, 3, 3, "silu"),
+    (63, 384, 256, 2, 1, "gelu"),
+    (64, 256, 256, 4, 2, "silu"),
+    (65, 128, 384, 1, 1, "silu"),
+    (127, 640, 128, 3, 2, "gelu"),
+    (129, 256, 512, 2, 2, "silu"),
+    (300, 384, 896, 5, 4, "silu"),
+    (513, 256, 1024, 8, 2, "gelu"),
+    (1000, 512, 384, 64, 2, "silu"),
+    (2049, 128, 256, 3, 2, "silu"),
+    (700, 1024, 2048, 16, 1, "silu"),
+])
+def test_step_matches_definition(num_tokens, d_model, ffn_dim, num_experts, k, act):
+    check(*make(num_tokens, d_model, ffn_dim, num_experts, k, seed=num_tokens), act=act)
+
+
+@pytest.mark.parametrize("case", ["random", "zipf", "skewed", "two_experts_only", "empty_middle"])
+def test_step_on_routing_patterns(case):
+    idx = routing_case(case, 333, 8, seed=5)
+    x, idx, gate, wg, wu, wd, go = make(333, 256, 384, 8, 2, idx=idx)
+    got = check(x, idx, gate, wg, wu, wd, go)
+    for e in range(8):
+        if not bool((idx == e).any()):  # experts nobody picked get zeros, not what the memory held
+            assert not any(bool(got[n][e].any()) for n in ("dw_gate", "dw_up", "dw_down"))
+
+
+def test_ids_out_of_range_and_the_same_expert_twice():
+    x, idx, gate, wg, wu, wd, go = make(200, 128, 256, 6, 3)
+    idx[::7, 0] = -1
+    idx[3::11, 1] = 6
+    idx[5::13] = idx[5::13, :1]  # one expert three times
+    got = check(x, idx, gate, wg, wu, wd, go)
+    assert not bool(got["dgate"][idx < 0].any()) and not bool(got["dgate"][idx == 6].any())
+    idx[:] = 17  # nothing routed anywhere
+    got = check(x, idx, gate, wg, wu, wd, go)
+    assert not any(bool(t.any()) for t in got.values())
+
+
+def test_int32_ids_and_fp32_gates():
+    x, idx, gate, wg, wu, wd, go = make(150, 256, 256, 4, 2, gate_dtype=torch.float32)
+    check(x, idx.int(), gate, wg, wu, wd, go)
+
+
+def test_empty_batch():
+    x, idx, gate, wg, wu, wd, go = make(0, 128, 256, 4, 2)
+    got = step(x, idx, gate, wg, wu, wd, go, "silu")
+    assert got["out"].shape == (0, 128) and got["dgate"].shape == (0, 2)
+    assert got["dw_gate"].shape == wg.shape and not any(bool(t.any()) for t in got.values())
+
+
+def test_gradients_against_differences():
+    # Central differences of the definition in 64 bits along random directions. They are off by their step squared
+    # (1e-8 of the third derivative); the kernel's gradient by NORM_TOL of its norm, in a random direction d of norm |d|
+    # by NORM_TOL |grad| |d| at most.
+    x, idx, gate, wg, wu, wd, go = make(90, 256, 384, 5, 2, seed=3)
+    got = step(x, idx, gate, wg, wu, wd, go, "silu")
+    leaves = [t.double() for t in (x, gate, wg, wu, wd)]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for i, name in enumerate(NAMES):
+        d = torch.randn(leaves[i].shape, generator=g, device="cuda", dtype=torch.float64)
+        sides = []
+        for sign in (1, -1):
+            moved = [t + sign * 1e-4 * d if n == i else t for n, t in enumerate(leaves)]
+            out = gated_layer(moved[0], idx, *moved[1:], "silu")
+            sides.append((out * go.double()).sum())
+        slope = float(sides[0] - sides[1]) / 2e-4
+        along = float((got[name].double() * d).sum())
+        assert abs(along - slope) <= NORM_TOL * float(got[name].double().norm() * d.norm()) + 1e-5, name
+
+
+def test_a_token_with_nan_or_inf_stays_alone():
+    x, idx, gate, wg, wu, wd, go = make(140, 128, 256, 4, 2)
+    want = step(x, idx, gate, wg, wu, wd, go, "silu")
+    for bad in (math.nan, math.inf):
+        y = x.clone()
+        y[17, 3] = bad
+        got = step(y, idx, gate, wg, wu, wd, go, "silu")
+        others = torch.arange(140, device="cuda") != 17
+        for n in ("out", "dx", "dgate"):
+            assert torch.equal(got[n][others], want[n][others]), n
+        untouched = [e for e in range(4) if e not in idx[17].tolist()]
+        for n in ("dw_gate", "dw_up", "dw_down"):
+            assert torch.equal(got[n][untouched], want[n][untouched]), n
+
+
+def test_memory_left_by_others_does_not_show():
+    # Every buffer of the step is torch.empty: with the allocator's memory full of NaN the results are the same.
+    args = make(210, 256, 384, 8, 2)
+    first = step(*args, "gelu")
+    torch.cuda.empty_cache()
+    for size in (1 << 26, 1 << 22, 1 << 20, 1 << 18):
+        junk = [torch.full((size,), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(8)]
+        del junk
+    again = step(*args, "gelu")
+    for n in first:
+        assert torch.equal(first[n], again[n]), n  # and run to run the same bits
+
+
+def test_captured_step_and_another_stream():
+    from sparsebench_b200 import moe_backward_gated, moe_forward_gated_saved
+
+    x, idx, gate, wg, wu, wd, go = make(260, 256, 256, 8, 2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = step(x, idx, gate, wg, wu, wd, go, "silu")
+    torch.cuda.current_stream().wait_stream(side)
+    for n, t in step(x, idx, gate, wg, wu, wd, go, "silu").items():
+        assert torch.equal(t, warm[n]), n
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, saved = moe_forward_gated_saved(x, idx, gate, wg, wu, wd)
+        grads = moe_backward_gated(go, saved)
+    for seed in (7, 8):
+        for dst, src in zip((x, idx, gate, wg, wu, wd, go), make(260, 256, 256, 8, 2, seed=seed)):
+            dst.copy_(src)
+        graph.replay()
+        eager = step(x, idx, gate, wg, wu, wd, go, "silu")
+        for n, t in zip(("out", *NAMES), (out, *grads)):
+            assert torch.equal(t, eager[n]), n
+
+
+def test_autograd_form():
+    from sparsebench_b200 import moe_gated
+
+    x, idx, gate, wg, wu, wd, go = make(100, 128, 256, 4, 2)
+    want = step(x, idx, gate, wg, wu, wd, go, "gelu")
+    leaves = [t.clone().requires_grad_() for t in (x, gate, wg, wu, wd)]
+    out = moe_gated(leaves[0], idx, *leaves[1:], activation="gelu")
+    assert torch.equal(out, want["out"])
+    grads = torch.autograd.grad(out, leaves, go, retain_graph=True)
+    for n, g in zip(NAMES, grads):
+        assert torch.equal(g, want[n]), n
+    out.sum().backward()  # an expanded gradient, all its strides 0
+    ones = step(x, idx, gate, wg, wu, wd, torch.ones_like(go), "gelu")
+    for n, leaf in zip(NAMES, leaves):
+        assert torch.equal(leaf.grad, ones[n]), n
+
+
+def test_sdd_gated_alone():
+    from sparsebench_b200 import route_device, sdd_gated
+
+    x, idx, gate, wg, wu, wd, go = make(180, 128, 384, 4, 2)
+    topo = route_device(idx, 4, 384, 128)
+    h = sdd_gated(x, wg, wu, topo)
+    trimmed = topo.to_topology()
+    for rb, e in enumerate(trimmed.row_block_expert.tolist()):
+        token = trimmed.row_token[rb * 128:(rb + 1) * 128].long()
+        rows = torch.where((token >= 0)[:, None], x[token.clamp(min=0)], torch.zeros((), device="cuda", dtype=x.dtype)).double()
+        g, u = rows @ wg[e].double(), rows @ wu[e].double()
+        want = g / (1 + torch.exp(-g)) * u
+        got = torch.cat(list(h[rb * 3:(rb + 1) * 3]), dim=1)
+        bound = 2.0**-8 * want.abs() + 128 * 2.0**-24 * 4 * (rows.abs() @ wg[e].double().abs() + 1) * (rows.abs() @ wu[e].double().abs() + 1)
+        assert bool(((got.double() - want).abs() <= bound).all())
+        assert not bool(got[token < 0].any())
+
+
+def test_refusals():
+    from sparsebench_b200 import moe_backward_gated, moe_forward_gated, moe_forward_gated_saved
+
+    x, idx, gate, wg, wu, wd, go = make(20, 128, 256, 4, 2)
+    for args, text in [
+        ((x, idx, gate, wg, wu[:, :, :128], wd), "w_gate and w_up"),
+        ((x, idx, gate, wg, wu, wd[:, :128]), "w_down must be"),
+        ((x[:, :64], idx, gate, wg, wu, wd), r"\[T, D\]"),
+        ((x, idx[:10], gate, wg, wu, wd), r"\[T, k\]"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            moe_forward_gated(*args)
+    wide = torch.empty(4, 128, 192, dtype=torch.bfloat16, device="cuda")
+    for args, kwargs, text in [
+        ((x.half(), idx, gate, wg, wu, wd), {}, "bfloat16"),
+        ((x, idx, gate, wg.float(), wu, wd), {}, "bfloat16"),
+        ((x.cpu(), idx, gate, wg, wu, wd), {}, "CUDA tensor"),
+        ((x, idx.cpu(), gate, wg, wu, wd), {}, "same GPU"),
+        ((x, idx, gate, wg.transpose(1, 2).contiguous().transpose(1, 2), wu, wd), {}, "contiguous"),
+        ((x, idx, gate, wide, wide, wide.transpose(1, 2).contiguous()), {}, "multiple of 128"),
+        ((x, idx, gate, wg, wu, wd), {"activation": "relu"}, "activation"),
+    ]:
+        with pytest.raises(RuntimeError, match=text):
+            moe_forward_gated(*args, **kwargs)
+    _, saved = moe_forward_gated_saved(x, idx, gate, wg, wu, wd)
+    with pytest.raises(ValueError, match="grad_out"):
+        moe_backward_gated(go[:10], saved)
+    with pytest.raises(RuntimeError, match="grad_out must be bfloat16"):
+        moe_backward_gated(go.float(), saved)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        moe_backward_gated(go[:1].expand(20, 128), saved)
+
+
+def test_autograd_backward_refuses_capture():
+    from sparsebench_b200 import moe_gated
+
+    x, idx, gate, wg, wu, wd, go = make(20, 128, 128, 2, 1)
+    leaf = x.clone().requires_grad_()
+    out = moe_gated(leaf, idx, gate, wg, wu, wd)
+
+    class Ctx:  # what the node hands its backward; the refusal comes before anything is launched or read
+        pass
+
+    from sparsebench_b200 import gated
+
+    real = torch.cuda.is_current_stream_capturing
+    torch.cuda.is_current_stream_capturing = lambda: True
+    try:
+        with pytest.raises(RuntimeError, match="moe_backward_gated"):
+            gated._GatedMoE.backward(Ctx(), go)
+    finally:
+        torch.cuda.is_current_stream_capturing = real
+    assert out.requires_grad
