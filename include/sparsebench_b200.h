@@ -446,6 +446,24 @@ int sb_gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void*
 int sb_gated_join(const void* dx_rows, const float* gate_partial, const int32_t* copy_row, void* dx, void* dgate,
                   int gate_dtype, int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, sb_stream_t stream);
 
+/*
+ * A projection with the low-rank adapters of many requests at once (no counterpart in the reference):
+ *   out[t] = x[t] . weight + scale[a] * sum_j (x[t] . lora_a[a][j]) lora_b[a][j],   a = adapter_idx[t]
+ * and only the first term for a token whose adapter is outside [0, num_adapters). x [T, D], weight [D, N],
+ * lora_a [num_adapters, rank, D], lora_b [num_adapters, rank, N] bf16; scale [num_adapters] fp32 (NULL: 1);
+ * adapter_idx int32 or int64 [T]; out [T, N] bf16, or fp32 with out_fp32. fp32 accumulation. D, N and rank are multiples
+ * of 8, rank <= 128; all buffers 16-byte aligned. Tokens may come in any order; few distinct adapters among neighbours
+ * (a batch of whole requests) is the fast case. A request's output does not depend on other requests' adapters, not
+ * even when those hold infinities or NaN. workspace: sb_lora_workspace_bytes (-1: sizes that are refused) bytes of
+ * device memory, nothing in it has to be set.
+ */
+int64_t sb_lora_workspace_bytes(int64_t num_tokens, int32_t d_model, int32_t width, int32_t rank, int32_t num_adapters,
+                                int out_fp32);
+int sb_lora_linear(const void* x, const void* weight, const void* lora_a, const void* lora_b, const void* adapter_idx,
+                   int idx_is_i64, const float* scale, void* out, int out_fp32, int64_t num_tokens, int32_t d_model,
+                   int32_t width, int32_t rank, int32_t num_adapters, void* workspace, int64_t workspace_bytes,
+                   int32_t* dev_status, sb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

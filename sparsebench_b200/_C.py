@@ -432,6 +432,45 @@ def gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weight: 
     return dx, dgate, dw_gate, dw_up, dw_down
 
 
+# ---- projections with the low-rank adapters of many requests (no counterpart in the reference) ----------
+
+def lora_linear_cuda(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                     adapter_idx: torch.Tensor, scale: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
+    """out [T, N] = x @ weight + scale[a] * (x @ lora_a[a]^T) @ lora_b[a] with a = adapter_idx[t] per token."""
+    lib = _lib.load()
+    _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
+    device = x.device
+    _check_bf16(device, x=x, weight=weight, lora_a=lora_a, lora_b=lora_b)
+    _check(x.dim() == 2 and weight.dim() == 2 and weight.shape[0] == x.shape[1],
+           f"x must be [T, D] and weight [D, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    num_tokens, d_model = x.shape
+    width = weight.shape[1]
+    _check(lora_a.dim() == 3 and lora_b.dim() == 3 and lora_a.shape[2] == d_model and
+           lora_b.shape == (lora_a.shape[0], lora_a.shape[1], width),
+           f"lora_a must be [L, r, {d_model}] and lora_b [L, r, {width}], got {tuple(lora_a.shape)} and {tuple(lora_b.shape)}")
+    num_adapters, rank = lora_a.shape[:2]
+    _check(adapter_idx.is_cuda and adapter_idx.device == device, "adapter_idx must be on x's GPU")
+    _check(adapter_idx.dtype in (torch.int32, torch.int64) and adapter_idx.shape == (num_tokens,) and
+           adapter_idx.is_contiguous(), f"adapter_idx must be a contiguous int32 or int64 [{num_tokens}] tensor")
+    if scale is not None:
+        _check(scale.is_cuda and scale.device == device and scale.dtype == torch.float32 and
+               scale.shape == (num_adapters,) and scale.is_contiguous(),
+               f"scale must be a contiguous float32 [{num_adapters}] tensor on x's GPU")
+    _check(out_dtype in (torch.bfloat16, torch.float32), f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    fp32 = int(out_dtype == torch.float32)
+    with torch.cuda.device(device):
+        nbytes = lib.sb_lora_workspace_bytes(num_tokens, d_model, width, rank, num_adapters, fp32)
+        if nbytes < 0:
+            _lib.check(1)
+        out = torch.empty((num_tokens, width), dtype=out_dtype, device=device)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _lib.check(lib.sb_lora_linear(_ptr(x), _ptr(weight), _ptr(lora_a), _ptr(lora_b), _ptr(adapter_idx),
+                                      int(adapter_idx.dtype == torch.int64), _ptr(scale), _ptr(out), fp32, num_tokens,
+                                      d_model, width, rank, num_adapters, _ptr(work), nbytes,
+                                      _ptr(device_status(device)), _stream()))
+    return out
+
+
 # ---- expert-parallel plumbing (no counterpart in the reference's extension) ----------------------
 
 def sort_copies_cuda(expert_idx: torch.Tensor, num_experts: int) -> list[torch.Tensor]:

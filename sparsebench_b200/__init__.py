@@ -14,6 +14,7 @@ from sparsebench_b200.gated import (
     moe_forward_gated_saved,
     moe_gated,
 )
+from sparsebench_b200.lora import lora_linear
 from sparsebench_b200.moe import moe_forward, moe_forward_assigned, moe_forward_from_logits
 from sparsebench_b200.routing import DeviceTopology, build_topology_cuda, route, route_and_layout, route_device
 from sparsebench_b200.rounding import DeviceAssignments, moe_forward_rounded, token_rounding
@@ -29,6 +30,7 @@ __all__ = [
     "build_topology_cuda",
     "combine",
     "dsd",
+    "lora_linear",
     "moe_backward_gated",
     "moe_forward",
     "moe_forward_assigned",

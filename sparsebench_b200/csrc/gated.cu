@@ -83,7 +83,7 @@ struct GatedUp {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr bool kGather = true, kAMnMajor = false, kBMnMajor = true;
+  static constexpr bool kVariable = false, kStepGather = false, kGather = true, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -124,9 +124,9 @@ struct GatedUp {
     uint32_t packed[32];
     if (p.keep) {
       load_packed_x64(gate, packed);
-      store_rows_x64(w, &maps.m[3], packed, col, row);
+      store_rows_128b(w, &maps.m[3], packed, col, row);
       load_packed_x64(up, packed);
-      store_rows_x64(w, &maps.m[4], packed, col, row);
+      store_rows_128b(w, &maps.m[4], packed, col, row);
     }
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
@@ -140,7 +140,7 @@ struct GatedUp {
             pack_bf16(act_value(__uint_as_float(g[2 * h]), p.activation) * __uint_as_float(u[2 * h]),
                       act_value(__uint_as_float(g[2 * h + 1]), p.activation) * __uint_as_float(u[2 * h + 1]));
     }
-    store_rows_x64(w, &maps.m[2], packed, col, row);
+    store_rows_128b(w, &maps.m[2], packed, col, row);
   }
 };
 
@@ -173,7 +173,7 @@ struct GradHidden {
     const uint4* u;
     uint4 g0[4], u0[4];
   };
-  static constexpr bool kGather = true, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = false, kStepGather = false, kGather = true, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -296,7 +296,7 @@ struct GradRows {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr bool kGather = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = false, kStepGather = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -331,7 +331,7 @@ struct GradRows {
       if (col >= p.d_model) break;
       uint32_t packed[32];
       load_packed_x64(w.taddr + w.half * 128 + g * 64, packed);
-      store_rows_x64(w, &maps.m[4], packed, col, t.row_block * kTileRows + w.quarter * 32);
+      store_rows_128b(w, &maps.m[4], packed, col, t.row_block * kTileRows + w.quarter * 32);
     }
   }
 };
@@ -354,7 +354,7 @@ struct GradWeights {
     bool live;
   };
   struct Early {};
-  static constexpr bool kGather = false, kAMnMajor = true, kBMnMajor = true;
+  static constexpr bool kVariable = false, kStepGather = false, kGather = false, kAMnMajor = true, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) {
     return p.num_experts * (p.down_tiles + 2 * p.up_tiles);
@@ -420,7 +420,7 @@ struct GradWeights {
 #pragma unroll
         for (int h = 0; h < 32; ++h) packed[h] = 0u;
       }
-      store_rows_x64(w, &maps.m[5 + t.which], packed, col, row);
+      store_rows_128b(w, &maps.m[5 + t.which], packed, col, row);
     }
   }
 };

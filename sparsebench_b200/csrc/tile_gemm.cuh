@@ -47,8 +47,9 @@ struct EpilogueWarp {
   uint32_t taddr;    // TMEM address of (lane quarter, column 0) of the finished accumulator
 };
 
-// bf16 pairs of 64 columns of this lane's row -> the warp's staging tile -> one TMA store of 32 rows x 64 columns.
-__device__ __forceinline__ void store_rows_x64(const EpilogueWarp& w, const CUtensorMap* map, const uint32_t (&packed)[32],
+// 128 bytes of this lane's row (64 bf16 columns as pairs, or 32 fp32 columns) -> the warp's staging tile -> one TMA store
+// of 32 rows.
+__device__ __forceinline__ void store_rows_128b(const EpilogueWarp& w, const CUtensorMap* map, const uint32_t (&packed)[32],
                                                int32_t col, int32_t row) {
   if (w.lane == 0) ptx::bulk_wait_read();  // the store before has read the staging tile
   __syncwarp();
@@ -103,7 +104,10 @@ struct BandOrder {
 //   Params, Tile (with int32_t k_steps: 0 = nothing to multiply; bool live: the epilogue has something to do)
 //   static constexpr bool kGather, kAMnMajor, kBMnMajor
 //   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar), tx_bytes
-//   gather_row(p, tile, row) -> source row of A or nullptr (zeros), for kGather
+//   gather_row(p, tile, row) -> source row of A or nullptr (zeros), for kGather; any_row(p): a readable address
+//   or, with kStepGather: Rows rows(p, tile, row0) once per tile and step_source(p, tile, rows, j, row, ks, chunk, &real),
+//   the address of 16-byte chunk `chunk` of row `row` = row0 + 16 j in K step ks (real = false: zeros)
+//   With kVariable: columns(p) <= 256 (a multiple of 16) accumulator columns in use, tx_bytes(p, tile, ks) per stage
 //   prefetch(p, tile, w) -> Early (global loads that can start before the accumulator is ready)
 //   epilogue(maps, p, tile, w, early)
 template <class Op>
@@ -183,7 +187,8 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
             break;
           }
           const uint32_t bar = full_bar + 8 * stage;
-          ptx::mbar_arrive_expect_tx(bar, S::kBBytes + (Op::kGather ? 0 : S::kABytes));
+          if constexpr (Op::kVariable) ptx::mbar_arrive_expect_tx(bar, Op::tx_bytes(p, tile, ks));
+          else ptx::mbar_arrive_expect_tx(bar, S::kBBytes + (Op::kGather ? 0 : S::kABytes));
           Op::load(maps, p, tile, ks, a_base + stage * S::kABytes, b_base + stage * S::kBBytes, bar);
           if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
         }
@@ -192,7 +197,9 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
-      constexpr uint32_t kIdesc = ptx::make_idesc_bf16(kTileRows, kTileCols, Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
+      uint32_t idesc = ptx::make_idesc_bf16(kTileRows, kTileCols, Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
+      if constexpr (Op::kVariable)
+        idesc = ptx::make_idesc_bf16(kTileRows, Op::columns(p), Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
       int32_t index = blockIdx.x;
@@ -224,7 +231,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
                                                   : ptx::make_smem_desc(a_addr + kk * 32, 16, 1024);
             const uint64_t desc_b = Op::kBMnMajor ? ptx::make_smem_desc(b_addr + kk * 2048, S::kSlabBytes, 1024)
                                                   : ptx::make_smem_desc(b_addr + kk * 32, 16, 1024);
-            ptx::umma_bf16(d_tmem, desc_a, desc_b, kIdesc, (ks | kk) != 0);
+            ptx::umma_bf16(d_tmem, desc_a, desc_b, idesc, (ks | kk) != 0);
           }
           ptx::umma_commit(empty_bar + 8 * stage);
           if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
@@ -273,38 +280,63 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
       const int row0 = gw * 4 + (lane >> 3);
       const uint32_t chunk = static_cast<uint32_t>(lane & 7);
       const uint32_t dst_off = static_cast<uint32_t>(row0) * 128u + ((chunk ^ static_cast<uint32_t>(row0 & 7)) << 4);
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      int32_t index = blockIdx.x;
-      typename Op::Tile next{};
-      const __nv_bfloat16* next_src[8];
-      auto fetch = [&](int32_t at) {
-        next = Op::tile(p, at);
+      if constexpr (Op::kStepGather) {
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (int32_t index = blockIdx.x; ok && index < total; index += step) {
+          const typename Op::Tile tile = Op::tile(p, index);
+          const typename Op::Rows rows = Op::rows(p, tile, row0);
+          for (int32_t ks = 0; ks < tile.k_steps; ++ks) {
+            if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
+              give_up(SB_DEV_TIMEOUT_PRODUCER);
+              ok = false;
+              break;
+            }
+            const uint32_t dst = a_base + stage * S::kABytes + dst_off;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) next_src[j] = next.k_steps > 0 ? Op::gather_row(p, next, row0 + j * 16) : nullptr;
-      };
-      if (index < total) fetch(index);
-      for (; ok && index < total; index += step) {
-        const int32_t k_steps = next.k_steps;
-        const __nv_bfloat16* src[8];
-        bool real[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          real[j] = next_src[j] != nullptr;
-          src[j] = (real[j] ? next_src[j] : Op::any_row(p)) + chunk * 8;  // padding still passes a valid address
-        }
-        if (index + step < total) fetch(index + step);
-        for (int32_t ks = 0; ks < k_steps; ++ks) {
-          if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
-            give_up(SB_DEV_TIMEOUT_PRODUCER);
-            ok = false;
-            break;
+            for (int j = 0; j < 8; ++j) {
+              bool real;
+              const void* src = Op::step_source(p, tile, rows, j, row0 + j * 16, ks, static_cast<int>(chunk), &real);
+              ptx::cp_async_16_zfill(dst + j * 2048, src, real);
+            }
+            ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
+            if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
           }
-          const uint32_t dst = a_base + stage * S::kABytes + dst_off;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ptx::cp_async_16_zfill(dst + j * 2048, src[j] + ks * kTileStep, real[j]);
-          ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
-          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+        }
+      } else {
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        int32_t index = blockIdx.x;
+        typename Op::Tile next{};
+        const __nv_bfloat16* next_src[8];
+        auto fetch = [&](int32_t at) {
+          next = Op::tile(p, at);
+  #pragma unroll
+          for (int j = 0; j < 8; ++j) next_src[j] = next.k_steps > 0 ? Op::gather_row(p, next, row0 + j * 16) : nullptr;
+        };
+        if (index < total) fetch(index);
+        for (; ok && index < total; index += step) {
+          const int32_t k_steps = next.k_steps;
+          const __nv_bfloat16* src[8];
+          bool real[8];
+  #pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            real[j] = next_src[j] != nullptr;
+            src[j] = (real[j] ? next_src[j] : Op::any_row(p)) + chunk * 8;  // padding still passes a valid address
+          }
+          if (index + step < total) fetch(index + step);
+          for (int32_t ks = 0; ks < k_steps; ++ks) {
+            if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
+              give_up(SB_DEV_TIMEOUT_PRODUCER);
+              ok = false;
+              break;
+            }
+            const uint32_t dst = a_base + stage * S::kABytes + dst_off;
+  #pragma unroll
+            for (int j = 0; j < 8; ++j) ptx::cp_async_16_zfill(dst + j * 2048, src[j] + ks * kTileStep, real[j]);
+            ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
+            if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+          }
         }
       }
       ptx::cp_async_wait_all();
