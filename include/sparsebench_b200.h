@@ -397,27 +397,26 @@ int sb_ep_sdd_dispatch(const void* recv_rows, const void* w1, const int32_t* row
                        int32_t capacity, int32_t push_warps, int32_t* dev_status, sb_stream_t stream);
 
 /*
- * The gated expert block and its backward pass, on the layout of sb_route at block size 128 (no counterpart in the
- * reference, whose experts have one up projection). bf16 in and out, fp32 accumulation. d_model and ffn_dim are
- * multiples of 128; w_gate and w_up are [E, D, F], w_down is [E, F, D]; every buffer 16-byte aligned.
+ * The gated expert block of the MoE layer and its backward pass (no counterpart in the reference, whose experts have one
+ * up projection). bf16 in and out, fp32 accumulation. d_model and ffn_dim are multiples of 128; w_gate and w_up are
+ * [E, D, F], w_down is [E, F, D]; gate (the picks' weights) is bf16 (gate_dtype 0) or fp32 (1); every buffer 16-byte
+ * aligned. A copy whose expert id is outside [0, num_experts) contributes nothing, and its gate's gradient is 0.
  *
- * sb_sdd_gated: h_blocks = act(x[row_token] . w_gate[e]) * (x[row_token] . w_up[e]) in one kernel, laid out like
- * sb_sdd's blocks; the down projection is sb_dsd. g_blocks / u_blocks (both or neither NULL): the two projections
- * before the activation, for the backward pass; every row of a 64-row half that holds real rows is then written
- * (padding rows as zeros). Without them skip_padding_rows works as in sb_sdd.
+ * sb_sdd_gated: h_blocks = act(x[row_token] . w_gate[e]) * (x[row_token] . w_up[e]) in one kernel, on sb_route's layout
+ * at block size 128, laid out like sb_sdd's blocks; the down projection is sb_dsd. g_blocks / u_blocks (both or neither
+ * NULL): the two projections before the activation; every row of a 64-row half of a row block that holds real rows is
+ * then written (padding rows as zeros). Without them skip_padding_rows works as in sb_sdd.
  *
- * The backward pass, in this order, from grad_out [T, D]:
- *   sb_gated_gather        x_rows[r] = x[token], grad_rows[r] = gate * grad_out[token], row_gate[r] = gate of the row's
- *                          copy; zeros for padding rows. [num_row_blocks * 128] rows; those past the real end stay as
- *                          they are. gate_dtype: 0 = bf16, 1 = fp32.
- *   sb_gated_grad_hidden   dg_blocks, du_blocks: gradients of the two projections; gate_partial
- *                          [num_row_blocks * 128, F / 128] fp32: each row's share of its gate's gradient per 128 hidden
- *                          columns (rows of real copies only).
- *   sb_gated_grad_weights  dw_gate, dw_up [E, D, F], dw_down [E, F, D]; zeros for an expert without rows.
- *   sb_gated_grad_rows     dx_rows[r] = dG w_gate^T + dU w_up^T; 32-row groups of padding are not written. May write over
- *                          x_rows once the weight gradients are done.
- *   sb_gated_join          dx[t] = sum of the token's rows, dgate[t, j] = sum of the copy's partials, in a fixed order.
- * A copy whose expert id was rejected contributes nothing and its gate's gradient is 0.
+ * sb_moe_gated_bytes: bytes[0] of the state, bytes[1] of the forward's scratch, bytes[2] of the backward's; keep = 0: for
+ * a forward pass alone (no state). Nothing in these buffers has to be set.
+ *
+ * sb_moe_gated_forward: out[t] = sum_j gate[t, j] * (act(x[t] . w_gate[e]) * (x[t] . w_up[e])) . w_down[e],
+ * e = expert_idx[t, j] (int32 or int64 [T, k]). With state (not NULL) it holds afterwards what the backward pass needs:
+ * the layout and the blocks of H, G and U.
+ *
+ * sb_moe_gated_backward: the gradients of x, gate (in gate's type), w_gate, w_up and w_down from grad_out [T, D], the
+ * inputs of that forward call and its state, which it leaves as it is. dw_*: written whole, zeros for an expert without
+ * rows. All sums are in a fixed order.
  */
 enum sb_activation { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* erf form */ };
 int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
@@ -425,26 +424,18 @@ int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int3
                  void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
                  int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
                  sb_stream_t stream);
-int sb_gated_gather(const void* x, const void* grad_out, const void* gate, int gate_dtype, const int32_t* row_token,
-                    const int32_t* copy_row, const int32_t* padded_offsets, int32_t num_experts, void* x_rows,
-                    void* grad_rows, float* row_gate, int64_t num_tokens, int32_t k, int32_t d_model,
-                    int32_t num_row_blocks, sb_stream_t stream);
-int sb_gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_blocks, const void* u_blocks,
-                         const float* row_gate, const int32_t* row_token, const int32_t* row_block_expert,
-                         const int32_t* row_offsets, void* dg_blocks, void* du_blocks, float* gate_partial,
-                         int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
-                         int32_t num_row_blocks, int32_t activation, int32_t* dev_status, sb_stream_t stream);
-int sb_gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_blocks, const void* dg_blocks,
-                          const void* du_blocks, const int32_t* padded_offsets, const int32_t* tokens_per_expert,
-                          const int32_t* row_offsets, void* dw_gate, void* dw_up, void* dw_down, int32_t d_model,
-                          int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status,
-                          sb_stream_t stream);
-int sb_gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up,
-                       const int32_t* row_token, const int32_t* row_block_expert, const int32_t* row_offsets,
-                       void* dx_rows, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
-                       int32_t* dev_status, sb_stream_t stream);
-int sb_gated_join(const void* dx_rows, const float* gate_partial, const int32_t* copy_row, void* dx, void* dgate,
-                  int gate_dtype, int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, sb_stream_t stream);
+int sb_moe_gated_bytes(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int keep,
+                       int64_t* bytes);
+int sb_moe_gated_forward(const void* x, const void* expert_idx, int idx_is_i64, const void* gate, int gate_dtype,
+                         const void* w_gate, const void* w_up, const void* w_down, void* out, int64_t num_tokens, int32_t k,
+                         int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t activation, void* state,
+                         int64_t state_bytes, void* scratch, int64_t scratch_bytes, int32_t* dev_status,
+                         sb_stream_t stream);
+int sb_moe_gated_backward(const void* grad_out, const void* x, const void* gate, int gate_dtype, const void* w_gate,
+                          const void* w_up, const void* w_down, const void* state, int64_t state_bytes, void* dx,
+                          void* dgate, void* dw_gate, void* dw_up, void* dw_down, int64_t num_tokens, int32_t k,
+                          int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t activation, void* scratch,
+                          int64_t scratch_bytes, int32_t* dev_status, sb_stream_t stream);
 
 /*
  * A projection with the low-rank adapters of many requests at once (no counterpart in the reference):

@@ -11,6 +11,7 @@ copies to the host or reads a size back from the GPU.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -335,10 +336,21 @@ def _check_activation(activation: str) -> int:
 
 def _check_bf16(device: torch.device, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
+        if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.bfloat16 and t.device == device
+                and t.is_contiguous()):
+            continue
         _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
         _check(t.device == device, f"all inputs must be on the same GPU: {name} is on {t.device}, not {device}")
         _check(t.dtype == torch.bfloat16, f"{name} must be bfloat16, got {t.dtype}")
         _check(t.is_contiguous(), f"{name} must be contiguous")
+
+
+_same_device = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """torch.cuda.device(device), which costs microseconds, only where another device is current."""
+    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _check_gated_weights(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor) -> None:
@@ -380,56 +392,63 @@ def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, ro
     return h, g, u
 
 
-def gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
-                        w_up: torch.Tensor, w_down: torch.Tensor, h: torch.Tensor, g: torch.Tensor, u: torch.Tensor,
-                        layout: list[torch.Tensor], activation: str) -> tuple[torch.Tensor, ...]:
-    """(dx, dexpert_weight, dw_gate, dw_up, dw_down) of the gated layer from grad_out [T, D]. h, g, u: what
-    sdd_gated_cuda kept; layout: build_topology_cuda's eight arrays for the same routing. Six launches."""
-    lib = _lib.load()
+def _check_gated_layer(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
+                       w_up: torch.Tensor, w_down: torch.Tensor, activation: str) -> int:
     _check_gated_weights(x, w_gate, w_up)
-    _check_bf16(x.device, grad_out=grad_out, w_down=w_down, h=h, g=g, u=u)
-    code = _check_activation(activation)
+    _check_bf16(x.device, w_down=w_down)
+    for name, t, dtypes, text in (("expert_idx", expert_idx, (torch.int32, torch.int64), "int32 or int64"),
+                                  ("expert_weight", expert_weight, (torch.bfloat16, torch.float32), "bfloat16 or float32")):
+        _check(t.device == x.device, f"all inputs must be on the same GPU: {name} is on {t.device}, not {x.device}")
+        _check(t.dtype in dtypes, f"{name} must be {text}, got {t.dtype}")
+        _check(t.is_contiguous(), f"{name} must be contiguous")
+    return _check_activation(activation)
+
+
+def moe_gated_forward_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
+                           w_up: torch.Tensor, w_down: torch.Tensor, activation: str, keep: bool
+                           ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(out [T, D], state): the gated layer; state (None unless keep) is what moe_gated_backward_cuda needs of it.
+    Shapes are the caller's to check; T * k must be positive."""
+    lib = _lib.load()
+    code = _check_gated_layer(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
+    device = x.device
+    num_tokens, k = expert_idx.shape
     num_experts, d_model, ffn_dim = w_gate.shape
+    with _on(device):
+        sizes = (ctypes.c_int64 * 3)()
+        _lib.check(lib.sb_moe_gated_bytes(num_tokens, k, d_model, ffn_dim, num_experts, int(keep), sizes))
+        out = torch.empty_like(x)
+        state = torch.empty(sizes[0], dtype=torch.uint8, device=device) if keep else None
+        scratch = torch.empty(sizes[1], dtype=torch.uint8, device=device)
+        _lib.check(lib.sb_moe_gated_forward(
+            x.data_ptr(), expert_idx.data_ptr(), int(expert_idx.dtype == torch.int64), expert_weight.data_ptr(),
+            int(expert_weight.dtype == torch.float32), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+            out.data_ptr(), num_tokens, k, d_model, ffn_dim, num_experts, code, state.data_ptr() if keep else None,
+            sizes[0], scratch.data_ptr(), sizes[1], device_status(device).data_ptr(), _stream()))
+    return out, state
+
+
+def moe_gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
+                            w_up: torch.Tensor, w_down: torch.Tensor, state: torch.Tensor, activation: str
+                            ) -> tuple[torch.Tensor, ...]:
+    """(dx, dexpert_weight, dw_gate, dw_up, dw_down) of moe_gated_forward_cuda, from grad_out [T, D] and its state."""
+    lib = _lib.load()
+    device = x.device
+    _check_bf16(device, grad_out=grad_out)
+    code = _check_activation(activation)
     num_tokens, k = expert_weight.shape
-    tokens_per_expert, padded_offsets, row_token, copy_row, row_block_expert, row_offsets = layout[:6]
-    num_row_blocks = row_offsets.numel() - 1
-    _check(grad_out.shape == x.shape, f"grad_out must be {tuple(x.shape)}, got {tuple(grad_out.shape)}")
-    _check(w_down.shape == (num_experts, ffn_dim, d_model), f"w_down must be {(num_experts, ffn_dim, d_model)}")
-    _check(expert_weight.dtype in (torch.bfloat16, torch.float32), "expert_weight must be bfloat16 or float32")
-    _check(expert_weight.is_contiguous() and expert_weight.device == x.device, "expert_weight must be contiguous, on x's GPU")
-    _check(num_tokens == x.shape[0] and copy_row.numel() == num_tokens * k, "the layout is of another batch")
-    _check(row_token.numel() == num_row_blocks * BLOCK and padded_offsets.numel() == num_experts + 1,
-           "the layout does not match block size 128 and the number of experts")
-    for t in (h, g, u):
-        _check(t.shape == (num_row_blocks * (ffn_dim // BLOCK), BLOCK, BLOCK), "the kept blocks are of another layout")
-    gate_dtype = int(expert_weight.dtype == torch.float32)
-    rows = num_row_blocks * BLOCK
-    with torch.cuda.device(x.device):
-        status, stream = _ptr(device_status(x.device)), _stream()
-        x_rows, grad_rows = (torch.empty((rows, d_model), dtype=torch.bfloat16, device=x.device) for _ in range(2))
-        row_gate = torch.empty(rows, dtype=torch.float32, device=x.device)
-        gate_partial = torch.empty((rows, ffn_dim // BLOCK), dtype=torch.float32, device=x.device)
-        dg, du = torch.empty_like(g), torch.empty_like(u)
-        dx, dgate = torch.empty_like(x), torch.empty_like(expert_weight)
-        dw_gate, dw_up, dw_down = (torch.empty_like(w) for w in (w_gate, w_up, w_down))
-        _lib.check(lib.sb_gated_gather(_ptr(x), _ptr(grad_out), _ptr(expert_weight), gate_dtype, _ptr(row_token),
-                                       _ptr(copy_row), _ptr(padded_offsets), num_experts, _ptr(x_rows), _ptr(grad_rows),
-                                       _ptr(row_gate), num_tokens, k, d_model, num_row_blocks, stream))
-        _lib.check(lib.sb_gated_grad_hidden(_ptr(grad_out), _ptr(w_down), _ptr(g), _ptr(u), _ptr(row_gate),
-                                            _ptr(row_token), _ptr(row_block_expert), _ptr(row_offsets), _ptr(dg),
-                                            _ptr(du), _ptr(gate_partial), num_tokens, d_model, ffn_dim, num_experts,
-                                            num_row_blocks, code, status, stream))
-        _lib.check(lib.sb_gated_grad_weights(_ptr(x_rows), _ptr(grad_rows), _ptr(h), _ptr(dg), _ptr(du),
-                                             _ptr(padded_offsets), _ptr(tokens_per_expert), _ptr(row_offsets),
-                                             _ptr(dw_gate), _ptr(dw_up), _ptr(dw_down), d_model, ffn_dim, num_experts,
-                                             num_row_blocks, status, stream))
-        # The rows of dx take the place of the gathered rows of x, which the weight gradients were the last to read.
-        _lib.check(lib.sb_gated_grad_rows(_ptr(dg), _ptr(du), _ptr(w_gate), _ptr(w_up), _ptr(row_token),
-                                          _ptr(row_block_expert), _ptr(row_offsets), _ptr(x_rows), d_model, ffn_dim,
-                                          num_experts, num_row_blocks, status, stream))
-        _lib.check(lib.sb_gated_join(_ptr(x_rows), _ptr(gate_partial), _ptr(copy_row), _ptr(dx), _ptr(dgate), gate_dtype,
-                                     num_tokens, k, d_model, ffn_dim, stream))
-    return dx, dgate, dw_gate, dw_up, dw_down
+    num_experts, d_model, ffn_dim = w_gate.shape
+    with _on(device):
+        sizes = (ctypes.c_int64 * 3)()
+        _lib.check(lib.sb_moe_gated_bytes(num_tokens, k, d_model, ffn_dim, num_experts, 1, sizes))
+        scratch = torch.empty(sizes[2], dtype=torch.uint8, device=device)
+        grads = tuple(torch.empty_like(t) for t in (x, expert_weight, w_gate, w_up, w_down))
+        _lib.check(lib.sb_moe_gated_backward(
+            grad_out.data_ptr(), x.data_ptr(), expert_weight.data_ptr(), int(expert_weight.dtype == torch.float32),
+            w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), state.data_ptr(), state.numel(),
+            *(g.data_ptr() for g in grads), num_tokens, k, d_model, ffn_dim, num_experts, code, scratch.data_ptr(), sizes[2],
+            device_status(device).data_ptr(), _stream()))
+    return grads
 
 
 # ---- projections with the low-rank adapters of many requests (no counterpart in the reference) ----------
@@ -458,7 +477,7 @@ def lora_linear_cuda(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor
                f"scale must be a contiguous float32 [{num_adapters}] tensor on x's GPU")
     _check(out_dtype in (torch.bfloat16, torch.float32), f"out_dtype must be bfloat16 or float32, got {out_dtype}")
     fp32 = int(out_dtype == torch.float32)
-    with torch.cuda.device(device):
+    with _on(device):
         nbytes = lib.sb_lora_workspace_bytes(num_tokens, d_model, width, rank, num_adapters, fp32)
         if nbytes < 0:
             _lib.check(1)

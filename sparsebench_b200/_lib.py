@@ -58,14 +58,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                _P, _P]),
     "sb_sdd_gated": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
                              c_int, _P, _P]),
-    "sb_gated_gather": (c_int, [_P, _P, _P, c_int, _P, _P, _P, c_int32, _P, _P, _P, c_int64, c_int32, c_int32, c_int32,
-                                _P]),
-    "sb_gated_grad_hidden": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32,
-                                     c_int32, c_int32, _P, _P]),
-    "sb_gated_grad_weights": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32,
-                                      _P, _P]),
-    "sb_gated_grad_rows": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, _P, _P]),
-    "sb_gated_join": (c_int, [_P, _P, _P, _P, _P, c_int, c_int64, c_int32, c_int32, c_int32, _P]),
+    "sb_moe_gated_bytes": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int, _P]),
+    "sb_moe_gated_forward": (c_int, [_P, _P, c_int, _P, c_int, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                     c_int32, _P, c_int64, _P, c_int64, _P, _P]),
+    "sb_moe_gated_backward": (c_int, [_P, _P, _P, c_int, _P, _P, _P, _P, c_int64, _P, _P, _P, _P, _P, c_int64, c_int32,
+                                      c_int32, c_int32, c_int32, c_int32, _P, c_int64, _P, _P]),
     "sb_lora_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int]),
     "sb_lora_linear": (c_int, [_P, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int64, c_int32, c_int32, c_int32, c_int32,
                                _P, c_int64, _P, _P]),

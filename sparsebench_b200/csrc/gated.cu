@@ -9,11 +9,15 @@
 // dgate comes from S and H, not from Y, so the forward has to keep only G, U and H (bf16); the gate multiplies S in
 // fp32, so dH is not rounded. Roundings to bf16: G, U, H, w dO, dG, dU, the rows of dx before their sum, the results.
 //
+// A decoding step (at most 64 copies, nothing kept) takes another way: no layout, the weights of the picked experts
+// streamed by the kernels of skinny.cuh (SkinnyUp, SkinnyDown, gated_small_combine_kernel).
+//
 // act is SiLU, v / (1 + exp(-v)), or the erf form of GELU.
 
 #include <algorithm>
 #include <initializer_list>
 
+#include "skinny.cuh"
 #include "tile_gemm.cuh"
 
 namespace sb {
@@ -296,7 +300,7 @@ struct GradRows {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr bool kVariable = false, kStepGather = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -354,7 +358,7 @@ struct GradWeights {
     bool live;
   };
   struct Early {};
-  static constexpr bool kVariable = false, kStepGather = false, kGather = false, kAMnMajor = true, kBMnMajor = true;
+  static constexpr bool kVariable = false, kGather = false, kAMnMajor = true, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) {
     return p.num_experts * (p.down_tiles + 2 * p.up_tiles);
@@ -425,6 +429,129 @@ struct GradWeights {
   }
 };
 
+// ---- a decoding step -----------------------------------------------------------------------------------------------
+// The blocks are numbered (picked expert in order of first appearance, column tile, split); every block finds its
+// expert and that expert's copies from the ids by itself, so there is no routing kernel in front.
+
+struct ExpertItem { int32_t expert, tile, rows; };
+
+// False: fewer distinct experts than block items. list: the expert's copies, ascending.
+__device__ __forceinline__ bool find_expert(const void* expert_idx, int idx_is_i64, int32_t copies, int32_t num_experts,
+                                            int32_t which, ExpertItem& item, int32_t* ids, int32_t* list) {
+  __shared__ int32_t count[4];
+  __shared__ int32_t found;
+  const int c = static_cast<int>(threadIdx.x);
+  int32_t mine = -1;
+  if (c < copies) {
+    const int64_t id = idx_is_i64 ? __ldg(static_cast<const long long*>(expert_idx) + c)
+                                  : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(expert_idx) + c));
+    if (id >= 0 && id < num_experts) mine = static_cast<int32_t>(id);
+  }
+  if (c < kSkinnyMaxRows) ids[c] = mine;
+  __syncthreads();
+  bool leads = mine >= 0;
+  for (int j = 0; leads && j < c; ++j) leads = ids[j] != mine;
+  const unsigned lead_mask = __ballot_sync(0xffffffffu, leads);
+  if (c < kSkinnyMaxRows && (c & 31) == 0) count[c >> 5] = __popc(lead_mask);
+  __syncthreads();
+  const unsigned below = (1u << (c & 31)) - 1u;
+  if (leads && __popc(lead_mask & below) + (c >= 32 ? count[0] : 0) == which) found = mine;
+  if (which >= count[0] + count[1]) return false;
+  __syncthreads();
+  item.expert = found;
+  const bool match = c < kSkinnyMaxRows && mine == item.expert;
+  const unsigned match_mask = __ballot_sync(0xffffffffu, match);
+  if (c < kSkinnyMaxRows && (c & 31) == 0) count[2 + (c >> 5)] = __popc(match_mask);
+  __syncthreads();
+  if (match) list[__popc(match_mask & below) + (c >= 32 ? count[2] : 0)] = c;
+  item.rows = count[2] + count[3];
+  return true;  // the caller's next barrier publishes the list
+}
+
+// H[copy] = act(x Wg) * (x Wu): the tile's 128 weight columns are 64 of Wg next to the same 64 of Wu.
+struct SkinnyUp {
+  struct Params {
+    SkinnyShape shape;
+    const void* expert_idx;
+    const __nv_bfloat16* x;
+    __nv_bfloat16* h;  // [copies, F]
+    int32_t idx_is_i64, copies, k, num_experts, d_model, ffn_dim, tiles, activation;
+  };
+  using Item = ExpertItem;
+  struct Extra {};
+  static constexpr bool kGather = true;
+  static __device__ __forceinline__ bool begin(const Params& p, Item& item, int32_t block_item, int32_t* ids, int32_t* list) {
+    const int32_t which = block_item / p.tiles;
+    item.tile = block_item - which * p.tiles;
+    return find_expert(p.expert_idx, p.idx_is_i64, p.copies, p.num_experts, which, item, ids, list);
+  }
+  static __device__ __forceinline__ void load_w(const SkinnyMaps& maps, const Params& p, const Item& item, int32_t ks,
+                                                uint32_t dst, uint32_t bar) {
+    const int32_t row = item.expert * p.d_model + ks * kSkinnyStep;
+    ptx::tma_load_2d(dst, &maps.w[0], item.tile * 64, row, bar);
+    ptx::tma_load_2d(dst + kSkinnyWBytes / 2, &maps.w[1], item.tile * 64, row, bar);
+  }
+  static __device__ __forceinline__ const __nv_bfloat16* gather_row(const Params& p, const Item&, const int32_t* list, int row) {
+    return p.x + static_cast<int64_t>(list[row] / p.k) * p.d_model;
+  }
+  static __device__ __forceinline__ void extra(const Params&, const Item&, int32_t, int, Extra&) {}
+  static __device__ __forceinline__ void finish(const Params& p, const Item& item, const int32_t* list, int32_t rank,
+                                                int worker, const SkinnySums& red, const Extra&) {
+    const int32_t c = (worker & 7) * 8;
+    for (int32_t r = rank + p.shape.splits * (worker >> 3); r < item.rows; r += p.shape.splits * 16) {
+      float g[8], u[8];
+      red.sum(r, c, g);
+      red.sum(r, 64 + c, u);
+      uint32_t packed[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        packed[q] = pack_bf16(act_value(g[2 * q], p.activation) * u[2 * q], act_value(g[2 * q + 1], p.activation) * u[2 * q + 1]);
+      *reinterpret_cast<uint4*>(p.h + static_cast<int64_t>(list[r]) * p.ffn_dim + item.tile * 64 + c) =
+          make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    }
+  }
+};
+
+// Y[copy] = H[copy] Wd in fp32.
+struct SkinnyDown {
+  struct Params {
+    SkinnyShape shape;
+    const void* expert_idx;
+    const __nv_bfloat16* h;
+    float* y;  // [copies, D]
+    int32_t idx_is_i64, copies, num_experts, d_model, ffn_dim, tiles;
+  };
+  using Item = ExpertItem;
+  struct Extra {};
+  static constexpr bool kGather = true;
+  static __device__ __forceinline__ bool begin(const Params& p, Item& item, int32_t block_item, int32_t* ids, int32_t* list) {
+    const int32_t which = block_item / p.tiles;
+    item.tile = block_item - which * p.tiles;
+    return find_expert(p.expert_idx, p.idx_is_i64, p.copies, p.num_experts, which, item, ids, list);
+  }
+  static __device__ __forceinline__ void load_w(const SkinnyMaps& maps, const Params& p, const Item& item, int32_t ks,
+                                                uint32_t dst, uint32_t bar) {
+    const int32_t row = item.expert * p.ffn_dim + ks * kSkinnyStep;
+    ptx::tma_load_2d(dst, &maps.w[0], item.tile * 128, row, bar);
+    ptx::tma_load_2d(dst + kSkinnyWBytes / 2, &maps.w[0], item.tile * 128 + 64, row, bar);
+  }
+  static __device__ __forceinline__ const __nv_bfloat16* gather_row(const Params& p, const Item&, const int32_t* list, int row) {
+    return p.h + static_cast<int64_t>(list[row]) * p.ffn_dim;
+  }
+  static __device__ __forceinline__ void extra(const Params&, const Item&, int32_t, int, Extra&) {}
+  static __device__ __forceinline__ void finish(const Params& p, const Item& item, const int32_t* list, int32_t rank,
+                                                int worker, const SkinnySums& red, const Extra&) {
+    const int32_t c = (worker & 15) * 8;
+    for (int32_t r = rank + p.shape.splits * (worker >> 4); r < item.rows; r += p.shape.splits * 8) {
+      float v[8];
+      red.sum(r, c, v);
+      float4* dst = reinterpret_cast<float4*>(p.y + static_cast<int64_t>(list[r]) * p.d_model + item.tile * 128 + c);
+      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  }
+};
+
 // ---- small kernels ------------------------------------------------------------------------------------------------
 
 constexpr int kSmallThreads = 256;
@@ -432,6 +559,31 @@ constexpr int kSmallThreads = 256;
 __device__ __forceinline__ float gate_at(const void* gate, int gate_dtype, int64_t i) {
   return gate_dtype == 1 ? __ldg(static_cast<const float*>(gate) + i)
                          : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(gate) + i));
+}
+
+// out[t] = sum over the picks j of gate[t, j] * Y[t k + j], in order, from the fp32 rows of a decoding step.
+__global__ void __launch_bounds__(128)
+gated_small_combine_kernel(const float4* __restrict__ y, const void* __restrict__ expert_idx, int idx_is_i64,
+                           const void* __restrict__ gate, int gate_dtype, uint2* __restrict__ out, int32_t k,
+                           int32_t num_experts, int32_t quads) {
+  grid_dependency_wait();
+  const int32_t t = static_cast<int32_t>(blockIdx.y);
+  const int32_t v = static_cast<int32_t>(blockIdx.x) * 128 + static_cast<int32_t>(threadIdx.x);
+  if (v >= quads) return;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int32_t j = 0; j < k; ++j) {
+    const int32_t c = t * k + j;
+    const int64_t id = idx_is_i64 ? __ldg(static_cast<const long long*>(expert_idx) + c)
+                                  : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(expert_idx) + c));
+    if (id < 0 || id >= num_experts) continue;
+    const float w = gate_at(gate, gate_dtype, c);
+    const float4 r = __ldcg(y + static_cast<int64_t>(c) * quads + v);
+    acc.x = fmaf(w, r.x, acc.x);
+    acc.y = fmaf(w, r.y, acc.y);
+    acc.z = fmaf(w, r.z, acc.z);
+    acc.w = fmaf(w, r.w, acc.w);
+  }
+  out[static_cast<int64_t>(t) * quads + v] = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
 }
 
 // One warp per row of the layout: X[r] = x[token], (w dO)[r] = w * grad_out[token], row_gate[r] = w; zeros for padding.
@@ -561,17 +713,11 @@ bool any_null(std::initializer_list<const void*> ptrs) {
   return false;
 }
 
-}  // namespace
-}  // namespace sb
-
-using namespace sb;
-
-extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
+int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
                             const int32_t* row_block_expert, const int32_t* row_offsets, void* h_blocks, void* g_blocks,
                             void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
                             int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
-                            sb_stream_t stream) {
-  clear_error();
+                            cudaStream_t stream) {
   if (int rc = check_gated("sdd_gated", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
   if (num_row_blocks == 0) return SB_OK;
   if (any_null({x, w_gate, w_up, row_token, row_block_expert, row_offsets, h_blocks}))
@@ -602,14 +748,13 @@ extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up,
   p.skip_padding = skip_padding_rows ? 1 : 0;
   p.keep = g_blocks != nullptr ? 1 : 0;
   return launch_tile_gemm<GatedUp>(maps, p, static_cast<int64_t>(num_row_blocks) * (ffn_dim / 128), dev_status,
-                                   as_stream(stream), "sdd_gated");
+                                   stream, "sdd_gated");
 }
 
-extern "C" int sb_gated_gather(const void* x, const void* grad_out, const void* gate, int gate_dtype,
+int gated_gather(const void* x, const void* grad_out, const void* gate, int gate_dtype,
                                const int32_t* row_token, const int32_t* copy_row, const int32_t* padded_offsets,
                                int32_t num_experts, void* x_rows, void* grad_rows, float* row_gate, int64_t num_tokens,
-                               int32_t k, int32_t d_model, int32_t num_row_blocks, sb_stream_t stream) {
-  clear_error();
+                               int32_t k, int32_t d_model, int32_t num_row_blocks, cudaStream_t stream) {
   if (int rc = check_gated("gated_gather", d_model, 128, num_experts, num_row_blocks, 0)) return rc;
   if (num_row_blocks == 0) return SB_OK;
   if (any_null({x, grad_out, gate, row_token, copy_row, padded_offsets, x_rows, grad_rows, row_gate}))
@@ -621,18 +766,17 @@ extern "C" int sb_gated_gather(const void* x, const void* grad_out, const void* 
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
-  gated_gather_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, as_stream(stream)>>>(
+  gated_gather_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, stream>>>(
       static_cast<const uint4*>(x), static_cast<const uint4*>(grad_out), gate, gate_dtype, row_token, copy_row,
       padded_offsets + num_experts, static_cast<uint4*>(x_rows), static_cast<uint4*>(grad_rows), row_gate, k, d_model / 8);
   return check_launch("gated_gather");
 }
 
-extern "C" int sb_gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_blocks, const void* u_blocks,
+int gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_blocks, const void* u_blocks,
                                     const float* row_gate, const int32_t* row_token, const int32_t* row_block_expert,
                                     const int32_t* row_offsets, void* dg_blocks, void* du_blocks, float* gate_partial,
                                     int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
-                                    int32_t num_row_blocks, int32_t activation, int32_t* dev_status, sb_stream_t stream) {
-  clear_error();
+                                    int32_t num_row_blocks, int32_t activation, int32_t* dev_status, cudaStream_t stream) {
   if (int rc = check_gated("gated_grad_hidden", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
   if (num_row_blocks == 0) return SB_OK;
   if (any_null({grad_out, w_down, g_blocks, u_blocks, row_gate, row_token, row_block_expert, row_offsets, dg_blocks,
@@ -660,16 +804,15 @@ extern "C" int sb_gated_grad_hidden(const void* grad_out, const void* w_down, co
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
   p.activation = activation;
-  return launch_tile_gemm<GradHidden>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, as_stream(stream),
+  return launch_tile_gemm<GradHidden>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream,
                                       "gated_grad_hidden");
 }
 
-extern "C" int sb_gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_blocks, const void* dg_blocks,
+int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_blocks, const void* dg_blocks,
                                      const void* du_blocks, const int32_t* padded_offsets, const int32_t* tokens_per_expert,
                                      const int32_t* row_offsets, void* dw_gate, void* dw_up, void* dw_down, int32_t d_model,
                                      int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status,
-                                     sb_stream_t stream) {
-  clear_error();
+                                     cudaStream_t stream) {
   if (int rc = check_gated("gated_grad_weights", d_model, ffn_dim, num_experts, num_row_blocks, 0)) return rc;
   if (num_row_blocks <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_weights: the layout has no row blocks");
   if (any_null({x_rows, grad_rows, h_blocks, dg_blocks, du_blocks, padded_offsets, tokens_per_expert, row_offsets, dw_gate,
@@ -703,14 +846,13 @@ extern "C" int sb_gated_grad_weights(const void* x_rows, const void* grad_rows, 
   p.up_cols = (ffn_dim + kTileCols - 1) / kTileCols;
   p.up_tiles = d_model / kTileRows * p.up_cols;
   const int64_t tiles = static_cast<int64_t>(num_experts) * (p.down_tiles + 2ll * p.up_tiles);
-  return launch_tile_gemm<GradWeights>(maps, p, tiles, dev_status, as_stream(stream), what);
+  return launch_tile_gemm<GradWeights>(maps, p, tiles, dev_status, stream, what);
 }
 
-extern "C" int sb_gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up,
+int gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up,
                                   const int32_t* row_token, const int32_t* row_block_expert, const int32_t* row_offsets,
                                   void* dx_rows, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
-                                  int32_t num_row_blocks, int32_t* dev_status, sb_stream_t stream) {
-  clear_error();
+                                  int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
   if (int rc = check_gated("gated_grad_rows", d_model, ffn_dim, num_experts, num_row_blocks, 0)) return rc;
   if (num_row_blocks == 0) return SB_OK;
   if (any_null({dg_blocks, du_blocks, w_gate, w_up, row_token, row_block_expert, row_offsets, dx_rows}))
@@ -734,13 +876,12 @@ extern "C" int sb_gated_grad_rows(const void* dg_blocks, const void* du_blocks, 
   p.row_block_expert = row_block_expert;
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
-  return launch_tile_gemm<GradRows>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, as_stream(stream), what);
+  return launch_tile_gemm<GradRows>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
 }
 
-extern "C" int sb_gated_join(const void* dx_rows, const float* gate_partial, const int32_t* copy_row, void* dx, void* dgate,
+int gated_join(const void* dx_rows, const float* gate_partial, const int32_t* copy_row, void* dx, void* dgate,
                              int gate_dtype, int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim,
-                             sb_stream_t stream) {
-  clear_error();
+                             cudaStream_t stream) {
   if (int rc = check_gated("gated_join", d_model, ffn_dim, 1, 0, 0)) return rc;
   if (any_null({dx_rows, gate_partial, copy_row, dx, dgate})) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: NULL buffer");
   if (num_tokens <= 0 || k <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: T and k must be positive");
@@ -749,8 +890,246 @@ extern "C" int sb_gated_join(const void* dx_rows, const float* gate_partial, con
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
   const int64_t blocks = std::min<int64_t>((num_tokens + 7) / 8, static_cast<int64_t>(info->sm_count) * 8);
-  gated_join_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, as_stream(stream)>>>(
+  gated_join_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, stream>>>(
       static_cast<const uint4*>(dx_rows), gate_partial, copy_row, static_cast<uint4*>(dx), dgate, gate_dtype, num_tokens, k,
       d_model / 8, ffn_dim / 128);
   return check_launch("gated_join");
+}
+
+int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
+
+// The two ways of the forward pass. The decoding way needs no layout and splits K over clusters; it starts a block per
+// 64 (128) weight columns of every picked expert. From 65 copies on (and wherever the backward pass needs the layout's
+// blocks) the persistent kernels of the layout are at least as fast.
+constexpr int64_t kSmallCopies = 64;
+
+// Parts of the buffers, in bytes from their start.
+struct GatedBuffers {
+  bool small;
+  int32_t row_blocks, ffn_blocks;
+  // state (keep) or scratch: the layout's arrays, then the blocks
+  int64_t tokens_per_expert, padded_offsets, row_token, copy_row, row_block_expert, row_offsets, col_indices, error, work;
+  int64_t h, g, u, y;
+  int64_t state_bytes, scratch_bytes;
+  // scratch of the backward pass
+  int64_t x_rows, grad_rows, row_gate, gate_partial, dg, du, backward_bytes;
+};
+
+int gated_buffers(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int keep,
+                  GatedBuffers* b) {
+  if (num_tokens <= 0 || k <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: T and k must be positive");
+  if (num_tokens > INT32_MAX / k) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: problem too large");
+  if (int rc = check_gated("moe_gated", d_model, ffn_dim, num_experts, 0, 0)) return rc;
+  const int64_t n = num_tokens * k;
+  int64_t row_blocks = 0, rows = 0, ffn_blocks = 0;
+  if (int rc = sb_route_sizes(n, num_experts, ffn_dim, 128, &row_blocks, &rows, &ffn_blocks)) return rc;
+  if (int rc = check_gated("moe_gated", d_model, ffn_dim, num_experts, static_cast<int32_t>(row_blocks), 0)) return rc;
+  *b = GatedBuffers{};
+  b->row_blocks = static_cast<int32_t>(row_blocks);
+  b->ffn_blocks = static_cast<int32_t>(ffn_blocks);
+  b->small = !keep && n <= kSmallCopies;
+  int64_t at = 0;
+  auto take = [&at](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  if (b->small) {
+    b->h = take(n * ffn_dim * 2);
+    b->y = take(n * d_model * 4);
+    b->scratch_bytes = at;
+    return SB_OK;
+  }
+  b->tokens_per_expert = take(num_experts * 4ll);
+  b->padded_offsets = take((num_experts + 1ll) * 4);
+  b->row_token = take(rows * 4);
+  b->copy_row = take(n * 4);
+  b->row_block_expert = take(row_blocks * 4);
+  b->row_offsets = take((row_blocks + 1) * 4);
+  b->col_indices = take(row_blocks * ffn_blocks * 4);
+  b->error = take(4);
+  b->h = take(rows * ffn_dim * 2);
+  if (keep) {
+    b->g = take(rows * ffn_dim * 2);
+    b->u = take(rows * ffn_dim * 2);
+    b->state_bytes = at;
+    at = 0;
+  }
+  b->work = take(static_cast<int64_t>(sb_route_workspace_bytes(n, num_experts)));
+  b->y = take(rows * d_model * 2);
+  b->scratch_bytes = at;
+  at = 0;
+  b->x_rows = take(rows * d_model * 2);
+  b->grad_rows = take(rows * d_model * 2);
+  b->row_gate = take(rows * 4);
+  b->gate_partial = take(rows * ffn_blocks * 4);
+  b->dg = take(rows * ffn_dim * 2);
+  b->du = take(rows * ffn_dim * 2);
+  b->backward_bytes = at;
+  return SB_OK;
+}
+
+int forward_small(const GatedBuffers& b, const void* x, const void* expert_idx, int idx_is_i64, const void* gate,
+                  int gate_dtype, const void* w_gate, const void* w_up, const void* w_down, void* out, int32_t num_tokens,
+                  int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t activation, uint8_t* scratch,
+                  int32_t* dev_status, cudaStream_t stream) {
+  const DeviceInfo* info = current_device_info();
+  if (info == nullptr) return SB_ERR_CUDA;
+  const int32_t copies = num_tokens * k;
+  const int32_t experts = std::min(copies, num_experts);  // at most so many different ones are picked
+  __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(scratch + b.h);
+  float* y = reinterpret_cast<float*>(scratch + b.y);
+  const uint64_t up_rows = static_cast<uint64_t>(num_experts) * d_model;
+  const uint64_t down_rows = static_cast<uint64_t>(num_experts) * ffn_dim;
+  SkinnyMaps maps{};
+  if (int rc = encode_2d_map(&maps.w[0], w_gate, up_rows, ffn_dim, 64, 64, 2, "moe_gated (w_gate)")) return rc;
+  if (int rc = encode_2d_map(&maps.w[1], w_up, up_rows, ffn_dim, 64, 64, 2, "moe_gated (w_up)")) return rc;
+  SkinnyUp::Params up{};
+  up.tiles = ffn_dim / 64;
+  up.shape = skinny_shape(static_cast<int64_t>(experts) * up.tiles, d_model / kSkinnyStep, copies, info->sm_count);
+  up.expert_idx = expert_idx;
+  up.x = static_cast<const __nv_bfloat16*>(x);
+  up.h = h;
+  up.idx_is_i64 = idx_is_i64;
+  up.copies = copies;
+  up.k = k;
+  up.num_experts = num_experts;
+  up.d_model = d_model;
+  up.ffn_dim = ffn_dim;
+  up.activation = activation;
+  if (int rc = launch_skinny<SkinnyUp>(maps, up, static_cast<int64_t>(experts) * up.tiles, false, dev_status, stream, "moe_gated (up)")) return rc;
+  SkinnyMaps down_maps{};
+  if (int rc = encode_2d_map(&down_maps.w[0], w_down, down_rows, d_model, 64, 64, 2, "moe_gated (w_down)")) return rc;
+  SkinnyDown::Params down{};
+  down.tiles = d_model / 128;
+  down.shape = skinny_shape(static_cast<int64_t>(experts) * down.tiles, ffn_dim / kSkinnyStep, copies, info->sm_count);
+  down.expert_idx = expert_idx;
+  down.h = h;
+  down.y = y;
+  down.idx_is_i64 = idx_is_i64;
+  down.copies = copies;
+  down.num_experts = num_experts;
+  down.d_model = d_model;
+  down.ffn_dim = ffn_dim;
+  if (int rc = launch_skinny<SkinnyDown>(down_maps, down, static_cast<int64_t>(experts) * down.tiles, true, dev_status, stream, "moe_gated (down)")) return rc;
+  cudaLaunchConfig_t cfg = {};
+  const int32_t quads = d_model / 4;
+  cfg.gridDim = dim3(static_cast<unsigned>((quads + 127) / 128), static_cast<unsigned>(num_tokens));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, gated_small_combine_kernel, reinterpret_cast<const float4*>(y), expert_idx,
+                                             idx_is_i64, gate, gate_dtype, static_cast<uint2*>(out), k, num_experts, quads);
+  if (err != cudaSuccess) return fail(SB_ERR_CUDA, "moe_gated (combine): %s", cudaGetErrorString(err));
+  return SB_OK;
+}
+
+}  // namespace
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
+                            const int32_t* row_block_expert, const int32_t* row_offsets, void* h_blocks, void* g_blocks,
+                            void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                            int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
+                            sb_stream_t stream) {
+  clear_error();
+  return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, row_offsets, h_blocks, g_blocks, u_blocks, num_tokens,
+                   d_model, ffn_dim, num_experts, num_row_blocks, activation, skip_padding_rows, dev_status, as_stream(stream));
+}
+
+extern "C" int sb_moe_gated_bytes(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                                  int keep, int64_t* bytes) {
+  clear_error();
+  if (bytes == nullptr) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_bytes: NULL output");
+  GatedBuffers b;
+  if (int rc = gated_buffers(num_tokens, k, d_model, ffn_dim, num_experts, keep, &b)) return rc;
+  bytes[0] = b.state_bytes;
+  bytes[1] = b.scratch_bytes;
+  bytes[2] = keep ? b.backward_bytes : 0;
+  return SB_OK;
+}
+
+extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int idx_is_i64, const void* gate, int gate_dtype,
+                                    const void* w_gate, const void* w_up, const void* w_down, void* out, int64_t num_tokens,
+                                    int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t activation,
+                                    void* state, int64_t state_bytes, void* scratch, int64_t scratch_bytes,
+                                    int32_t* dev_status, sb_stream_t stream) {
+  clear_error();
+  const int keep = state != nullptr ? 1 : 0;
+  GatedBuffers b;
+  if (int rc = gated_buffers(num_tokens, k, d_model, ffn_dim, num_experts, keep, &b)) return rc;
+  if (int rc = check_gated("moe_gated", d_model, ffn_dim, num_experts, b.row_blocks, activation)) return rc;
+  if (any_null({x, expert_idx, gate, w_gate, w_up, w_down, out, scratch})) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: NULL buffer");
+  if (any_misaligned({x, w_gate, w_up, w_down, out, state, scratch}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: buffers must be 16-byte aligned");
+  if (gate_dtype != 0 && gate_dtype != 1) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: gate_dtype must be 0 (bf16) or 1 (fp32)");
+  if ((keep && state_bytes < b.state_bytes) || scratch_bytes < b.scratch_bytes)
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: the buffers have %lld and %lld bytes, %lld and %lld are needed",
+                (long long)state_bytes, (long long)scratch_bytes, (long long)b.state_bytes, (long long)b.scratch_bytes);
+  uint8_t* temp = static_cast<uint8_t*>(scratch);
+  if (b.small)
+    return forward_small(b, x, expert_idx, idx_is_i64, gate, gate_dtype, w_gate, w_up, w_down, out,
+                         static_cast<int32_t>(num_tokens), k, d_model, ffn_dim, num_experts, activation, temp, dev_status,
+                         as_stream(stream));
+  uint8_t* base = keep ? static_cast<uint8_t*>(state) : temp;
+  auto ints = [base](int64_t at) { return reinterpret_cast<int32_t*>(base + at); };
+  if (int rc = sb_route(expert_idx, idx_is_i64, num_tokens * k, k, num_experts, b.ffn_blocks, 128, b.row_blocks,
+                        ints(b.tokens_per_expert), ints(b.padded_offsets), ints(b.row_token), ints(b.copy_row),
+                        ints(b.row_block_expert), ints(b.row_offsets), ints(b.col_indices), ints(b.error), temp + b.work, stream))
+    return rc;
+  if (int rc = sdd_gated(x, w_gate, w_up, ints(b.row_token), ints(b.row_block_expert), ints(b.row_offsets), base + b.h,
+                         keep ? base + b.g : nullptr, keep ? base + b.u : nullptr, num_tokens, d_model, ffn_dim, num_experts,
+                         b.row_blocks, activation, 1, dev_status, as_stream(stream)))
+    return rc;
+  if (int rc = sb_dsd(base + b.h, static_cast<int64_t>(b.row_blocks) * b.ffn_blocks, w_down,
+                      static_cast<int64_t>(num_experts) * ffn_dim, d_model, ints(b.row_offsets), ints(b.col_indices),
+                      b.row_blocks, 128, 0, ints(b.row_token), temp + b.y, ints(b.padded_offsets), num_experts, dev_status, stream))
+    return rc;
+  return sb_combine(temp + b.y, ints(b.copy_row), gate, gate_dtype, out, num_tokens, k, d_model, stream);
+}
+
+extern "C" int sb_moe_gated_backward(const void* grad_out, const void* x, const void* gate, int gate_dtype,
+                                     const void* w_gate, const void* w_up, const void* w_down, const void* state,
+                                     int64_t state_bytes, void* dx, void* dgate, void* dw_gate, void* dw_up, void* dw_down,
+                                     int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                                     int32_t activation, void* scratch, int64_t scratch_bytes, int32_t* dev_status,
+                                     sb_stream_t stream) {
+  clear_error();
+  GatedBuffers b;
+  if (int rc = gated_buffers(num_tokens, k, d_model, ffn_dim, num_experts, 1, &b)) return rc;
+  if (any_null({grad_out, x, gate, w_gate, w_up, w_down, state, dx, dgate, dw_gate, dw_up, dw_down, scratch}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: NULL buffer");
+  if (any_misaligned({state, scratch})) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: buffers must be 16-byte aligned");
+  if (state_bytes < b.state_bytes || scratch_bytes < b.backward_bytes)
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: the buffers have %lld and %lld bytes, %lld and %lld are needed",
+                (long long)state_bytes, (long long)scratch_bytes, (long long)b.state_bytes, (long long)b.backward_bytes);
+  const uint8_t* base = static_cast<const uint8_t*>(state);
+  uint8_t* temp = static_cast<uint8_t*>(scratch);
+  const cudaStream_t st = as_stream(stream);
+  auto ints = [base](int64_t at) { return reinterpret_cast<const int32_t*>(base + at); };
+  const int32_t* row_token = ints(b.row_token);
+  float* row_gate = reinterpret_cast<float*>(temp + b.row_gate);
+  float* gate_partial = reinterpret_cast<float*>(temp + b.gate_partial);
+  if (int rc = gated_gather(x, grad_out, gate, gate_dtype, row_token, ints(b.copy_row), ints(b.padded_offsets), num_experts,
+                            temp + b.x_rows, temp + b.grad_rows, row_gate, num_tokens, k, d_model, b.row_blocks, st))
+    return rc;
+  if (int rc = gated_grad_hidden(grad_out, w_down, base + b.g, base + b.u, row_gate, row_token, ints(b.row_block_expert),
+                                 ints(b.row_offsets), temp + b.dg, temp + b.du, gate_partial, num_tokens, d_model, ffn_dim,
+                                 num_experts, b.row_blocks, activation, dev_status, st))
+    return rc;
+  if (int rc = gated_grad_weights(temp + b.x_rows, temp + b.grad_rows, base + b.h, temp + b.dg, temp + b.du,
+                                  ints(b.padded_offsets), ints(b.tokens_per_expert), ints(b.row_offsets), dw_gate, dw_up,
+                                  dw_down, d_model, ffn_dim, num_experts, b.row_blocks, dev_status, st))
+    return rc;
+  // The rows of dx take the place of the gathered rows of x, which the weight gradients were the last to read.
+  if (int rc = gated_grad_rows(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert),
+                               ints(b.row_offsets), temp + b.x_rows, d_model, ffn_dim, num_experts, b.row_blocks, dev_status, st))
+    return rc;
+  return gated_join(temp + b.x_rows, gate_partial, ints(b.copy_row), dx, dgate, gate_dtype, num_tokens, k, d_model, ffn_dim, st);
 }

@@ -128,7 +128,7 @@ struct LoraShrink {
     bool live;
   };
   struct Early { int32_t slot; };
-  static constexpr bool kVariable = true, kStepGather = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = true, kGather = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.row_tiles * p.groups * p.splits; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {

@@ -2,29 +2,26 @@
 
     out[t] = sum over the token's picks of gate * (act(x w_gate[e]) * (x w_up[e])) w_down[e]
 
-Forward: routing -> sdd_gated -> DSD -> combine, like moe_forward. The backward pass is a call of its own
-(moe_backward_gated), so that a training step can be captured into a CUDA graph as it is; moe_gated() wraps the two
-for torch.autograd. No host sync anywhere.
+Routing, the gated SDD, DSD and the combine as in moe_forward; a decoding step (at most 64 token copies) streams the picked
+experts' weights without a layout. The backward pass is a call of its own (moe_backward_gated), so that a training step can
+be captured into a CUDA graph as it is; moe_gated() wraps the two for torch.autograd. No host sync anywhere.
 """
 
 from __future__ import annotations
 
-from collections.abc import Callable
 from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
 
 from sparsebench_b200 import _C
-from sparsebench_b200.moe import BLOCK_SIZE, _no_mark
-from sparsebench_b200.routing import DeviceTopology, route_device
-from sparsebench_b200.spmm import combine, dsd
 
 
 @dataclass(frozen=True)
 class GatedSaved:
     """What moe_forward_gated_saved keeps for moe_backward_gated: the inputs by reference (they must still hold the
-    same values then), the layout, and the blocks of H, G and U (3 * rows * F bf16). topo is None for an empty batch."""
+    same values then) and the layout with the blocks of H, G and U (3 * rows * F bf16). state is None for an empty
+    batch."""
 
     x: torch.Tensor
     expert_weight: torch.Tensor
@@ -32,10 +29,7 @@ class GatedSaved:
     w_up: torch.Tensor
     w_down: torch.Tensor
     activation: str
-    topo: DeviceTopology | None
-    h: torch.Tensor | None
-    g: torch.Tensor | None
-    u: torch.Tensor | None
+    state: torch.Tensor | None
 
 
 class GatedGrads(NamedTuple):
@@ -57,27 +51,12 @@ def _check_shapes(x, expert_idx, expert_weight, w_gate, w_up, w_down) -> None:
         raise ValueError("x must be [T, D] and expert_idx / expert_weight [T, k]")
 
 
-def _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, keep, mark):
+def _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, keep):
     _check_shapes(x, expert_idx, expert_weight, w_gate, w_up, w_down)
-    _C._check_gated_weights(x, w_gate, w_up)
-    _C._check_bf16(x.device, w_down=w_down)
-    _C._check_activation(activation)
-    for t, name in ((expert_idx, "expert_idx"), (expert_weight, "expert_weight")):
-        _C._check(t.device == x.device, f"all inputs must be on the same GPU: {name} is on {t.device}, not {x.device}")
-    num_experts, d_model, ffn_dim = w_gate.shape
     if expert_idx.numel() == 0:  # host-known size: nothing routed anywhere
-        return torch.zeros_like(x), None, None, None, None
-    topo = route_device(expert_idx, num_experts, ffn_dim, BLOCK_SIZE)
-    mark("routing")
-    h, g, u = _C.sdd_gated_cuda(x, w_gate, w_up, topo.row_token, topo.row_block_expert, topo.row_offsets,
-                                topo.col_indices.numel(), activation, skip_padding_rows=True, keep=keep)
-    mark("gated SDD")
-    y = dsd(h, w_down.view(num_experts * ffn_dim, d_model), topo, version=4, skip_padding_rows=True,
-            layout_from_routing=True)
-    mark("DSD")
-    out = combine(y, expert_weight, topo)
-    mark("combine")
-    return out, topo, h, g, u
+        _C._check_gated_layer(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
+        return torch.zeros_like(x), None
+    return _C.moe_gated_forward_cuda(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, keep)
 
 
 def moe_forward_gated(
@@ -88,13 +67,11 @@ def moe_forward_gated(
     w_up: torch.Tensor,
     w_down: torch.Tensor,
     activation: str = "silu",
-    mark: Callable[[str], None] = _no_mark,
 ) -> torch.Tensor:
     """x [T, D], expert_idx / expert_weight [T, k], w_gate and w_up [E, D, F], w_down [E, F, D] -> [T, D]; bf16 (gates
     bf16 or fp32), fp32 accumulation inside the kernels, D and F multiples of 128. activation: "silu" (SwiGLU experts)
-    or "gelu" (erf form). An expert id outside [0, E) is skipped, as in moe_forward. mark as in moe_forward, with
-    "gated SDD" for the second stage."""
-    return _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, False, mark)[0]
+    or "gelu" (erf form). An expert id outside [0, E) is skipped, as in moe_forward."""
+    return _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, False)[0]
 
 
 def moe_forward_gated_saved(
@@ -107,8 +84,8 @@ def moe_forward_gated_saved(
     activation: str = "silu",
 ) -> tuple[torch.Tensor, GatedSaved]:
     """moe_forward_gated that also returns what moe_backward_gated needs."""
-    out, topo, h, g, u = _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, True, _no_mark)
-    return out, GatedSaved(x, expert_weight, w_gate, w_up, w_down, activation, topo, h, g, u)
+    out, state = _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, True)
+    return out, GatedSaved(x, expert_weight, w_gate, w_up, w_down, activation, state)
 
 
 def moe_backward_gated(grad_out: torch.Tensor, saved: GatedSaved) -> GatedGrads:
@@ -117,12 +94,10 @@ def moe_backward_gated(grad_out: torch.Tensor, saved: GatedSaved) -> GatedGrads:
     s = saved
     if grad_out.shape != s.x.shape:
         raise ValueError(f"grad_out must be {tuple(s.x.shape)}, got {tuple(grad_out.shape)}")
-    if s.topo is None:
+    if s.state is None:
         return GatedGrads(*(torch.zeros_like(t) for t in (s.x, s.expert_weight, s.w_gate, s.w_up, s.w_down)))
-    t = s.topo
-    layout = [t.tokens_per_expert, t.padded_offsets, t.row_token, t.copy_row, t.row_block_expert, t.row_offsets]
-    return GatedGrads(*_C.gated_backward_cuda(grad_out, s.x, s.expert_weight, s.w_gate, s.w_up, s.w_down, s.h, s.g, s.u,
-                                              layout, s.activation))
+    return GatedGrads(*_C.moe_gated_backward_cuda(grad_out, s.x, s.expert_weight, s.w_gate, s.w_up, s.w_down, s.state,
+                                                  s.activation))
 
 
 class _GatedMoE(torch.autograd.Function):
@@ -130,7 +105,7 @@ class _GatedMoE(torch.autograd.Function):
     def forward(ctx, x, expert_idx, expert_weight, w_gate, w_up, w_down, activation):
         out, saved = moe_forward_gated_saved(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
         ctx.save_for_backward(x, expert_weight, w_gate, w_up, w_down)  # autograd checks them for in-place changes
-        ctx.rest = (activation, saved.topo, saved.h, saved.g, saved.u)
+        ctx.rest = (activation, saved.state)
         return out
 
     @staticmethod
@@ -139,8 +114,7 @@ class _GatedMoE(torch.autograd.Function):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the autograd form of the gated layer cannot be captured into a CUDA graph: "
                                "capture moe_forward_gated_saved and moe_backward_gated")
-        activation, topo, h, g, u = ctx.rest
-        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*ctx.saved_tensors, activation, topo, h, g, u))
+        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*ctx.saved_tensors, *ctx.rest))
         return grads.x, None, grads.expert_weight, grads.w_gate, grads.w_up, grads.w_down, None
 
 
