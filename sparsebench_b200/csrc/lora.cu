@@ -11,16 +11,20 @@
 //   expand   y = [x | V in its slot's columns, zeros elsewhere] [W ; B of the slots]: the second term is a few more K
 //            steps of the projection itself, so y is written once and never read back
 //
-// V is rounded to bf16 for y in bf16; for y in fp32 it travels as a pair of bf16 (V and what rounding took from it,
+// Up to 64 tokens (a decoding step) the weights are streamed by the kernel of skinny.cuh and the second term is plain
+// fp32 arithmetic on each token's own rows of A and B (lora_rows_kernel, SkinnyLora): no plan, no pairing of tokens.
+//
+// In the products V is rounded to bf16 for y in bf16; for y in fp32 it travels as a pair of bf16 (V and what rounding took from it,
 // against the same rows of B), 2^-17 of V off.
 //
-// A zero of V meets B of other requests' adapters there: an infinity or NaN in one adapter would reach its neighbours'
+// There a zero of V meets B of other requests' adapters: an infinity or NaN in one adapter would reach its neighbours'
 // rows. So an adapter whose B is not finite stays out of the product (plan finds it, reading B once, on its way into
 // L2) and its own rows get their term from the epilogue, number by number.
 
 #include <algorithm>
 #include <initializer_list>
 
+#include "skinny.cuh"
 #include "tile_gemm.cuh"
 
 namespace sb {
@@ -332,6 +336,174 @@ struct LoraExpand {
   }
 };
 
+// ---- a decoding step -----------------------------------------------------------------------------------------------
+
+// V[t, j] = scale[a] * x[t] . A[a, j] in fp32, one warp each; tokens without an adapter are left out here and later.
+template <typename index_t>
+__global__ void __launch_bounds__(256)
+lora_rows_kernel(const uint4* __restrict__ x, const uint4* __restrict__ a, const index_t* __restrict__ adapter_idx,
+                 const float* __restrict__ scale, float* __restrict__ v, int32_t num_adapters, int32_t rank, int32_t vecs) {
+  grid_launch_dependents();
+  const int32_t t = static_cast<int32_t>(blockIdx.x);
+  const int32_t j = static_cast<int32_t>(blockIdx.y) * 8 + static_cast<int32_t>(threadIdx.x >> 5);
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int64_t id = static_cast<int64_t>(__ldg(adapter_idx + t));
+  if (id < 0 || id >= num_adapters || j >= rank) return;
+  const uint4* xr = x + static_cast<int64_t>(t) * vecs;
+  const uint4* ar = a + (id * rank + j) * vecs;
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int32_t i = lane; i < vecs; i += 32) {
+    const uint4 xq = __ldg(xr + i);
+    const uint4 aq = __ldg(ar + i);
+    const __nv_bfloat162* xp = reinterpret_cast<const __nv_bfloat162*>(&xq);
+    const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&aq);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 xf = __bfloat1622float2(xp[q]);
+      const float2 af = __bfloat1622float2(ap[q]);
+      sum = fmaf(xf.x, af.x, sum);
+      sum = fmaf(xf.y, af.y, sum);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) v[static_cast<int64_t>(t) * rank + j] = scale != nullptr ? sum * __ldg(scale + id) : sum;
+}
+
+// y: 128 columns of x W by the tensor cores; the workers compute the adapters' term of their share of the tokens while
+// the weights stream (thread: 8 columns of every 8th token), and add it to the sums of the splits.
+template <int kPasses>
+struct SkinnyLora {
+  struct Params {
+    SkinnyShape shape;
+    const void* adapter_idx;
+    const float* v;
+    const __nv_bfloat16* b;
+    void* out;
+    int32_t idx_is_i64, num_tokens, num_adapters, rank, width, out_fp32;
+  };
+  struct Item { int32_t n0, rows; };
+  struct Extra { float y[kPasses][8]; };
+  static constexpr bool kGather = false;
+  static __device__ __forceinline__ bool begin(const Params& p, Item& item, int32_t block_item, int32_t*, int32_t*) {
+    item.n0 = block_item * kSkinnyCols;
+    item.rows = p.num_tokens;
+    return true;
+  }
+  static __device__ __forceinline__ void load_w(const SkinnyMaps& maps, const Params&, const Item& item, int32_t ks, uint32_t dst,
+                                                uint32_t bar) {
+    ptx::tma_load_2d(dst, &maps.w[0], item.n0, ks * kSkinnyStep, bar);
+    ptx::tma_load_2d(dst + kSkinnyWBytes / 2, &maps.w[0], item.n0 + 64, ks * kSkinnyStep, bar);
+  }
+  static __device__ __forceinline__ int32_t token(const Params& p, int32_t rank, int worker, int pass) {
+    return rank + p.shape.splits * (pass * 8 + (worker >> 4));
+  }
+  static __device__ __forceinline__ void extra(const Params& p, const Item& item, int32_t rank, int worker, Extra& e) {
+    const int32_t col = item.n0 + (worker & 15) * 8;
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) e.y[pass][q] = 0.0f;
+      const int32_t t = token(p, rank, worker, pass);
+      if (t >= p.num_tokens || col >= p.width) continue;
+      const int64_t a = p.idx_is_i64 ? __ldg(static_cast<const long long*>(p.adapter_idx) + t)
+                                     : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.adapter_idx) + t));
+      if (a < 0 || a >= p.num_adapters) continue;
+      const uint4* b = reinterpret_cast<const uint4*>(p.b + a * p.rank * p.width + col);
+      const float* v = p.v + static_cast<int64_t>(t) * p.rank;
+      const int32_t stride = p.width / 8;
+      for (int32_t j = 0; j < p.rank; j += 8) {
+        uint4 raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = __ldg(b + static_cast<int64_t>(j + i) * stride);
+        float f[8];
+        *reinterpret_cast<float4*>(f) = __ldcg(reinterpret_cast<const float4*>(v + j));
+        *reinterpret_cast<float4*>(f + 4) = __ldcg(reinterpret_cast<const float4*>(v + j + 4));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162* pair = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 bf = __bfloat1622float2(pair[q]);
+            e.y[pass][2 * q] = fmaf(f[i], bf.x, e.y[pass][2 * q]);
+            e.y[pass][2 * q + 1] = fmaf(f[i], bf.y, e.y[pass][2 * q + 1]);
+          }
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ void finish(const Params& p, const Item& item, const int32_t*, int32_t rank, int worker,
+                                                const SkinnySums& red, const Extra& e) {
+    const int32_t c = (worker & 15) * 8;
+    if (item.n0 + c >= p.width) return;
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+      const int32_t t = token(p, rank, worker, pass);
+      if (t >= p.num_tokens) break;
+      float v[8];
+      red.sum(t, c, v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += e.y[pass][q];
+      const int64_t at = static_cast<int64_t>(t) * p.width + item.n0 + c;
+      if (p.out_fp32) {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+      }
+    }
+  }
+};
+
+template <int kPasses>
+int launch_lora_small(const SkinnyMaps& maps, const SkinnyShape& shape, const void* adapter_idx, int idx_is_i64, const float* v,
+                      const void* lora_b, void* out, int out_fp32, int32_t num_tokens, int32_t width, int32_t rank,
+                      int32_t num_adapters, int64_t items, int32_t* dev_status, cudaStream_t stream) {
+  typename SkinnyLora<kPasses>::Params p{};
+  p.shape = shape;
+  p.adapter_idx = adapter_idx;
+  p.v = v;
+  p.b = static_cast<const __nv_bfloat16*>(lora_b);
+  p.out = out;
+  p.idx_is_i64 = idx_is_i64;
+  p.num_tokens = num_tokens;
+  p.num_adapters = num_adapters;
+  p.rank = rank;
+  p.width = width;
+  p.out_fp32 = out_fp32;
+  return launch_skinny<SkinnyLora<kPasses>>(maps, p, items, true, dev_status, stream, "lora_linear (small)");
+}
+
+int lora_small(const void* x, const void* weight, const void* lora_a, const void* lora_b, const void* adapter_idx,
+               int idx_is_i64, const float* scale, void* out, int out_fp32, int32_t num_tokens, int32_t d_model, int32_t width,
+               int32_t rank, int32_t num_adapters, float* v, const DeviceInfo* info, int32_t* dev_status, cudaStream_t stream) {
+  const int64_t items = (width + kSkinnyCols - 1) / kSkinnyCols;
+  const SkinnyShape shape = skinny_shape(items, (d_model + kSkinnyStep - 1) / kSkinnyStep, num_tokens, info->sm_count);
+  SkinnyMaps maps{};
+  if (int rc = encode_2d_map(&maps.w[0], weight, d_model, width, 64, 64, 2, "lora_linear (weight)")) return rc;
+  if (int rc = encode_2d_map(&maps.x, x, num_tokens, d_model, shape.rows_pad, 64, 2, "lora_linear (x)")) return rc;
+  const dim3 grid(static_cast<unsigned>(num_tokens), static_cast<unsigned>((rank + 7) / 8));
+  if (idx_is_i64)
+    lora_rows_kernel<long long><<<grid, 256, 0, stream>>>(static_cast<const uint4*>(x), static_cast<const uint4*>(lora_a),
+        static_cast<const long long*>(adapter_idx), scale, v, num_adapters, rank, d_model / 8);
+  else
+    lora_rows_kernel<int32_t><<<grid, 256, 0, stream>>>(static_cast<const uint4*>(x), static_cast<const uint4*>(lora_a),
+        static_cast<const int32_t*>(adapter_idx), scale, v, num_adapters, rank, d_model / 8);
+  if (int rc = check_launch("lora_linear (rows)")) return rc;
+  const int32_t per_rank = (num_tokens + shape.splits - 1) / shape.splits;  // tokens of a block, 8 at a time
+#define SB_LORA_SMALL(PASSES)                                                                                               \
+  launch_lora_small<PASSES>(maps, shape, adapter_idx, idx_is_i64, v, lora_b, out, out_fp32, num_tokens, width, rank,         \
+                            num_adapters, items, dev_status, stream)
+  if (per_rank <= 8) return SB_LORA_SMALL(1);
+  if (per_rank <= 16) return SB_LORA_SMALL(2);
+  if (per_rank <= 32) return SB_LORA_SMALL(4);
+  return SB_LORA_SMALL(8);
+#undef SB_LORA_SMALL
+}
+
 struct LoraSizes {
   int64_t row_tiles, tables, not_finite, partial, v, total;  // bytes of each part, 256-byte aligned, then all
   int32_t splits, steps, total_steps, parts;
@@ -341,6 +513,11 @@ int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
 LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t rank, int32_t num_adapters, int out_fp32, int sm_count) {
   LoraSizes s{};
+  if (num_tokens <= kSkinnyMaxRows) {
+    s.v = align256(num_tokens * rank * 4);
+    s.total = s.v;
+    return s;
+  }
   s.row_tiles = (num_tokens + kTileRows - 1) / kTileRows;
   s.parts = out_fp32 ? 2 : 1;
   s.total_steps = (d_model + kTileStep - 1) / kTileStep;
@@ -400,6 +577,9 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
     return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: the workspace has %lld bytes, %lld are needed",
                 (long long)workspace_bytes, (long long)s.total);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (num_tokens <= kSkinnyMaxRows)
+    return lora_small(x, weight, lora_a, lora_b, adapter_idx, idx_is_i64, scale, out, out_fp32, static_cast<int32_t>(num_tokens),
+                      d_model, width, rank, num_adapters, reinterpret_cast<float*>(ws), info, dev_status, as_stream(stream));
   int32_t* tables = reinterpret_cast<int32_t*>(ws);
   uint8_t* not_finite = ws + s.tables;
   float* partial = reinterpret_cast<float*>(not_finite + s.not_finite);
