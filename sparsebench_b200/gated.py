@@ -41,13 +41,15 @@ class GatedGrads(NamedTuple):
 
 
 def _check_shapes(x, expert_idx, expert_weight, w_gate, w_up, w_down) -> None:
-    if w_gate.dim() != 3 or w_up.shape != w_gate.shape:
-        raise ValueError(f"w_gate and w_up must be [E, D, F], got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
-    num_experts, d_model, ffn_dim = w_gate.shape
-    if w_down.shape != (num_experts, ffn_dim, d_model):
+    shape = w_gate.shape
+    if len(shape) != 3 or w_up.shape != shape:
+        raise ValueError(f"w_gate and w_up must be [E, D, F], got {tuple(shape)} and {tuple(w_up.shape)}")
+    num_experts, d_model, ffn_dim = shape
+    if tuple(w_down.shape) != (num_experts, ffn_dim, d_model):
         raise ValueError(f"w_down must be {(num_experts, ffn_dim, d_model)}, got {tuple(w_down.shape)}")
-    if (x.dim() != 2 or x.shape[1] != d_model or expert_idx.dim() != 2 or expert_idx.shape != expert_weight.shape
-            or expert_idx.shape[0] != x.shape[0]):
+    x_shape, idx_shape = x.shape, expert_idx.shape
+    if (len(x_shape) != 2 or x_shape[1] != d_model or len(idx_shape) != 2 or idx_shape != expert_weight.shape
+            or idx_shape[0] != x_shape[0]):
         raise ValueError("x must be [T, D] and expert_idx / expert_weight [T, k]")
 
 
