@@ -408,7 +408,7 @@ int sb_ep_sdd_dispatch(const void* recv_rows, const void* w1, const int32_t* row
  * then written (padding rows as zeros). Without them skip_padding_rows works as in sb_sdd.
  *
  * sb_moe_gated_bytes: bytes[0] of the state, bytes[1] of the forward's scratch, bytes[2] of the backward's; keep = 0: for
- * a forward pass alone (no state). Nothing in these buffers has to be set.
+ * a forward pass alone (no state). Nothing in these buffers has to be set; they are 256-byte aligned.
  *
  * sb_moe_gated_forward: out[t] = sum_j gate[t, j] * (act(x[t] . w_gate[e]) * (x[t] . w_up[e])) . w_down[e],
  * e = expert_idx[t, j] (int32 or int64 [T, k]). With state (not NULL) it holds afterwards what the backward pass needs:

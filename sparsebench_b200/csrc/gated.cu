@@ -34,13 +34,15 @@ __device__ __forceinline__ float fast_rcp(float v) {
 // exp(-v) overflows to inf below v = -88: the reciprocal is then 0, the limit.
 __device__ __forceinline__ float sigmoid(float v) { return fast_rcp(1.0f + __expf(-v)); }
 
-__device__ __forceinline__ float act_value(float v, int32_t activation) {
-  return activation == 0 ? v * sigmoid(v) : gelu_erf(v);
+template <int kActivation>
+__device__ __forceinline__ float act_value(float v) {
+  return kActivation == SB_ACT_SILU ? v * sigmoid(v) : gelu_erf(v);
 }
 
 // act(v) and its derivative.
-__device__ __forceinline__ void act_and_slope(float v, int32_t activation, float* value, float* slope) {
-  if (activation == 0) {
+template <int kActivation>
+__device__ __forceinline__ void act_and_slope(float v, float* value, float* slope) {
+  if (kActivation == SB_ACT_SILU) {
     const float s = sigmoid(v);
     *value = v * s;
     *slope = s * fmaf(v, 1.0f - s, 1.0f);
@@ -87,7 +89,8 @@ struct GatedUp {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr bool kVariable = false, kStepGather = false, kGather = true, kAMnMajor = false, kBMnMajor = true;
+  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kVariable = false, kExtension = false, kGather = true, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -118,20 +121,8 @@ struct GatedUp {
     if (p.keep) return {half_has_rows(p.row_token, t.row_block, w.quarter)};
     return {!p.skip_padding || __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32) >= 0};
   }
-  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
-                                                  const Early& early) {
-    if (!early.store) return;
-    const int32_t col = w.half * 64;
-    const int32_t row = (t.first_block + (t.n0 >> 7)) * kTileRows + w.quarter * 32;
-    const uint32_t gate = w.taddr + w.half * 64;
-    const uint32_t up = gate + 128;
-    uint32_t packed[32];
-    if (p.keep) {
-      load_packed_x64(gate, packed);
-      store_rows_128b(w, &maps.m[3], packed, col, row);
-      load_packed_x64(up, packed);
-      store_rows_128b(w, &maps.m[4], packed, col, row);
-    }
+  template <int kActivation>
+  static __device__ __forceinline__ void product(uint32_t gate, uint32_t up, uint32_t (&packed)[32]) {
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
       uint32_t g[32], u[32];
@@ -141,17 +132,35 @@ struct GatedUp {
 #pragma unroll
       for (int h = 0; h < 16; ++h)
         packed[part * 16 + h] =
-            pack_bf16(act_value(__uint_as_float(g[2 * h]), p.activation) * __uint_as_float(u[2 * h]),
-                      act_value(__uint_as_float(g[2 * h + 1]), p.activation) * __uint_as_float(u[2 * h + 1]));
+            pack_bf16(act_value<kActivation>(__uint_as_float(g[2 * h])) * __uint_as_float(u[2 * h]),
+                      act_value<kActivation>(__uint_as_float(g[2 * h + 1])) * __uint_as_float(u[2 * h + 1]));
     }
-    store_rows_128b(w, &maps.m[2], packed, col, row);
+  }
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, EpilogueWarp& w,
+                                                  const Early& early) {
+    if (!early.store) return;
+    const int32_t col = w.half * 64;
+    const int32_t row = (t.first_block + (t.n0 >> 7)) * kTileRows + w.quarter * 32;
+    const uint32_t gate = w.taddr + w.half * 64;
+    const uint32_t up = gate + 128;
+    uint32_t packed[32];
+    if (p.keep) {
+      load_packed_x64(gate, packed);
+      store_rows_128b<kBuffers>(w, &maps.m[3], packed, col, row);
+      load_packed_x64(up, packed);
+      store_rows_128b<kBuffers>(w, &maps.m[4], packed, col, row);
+    }
+    if (p.activation == SB_ACT_SILU) product<SB_ACT_SILU>(gate, up, packed);
+    else product<SB_ACT_GELU>(gate, up, packed);
+    store_rows_128b<kBuffers>(w, &maps.m[2], packed, col, row);
   }
 };
 
 // ---- backward: gradients of G, U and of the gates -----------------------------------------------------------------
-// S = dO Wd^T over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. The epilogue reads G and U of
-// its own row (32 columns at a time, the next 32 on their way while the current ones are worked on) and leaves dG, dU
-// and, per row and 128 columns, its share of dgate, summed in a fixed order by the join kernel.
+// S = dO Wd^T over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. In the epilogue a lane has a row
+// to itself: it reads G and U and writes dG and dU a sector (16 columns) at a time, two sectors ahead of the one it works
+// on, and leaves per row and 128 columns its share of dgate, summed in a fixed order by the join kernel. Staging the
+// results for TMA stores instead made the warps wait for their 4 KB tile at every step.
 struct GradHidden {
   struct Params {
     BandOrder order;
@@ -162,10 +171,13 @@ struct GradHidden {
     const __nv_bfloat16* g;
     const __nv_bfloat16* u;
     const float* row_gate;
+    __nv_bfloat16* dg;
+    __nv_bfloat16* du;
     float* gate_partial;  // [rows, F / 128]
     int32_t d_model, ffn_dim;
     int32_t activation;
   };
+  static constexpr int kPart = 16;  // columns at a time: 32 bytes of a row, one sector
   struct Tile {
     int32_t k_steps, row_block, n0, expert, first_block;
     bool live;
@@ -173,11 +185,13 @@ struct GradHidden {
   struct Early {
     bool store, real;
     float gate;
-    const uint4* g;  // this row's 128 columns
-    const uint4* u;
-    uint4 g0[4], u0[4];
+    const __nv_bfloat16* g;  // this row's 128 columns, as U's and the results' are
+    const __nv_bfloat16* u;
+    int64_t at;
+    uint32_t first[2][2][8];  // G and U of the first two parts
   };
-  static constexpr bool kVariable = false, kStepGather = false, kGather = true, kAMnMajor = false, kBMnMajor = false;
+  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kVariable = false, kExtension = false, kGather = true, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -202,13 +216,6 @@ struct GradHidden {
     const int32_t token = __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + row);
     return token >= 0 ? p.grad_out + static_cast<int64_t>(token) * p.d_model : nullptr;
   }
-  static __device__ __forceinline__ void fetch(const Early& e, int part, uint4 (&g)[4], uint4 (&u)[4]) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      g[c] = __ldg(e.g + part * 4 + c);
-      u[c] = __ldg(e.u + part * 4 + c);
-    }
-  }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
     Early e;
     const int32_t n = t.n0 + w.half * 128;
@@ -217,43 +224,55 @@ struct GradHidden {
     e.gate = 0.0f;
     if (!e.store) return e;
     const int64_t row = static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane;
+    e.at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128;
+    e.g = p.g + e.at;
+    e.u = p.u + e.at;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      ptx::ld_global_v8(e.g + part * kPart, e.first[part][0]);
+      ptx::ld_global_v8(e.u + part * kPart, e.first[part][1]);
+    }
     e.real = __ldg(p.row_token + row) >= 0;
     e.gate = __ldg(p.row_gate + row);
-    const int64_t at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128;
-    e.g = reinterpret_cast<const uint4*>(p.g + at);
-    e.u = reinterpret_cast<const uint4*>(p.u + at);
-    fetch(e, 0, e.g0, e.u0);
     return e;
   }
-  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+  static __device__ __forceinline__ void epilogue(const TileMaps&, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
     if (!early.store) return;
+    if (p.activation == SB_ACT_SILU) work<SB_ACT_SILU>(p, t, w, early);
+    else work<SB_ACT_GELU>(p, t, w, early);
+  }
+  template <int kActivation>
+  static __device__ __forceinline__ void work(const Params& p, const Tile& t, const EpilogueWarp& w, const Early& early) {
     const int32_t n = t.n0 + w.half * 128;
-    const int32_t out_row = (t.first_block + (n >> 7)) * kTileRows + w.quarter * 32;
-    // Two 32 x 32 pieces of 64-byte rows share the staging tile: dG in front, dU behind (64-byte swizzle).
-    const uint32_t swz = static_cast<uint32_t>((w.lane >> 1) & 3);
-    const uint32_t dst = w.staging + static_cast<uint32_t>(w.lane) * 64u;
-    uint4 gq[4], uq[4];
+    __nv_bfloat16* dg_row = p.dg + early.at;
+    __nv_bfloat16* du_row = p.du + early.at;
+    uint32_t held[3][2][8];  // G and U of this part and the next two
 #pragma unroll
-    for (int c = 0; c < 4; ++c) { gq[c] = early.g0[c]; uq[c] = early.u0[c]; }
+    for (int q = 0; q < 8; ++q) {
+      held[0][0][q] = early.first[0][0][q];
+      held[0][1][q] = early.first[0][1][q];
+      held[1][0][q] = early.first[1][0][q];
+      held[1][1][q] = early.first[1][1][q];
+    }
     float dgate = 0.0f;
 #pragma unroll
-    for (int part = 0; part < 4; ++part) {
-      uint32_t s[32];
-      ptx::tmem_ld_32x32b_x32(w.taddr + w.half * 128 + part * 32, s);
-      uint4 gn[4], un[4];
-      if (part < 3) fetch(early, part + 1, gn, un);
+    for (int part = 0; part < 128 / kPart; ++part) {
+      uint32_t s[16];
+      ptx::tmem_ld_32x32b_x16(w.taddr + w.half * 128 + part * kPart, s);
+      if (part + 2 < 128 / kPart) {
+        ptx::ld_global_v8(early.g + (part + 2) * kPart, held[(part + 2) % 3][0]);
+        ptx::ld_global_v8(early.u + (part + 2) * kPart, held[(part + 2) % 3][1]);
+      }
       ptx::tmem_ld_wait();
-      uint32_t dg[16], du[16];
+      uint32_t dg[8], du[8];
 #pragma unroll
-      for (int h = 0; h < 16; ++h) {
-        const uint32_t graw = reinterpret_cast<const uint32_t*>(gq)[h];
-        const uint32_t uraw = reinterpret_cast<const uint32_t*>(uq)[h];
-        const float2 gf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&graw));
-        const float2 uf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&uraw));
+      for (int h = 0; h < 8; ++h) {
+        const float2 gf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[part % 3][0][h]));
+        const float2 uf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[part % 3][1][h]));
         float a0, a1, d0, d1;
-        act_and_slope(gf.x, p.activation, &a0, &d0);
-        act_and_slope(gf.y, p.activation, &a1, &d1);
+        act_and_slope<kActivation>(gf.x, &a0, &d0);
+        act_and_slope<kActivation>(gf.y, &a1, &d1);
         const float s0 = __uint_as_float(s[2 * h]);
         const float s1 = __uint_as_float(s[2 * h + 1]);
         dgate = fmaf(a0 * uf.x, s0, dgate);
@@ -263,22 +282,8 @@ struct GradHidden {
         dg[h] = early.real ? pack_bf16(h0 * uf.x * d0, h1 * uf.y * d1) : 0u;
         du[h] = early.real ? pack_bf16(h0 * a0, h1 * a1) : 0u;
       }
-      if (w.lane == 0) ptx::bulk_wait_read();
-      __syncwarp();
-#pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) {
-        ptx::st_shared_v4(dst + ((c ^ swz) << 4), dg[4 * c], dg[4 * c + 1], dg[4 * c + 2], dg[4 * c + 3]);
-        ptx::st_shared_v4(dst + 2048u + ((c ^ swz) << 4), du[4 * c], du[4 * c + 1], du[4 * c + 2], du[4 * c + 3]);
-      }
-      ptx::fence_proxy_async_shared();
-      __syncwarp();
-      if (w.lane == 0) {
-        ptx::tma_store_2d(&maps.m[1], w.staging, part * 32, out_row);
-        ptx::tma_store_2d(&maps.m[2], w.staging + 2048u, part * 32, out_row);
-        ptx::bulk_commit();
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) { gq[c] = gn[c]; uq[c] = un[c]; }
+      ptx::st_global_v8(dg_row + part * kPart, dg);
+      ptx::st_global_v8(du_row + part * kPart, du);
     }
     if (early.real)
       p.gate_partial[(static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane) * (p.ffn_dim / 128) + (n >> 7)] = dgate;
@@ -300,7 +305,8 @@ struct GradRows {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr bool kVariable = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kVariable = false, kExtension = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -326,7 +332,7 @@ struct GradRows {
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
     return {__ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32) >= 0};
   }
-  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
     if (!early.store) return;
 #pragma unroll 1
@@ -335,7 +341,7 @@ struct GradRows {
       if (col >= p.d_model) break;
       uint32_t packed[32];
       load_packed_x64(w.taddr + w.half * 128 + g * 64, packed);
-      store_rows_128b(w, &maps.m[4], packed, col, t.row_block * kTileRows + w.quarter * 32);
+      store_rows_128b<kBuffers>(w, &maps.m[4], packed, col, t.row_block * kTileRows + w.quarter * 32);
     }
   }
 };
@@ -358,7 +364,8 @@ struct GradWeights {
     bool live;
   };
   struct Early {};
-  static constexpr bool kVariable = false, kGather = false, kAMnMajor = true, kBMnMajor = true;
+  static constexpr int kStages = 3, kBuffers = 2;
+  static constexpr bool kVariable = false, kExtension = false, kGather = false, kAMnMajor = true, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) {
     return p.num_experts * (p.down_tiles + 2 * p.up_tiles);
@@ -409,7 +416,7 @@ struct GradWeights {
     }
   }
   static __device__ __forceinline__ Early prefetch(const Params&, const Tile&, const EpilogueWarp&) { return {}; }
-  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early&) {
     const int32_t width = t.which == 0 ? p.d_model : p.ffn_dim;
     const int32_t row = t.expert * (t.which == 0 ? p.ffn_dim : p.d_model) + t.m0 + w.quarter * 32;
@@ -424,7 +431,7 @@ struct GradWeights {
 #pragma unroll
         for (int h = 0; h < 32; ++h) packed[h] = 0u;
       }
-      store_rows_128b(w, &maps.m[5 + t.which], packed, col, row);
+      store_rows_128b<kBuffers>(w, &maps.m[5 + t.which], packed, col, row);
     }
   }
 };
@@ -505,7 +512,9 @@ struct SkinnyUp {
       uint32_t packed[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        packed[q] = pack_bf16(act_value(g[2 * q], p.activation) * u[2 * q], act_value(g[2 * q + 1], p.activation) * u[2 * q + 1]);
+        packed[q] = p.activation == SB_ACT_SILU
+                        ? pack_bf16(act_value<SB_ACT_SILU>(g[2 * q]) * u[2 * q], act_value<SB_ACT_SILU>(g[2 * q + 1]) * u[2 * q + 1])
+                        : pack_bf16(act_value<SB_ACT_GELU>(g[2 * q]) * u[2 * q], act_value<SB_ACT_GELU>(g[2 * q + 1]) * u[2 * q + 1]);
       *reinterpret_cast<uint4*>(p.h + static_cast<int64_t>(list[r]) * p.ffn_dim + item.tile * 64 + c) =
           make_uint4(packed[0], packed[1], packed[2], packed[3]);
     }
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(128)
 gated_small_combine_kernel(const float4* __restrict__ y, const void* __restrict__ expert_idx, int idx_is_i64,
                            const void* __restrict__ gate, int gate_dtype, uint2* __restrict__ out, int32_t k,
                            int32_t num_experts, int32_t quads) {
-  grid_dependency_wait();
+  ptx::grid_dependency_wait();
   const int32_t t = static_cast<int32_t>(blockIdx.y);
   const int32_t v = static_cast<int32_t>(blockIdx.x) * 128 + static_cast<int32_t>(threadIdx.x);
   if (v >= quads) return;
@@ -592,6 +601,7 @@ gated_gather_kernel(const uint4* __restrict__ x, const uint4* __restrict__ grad_
                     int gate_dtype, const int32_t* __restrict__ row_token, const int32_t* __restrict__ copy_row,
                     const int32_t* __restrict__ num_rows, uint4* __restrict__ x_rows, uint4* __restrict__ grad_rows,
                     float* __restrict__ row_gate, int32_t k, int32_t vecs) {
+  ptx::grid_launch_dependents();
   const int lane = static_cast<int>(threadIdx.x & 31);
   const int32_t rows = __ldg(num_rows);
   const int32_t warps = static_cast<int32_t>(gridDim.x * (kSmallThreads / 32));
@@ -785,11 +795,8 @@ int gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_bl
   if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: T must be positive");
   if (any_misaligned({grad_out, w_down, g_blocks, u_blocks, dg_blocks, du_blocks}))
     return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: buffers must be 16-byte aligned");
-  const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
   TileMaps maps{};
   if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, 256, 64, 2, "gated_grad_hidden (w_down)")) return rc;
-  if (int rc = encode_2d_map(&maps.m[1], dg_blocks, b_rows, 128, 32, 32, 2, "gated_grad_hidden (dG)")) return rc;
-  if (int rc = encode_2d_map(&maps.m[2], du_blocks, b_rows, 128, 32, 32, 2, "gated_grad_hidden (dU)")) return rc;
   GradHidden::Params p{};
   const int32_t slices = (ffn_dim + kTileCols - 1) / kTileCols;
   p.order = {num_row_blocks, slices, band_for(num_row_blocks, num_experts)};
@@ -800,6 +807,8 @@ int gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_bl
   p.g = static_cast<const __nv_bfloat16*>(g_blocks);
   p.u = static_cast<const __nv_bfloat16*>(u_blocks);
   p.row_gate = row_gate;
+  p.dg = static_cast<__nv_bfloat16*>(dg_blocks);
+  p.du = static_cast<__nv_bfloat16*>(du_blocks);
   p.gate_partial = gate_partial;
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
@@ -896,6 +905,7 @@ int gated_join(const void* dx_rows, const float* gate_partial, const int32_t* co
   return check_launch("gated_join");
 }
 
+bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
 int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
 // The two ways of the forward pass. The decoding way needs no layout and splits K over clusters; it starts a block per
@@ -1066,8 +1076,8 @@ extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int i
   if (int rc = gated_buffers(num_tokens, k, d_model, ffn_dim, num_experts, keep, &b)) return rc;
   if (int rc = check_gated("moe_gated", d_model, ffn_dim, num_experts, b.row_blocks, activation)) return rc;
   if (any_null({x, expert_idx, gate, w_gate, w_up, w_down, out, scratch})) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: NULL buffer");
-  if (any_misaligned({x, w_gate, w_up, w_down, out, state, scratch}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: buffers must be 16-byte aligned");
+  if (any_misaligned({x, w_gate, w_up, w_down, out}) || !aligned256(state) || !aligned256(scratch))
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: buffers must be 16-byte aligned, state and scratch 256-byte aligned");
   if (gate_dtype != 0 && gate_dtype != 1) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: gate_dtype must be 0 (bf16) or 1 (fp32)");
   if ((keep && state_bytes < b.state_bytes) || scratch_bytes < b.scratch_bytes)
     return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated: the buffers have %lld and %lld bytes, %lld and %lld are needed",
@@ -1105,7 +1115,8 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* x, const 
   if (int rc = gated_buffers(num_tokens, k, d_model, ffn_dim, num_experts, 1, &b)) return rc;
   if (any_null({grad_out, x, gate, w_gate, w_up, w_down, state, dx, dgate, dw_gate, dw_up, dw_down, scratch}))
     return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: NULL buffer");
-  if (any_misaligned({state, scratch})) return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: buffers must be 16-byte aligned");
+  if (!aligned256(state) || !aligned256(scratch))
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: state and scratch must be 256-byte aligned");
   if (state_bytes < b.state_bytes || scratch_bytes < b.backward_bytes)
     return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: the buffers have %lld and %lld bytes, %lld and %lld are needed",
                 (long long)state_bytes, (long long)scratch_bytes, (long long)b.state_bytes, (long long)b.backward_bytes);

@@ -31,21 +31,28 @@ namespace sb {
 namespace {
 
 constexpr int kMaxSlots = kTileRows;
-constexpr int kTableInts = 1 + kMaxSlots + kTileRows;  // slot count, adapter of each slot, slot of each row (-1: none)
-constexpr int kScanParts = 16;                         // each used adapter's B is read by so many thread blocks
+// Per tile: the slot count, the adapter of each slot, the slot of each row (-1: none), and again the adapter of each slot,
+// or -1 where its B is not finite.
+constexpr int kSlotAdapter = 1, kRowSlot = kSlotAdapter + kMaxSlots, kSlotShared = kRowSlot + kTileRows;
+constexpr int kTableInts = kSlotShared + kMaxSlots;
 constexpr int kPlanThreads = 256;
 
 // ---- plan ---------------------------------------------------------------------------------------------------------
 
+// Block (tile, part): the tile's slots; part 0 writes them down, and every part looks through its part of the B of those
+// of the tile's adapters that the tile before does not have (they are being looked through there, or further up). For a
+// batch of whole requests that is once per request; in any order it is at most what expand reads of B anyway. Tiles that
+// share an adapter write the same answer.
 template <typename index_t>
 __global__ void __launch_bounds__(kPlanThreads)
 lora_plan_kernel(const index_t* __restrict__ adapter_idx, const uint4* __restrict__ b, int32_t* __restrict__ tables,
-                 uint8_t* __restrict__ not_finite, int32_t num_tokens, int32_t num_adapters, int64_t vecs_per_adapter) {
-  __shared__ int32_t id[kTileRows];
+                 uint8_t* __restrict__ not_finite, int32_t num_tokens, int32_t num_adapters, int32_t vecs_per_adapter) {
+  __shared__ alignas(16) int32_t id[kTileRows];
   __shared__ int32_t slot_adapter[kMaxSlots];
   __shared__ int32_t slot_of_first[kTileRows];
   __shared__ int32_t warp_count[4];
   __shared__ int32_t seen[kMaxSlots];
+  ptx::grid_launch_dependents();
   const int i = static_cast<int>(threadIdx.x);
   const int32_t first_token = static_cast<int32_t>(blockIdx.x) * kTileRows;
   int32_t mine = -1;
@@ -59,12 +66,16 @@ lora_plan_kernel(const index_t* __restrict__ adapter_idx, const uint4* __restric
   }
   __syncthreads();
   int first = i;
-  bool leads = false;
   if (i < kTileRows && mine >= 0) {
-    for (int j = 0; j < i; ++j)
-      if (id[j] == mine) { first = j; break; }
-    leads = first == i;
+    for (int j = 0; j < i; j += 4) {
+      const int4 four = *reinterpret_cast<const int4*>(id + j);
+      if (four.x == mine) { first = j; break; }
+      if (four.y == mine) { first = j + 1; break; }
+      if (four.z == mine) { first = j + 2; break; }
+      if (four.w == mine) { first = j + 3; break; }
+    }
   }
+  const bool leads = i < kTileRows && mine >= 0 && first == i;  // first never lies behind i: id[i] itself matches
   const unsigned ballot = __ballot_sync(0xffffffffu, leads);
   if (i < kTileRows && (i & 31) == 0) warp_count[i >> 5] = __popc(ballot);
   __syncthreads();
@@ -82,26 +93,26 @@ lora_plan_kernel(const index_t* __restrict__ adapter_idx, const uint4* __restric
   if (blockIdx.y == 0) {
     int32_t* table = tables + static_cast<int64_t>(blockIdx.x) * kTableInts;
     if (i == 0) table[0] = slots;
-    if (i < slots) table[1 + i] = slot_adapter[i];
-    if (i < kTileRows) table[1 + kMaxSlots + i] = mine >= 0 ? slot_of_first[first] : -1;
+    if (i < slots) table[kSlotAdapter + i] = slot_adapter[i];
+    if (i < kTileRows) table[kRowSlot + i] = mine >= 0 ? slot_of_first[first] : -1;
   }
-  // A tile looks through the B of those of its adapters that the tile before does not have (they are being looked
-  // through there, or further up); block y takes the y-th part. For a batch of whole requests that is once per request;
-  // in any order it is at most what expand reads of B anyway. Tiles that share an adapter write the same answer.
   if (i < kTileRows && first_token > 0) {
     const int64_t a = static_cast<int64_t>(__ldg(adapter_idx + first_token - kTileRows + i));
     for (int32_t s = 0; s < slots; ++s)
       if (slot_adapter[s] == a) seen[s] = 1;
   }
   __syncthreads();
+  const int32_t parts = static_cast<int32_t>(gridDim.y);
+  const int32_t per_part = (vecs_per_adapter + parts - 1) / parts;
+  const int32_t begin = static_cast<int32_t>(blockIdx.y) * per_part;
+  const int32_t end = min(vecs_per_adapter, begin + per_part);
   for (int32_t s = 0; s < slots; ++s) {
     if (seen[s] != 0) continue;
     const int32_t a = slot_adapter[s];
     const uint4* rows = b + static_cast<int64_t>(a) * vecs_per_adapter;
-    const int64_t per_part = (vecs_per_adapter + kScanParts - 1) / kScanParts;
-    const int64_t end = min(vecs_per_adapter, (static_cast<int64_t>(blockIdx.y) + 1) * per_part);
     bool bad = false;
-    for (int64_t v = static_cast<int64_t>(blockIdx.y) * per_part + i; v < end; v += kPlanThreads) {
+#pragma unroll 4
+    for (int32_t v = begin + i; v < end; v += kPlanThreads) {
       const uint4 raw = __ldg(rows + v);
       const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
@@ -109,13 +120,8 @@ lora_plan_kernel(const index_t* __restrict__ adapter_idx, const uint4* __restric
         bad |= (words[q] & 0x7f80u) == 0x7f80u || (words[q] & 0x7f800000u) == 0x7f800000u;
     }
     const int any = __syncthreads_or(bad);
-    if (i == 0) not_finite[static_cast<int64_t>(a) * kScanParts + blockIdx.y] = any ? 1 : 0;
+    if (i == 0) not_finite[static_cast<int64_t>(a) * parts + blockIdx.y] = any ? 1 : 0;
   }
-}
-
-__device__ __forceinline__ bool adapter_finite(const uint8_t* not_finite, int32_t adapter) {
-  const uint4 f = __ldg(reinterpret_cast<const uint4*>(not_finite) + adapter);  // kScanParts bytes
-  return (f.x | f.y | f.z | f.w) == 0u;
 }
 
 // ---- shrink -------------------------------------------------------------------------------------------------------
@@ -132,7 +138,8 @@ struct LoraShrink {
     bool live;
   };
   struct Early { int32_t slot; };
-  static constexpr bool kVariable = true, kGather = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kVariable = true, kExtension = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.row_tiles * p.groups * p.splits; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -145,7 +152,7 @@ struct LoraShrink {
     const int32_t* table = p.tables + static_cast<int64_t>(t.row_tile) * kTableInts;
     t.first_slot = group * p.group_slots;
     t.slots = min(p.group_slots, __ldg(table) - t.first_slot);
-    t.adapters = table + 1 + t.first_slot;
+    t.adapters = table + kSlotAdapter + t.first_slot;
     t.step0 = t.split * p.steps;
     t.live = t.slots > 0;
     t.k_steps = t.live ? min(p.steps, p.total_steps - t.step0) : 0;
@@ -163,9 +170,9 @@ struct LoraShrink {
       ptx::tma_load_2d(b + static_cast<uint32_t>(s * p.rank) * 128u, &maps.m[1], k, __ldg(t.adapters + s) * p.rank, bar);
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
-    return {__ldg(p.tables + static_cast<int64_t>(t.row_tile) * kTableInts + 1 + kMaxSlots + w.quarter * 32 + w.lane)};
+    return {__ldg(p.tables + static_cast<int64_t>(t.row_tile) * kTableInts + kRowSlot + w.quarter * 32 + w.lane)};
   }
-  static __device__ __forceinline__ void epilogue(const TileMaps&, const Params& p, const Tile& t, const EpilogueWarp& w,
+  static __device__ __forceinline__ void epilogue(const TileMaps&, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
     const int32_t token = t.row_tile * kTileRows + w.quarter * 32 + w.lane;
     float* dst = p.partial + (static_cast<int64_t>(t.split) * p.num_tokens + token) * p.rank;
@@ -186,21 +193,35 @@ struct LoraShrink {
 };
 
 // V[t] = scale * sum over the parts, in order, as one bf16 (parts = 1) or as a pair (parts = 2: r values, then r
-// remainders). Tokens without an adapter are not read later and not written.
+// remainders). Tokens without an adapter are not read later and not written. Also the last column of the tables.
 template <typename index_t>
 __global__ void __launch_bounds__(256)
 lora_join_kernel(const float* __restrict__ partial, const index_t* __restrict__ adapter_idx, const float* __restrict__ scale,
                  __nv_bfloat16* __restrict__ v, int32_t num_tokens, int32_t num_adapters, int32_t rank, int32_t splits,
-                 int32_t parts) {
+                 int32_t parts, int32_t* __restrict__ tables, const uint8_t* __restrict__ not_finite, int32_t row_tiles,
+                 int32_t scan_parts) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t start = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (int64_t i = start; i < static_cast<int64_t>(row_tiles) * kMaxSlots; i += stride) {
+    int32_t* table = tables + i / kMaxSlots * kTableInts;
+    const int32_t s = static_cast<int32_t>(i % kMaxSlots);
+    if (s >= __ldcg(table)) continue;
+    int32_t a = __ldcg(table + kSlotAdapter + s);
+    const uint8_t* flags = not_finite + static_cast<int64_t>(a) * scan_parts;
+    unsigned bad = 0;
+    for (int32_t q = 0; q < scan_parts; ++q) bad |= __ldcg(flags + q);
+    table[kSlotShared + s] = bad != 0 ? -1 : a;
+  }
   const int64_t total = static_cast<int64_t>(num_tokens) * rank;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+  for (int64_t i = start; i < total; i += stride) {
     const int32_t t = static_cast<int32_t>(i / rank);
     const int32_t j = static_cast<int32_t>(i - static_cast<int64_t>(t) * rank);
     const int64_t a = static_cast<int64_t>(__ldg(adapter_idx + t));
     if (a < 0 || a >= num_adapters) continue;
     float sum = 0.0f;
-    for (int32_t s = 0; s < splits; ++s) sum += __ldg(partial + s * total + i);
+    for (int32_t s = 0; s < splits; ++s) sum += __ldcg(partial + s * total + i);
     if (scale != nullptr) sum *= __ldg(scale + a);
     const __nv_bfloat16 high = __float2bfloat16_rn(sum);
     __nv_bfloat16* row = v + static_cast<int64_t>(t) * rank * parts;
@@ -214,20 +235,19 @@ struct LoraExpand {
   struct Params {
     BandOrder order;
     const int32_t* tables;
-    const uint8_t* not_finite;
-    const __nv_bfloat16* x;
     const __nv_bfloat16* v;
     const __nv_bfloat16* b;
-    int32_t num_tokens, d_model, width, rank, v_cols, base_steps, adapter_rows, cols, out_fp32;  // v_cols = rank * parts
+    int32_t num_tokens, width, rank, v_cols, base_steps, adapter_rows, cols, out_fp32;  // v_cols = rank * parts
   };
   struct Tile {
-    int32_t k_steps, row_tile, n0, slots;
+    int32_t k_steps, base_steps, row_tile, n0, slots;
     const int32_t* table;
     bool live;
   };
   struct Rows { int32_t slot[8]; };
   struct Early { int32_t loner; };  // this row's adapter when its B is not finite, else -1
-  static constexpr bool kVariable = true, kStepGather = true, kGather = true, kAMnMajor = false, kBMnMajor = true;
+  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kVariable = true, kExtension = true, kGather = false, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -237,67 +257,64 @@ struct LoraExpand {
     t.n0 = slice * kTileCols;
     t.table = p.tables + static_cast<int64_t>(t.row_tile) * kTableInts;
     t.slots = __ldg(t.table);
+    t.base_steps = p.base_steps;
     t.k_steps = p.base_steps + (t.slots * p.v_cols + kTileStep - 1) / kTileStep;
     t.live = true;
     return t;
   }
   static __device__ __forceinline__ int columns(const Params& p) { return p.cols; }
   static __device__ __forceinline__ int slabs(const Params& p) { return (p.cols + 63) >> 6; }
-  static __device__ __forceinline__ uint32_t tx_bytes(const Params& p, const Tile&, int32_t) {
-    return static_cast<uint32_t>(slabs(p)) * TileSmem::kSlabBytes;
+  static __device__ __forceinline__ uint32_t tx_bytes(const Params& p, const Tile& t, int32_t ks) {
+    return static_cast<uint32_t>(slabs(p)) * TileSmem::kSlabBytes + (ks < t.base_steps ? TileSmem::kABytes : 0);
   }
-  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t,
+  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
     const int n = slabs(p);
-    if (ks < p.base_steps) {
+    if (ks < t.base_steps) {
+      ptx::tma_load_2d(a, &maps.m[3], ks * kTileStep, t.row_tile * kTileRows, bar);
       for (int j = 0; j < n; ++j)
         ptx::tma_load_2d(b + j * TileSmem::kSlabBytes, &maps.m[0], t.n0 + j * 64, ks * kTileStep, bar);
       return;
     }
-    // Eight K rows at a time: rows of one adapter's B, or of none (past the end: zeros).
+    // Eight K rows at a time: rows of one adapter's B, or of none (past the end, or not finite: zeros).
+    int32_t row[8];
+#pragma unroll
     for (int g = 0; g < 8; ++g) {
-      const int32_t q = (ks - p.base_steps) * kTileStep + g * 8;
+      const int32_t q = (ks - t.base_steps) * kTileStep + g * 8;
       const int32_t slot = q / p.v_cols;
-      int32_t row = p.adapter_rows;
-      if (slot < t.slots) {
-        const int32_t a = __ldg(t.table + 1 + slot);
-        int32_t j = q - slot * p.v_cols;
-        if (j >= p.rank) j -= p.rank;
-        if (adapter_finite(p.not_finite, a)) row = a * p.rank + j;
-      }
-      for (int j = 0; j < n; ++j)
-        ptx::tma_load_2d(b + j * TileSmem::kSlabBytes + g * 1024, &maps.m[1], t.n0 + j * 64, row, bar);
+      const int32_t a_id = slot < t.slots ? __ldg(t.table + kSlotShared + slot) : -1;
+      int32_t j = q - slot * p.v_cols;
+      if (j >= p.rank) j -= p.rank;
+      row[g] = a_id >= 0 ? a_id * p.rank + j : p.adapter_rows;
     }
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+      for (int j = 0; j < n; ++j)
+        ptx::tma_load_2d(b + j * TileSmem::kSlabBytes + g * 1024, &maps.m[1], t.n0 + j * 64, row[g], bar);
   }
-  static __device__ __forceinline__ Rows rows(const Params& p, const Tile& t, int row0) {
+  static __device__ __forceinline__ Rows rows(const Params&, const Tile& t, int row0) {
     Rows r;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      r.slot[j] = __ldg(t.table + 1 + kMaxSlots + row0 + j * 16);
-      if (r.slot[j] >= 0 && !adapter_finite(p.not_finite, __ldg(t.table + 1 + r.slot[j]))) r.slot[j] = -1;
+      r.slot[j] = __ldg(t.table + kRowSlot + row0 + j * 16);
+      if (r.slot[j] >= 0 && __ldg(t.table + kSlotShared + r.slot[j]) < 0) r.slot[j] = -1;
     }
     return r;
   }
-  static __device__ __forceinline__ const void* step_source(const Params& p, const Tile& t, const Rows& r, int j, int row,
-                                                            int32_t ks, int chunk, bool* real) {
-    const int64_t token = static_cast<int64_t>(t.row_tile) * kTileRows + row;
-    if (ks < p.base_steps) {
-      const int32_t k = ks * kTileStep + chunk * 8;
-      *real = token < p.num_tokens && k < p.d_model;
-      return p.x + (*real ? token * p.d_model + k : 0);
-    }
-    const int32_t q = (ks - p.base_steps) * kTileStep + chunk * 8;
+  static __device__ __forceinline__ uint4 extension_chunk(const Params& p, const Tile& t, const Rows& r, int j, int row,
+                                                          int32_t ks, int chunk) {
+    const int32_t q = (ks - t.base_steps) * kTileStep + chunk * 8;
     const int32_t slot = q / p.v_cols;
-    *real = r.slot[j] == slot;  // rows past the end have no slot
-    return p.v + (*real ? token * p.v_cols + (q - slot * p.v_cols) : 0);
+    if (r.slot[j] != slot) return make_uint4(0u, 0u, 0u, 0u);  // rows past the end have no slot
+    const int64_t token = static_cast<int64_t>(t.row_tile) * kTileRows + row;
+    return __ldg(reinterpret_cast<const uint4*>(p.v + token * p.v_cols + (q - slot * p.v_cols)));
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
-    const int32_t slot = __ldg(t.table + 1 + kMaxSlots + w.quarter * 32 + w.lane);
-    if (slot < 0) return {-1};
-    const int32_t a = __ldg(t.table + 1 + slot);
-    return {adapter_finite(p.not_finite, a) ? -1 : a};
+    const int32_t slot = __ldg(t.table + kRowSlot + w.quarter * 32 + w.lane);
+    if (slot < 0 || __ldg(t.table + kSlotShared + slot) >= 0) return {-1};
+    return {__ldg(t.table + kSlotAdapter + slot)};
   }
-  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, const EpilogueWarp& w,
+  static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
     const int32_t row = t.row_tile * kTileRows + w.quarter * 32;
     if (row >= p.num_tokens) return;
@@ -324,14 +341,14 @@ struct LoraExpand {
           }
         }
         if (p.out_fp32) {
-          if (col + part * 32 < p.width) store_rows_128b(w, &maps.m[2], v, col + part * 32, row);
+          if (col + part * 32 < p.width) store_rows_128b<kBuffers>(w, &maps.m[2], v, col + part * 32, row);
         } else {
 #pragma unroll
           for (int h = 0; h < 16; ++h)
             packed[part * 16 + h] = pack_bf16(__uint_as_float(v[2 * h]), __uint_as_float(v[2 * h + 1]));
         }
       }
-      if (!p.out_fp32) store_rows_128b(w, &maps.m[2], packed, col, row);
+      if (!p.out_fp32) store_rows_128b<kBuffers>(w, &maps.m[2], packed, col, row);
     }
   }
 };
@@ -343,7 +360,7 @@ template <typename index_t>
 __global__ void __launch_bounds__(256)
 lora_rows_kernel(const uint4* __restrict__ x, const uint4* __restrict__ a, const index_t* __restrict__ adapter_idx,
                  const float* __restrict__ scale, float* __restrict__ v, int32_t num_adapters, int32_t rank, int32_t vecs) {
-  grid_launch_dependents();
+  ptx::grid_launch_dependents();
   const int32_t t = static_cast<int32_t>(blockIdx.x);
   const int32_t j = static_cast<int32_t>(blockIdx.y) * 8 + static_cast<int32_t>(threadIdx.x >> 5);
   const int lane = static_cast<int>(threadIdx.x & 31);
@@ -506,12 +523,12 @@ int lora_small(const void* x, const void* weight, const void* lora_a, const void
 
 struct LoraSizes {
   int64_t row_tiles, tables, not_finite, partial, v, total;  // bytes of each part, 256-byte aligned, then all
-  int32_t splits, steps, total_steps, parts;
+  int32_t splits, steps, total_steps, parts, scan_parts;
 };
 
 int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
-LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t rank, int32_t num_adapters, int out_fp32, int sm_count) {
+LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t width, int32_t rank, int32_t num_adapters, int out_fp32, int sm_count) {
   LoraSizes s{};
   if (num_tokens <= kSkinnyMaxRows) {
     s.v = align256(num_tokens * rank * 4);
@@ -527,7 +544,10 @@ LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t rank, int32_t 
   s.steps = static_cast<int32_t>((s.total_steps + parts - 1) / parts);
   s.splits = (s.total_steps + s.steps - 1) / s.steps;
   s.tables = align256(s.row_tiles * kTableInts * 4);
-  s.not_finite = align256(static_cast<int64_t>(num_adapters) * kScanParts);
+  // Thread blocks that look through one adapter's B: about four per SM over all tiles, each for 8 KB at least.
+  const int64_t b_bytes = static_cast<int64_t>(rank) * width * 2;
+  s.scan_parts = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({64, 4 * sm_count / s.row_tiles, b_bytes / 8192})));
+  s.not_finite = align256(static_cast<int64_t>(num_adapters) * s.scan_parts);
   s.partial = align256(static_cast<int64_t>(s.splits) * num_tokens * rank * 4);
   s.v = align256(num_tokens * rank * s.parts * 2);
   s.total = s.tables + s.not_finite + s.partial + s.v;
@@ -556,7 +576,7 @@ extern "C" int64_t sb_lora_workspace_bytes(int64_t num_tokens, int32_t d_model, 
   if (check_lora(num_tokens, d_model, width, rank, num_adapters) != SB_OK) return -1;
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return -1;
-  return lora_sizes(num_tokens, d_model, rank, num_adapters, out_fp32, info->sm_count).total;
+  return lora_sizes(num_tokens, d_model, width, rank, num_adapters, out_fp32, info->sm_count).total;
 }
 
 extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lora_a, const void* lora_b,
@@ -572,7 +592,7 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
     if (!aligned16(q)) return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: buffers must be 16-byte aligned");
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
-  const LoraSizes s = lora_sizes(num_tokens, d_model, rank, num_adapters, out_fp32, info->sm_count);
+  const LoraSizes s = lora_sizes(num_tokens, d_model, width, rank, num_adapters, out_fp32, info->sm_count);
   if (workspace_bytes < s.total)
     return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: the workspace has %lld bytes, %lld are needed",
                 (long long)workspace_bytes, (long long)s.total);
@@ -588,8 +608,8 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
   const int32_t tokens = static_cast<int32_t>(num_tokens);
   const int32_t row_tiles = static_cast<int32_t>(s.row_tiles);
 
-  const dim3 plan_grid(static_cast<unsigned>(row_tiles), kScanParts);
-  const int64_t b_vecs = static_cast<int64_t>(rank) * width / 8;
+  const dim3 plan_grid(static_cast<unsigned>(row_tiles), static_cast<unsigned>(s.scan_parts));
+  const int32_t b_vecs = rank * (width / 8);
   if (idx_is_i64)
     lora_plan_kernel<int64_t><<<plan_grid, kPlanThreads, 0, st>>>(static_cast<const int64_t*>(adapter_idx),
         static_cast<const uint4*>(lora_b), tables, not_finite, tokens, num_adapters, b_vecs);
@@ -616,30 +636,39 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
     p.total_steps = s.total_steps;
     if (int rc = launch_tile_gemm<LoraShrink>(maps, p, static_cast<int64_t>(row_tiles) * p.groups * p.splits, dev_status, st, "lora_linear (shrink)")) return rc;
   }
-  const int64_t values = num_tokens * rank;
-  const unsigned join_blocks = static_cast<unsigned>(std::min<int64_t>((values + 255) / 256, static_cast<int64_t>(info->sm_count) * 8));
-  if (idx_is_i64)
-    lora_join_kernel<int64_t><<<join_blocks, 256, 0, st>>>(partial, static_cast<const int64_t*>(adapter_idx), scale, v, tokens,
-                                                            num_adapters, rank, s.splits, s.parts);
-  else
-    lora_join_kernel<int32_t><<<join_blocks, 256, 0, st>>>(partial, static_cast<const int32_t*>(adapter_idx), scale, v, tokens,
-                                                            num_adapters, rank, s.splits, s.parts);
-  if (int rc = check_launch("lora_linear (join)")) return rc;
+  {
+    const int64_t values = std::max<int64_t>(num_tokens * rank, static_cast<int64_t>(row_tiles) * kMaxSlots);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((values + 255) / 256, static_cast<int64_t>(info->sm_count) * 8)));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const float* parts = partial;
+    const uint8_t* flags = not_finite;
+    const cudaError_t err =
+        idx_is_i64 ? cudaLaunchKernelEx(&cfg, lora_join_kernel<int64_t>, parts, static_cast<const int64_t*>(adapter_idx), scale, v, tokens,
+                                        num_adapters, rank, s.splits, s.parts, tables, flags, row_tiles, s.scan_parts)
+                   : cudaLaunchKernelEx(&cfg, lora_join_kernel<int32_t>, parts, static_cast<const int32_t*>(adapter_idx), scale, v, tokens,
+                                        num_adapters, rank, s.splits, s.parts, tables, flags, row_tiles, s.scan_parts);
+    if (err != cudaSuccess) return fail(SB_ERR_CUDA, "lora_linear (join): %s", cudaGetErrorString(err));
+  }
 
   TileMaps maps{};
   if (int rc = encode_2d_map(&maps.m[0], weight, d_model, width, 64, 64, 2, "lora_linear (weight)")) return rc;
   if (int rc = encode_2d_map(&maps.m[1], lora_b, static_cast<uint64_t>(num_adapters) * rank, width, 8, 64, 2, "lora_linear (B)")) return rc;
   if (int rc = encode_2d_map(&maps.m[2], out, num_tokens, width, 32, out_fp32 ? 32 : 64, out_fp32 ? 4 : 2, "lora_linear (out)")) return rc;
+  if (int rc = encode_2d_map(&maps.m[3], x, num_tokens, d_model, kTileRows, 64, 2, "lora_linear (x)")) return rc;
   LoraExpand::Params p{};
   const int32_t slices = (width + kTileCols - 1) / kTileCols;
   p.order = {row_tiles, slices, 8};
   p.tables = tables;
-  p.not_finite = not_finite;
-  p.x = static_cast<const __nv_bfloat16*>(x);
   p.v = v;
   p.b = static_cast<const __nv_bfloat16*>(lora_b);
   p.num_tokens = tokens;
-  p.d_model = d_model;
   p.width = width;
   p.rank = rank;
   p.v_cols = rank * s.parts;

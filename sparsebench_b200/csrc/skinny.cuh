@@ -26,9 +26,6 @@ constexpr int kSkinnyStep = 64;
 constexpr int kSkinnyWBytes = kSkinnyCols * kSkinnyStep * 2;
 constexpr int kSkinnyMaxRows = 64;
 
-__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -110,10 +107,10 @@ skinny_kernel(const __grid_constant__ SkinnyMaps maps, const __grid_constant__ t
   const int32_t rank = static_cast<int32_t>(blockIdx.x) % sh.splits;
   const int32_t block_item = static_cast<int32_t>(blockIdx.x) / sh.splits;
 
-  grid_launch_dependents();
+  ptx::grid_launch_dependents();
   typename Op::Item item;
   if (!Op::begin(p, item, block_item, ids, list)) {
-    grid_dependency_wait();
+    ptx::grid_dependency_wait();
     return;
   }
   if (threadIdx.x == 0) {
@@ -183,7 +180,7 @@ skinny_kernel(const __grid_constant__ SkinnyMaps maps, const __grid_constant__ t
     __syncwarp();
   } else {
     const int worker = static_cast<int>(threadIdx.x) - 64;
-    grid_dependency_wait();
+    ptx::grid_dependency_wait();
     if constexpr (Op::kGather) {
       // Eight lanes share a row's 128 bytes of the K step; 128 threads move 16 rows at a time.
       const int row0 = worker >> 3;

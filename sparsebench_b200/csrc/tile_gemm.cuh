@@ -27,15 +27,12 @@ struct alignas(64) TileMaps {
 };
 
 struct TileSmem {
-  static constexpr int kStages = 4;
   static constexpr int kABytes = kTileRows * kTileStep * 2;
   static constexpr int kBBytes = kTileCols * kTileStep * 2;
   static constexpr int kSlabBytes = kTileStep * 128;
   static constexpr int kEpilogueWarps = 8;
-  static constexpr int kStagingBytes = 32 * 128;  // per epilogue warp: 32 rows x 64 bf16
+  static constexpr int kStagingBytes = 32 * 128;  // one staging tile of an epilogue warp: 32 rows x 128 bytes
   static constexpr int kBarrierBytes = 256;
-  static constexpr int kBytes = 1024 + kStages * (kABytes + kBBytes) + kEpilogueWarps * kStagingBytes + kBarrierBytes;
-  static_assert(kBytes <= 227 * 1024, "shared memory budget");
 };
 
 // What an epilogue warp works with.
@@ -43,25 +40,29 @@ struct EpilogueWarp {
   int quarter;       // rows quarter * 32 .. + 31 of the tile (TMEM lanes this warp may read)
   int half;          // 0 or 1: which half of the tile's columns is this warp's
   int lane;
-  uint32_t staging;  // this warp's 4 KB in shared memory
+  uint32_t staging;  // this warp's staging tiles in shared memory, 4 KB each
+  uint32_t buffer;   // the one to use next
   uint32_t taddr;    // TMEM address of (lane quarter, column 0) of the finished accumulator
 };
 
-// 128 bytes of this lane's row (64 bf16 columns as pairs, or 32 fp32 columns) -> the warp's staging tile -> one TMA store
-// of 32 rows.
-__device__ __forceinline__ void store_rows_128b(const EpilogueWarp& w, const CUtensorMap* map, const uint32_t (&packed)[32],
-                                               int32_t col, int32_t row) {
-  if (w.lane == 0) ptx::bulk_wait_read();  // the store before has read the staging tile
+// 128 bytes of this lane's row (64 bf16 columns as pairs, or 32 fp32 columns) -> a staging tile of the warp -> one TMA
+// store of 32 rows. kBuffers staging tiles are used in turn.
+template <int kBuffers>
+__device__ __forceinline__ void store_rows_128b(EpilogueWarp& w, const CUtensorMap* map, const uint32_t (&packed)[32],
+                                                int32_t col, int32_t row) {
+  if (w.lane == 0) ptx::bulk_wait_read_but<kBuffers - 1>();  // the tile's last store has read it
   __syncwarp();
+  const uint32_t tile = w.staging + w.buffer * TileSmem::kStagingBytes;
+  if (kBuffers > 1) w.buffer ^= 1u;
   const uint32_t swz = static_cast<uint32_t>(w.lane & 7);
-  const uint32_t dst = w.staging + static_cast<uint32_t>(w.lane) * 128u;
+  const uint32_t dst = tile + static_cast<uint32_t>(w.lane) * 128u;
 #pragma unroll
   for (uint32_t c = 0; c < 8; ++c)
     ptx::st_shared_v4(dst + ((c ^ swz) << 4), packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
   ptx::fence_proxy_async_shared();
   __syncwarp();
   if (w.lane == 0) {
-    ptx::tma_store_2d(map, w.staging, col, row);
+    ptx::tma_store_2d(map, tile, col, row);
     ptx::bulk_commit();
   }
 }
@@ -105,17 +106,20 @@ struct BandOrder {
 //   static constexpr bool kGather, kAMnMajor, kBMnMajor
 //   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar), tx_bytes
 //   gather_row(p, tile, row) -> source row of A or nullptr (zeros), for kGather; any_row(p): a readable address
-//   or, with kStepGather: Rows rows(p, tile, row0) once per tile and step_source(p, tile, rows, j, row, ks, chunk, &real),
-//   the address of 16-byte chunk `chunk` of row `row` = row0 + 16 j in K step ks (real = false: zeros)
+//   static constexpr int kStages (of the ring), kBuffers (staging tiles per epilogue warp)
+//   With kExtension: Tile has base_steps; A of the K steps behind them is written by four warps from registers:
+//   Rows rows(p, tile, row0) once per tile, extension_chunk(p, tile, rows, j, row, ks, chunk) = the 16 bytes of chunk
+//   `chunk` of row `row` = row0 + 16 j.
 //   With kVariable: columns(p) <= 256 (a multiple of 16) accumulator columns in use, tx_bytes(p, tile, ks) per stage
-//   prefetch(p, tile, w) -> Early (global loads that can start before the accumulator is ready)
-//   epilogue(maps, p, tile, w, early)
 template <class Op>
 struct TileConfig {
-  static constexpr int kGatherWarps = Op::kGather ? 4 : 0;
+  static constexpr int kGatherWarps = Op::kGather || Op::kExtension ? 4 : 0;
   static constexpr int kFirstGatherWarp = 2 + TileSmem::kEpilogueWarps;
   static constexpr int kThreads = 32 * (kFirstGatherWarp + kGatherWarps);
-  static constexpr uint32_t kFullArrivals = 1 + 32 * kGatherWarps;
+  static constexpr uint32_t kFullArrivals = Op::kGather ? 1 + 32 * kGatherWarps : 1;
+  static constexpr int kSmemBytes = 1024 + Op::kStages * (TileSmem::kABytes + TileSmem::kBBytes) +
+                                    TileSmem::kEpilogueWarps * Op::kBuffers * TileSmem::kStagingBytes + TileSmem::kBarrierBytes;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
 template <class Op>
@@ -126,14 +130,16 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t a_base = smem_base;
-  const uint32_t b_base = a_base + S::kStages * S::kABytes;
-  const uint32_t staging_base = b_base + S::kStages * S::kBBytes;
-  const uint32_t full_bar = staging_base + S::kEpilogueWarps * S::kStagingBytes;  // [kStages]
-  const uint32_t empty_bar = full_bar + 8 * S::kStages;                           // [kStages]
-  const uint32_t acc_full_bar = empty_bar + 8 * S::kStages;                       // [2]
+  const uint32_t b_base = a_base + Op::kStages * S::kABytes;
+  const uint32_t staging_base = b_base + Op::kStages * S::kBBytes;
+  const uint32_t full_bar = staging_base + S::kEpilogueWarps * Op::kBuffers * S::kStagingBytes;  // [kStages]
+  const uint32_t empty_bar = full_bar + 8 * Op::kStages;                          // [kStages]
+  const uint32_t acc_full_bar = empty_bar + 8 * Op::kStages;                      // [2]
   const uint32_t acc_empty_bar = acc_full_bar + 16;                               // [2]
   const uint32_t tmem_slot = acc_empty_bar + 16;
   const uint32_t abort_slot = tmem_slot + 4;
+  const uint32_t go_bar = abort_slot + 4;             // [kStages] extension: the stage is free for the warps' A rows
+  const uint32_t ready_bar = go_bar + 8 * Op::kStages;  // [kStages] extension: they are written
   uint8_t* smem_aligned = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
   volatile uint32_t* tmem_word = reinterpret_cast<volatile uint32_t*>(smem_aligned + (tmem_slot - smem_base));
   volatile uint32_t* abort_word = reinterpret_cast<volatile uint32_t*>(smem_aligned + (abort_slot - smem_base));
@@ -142,9 +148,13 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
   const int lane = static_cast<int>(threadIdx.x & 31);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < Op::kStages; ++s) {
       ptx::mbar_init(full_bar + 8 * s, Cfg::kFullArrivals);
       ptx::mbar_init(empty_bar + 8 * s, 1);
+      if (Op::kExtension) {
+        ptx::mbar_init(go_bar + 8 * s, 1);
+        ptx::mbar_init(ready_bar + 8 * s, Cfg::kGatherWarps);
+      }
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(acc_full_bar + 8 * a, 1);
@@ -161,6 +171,10 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
   __syncthreads();
   ptx::tcgen05_fence_after_sync();
   const uint32_t tmem_base = *tmem_word;
+  // Launched with programmatic dependence: everything up to here may overlap the end of the kernel before.
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  ptx::fence_proxy_async_global();  // what earlier kernels stored is read by TMA
 
   const int32_t total = Op::total_tiles(p);
   const int32_t step = static_cast<int32_t>(gridDim.x);
@@ -187,10 +201,13 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
             break;
           }
           const uint32_t bar = full_bar + 8 * stage;
+          if constexpr (Op::kExtension) {
+            if (ks >= tile.base_steps) ptx::mbar_arrive(go_bar + 8 * stage);
+          }
           if constexpr (Op::kVariable) ptx::mbar_arrive_expect_tx(bar, Op::tx_bytes(p, tile, ks));
           else ptx::mbar_arrive_expect_tx(bar, S::kBBytes + (Op::kGather ? 0 : S::kABytes));
           Op::load(maps, p, tile, ks, a_base + stage * S::kABytes, b_base + stage * S::kBBytes, bar);
-          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == Op::kStages) { stage = 0; phase ^= 1u; }
         }
       }
     }
@@ -200,13 +217,15 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
       uint32_t idesc = ptx::make_idesc_bf16(kTileRows, kTileCols, Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
       if constexpr (Op::kVariable)
         idesc = ptx::make_idesc_bf16(kTileRows, Op::columns(p), Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, ready_phases = 0;
       bool ok = true;
       int32_t index = blockIdx.x;
       typename Op::Tile next{};
       if (index < total) next = Op::tile(p, index);
       for (; ok && index < total; index += step) {
         const int32_t k_steps = next.k_steps;
+        int32_t base_steps = k_steps;
+        if constexpr (Op::kExtension) base_steps = next.base_steps;
         if (index + step < total) next = Op::tile(p, index + step);
         if (k_steps == 0) continue;
         if (!ptx::mbar_wait_bounded(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_word)) {
@@ -221,6 +240,14 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
             ok = false;
             break;
           }
+          if (Op::kExtension && ks >= base_steps) {
+            if (!ptx::mbar_wait_bounded(ready_bar + 8 * stage, (ready_phases >> stage) & 1u, abort_word)) {
+              give_up(SB_DEV_TIMEOUT_MMA);
+              ok = false;
+              break;
+            }
+            ready_phases ^= 1u << stage;
+          }
           if (Op::kGather) ptx::fence_proxy_async_shared();  // rows written by cp.async, read by the tensor core
           ptx::tcgen05_fence_after_sync();
           const uint32_t a_addr = a_base + stage * S::kABytes;
@@ -234,7 +261,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
             ptx::umma_bf16(d_tmem, desc_a, desc_b, idesc, (ks | kk) != 0);
           }
           ptx::umma_commit(empty_bar + 8 * stage);
-          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == Op::kStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
         ptx::umma_commit(acc_full_bar + 8 * acc);
@@ -248,7 +275,8 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     w.quarter = warp & 3;
     w.half = (warp - 2) >> 2;
     w.lane = lane;
-    w.staging = staging_base + static_cast<uint32_t>(warp - 2) * S::kStagingBytes;
+    w.staging = staging_base + static_cast<uint32_t>(warp - 2) * (Op::kBuffers * S::kStagingBytes);
+    w.buffer = 0;
     uint32_t acc = 0, acc_phase = 0;
     for (int32_t index = blockIdx.x; index < total; index += step) {
       const typename Op::Tile tile = Op::tile(p, index);
@@ -280,66 +308,74 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
       const int row0 = gw * 4 + (lane >> 3);
       const uint32_t chunk = static_cast<uint32_t>(lane & 7);
       const uint32_t dst_off = static_cast<uint32_t>(row0) * 128u + ((chunk ^ static_cast<uint32_t>(row0 & 7)) << 4);
-      if constexpr (Op::kStepGather) {
-        uint32_t stage = 0, phase = 0;
-        bool ok = true;
-        for (int32_t index = blockIdx.x; ok && index < total; index += step) {
-          const typename Op::Tile tile = Op::tile(p, index);
-          const typename Op::Rows rows = Op::rows(p, tile, row0);
-          for (int32_t ks = 0; ks < tile.k_steps; ++ks) {
-            if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
-              give_up(SB_DEV_TIMEOUT_PRODUCER);
-              ok = false;
-              break;
-            }
-            const uint32_t dst = a_base + stage * S::kABytes + dst_off;
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      int32_t index = blockIdx.x;
+      typename Op::Tile next{};
+      const __nv_bfloat16* next_src[8];
+      auto fetch = [&](int32_t at) {
+        next = Op::tile(p, at);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              bool real;
-              const void* src = Op::step_source(p, tile, rows, j, row0 + j * 16, ks, static_cast<int>(chunk), &real);
-              ptx::cp_async_16_zfill(dst + j * 2048, src, real);
-            }
-            ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
-            if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
-          }
+        for (int j = 0; j < 8; ++j) next_src[j] = next.k_steps > 0 ? Op::gather_row(p, next, row0 + j * 16) : nullptr;
+      };
+      if (index < total) fetch(index);
+      for (; ok && index < total; index += step) {
+        const int32_t k_steps = next.k_steps;
+        const __nv_bfloat16* src[8];
+        bool real[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          real[j] = next_src[j] != nullptr;
+          src[j] = (real[j] ? next_src[j] : Op::any_row(p)) + chunk * 8;  // padding still passes a valid address
         }
-      } else {
-        uint32_t stage = 0, phase = 0;
-        bool ok = true;
-        int32_t index = blockIdx.x;
-        typename Op::Tile next{};
-        const __nv_bfloat16* next_src[8];
-        auto fetch = [&](int32_t at) {
-          next = Op::tile(p, at);
-  #pragma unroll
-          for (int j = 0; j < 8; ++j) next_src[j] = next.k_steps > 0 ? Op::gather_row(p, next, row0 + j * 16) : nullptr;
-        };
-        if (index < total) fetch(index);
-        for (; ok && index < total; index += step) {
-          const int32_t k_steps = next.k_steps;
-          const __nv_bfloat16* src[8];
-          bool real[8];
-  #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            real[j] = next_src[j] != nullptr;
-            src[j] = (real[j] ? next_src[j] : Op::any_row(p)) + chunk * 8;  // padding still passes a valid address
+        if (index + step < total) fetch(index + step);
+        for (int32_t ks = 0; ks < k_steps; ++ks) {
+          if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
+            give_up(SB_DEV_TIMEOUT_PRODUCER);
+            ok = false;
+            break;
           }
-          if (index + step < total) fetch(index + step);
-          for (int32_t ks = 0; ks < k_steps; ++ks) {
-            if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
-              give_up(SB_DEV_TIMEOUT_PRODUCER);
-              ok = false;
-              break;
-            }
-            const uint32_t dst = a_base + stage * S::kABytes + dst_off;
-  #pragma unroll
-            for (int j = 0; j < 8; ++j) ptx::cp_async_16_zfill(dst + j * 2048, src[j] + ks * kTileStep, real[j]);
-            ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
-            if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
-          }
+          const uint32_t dst = a_base + stage * S::kABytes + dst_off;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ptx::cp_async_16_zfill(dst + j * 2048, src[j] + ks * kTileStep, real[j]);
+          ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
+          if (++stage == Op::kStages) { stage = 0; phase ^= 1u; }
         }
       }
       ptx::cp_async_wait_all();
+    }
+    if constexpr (Op::kExtension) {
+      // The same rows and chunks, for the steps behind the base steps only. The producer says when a stage is free
+      // (its own wait on empty_bar passed), so that these warps need not follow the ring through the base steps.
+      const int row0 = (warp - Cfg::kFirstGatherWarp) * 4 + (lane >> 3);
+      const int chunk = lane & 7;
+      const uint32_t dst_off = static_cast<uint32_t>(row0) * 128u + (static_cast<uint32_t>(chunk ^ (row0 & 7)) << 4);
+      uint32_t stage = 0, go_phases = 0;
+      bool ok = true;
+      for (int32_t index = blockIdx.x; ok && index < total; index += step) {
+        const typename Op::Tile tile = Op::tile(p, index);
+        stage = (stage + static_cast<uint32_t>(tile.base_steps)) % Op::kStages;
+        if (tile.base_steps >= tile.k_steps) continue;
+        const typename Op::Rows rows = Op::rows(p, tile, row0);
+        for (int32_t ks = tile.base_steps; ks < tile.k_steps; ++ks) {
+          uint4 chunks[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) chunks[j] = Op::extension_chunk(p, tile, rows, j, row0 + j * 16, ks, chunk);
+          if (!ptx::mbar_wait_bounded(go_bar + 8 * stage, (go_phases >> stage) & 1u, abort_word)) {
+            give_up(SB_DEV_TIMEOUT_PRODUCER);
+            ok = false;
+            break;
+          }
+          go_phases ^= 1u << stage;
+          const uint32_t dst = a_base + stage * S::kABytes + dst_off;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ptx::st_shared_v4(dst + j * 2048, chunks[j].x, chunks[j].y, chunks[j].z, chunks[j].w);
+          ptx::fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ready_bar + 8 * stage);
+          if (++stage == Op::kStages) stage = 0;
+        }
+      }
     }
   }
 
@@ -371,15 +407,25 @@ int launch_tile_gemm(const TileMaps& maps, const typename Op::Params& p, int64_t
   if (info == nullptr) return SB_ERR_CUDA;
   static std::atomic<bool> done[kMaxDevices] = {};
   if (!done[device].load(std::memory_order_acquire)) {
-    const cudaError_t err = cudaFuncSetAttribute(tile_gemm_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem::kBytes);
+    const cudaError_t err = cudaFuncSetAttribute(tile_gemm_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileConfig<Op>::kSmemBytes);
     if (err != cudaSuccess) return fail(SB_ERR_CUDA, "%s: shared memory opt-in: %s", what, cudaGetErrorString(err));
     done[device].store(true, std::memory_order_release);
   }
   if (tiles <= 0) return SB_OK;
   if (tiles > INT32_MAX - info->sm_count) return fail(SB_ERR_INVALID_ARGUMENT, "%s: problem too large", what);
-  const unsigned grid = static_cast<unsigned>(tiles < info->sm_count ? tiles : info->sm_count);
-  tile_gemm_kernel<Op><<<grid, TileConfig<Op>::kThreads, TileSmem::kBytes, stream>>>(maps, p, dev_status);
-  return check_launch(what);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles < info->sm_count ? tiles : info->sm_count));
+  cfg.blockDim = dim3(TileConfig<Op>::kThreads);
+  cfg.dynamicSmemBytes = TileConfig<Op>::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, tile_gemm_kernel<Op>, maps, p, dev_status);
+  if (err != cudaSuccess) return fail(SB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
+  return SB_OK;
 }
 
 }  // namespace sb
