@@ -90,6 +90,7 @@ struct GatedUp {
   };
   struct Early { bool store; };
   static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kGather = true, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
@@ -191,6 +192,7 @@ struct GradHidden {
     uint32_t first[2][2][8];  // G and U of the first two parts
   };
   static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kAhead = true;
   static constexpr bool kVariable = false, kExtension = false, kGather = true, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
@@ -235,6 +237,15 @@ struct GradHidden {
     e.real = __ldg(p.row_token + row) >= 0;
     e.gate = __ldg(p.row_gate + row);
     return e;
+  }
+  // The warp's 32 rows of a block are 8 KB in one piece: the next tile's are asked into L2 before this one is worked on,
+  // because what a warp can hold in flight in registers does not cover the way to memory.
+  static __device__ __forceinline__ void ahead(const Params& p, const Tile& next, const EpilogueWarp& w) {
+    const int32_t n = next.n0 + w.half * 128;
+    if (!next.live || n >= p.ffn_dim || w.lane != 0 || !half_has_rows(p.row_token, next.row_block, w.quarter)) return;
+    const int64_t at = ((static_cast<int64_t>(next.first_block) + (n >> 7)) * kTileRows + w.quarter * 32) * 128;
+    ptx::bulk_prefetch_l2(p.g + at, 32 * 256);
+    ptx::bulk_prefetch_l2(p.u + at, 32 * 256);
   }
   static __device__ __forceinline__ void epilogue(const TileMaps&, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
@@ -306,6 +317,7 @@ struct GradRows {
   };
   struct Early { bool store; };
   static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
@@ -364,7 +376,8 @@ struct GradWeights {
     bool live;
   };
   struct Early {};
-  static constexpr int kStages = 3, kBuffers = 2;
+  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kGather = false, kAMnMajor = true, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) {

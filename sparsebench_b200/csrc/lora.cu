@@ -139,6 +139,7 @@ struct LoraShrink {
   };
   struct Early { int32_t slot; };
   static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.row_tiles * p.groups * p.splits; }
@@ -247,6 +248,7 @@ struct LoraExpand {
   struct Rows { int32_t slot[8]; };
   struct Early { int32_t loner; };  // this row's adapter when its B is not finite, else -1
   static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = true, kGather = false, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
@@ -355,22 +357,24 @@ struct LoraExpand {
 
 // ---- a decoding step -----------------------------------------------------------------------------------------------
 
-// V[t, j] = scale[a] * x[t] . A[a, j] in fp32, one warp each; tokens without an adapter are left out here and later.
+// V[t, j] = scale[a] * x[t] . A[a, j] in fp32, a block each (with one warp the row's loads would wait for each other);
+// tokens without an adapter are left out here and later.
+constexpr int kRowsThreads = 256;
 template <typename index_t>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kRowsThreads)
 lora_rows_kernel(const uint4* __restrict__ x, const uint4* __restrict__ a, const index_t* __restrict__ adapter_idx,
                  const float* __restrict__ scale, float* __restrict__ v, int32_t num_adapters, int32_t rank, int32_t vecs) {
+  __shared__ float warp_sum[kRowsThreads / 32];
   ptx::grid_launch_dependents();
   const int32_t t = static_cast<int32_t>(blockIdx.x);
-  const int32_t j = static_cast<int32_t>(blockIdx.y) * 8 + static_cast<int32_t>(threadIdx.x >> 5);
-  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int32_t j = static_cast<int32_t>(blockIdx.y);
   const int64_t id = static_cast<int64_t>(__ldg(adapter_idx + t));
-  if (id < 0 || id >= num_adapters || j >= rank) return;
+  if (id < 0 || id >= num_adapters) return;
   const uint4* xr = x + static_cast<int64_t>(t) * vecs;
   const uint4* ar = a + (id * rank + j) * vecs;
   float sum = 0.0f;
-#pragma unroll 4
-  for (int32_t i = lane; i < vecs; i += 32) {
+#pragma unroll 2
+  for (int32_t i = static_cast<int32_t>(threadIdx.x); i < vecs; i += kRowsThreads) {
     const uint4 xq = __ldg(xr + i);
     const uint4 aq = __ldg(ar + i);
     const __nv_bfloat162* xp = reinterpret_cast<const __nv_bfloat162*>(&xq);
@@ -385,7 +389,14 @@ lora_rows_kernel(const uint4* __restrict__ x, const uint4* __restrict__ a, const
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) v[static_cast<int64_t>(t) * rank + j] = scale != nullptr ? sum * __ldg(scale + id) : sum;
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kRowsThreads / 32; ++w) sum += warp_sum[w];
+    v[static_cast<int64_t>(t) * rank + j] = scale != nullptr ? sum * __ldg(scale + id) : sum;
+  }
 }
 
 // y: 128 columns of x W by the tensor cores; the workers compute the adapters' term of their share of the tokens while
@@ -502,12 +513,12 @@ int lora_small(const void* x, const void* weight, const void* lora_a, const void
   SkinnyMaps maps{};
   if (int rc = encode_2d_map(&maps.w[0], weight, d_model, width, 64, 64, 2, "lora_linear (weight)")) return rc;
   if (int rc = encode_2d_map(&maps.x, x, num_tokens, d_model, shape.rows_pad, 64, 2, "lora_linear (x)")) return rc;
-  const dim3 grid(static_cast<unsigned>(num_tokens), static_cast<unsigned>((rank + 7) / 8));
+  const dim3 grid(static_cast<unsigned>(num_tokens), static_cast<unsigned>(rank));
   if (idx_is_i64)
-    lora_rows_kernel<long long><<<grid, 256, 0, stream>>>(static_cast<const uint4*>(x), static_cast<const uint4*>(lora_a),
+    lora_rows_kernel<long long><<<grid, kRowsThreads, 0, stream>>>(static_cast<const uint4*>(x), static_cast<const uint4*>(lora_a),
         static_cast<const long long*>(adapter_idx), scale, v, num_adapters, rank, d_model / 8);
   else
-    lora_rows_kernel<int32_t><<<grid, 256, 0, stream>>>(static_cast<const uint4*>(x), static_cast<const uint4*>(lora_a),
+    lora_rows_kernel<int32_t><<<grid, kRowsThreads, 0, stream>>>(static_cast<const uint4*>(x), static_cast<const uint4*>(lora_a),
         static_cast<const int32_t*>(adapter_idx), scale, v, num_adapters, rank, d_model / 8);
   if (int rc = check_launch("lora_linear (rows)")) return rc;
   const int32_t per_rank = (num_tokens + shape.splits - 1) / shape.splits;  // tokens of a block, 8 at a time

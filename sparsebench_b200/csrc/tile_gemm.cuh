@@ -280,6 +280,9 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     uint32_t acc = 0, acc_phase = 0;
     for (int32_t index = blockIdx.x; index < total; index += step) {
       const typename Op::Tile tile = Op::tile(p, index);
+      if constexpr (Op::kAhead) {
+        if (index + step < total) Op::ahead(p, Op::tile(p, index + step), w);
+      }
       if (!tile.live) continue;
       const typename Op::Early early = Op::prefetch(p, tile, w);
       if (tile.k_steps > 0) {
