@@ -402,26 +402,25 @@ int sb_ep_sdd_dispatch(const void* recv_rows, const void* w1, const int32_t* row
  * [E, D, F], w_down is [E, F, D]; gate (the picks' weights) is bf16 (gate_dtype 0) or fp32 (1); every buffer 16-byte
  * aligned. A copy whose expert id is outside [0, num_experts) contributes nothing, and its gate's gradient is 0.
  *
- * sb_sdd_gated: h_blocks = act(x[row_token] . w_gate[e]) * (x[row_token] . w_up[e]) in one kernel, on sb_route's layout
- * at block size 128, laid out like sb_sdd's blocks; the down projection is sb_dsd. g_blocks / u_blocks (both or neither
- * NULL): the two projections before the activation; every row of a 64-row half of a row block that holds real rows is
- * then written (padding rows as zeros). Without them skip_padding_rows works as in sb_sdd.
+ * sb_sdd_gated: h_blocks = act(x[row_token] . w_gate[e]) * (x[row_token] . w_up[e]) in one matmul kernel, on sb_route's
+ * layout at block size 128, laid out like sb_sdd's blocks; the down projection is sb_dsd. x_rows: scratch for
+ * [num_row_blocks * 128, D] bf16, x in layout order (padding rows 0). skip_padding_rows works as in sb_sdd.
  *
  * sb_moe_gated_bytes: bytes[0] of the state, bytes[1] of the forward's scratch, bytes[2] of the backward's; keep = 0: for
  * a forward pass alone (no state). Nothing in these buffers has to be set; they are 256-byte aligned.
  *
  * sb_moe_gated_forward: out[t] = sum_j gate[t, j] * (act(x[t] . w_gate[e]) * (x[t] . w_up[e])) . w_down[e],
  * e = expert_idx[t, j] (int32 or int64 [T, k]). With state (not NULL) it holds afterwards what the backward pass needs:
- * the layout and the blocks of H, G and U.
+ * the layout, x and Y in layout order and the blocks of H, G and U.
  *
- * sb_moe_gated_backward: the gradients of x, gate (in gate's type), w_gate, w_up and w_down from grad_out [T, D], the
- * inputs of that forward call and its state, which it leaves as it is. dw_*: written whole, zeros for an expert without
+ * sb_moe_gated_backward: the gradients of x, gate (in gate's type), w_gate, w_up and w_down from grad_out [T, D], gate and
+ * the weights of that forward call and its state, which it leaves as it is. dw_*: written whole, zeros for an expert without
  * rows. All sums are in a fixed order.
  */
 enum sb_activation { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* erf form */ };
 int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
-                 const int32_t* row_block_expert, const int32_t* row_offsets, void* h_blocks, void* g_blocks,
-                 void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                 const int32_t* row_block_expert, const int32_t* row_offsets, const int32_t* padded_offsets, void* x_rows,
+                 void* h_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
                  int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
                  sb_stream_t stream);
 int sb_moe_gated_bytes(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int keep,
@@ -431,8 +430,8 @@ int sb_moe_gated_forward(const void* x, const void* expert_idx, int idx_is_i64, 
                          int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t activation, void* state,
                          int64_t state_bytes, void* scratch, int64_t scratch_bytes, int32_t* dev_status,
                          sb_stream_t stream);
-int sb_moe_gated_backward(const void* grad_out, const void* x, const void* gate, int gate_dtype, const void* w_gate,
-                          const void* w_up, const void* w_down, const void* state, int64_t state_bytes, void* dx,
+int sb_moe_gated_backward(const void* grad_out, const void* gate, int gate_dtype, const void* w_gate, const void* w_up,
+                          const void* w_down, const void* state, int64_t state_bytes, void* dx,
                           void* dgate, void* dw_gate, void* dw_up, void* dw_down, int64_t num_tokens, int32_t k,
                           int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t activation, void* scratch,
                           int64_t scratch_bytes, int32_t* dev_status, sb_stream_t stream);

@@ -81,16 +81,14 @@ def gated_reference(x, expert_idx, gate, w_gate, w_up, w_down, act: str = "silu"
         a_b = 1.13 * g_b + ACT_ERROR * g.abs()
         s_b = CURVATURE * g_b + ACT_ERROR * (1 + g.abs())
         do = go[t]
-        sv = do @ wd.T
-        sv_b = d_model * HALF_FP32 * (do.abs() @ wd.abs().T)
-        hh_b = a_b * u.abs() + a.abs() * u_b
-        val["dgate"][t, j] = (h * sv).sum(1)
-        bnd["dgate"][t, j] = (hh_b * sv.abs() + h.abs() * sv_b + ffn_dim * HALF_FP32 * (h * sv).abs()).sum(1)
-        dh, dh_b = w * sv, w.abs() * sv_b
+        val["dgate"][t, j] = (do * y).sum(1)
+        bnd["dgate"][t, j] = (do.abs() * y_b + d_model * HALF_FP32 * (do * y).abs()).sum(1)
+        wdo = w * do  # held as bf16
+        dh = wdo @ wd.T
+        dh_b = (HALF_BF16 + d_model * HALF_FP32) * (wdo.abs() @ wd.abs().T)
         du, dg = dh * a, dh * u * s
         du_b = dh_b * a.abs() + dh.abs() * a_b + HALF_BF16 * du.abs()
         dg_b = dh_b * (u * s).abs() + dh.abs() * (u_b * s.abs() + u.abs() * s_b) + HALF_BF16 * dg.abs()
-        wdo = w * do
         n = t.numel()
         val["dw_down"][e] = h.T @ wdo
         bnd["dw_down"][e] = h_b.T @ wdo.abs() + (HALF_BF16 + n * HALF_FP32) * (h.abs().T @ wdo.abs())

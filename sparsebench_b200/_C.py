@@ -370,33 +370,32 @@ def _check_gated_weights(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
 
 
 def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, row_token: torch.Tensor,
-                   row_block_expert: torch.Tensor, row_offsets: torch.Tensor, num_nnz: int, activation: str,
-                   skip_padding_rows: bool = False, keep: bool = False
-                   ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
-    """(H, G, U), blocks [num_nnz, 128, 128] each: G = x[row_token] @ w_gate[expert], U the same with w_up,
-    H = act(G) * U, in one kernel. G and U are None unless keep: then all three have every row the backward pass
-    reads (padding rows of a 64-row half that holds real rows as zeros). Dead row blocks are left unwritten."""
+                   row_block_expert: torch.Tensor, row_offsets: torch.Tensor, padded_offsets: torch.Tensor, num_nnz: int,
+                   activation: str, skip_padding_rows: bool = False) -> torch.Tensor:
+    """Blocks [num_nnz, 128, 128] = act(x[row_token] @ w_gate[expert]) * (x[row_token] @ w_up[expert]) on the layout's
+    blocks. Dead row blocks are left unwritten, with skip_padding_rows 32-row groups of padding too."""
     lib = _lib.load()
     _check_gated_weights(x, w_gate, w_up)
     code = _check_activation(activation)
-    for t, name in ((row_token, "row_token"), (row_block_expert, "row_block_expert"), (row_offsets, "row_offsets")):
+    for t, name in ((row_token, "row_token"), (row_block_expert, "row_block_expert"), (row_offsets, "row_offsets"),
+                    (padded_offsets, "padded_offsets")):
         _check_index(t, name)
         _check(t.device == x.device, f"{name} must be on x's GPU")
     num_experts, d_model, ffn_dim = w_gate.shape
     num_row_blocks = row_offsets.numel() - 1
-    _check(row_token.numel() == num_row_blocks * BLOCK and row_block_expert.numel() == num_row_blocks,
-           "the layout does not match block size 128")
+    _check(row_token.numel() == num_row_blocks * BLOCK and row_block_expert.numel() == num_row_blocks and
+           padded_offsets.numel() == num_experts + 1, "the layout does not match block size 128 and the number of experts")
     _check(num_nnz == num_row_blocks * (ffn_dim // BLOCK),
            f"expected {num_row_blocks * (ffn_dim // BLOCK)} blocks (row blocks x F/128), got {num_nnz}")
     with torch.cuda.device(x.device):
         h = torch.empty((num_nnz, BLOCK, BLOCK), dtype=torch.bfloat16, device=x.device)
-        g, u = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
         if num_row_blocks > 0:
+            rows = torch.empty((num_row_blocks * BLOCK, d_model), dtype=torch.bfloat16, device=x.device)
             _lib.check(lib.sb_sdd_gated(_ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(row_token), _ptr(row_block_expert),
-                                        _ptr(row_offsets), _ptr(h), _ptr(g), _ptr(u), x.shape[0], d_model, ffn_dim,
-                                        num_experts, num_row_blocks, code, int(bool(skip_padding_rows)),
+                                        _ptr(row_offsets), _ptr(padded_offsets), _ptr(rows), _ptr(h), x.shape[0], d_model,
+                                        ffn_dim, num_experts, num_row_blocks, code, int(bool(skip_padding_rows)),
                                         _ptr(device_status(x.device)), _stream()))
-    return h, g, u
+    return h
 
 
 def _check_gated_layer(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
@@ -457,7 +456,7 @@ def moe_gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weig
         scratch = torch.empty(sizes[2], dtype=torch.uint8, device=device)
         grads = tuple(torch.empty_like(t) for t in (x, expert_weight, w_gate, w_up, w_down))
         _lib.check(lib.sb_moe_gated_backward(
-            grad_out.data_ptr(), x.data_ptr(), expert_weight.data_ptr(), int(expert_weight.dtype == torch.float32),
+            grad_out.data_ptr(), expert_weight.data_ptr(), int(expert_weight.dtype == torch.float32),
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), state.data_ptr(), state.numel(),
             *(g.data_ptr() for g in grads), num_tokens, k, d_model, ffn_dim, num_experts, code, scratch.data_ptr(), sizes[2],
             device_status(device).data_ptr(), _raw_stream(index)))

@@ -61,7 +61,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sb_moe_gated_bytes": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int, _P]),
     "sb_moe_gated_forward": (c_int, [_P, _P, c_int, _P, c_int, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32,
                                      c_int32, _P, c_int64, _P, c_int64, _P, _P]),
-    "sb_moe_gated_backward": (c_int, [_P, _P, _P, c_int, _P, _P, _P, _P, c_int64, _P, _P, _P, _P, _P, c_int64, c_int32,
+    "sb_moe_gated_backward": (c_int, [_P, _P, c_int, _P, _P, _P, _P, c_int64, _P, _P, _P, _P, _P, c_int64, c_int32,
                                       c_int32, c_int32, c_int32, c_int32, _P, c_int64, _P, _P]),
     "sb_lora_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int]),
     "sb_lora_linear": (c_int, [_P, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int64, c_int32, c_int32, c_int32, c_int32,

@@ -1,13 +1,14 @@
 // The gated expert block of the MoE layer and its backward pass, on the block-sparse layout of sb_route.
 //
-//   forward    G = X Wg[e], U = X Wu[e], H = act(G) * U            (GatedUp; the product H Wd[e] is sb_dsd)
-//   backward   S = dO Wd[e]^T (dO = grad_out of the row's token, before the gate w of its copy is applied)
-//              dgate = sum_f H S, dH = w S, dU = dH act(G), dG = dH U act'(G)                      (GradHidden)
-//              dWd = H^T (w dO), dWg = X^T dG, dWu = X^T dU                                         (GradWeights)
-//              dx[t] = sum over the token's copies of dG Wg^T + dU Wu^T                             (GradRows, join)
+//   forward    G = X Wg[e], U = X Wu[e], H = act(G) * U            (GatedUp; Y = H Wd[e] is sb_dsd)
+//   backward   with dO = grad_out of the row's token and w the gate of its copy:
+//              dgate = dO . Y, dH = (w dO) Wd[e]^T, dU = dH act(G), dG = dH U act'(G)     (grad rows kernel, GradHidden)
+//              dWd = H^T (w dO), dWg = X^T dG, dWu = X^T dU                               (GradWeights)
+//              dx[t] = sum over the token's copies of dG Wg^T + dU Wu^T                   (GradRows, join)
 //
-// dgate comes from S and H, not from Y, so the forward has to keep only G, U and H (bf16); the gate multiplies S in
-// fp32, so dH is not rounded. Roundings to bf16: G, U, H, w dO, dG, dU, the rows of dx before their sum, the results.
+// The forward keeps X (rows in layout order), G, U, H and Y. Everything that is an operand of a product is bf16, as the
+// weights are: G, U, H, Y, w dO, dG, dU and the rows of dx are each rounded once; sums, the activation and its derivative
+// are in fp32. dgate takes Y, not H dH / w, which a gate of 0 would spoil.
 //
 // A decoding step (at most 64 copies, nothing kept) takes another way: no layout, the weights of the picked experts
 // streamed by the kernels of skinny.cuh (SkinnyUp, SkinnyDown, gated_small_combine_kernel).
@@ -78,7 +79,6 @@ struct GatedUp {
     const int32_t* row_offsets;
     const int32_t* row_token;
     const int32_t* row_block_expert;
-    const __nv_bfloat16* x;
     int32_t d_model;
     int32_t activation;
     int32_t skip_padding;  // 32-row groups of padding are not stored
@@ -91,7 +91,7 @@ struct GatedUp {
   struct Early { bool store; };
   static constexpr int kStages = 4, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = false, kExtension = false, kGather = true, kAMnMajor = false, kBMnMajor = true;
+  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -105,18 +105,14 @@ struct GatedUp {
     t.expert = __ldg(p.row_block_expert + t.row_block);
     return t;
   }
-  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t,
+  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
     const uint64_t once = ptx::policy_evict_first();
+    ptx::tma_load_2d(a, &maps.m[5], ks * kTileStep, t.row_block * kTileRows, bar);
     const int32_t row = t.expert * p.d_model + ks * kTileStep;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       ptx::tma_load_2d_hint(b + j * TileSmem::kSlabBytes, &maps.m[j >> 1], t.n0 + (j & 1) * 64, row, bar, once);
-  }
-  static __device__ __forceinline__ const __nv_bfloat16* any_row(const Params& p) { return p.x; }
-  static __device__ __forceinline__ const __nv_bfloat16* gather_row(const Params& p, const Tile& t, int row) {
-    const int32_t token = __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + row);
-    return token >= 0 ? p.x + static_cast<int64_t>(token) * p.d_model : nullptr;
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
     if (p.keep) return {half_has_rows(p.row_token, t.row_block, w.quarter)};
@@ -168,13 +164,10 @@ struct GradHidden {
     const int32_t* row_offsets;
     const int32_t* row_token;
     const int32_t* row_block_expert;
-    const __nv_bfloat16* grad_out;
     const __nv_bfloat16* g;
     const __nv_bfloat16* u;
-    const float* row_gate;
     __nv_bfloat16* dg;
     __nv_bfloat16* du;
-    float* gate_partial;  // [rows, F / 128]
     int32_t d_model, ffn_dim;
     int32_t activation;
   };
@@ -184,8 +177,7 @@ struct GradHidden {
     bool live;
   };
   struct Early {
-    bool store, real;
-    float gate;
+    bool store;
     const __nv_bfloat16* g;  // this row's 128 columns, as U's and the results' are
     const __nv_bfloat16* u;
     int64_t at;
@@ -193,7 +185,7 @@ struct GradHidden {
   };
   static constexpr int kStages = 4, kBuffers = 1;
   static constexpr bool kAhead = true;
-  static constexpr bool kVariable = false, kExtension = false, kGather = true, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -207,25 +199,18 @@ struct GradHidden {
     t.expert = __ldg(p.row_block_expert + t.row_block);
     return t;
   }
-  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t,
+  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
+    ptx::tma_load_2d(a, &maps.m[1], ks * kTileStep, t.row_block * kTileRows, bar);
     // With F an odd multiple of 128 the last tile's upper 128 columns are rows of the next expert (or zeros past the
     // end): computed, never stored.
     ptx::tma_load_2d_hint(b, &maps.m[0], ks * kTileStep, t.expert * p.ffn_dim + t.n0, bar, ptx::policy_evict_first());
-  }
-  static __device__ __forceinline__ const __nv_bfloat16* any_row(const Params& p) { return p.grad_out; }
-  static __device__ __forceinline__ const __nv_bfloat16* gather_row(const Params& p, const Tile& t, int row) {
-    const int32_t token = __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + row);
-    return token >= 0 ? p.grad_out + static_cast<int64_t>(token) * p.d_model : nullptr;
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
     Early e;
     const int32_t n = t.n0 + w.half * 128;
     e.store = n < p.ffn_dim && half_has_rows(p.row_token, t.row_block, w.quarter);
-    e.real = false;
-    e.gate = 0.0f;
     if (!e.store) return e;
-    const int64_t row = static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane;
     e.at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128;
     e.g = p.g + e.at;
     e.u = p.u + e.at;
@@ -234,8 +219,6 @@ struct GradHidden {
       ptx::ld_global_v8(e.g + part * kPart, e.first[part][0]);
       ptx::ld_global_v8(e.u + part * kPart, e.first[part][1]);
     }
-    e.real = __ldg(p.row_token + row) >= 0;
-    e.gate = __ldg(p.row_gate + row);
     return e;
   }
   // The warp's 32 rows of a block are 8 KB in one piece: the next tile's are asked into L2 before this one is worked on,
@@ -255,7 +238,6 @@ struct GradHidden {
   }
   template <int kActivation>
   static __device__ __forceinline__ void work(const Params& p, const Tile& t, const EpilogueWarp& w, const Early& early) {
-    const int32_t n = t.n0 + w.half * 128;
     __nv_bfloat16* dg_row = p.dg + early.at;
     __nv_bfloat16* du_row = p.du + early.at;
     uint32_t held[3][2][8];  // G and U of this part and the next two
@@ -266,7 +248,6 @@ struct GradHidden {
       held[1][0][q] = early.first[1][0][q];
       held[1][1][q] = early.first[1][1][q];
     }
-    float dgate = 0.0f;
 #pragma unroll
     for (int part = 0; part < 128 / kPart; ++part) {
       uint32_t s[16];
@@ -286,18 +267,12 @@ struct GradHidden {
         act_and_slope<kActivation>(gf.y, &a1, &d1);
         const float s0 = __uint_as_float(s[2 * h]);
         const float s1 = __uint_as_float(s[2 * h + 1]);
-        dgate = fmaf(a0 * uf.x, s0, dgate);
-        dgate = fmaf(a1 * uf.y, s1, dgate);
-        const float h0 = s0 * early.gate;
-        const float h1 = s1 * early.gate;
-        dg[h] = early.real ? pack_bf16(h0 * uf.x * d0, h1 * uf.y * d1) : 0u;
-        du[h] = early.real ? pack_bf16(h0 * a0, h1 * a1) : 0u;
+        dg[h] = pack_bf16(s0 * uf.x * d0, s1 * uf.y * d1);
+        du[h] = pack_bf16(s0 * a0, s1 * a1);
       }
       ptx::st_global_v8(dg_row + part * kPart, dg);
       ptx::st_global_v8(du_row + part * kPart, du);
     }
-    if (early.real)
-      p.gate_partial[(static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane) * (p.ffn_dim / 128) + (n >> 7)] = dgate;
   }
 };
 
@@ -318,7 +293,7 @@ struct GradRows {
   struct Early { bool store; };
   static constexpr int kStages = 4, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = false, kExtension = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -366,7 +341,6 @@ struct GradWeights {
   struct Params {
     const int32_t* padded_offsets;
     const int32_t* tokens_per_expert;
-    const int32_t* row_offsets;
     int32_t num_experts, d_model, ffn_dim;
     int32_t down_cols, down_tiles;  // column tiles of dWd [F, D], its tiles per expert
     int32_t up_cols, up_tiles;      // the same of dWg and dWu [D, F]
@@ -378,7 +352,7 @@ struct GradWeights {
   struct Early {};
   static constexpr int kStages = 4, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = false, kExtension = false, kGather = false, kAMnMajor = true, kBMnMajor = true;
+  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = true, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) {
     return p.num_experts * (p.down_tiles + 2 * p.up_tiles);
@@ -402,7 +376,7 @@ struct GradWeights {
     t.live = true;
     t.k_steps = (__ldg(p.tokens_per_expert + t.expert) + kTileStep - 1) / kTileStep;
     t.row0 = __ldg(p.padded_offsets + t.expert);
-    t.block0 = __ldg(p.row_offsets + t.row0 / kTileRows);
+    t.block0 = t.row0 / kTileRows * (p.ffn_dim >> 7);  // the layout's row_offsets, which are regular where rows are
     return t;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
@@ -608,63 +582,99 @@ gated_small_combine_kernel(const float4* __restrict__ y, const void* __restrict_
   out[static_cast<int64_t>(t) * quads + v] = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
 }
 
-// One warp per row of the layout: X[r] = x[token], (w dO)[r] = w * grad_out[token], row_gate[r] = w; zeros for padding.
+// One warp per row of the layout: x_rows[r] = x[token], zeros for padding (the rows that the products' TMA loads want side
+// by side; gathering them inside the products with cp.async took a quarter of their time instead).
 __global__ void __launch_bounds__(kSmallThreads)
-gated_gather_kernel(const uint4* __restrict__ x, const uint4* __restrict__ grad_out, const void* __restrict__ gate,
-                    int gate_dtype, const int32_t* __restrict__ row_token, const int32_t* __restrict__ copy_row,
-                    const int32_t* __restrict__ num_rows, uint4* __restrict__ x_rows, uint4* __restrict__ grad_rows,
-                    float* __restrict__ row_gate, int32_t k, int32_t vecs) {
+gated_rows_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ row_token, const int32_t* __restrict__ num_rows,
+                  uint4* __restrict__ x_rows, int32_t vecs) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int32_t rows = __ldg(num_rows);
+  const int32_t warps = static_cast<int32_t>(gridDim.x * (kSmallThreads / 32));
+  for (int32_t r = static_cast<int32_t>(blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)); r < rows; r += warps) {
+    const int32_t token = __ldg(row_token + r);
+    uint4* dst = x_rows + static_cast<int64_t>(r) * vecs;
+    const uint4* src = x + static_cast<int64_t>(max(token, 0)) * vecs;
+#pragma unroll 4
+    for (int32_t v = lane; v < vecs; v += 32) dst[v] = token >= 0 ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// One warp per row of the layout, for the copy that it is: grad_rows[r] = w grad_out[token], rounded to bf16 (an operand
+// of both gradient products), zeros for padding, and dgate = grad_out[token] . Y[r] in fp32.
+__global__ void __launch_bounds__(kSmallThreads)
+gated_grad_rows_kernel(const uint4* __restrict__ grad_out, const uint4* __restrict__ y_rows, const void* __restrict__ gate,
+                       int gate_dtype, const int32_t* __restrict__ row_token, const int32_t* __restrict__ copy_row,
+                       const int32_t* __restrict__ num_rows, uint4* __restrict__ grad_rows, void* __restrict__ dgate,
+                       int32_t k, int32_t vecs) {
   ptx::grid_launch_dependents();
   const int lane = static_cast<int>(threadIdx.x & 31);
   const int32_t rows = __ldg(num_rows);
   const int32_t warps = static_cast<int32_t>(gridDim.x * (kSmallThreads / 32));
   for (int32_t r = static_cast<int32_t>(blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)); r < rows; r += warps) {
     const int32_t token = __ldg(row_token + r);
-    uint4* xr = x_rows + static_cast<int64_t>(r) * vecs;
-    uint4* gr = grad_rows + static_cast<int64_t>(r) * vecs;
+    uint4* dst = grad_rows + static_cast<int64_t>(r) * vecs;
     if (token < 0) {
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-      for (int32_t v = lane; v < vecs; v += 32) { xr[v] = zero; gr[v] = zero; }
-      if (lane == 0) row_gate[r] = 0.0f;
+      for (int32_t v = lane; v < vecs; v += 32) dst[v] = make_uint4(0u, 0u, 0u, 0u);
       continue;
     }
     // The copy of the token that this row is: the one whose row it is (rows are unique).
-    float w = 0.0f;
+    int64_t copy = 0;
     for (int32_t j0 = 0; j0 < k; j0 += 32) {
       const int32_t j = j0 + lane;
       const bool mine = j < k && __ldg(copy_row + static_cast<int64_t>(token) * k + j) == r;
       const unsigned who = __ballot_sync(0xffffffffu, mine);
       if (who != 0u) {
-        w = gate_at(gate, gate_dtype, static_cast<int64_t>(token) * k + j0 + __ffs(who) - 1);
+        copy = static_cast<int64_t>(token) * k + j0 + __ffs(who) - 1;
         break;
       }
     }
-    if (lane == 0) row_gate[r] = w;
-    const uint4* xs = x + static_cast<int64_t>(token) * vecs;
+    const float w = gate_at(gate, gate_dtype, copy);
     const uint4* gs = grad_out + static_cast<int64_t>(token) * vecs;
+    const uint4* ys = y_rows + static_cast<int64_t>(r) * vecs;
+    float dot = 0.0f;
+#pragma unroll 2
     for (int32_t v = lane; v < vecs; v += 32) {
-      xr[v] = __ldg(xs + v);
-      uint4 raw = __ldg(gs + v);
-      uint32_t* q = reinterpret_cast<uint32_t*>(&raw);
+      const uint4 raw = __ldg(gs + v);
+      const uint4 yraw = __ldg(ys + v);
+      const uint32_t gq[4] = {raw.x, raw.y, raw.z, raw.w};
+      const uint32_t yq[4] = {yraw.x, yraw.y, yraw.z, yraw.w};
+      uint32_t q[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[c]));
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&gq[c]));
+        const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&yq[c]));
+        dot = fmaf(f.x, y.x, dot);
+        dot = fmaf(f.y, y.y, dot);
         q[c] = pack_bf16(f.x * w, f.y * w);
       }
-      gr[v] = raw;
+      dst[v] = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    if (lane == 0) {
+      if (gate_dtype == 1) static_cast<float*>(dgate)[copy] = dot;
+      else static_cast<__nv_bfloat16*>(dgate)[copy] = __float2bfloat16_rn(dot);
     }
   }
 }
 
-// dx[t] = sum over the token's copies of their rows, in copy order in fp32; dgate[t, j] = sum of the row's partial
-// sums in column order. One warp per token.
+// dx[t] = sum over the token's copies of their rows, in copy order in fp32, one warp per token; and zeros into the dgate
+// of copies that have no row.
 __global__ void __launch_bounds__(kSmallThreads)
-gated_join_kernel(const uint4* __restrict__ dx_rows, const float* __restrict__ gate_partial,
-                  const int32_t* __restrict__ copy_row, uint4* __restrict__ dx, void* __restrict__ dgate, int gate_dtype,
-                  int64_t num_tokens, int32_t k, int32_t vecs, int32_t partials) {
+gated_join_kernel(const uint4* __restrict__ dx_rows, const int32_t* __restrict__ copy_row, uint4* __restrict__ dx,
+                  void* __restrict__ dgate, int gate_dtype, int64_t num_tokens, int32_t k, int32_t vecs) {
+  ptx::grid_dependency_wait();
   const int lane = static_cast<int>(threadIdx.x & 31);
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kSmallThreads / 32);
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kSmallThreads / 32) + (threadIdx.x >> 5); t < num_tokens; t += warps) {
+    for (int32_t j = lane; j < k; j += 32) {
+      if (__ldg(copy_row + t * k + j) >= 0) continue;
+      if (gate_dtype == 1) static_cast<float*>(dgate)[t * k + j] = 0.0f;
+      else static_cast<__nv_bfloat16*>(dgate)[t * k + j] = __float2bfloat16_rn(0.0f);
+    }
+#pragma unroll 2
     for (int32_t v = lane; v < vecs; v += 32) {
       float acc[8];
 #pragma unroll
@@ -672,7 +682,7 @@ gated_join_kernel(const uint4* __restrict__ dx_rows, const float* __restrict__ g
       for (int32_t j = 0; j < k; ++j) {
         const int32_t row = __ldg(copy_row + t * k + j);
         if (row < 0) continue;
-        const uint4 raw = __ldg(dx_rows + static_cast<int64_t>(row) * vecs + v);
+        const uint4 raw = __ldcg(dx_rows + static_cast<int64_t>(row) * vecs + v);
         const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -686,18 +696,6 @@ gated_join_kernel(const uint4* __restrict__ dx_rows, const float* __restrict__ g
 #pragma unroll
       for (int q = 0; q < 4; ++q) o[q] = pack_bf16(acc[2 * q], acc[2 * q + 1]);
       dx[t * vecs + v] = packed;
-    }
-    for (int32_t j = 0; j < k; ++j) {
-      const int32_t row = __ldg(copy_row + t * k + j);
-      float sum = 0.0f;
-      if (row >= 0)
-        for (int32_t b = lane; b < partials; b += 32) sum += __ldg(gate_partial + static_cast<int64_t>(row) * partials + b);
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == 0) {
-        if (gate_dtype == 1) static_cast<float*>(dgate)[t * k + j] = sum;
-        else static_cast<__nv_bfloat16*>(dgate)[t * k + j] = __float2bfloat16_rn(sum);
-      }
     }
   }
 }
@@ -736,20 +734,30 @@ bool any_null(std::initializer_list<const void*> ptrs) {
   return false;
 }
 
-int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
-                            const int32_t* row_block_expert, const int32_t* row_offsets, void* h_blocks, void* g_blocks,
-                            void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
-                            int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
-                            cudaStream_t stream) {
-  if (int rc = check_gated("sdd_gated", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
-  if (num_row_blocks == 0) return SB_OK;
-  if (any_null({x, w_gate, w_up, row_token, row_block_expert, row_offsets, h_blocks}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: NULL buffer");
-  if ((g_blocks == nullptr) != (u_blocks == nullptr))
-    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: pass both kept arrays or neither");
-  if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: T must be positive");
-  if (any_misaligned({x, w_gate, w_up, h_blocks, g_blocks, u_blocks}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: x, the weights and the blocks must be 16-byte aligned");
+// Launches one of the small kernels with programmatic dependence.
+template <class... Params, class... Args>
+int launch_small(void (*kernel)(Params...), int64_t blocks, int threads, cudaStream_t stream, const char* what, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  if (err != cudaSuccess) return fail(SB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
+  return SB_OK;
+}
+
+// x_rows, then H (and G, U) on the layout; num_rows: the real row count on the device.
+int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token, const int32_t* row_block_expert,
+              const int32_t* row_offsets, const int32_t* num_rows, void* x_rows, void* h_blocks, void* g_blocks,
+              void* u_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
+              int32_t activation, int skip_padding_rows, int32_t* dev_status, cudaStream_t stream) {
+  const DeviceInfo* info = current_device_info();
+  if (info == nullptr) return SB_ERR_CUDA;
   const uint64_t w_rows = static_cast<uint64_t>(num_experts) * d_model;
   const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;  // nnz * 128
   TileMaps maps{};
@@ -760,89 +768,64 @@ int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t
     if (int rc = encode_2d_map(&maps.m[3], g_blocks, b_rows, 128, 32, 64, 2, "sdd_gated (kept gate)")) return rc;
     if (int rc = encode_2d_map(&maps.m[4], u_blocks, b_rows, 128, 32, 64, 2, "sdd_gated (kept up)")) return rc;
   }
+  if (int rc = encode_2d_map(&maps.m[5], x_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, "sdd_gated (rows)")) return rc;
+  const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
+  if (int rc = launch_small(gated_rows_kernel, blocks, kSmallThreads, stream, "sdd_gated (rows)", static_cast<const uint4*>(x),
+                            row_token, num_rows, static_cast<uint4*>(x_rows), d_model / 8))
+    return rc;
   GatedUp::Params p{};
   p.order = {num_row_blocks, ffn_dim / 128, band_for(num_row_blocks, num_experts)};
   p.row_offsets = row_offsets;
   p.row_token = row_token;
   p.row_block_expert = row_block_expert;
-  p.x = static_cast<const __nv_bfloat16*>(x);
   p.d_model = d_model;
   p.activation = activation;
   p.skip_padding = skip_padding_rows ? 1 : 0;
   p.keep = g_blocks != nullptr ? 1 : 0;
-  return launch_tile_gemm<GatedUp>(maps, p, static_cast<int64_t>(num_row_blocks) * (ffn_dim / 128), dev_status,
-                                   stream, "sdd_gated");
+  return launch_tile_gemm<GatedUp>(maps, p, static_cast<int64_t>(num_row_blocks) * (ffn_dim / 128), dev_status, stream, "sdd_gated");
 }
 
-int gated_gather(const void* x, const void* grad_out, const void* gate, int gate_dtype,
-                               const int32_t* row_token, const int32_t* copy_row, const int32_t* padded_offsets,
-                               int32_t num_experts, void* x_rows, void* grad_rows, float* row_gate, int64_t num_tokens,
-                               int32_t k, int32_t d_model, int32_t num_row_blocks, cudaStream_t stream) {
-  if (int rc = check_gated("gated_gather", d_model, 128, num_experts, num_row_blocks, 0)) return rc;
-  if (num_row_blocks == 0) return SB_OK;
-  if (any_null({x, grad_out, gate, row_token, copy_row, padded_offsets, x_rows, grad_rows, row_gate}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: NULL buffer");
-  if (num_tokens <= 0 || k <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: T and k must be positive");
-  if (gate_dtype != 0 && gate_dtype != 1) return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: gate_dtype must be 0 (bf16) or 1 (fp32)");
-  if (any_misaligned({x, grad_out, x_rows, grad_rows}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_gather: rows must be 16-byte aligned");
+int gated_grad_rows_of(const void* grad_out, const void* y_rows, const void* gate, int gate_dtype, const int32_t* row_token,
+                       const int32_t* copy_row, const int32_t* num_rows, void* grad_rows, void* dgate, int32_t k,
+                       int32_t d_model, int32_t num_row_blocks, cudaStream_t stream) {
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
-  gated_gather_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, stream>>>(
-      static_cast<const uint4*>(x), static_cast<const uint4*>(grad_out), gate, gate_dtype, row_token, copy_row,
-      padded_offsets + num_experts, static_cast<uint4*>(x_rows), static_cast<uint4*>(grad_rows), row_gate, k, d_model / 8);
-  return check_launch("gated_gather");
+  gated_grad_rows_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, stream>>>(
+      static_cast<const uint4*>(grad_out), static_cast<const uint4*>(y_rows), gate, gate_dtype, row_token, copy_row, num_rows,
+      static_cast<uint4*>(grad_rows), dgate, k, d_model / 8);
+  return check_launch("moe_gated_backward (rows)");
 }
 
-int gated_grad_hidden(const void* grad_out, const void* w_down, const void* g_blocks, const void* u_blocks,
-                                    const float* row_gate, const int32_t* row_token, const int32_t* row_block_expert,
-                                    const int32_t* row_offsets, void* dg_blocks, void* du_blocks, float* gate_partial,
-                                    int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
-                                    int32_t num_row_blocks, int32_t activation, int32_t* dev_status, cudaStream_t stream) {
-  if (int rc = check_gated("gated_grad_hidden", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
-  if (num_row_blocks == 0) return SB_OK;
-  if (any_null({grad_out, w_down, g_blocks, u_blocks, row_gate, row_token, row_block_expert, row_offsets, dg_blocks,
-                du_blocks, gate_partial}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: NULL buffer");
-  if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: T must be positive");
-  if (any_misaligned({grad_out, w_down, g_blocks, u_blocks, dg_blocks, du_blocks}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_hidden: buffers must be 16-byte aligned");
+int gated_grad_hidden(const void* grad_rows, const void* w_down, const void* g_blocks, const void* u_blocks,
+                      const int32_t* row_token, const int32_t* row_block_expert, const int32_t* row_offsets, void* dg_blocks,
+                      void* du_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
+                      int32_t activation, int32_t* dev_status, cudaStream_t stream) {
+  const char* what = "moe_gated_backward (hidden)";
   TileMaps maps{};
-  if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, 256, 64, 2, "gated_grad_hidden (w_down)")) return rc;
+  if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, 256, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[1], grad_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, what)) return rc;
   GradHidden::Params p{};
   const int32_t slices = (ffn_dim + kTileCols - 1) / kTileCols;
   p.order = {num_row_blocks, slices, band_for(num_row_blocks, num_experts)};
   p.row_offsets = row_offsets;
   p.row_token = row_token;
   p.row_block_expert = row_block_expert;
-  p.grad_out = static_cast<const __nv_bfloat16*>(grad_out);
   p.g = static_cast<const __nv_bfloat16*>(g_blocks);
   p.u = static_cast<const __nv_bfloat16*>(u_blocks);
-  p.row_gate = row_gate;
   p.dg = static_cast<__nv_bfloat16*>(dg_blocks);
   p.du = static_cast<__nv_bfloat16*>(du_blocks);
-  p.gate_partial = gate_partial;
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
   p.activation = activation;
-  return launch_tile_gemm<GradHidden>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream,
-                                      "gated_grad_hidden");
+  return launch_tile_gemm<GradHidden>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
 }
 
 int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_blocks, const void* dg_blocks,
-                                     const void* du_blocks, const int32_t* padded_offsets, const int32_t* tokens_per_expert,
-                                     const int32_t* row_offsets, void* dw_gate, void* dw_up, void* dw_down, int32_t d_model,
-                                     int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status,
-                                     cudaStream_t stream) {
-  if (int rc = check_gated("gated_grad_weights", d_model, ffn_dim, num_experts, num_row_blocks, 0)) return rc;
-  if (num_row_blocks <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_weights: the layout has no row blocks");
-  if (any_null({x_rows, grad_rows, h_blocks, dg_blocks, du_blocks, padded_offsets, tokens_per_expert, row_offsets, dw_gate,
-                dw_up, dw_down}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_weights: NULL buffer");
-  if (any_misaligned({x_rows, grad_rows, h_blocks, dg_blocks, du_blocks, dw_gate, dw_up, dw_down}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_weights: buffers must be 16-byte aligned");
-  const char* what = "gated_grad_weights";
+                       const void* du_blocks, const int32_t* padded_offsets, const int32_t* tokens_per_expert, void* dw_gate,
+                       void* dw_up, void* dw_down, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                       int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
+  const char* what = "moe_gated_backward (weights)";
   const uint64_t rows = static_cast<uint64_t>(num_row_blocks) * kTileRows;
   const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
   const uint64_t up_rows = static_cast<uint64_t>(num_experts) * d_model;
@@ -859,7 +842,6 @@ int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_
   GradWeights::Params p{};
   p.padded_offsets = padded_offsets;
   p.tokens_per_expert = tokens_per_expert;
-  p.row_offsets = row_offsets;
   p.num_experts = num_experts;
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
@@ -871,17 +853,10 @@ int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_
   return launch_tile_gemm<GradWeights>(maps, p, tiles, dev_status, stream, what);
 }
 
-int gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up,
-                                  const int32_t* row_token, const int32_t* row_block_expert, const int32_t* row_offsets,
-                                  void* dx_rows, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
-                                  int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
-  if (int rc = check_gated("gated_grad_rows", d_model, ffn_dim, num_experts, num_row_blocks, 0)) return rc;
-  if (num_row_blocks == 0) return SB_OK;
-  if (any_null({dg_blocks, du_blocks, w_gate, w_up, row_token, row_block_expert, row_offsets, dx_rows}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_rows: NULL buffer");
-  if (any_misaligned({dg_blocks, du_blocks, w_gate, w_up, dx_rows}))
-    return fail(SB_ERR_INVALID_ARGUMENT, "gated_grad_rows: buffers must be 16-byte aligned");
-  const char* what = "gated_grad_rows";
+int gated_grad_x(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up, const int32_t* row_token,
+                 const int32_t* row_block_expert, const int32_t* row_offsets, void* dx_rows, int32_t d_model,
+                 int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
+  const char* what = "moe_gated_backward (x)";
   const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
   const uint64_t w_rows = static_cast<uint64_t>(num_experts) * d_model;
   TileMaps maps{};
@@ -901,21 +876,14 @@ int gated_grad_rows(const void* dg_blocks, const void* du_blocks, const void* w_
   return launch_tile_gemm<GradRows>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
 }
 
-int gated_join(const void* dx_rows, const float* gate_partial, const int32_t* copy_row, void* dx, void* dgate,
-                             int gate_dtype, int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim,
-                             cudaStream_t stream) {
-  if (int rc = check_gated("gated_join", d_model, ffn_dim, 1, 0, 0)) return rc;
-  if (any_null({dx_rows, gate_partial, copy_row, dx, dgate})) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: NULL buffer");
-  if (num_tokens <= 0 || k <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: T and k must be positive");
-  if (gate_dtype != 0 && gate_dtype != 1) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: gate_dtype must be 0 (bf16) or 1 (fp32)");
-  if (any_misaligned({dx_rows, dx})) return fail(SB_ERR_INVALID_ARGUMENT, "gated_join: rows must be 16-byte aligned");
+int gated_join(const void* dx_rows, const int32_t* copy_row, void* dx, void* dgate, int gate_dtype, int64_t num_tokens,
+               int32_t k, int32_t d_model, cudaStream_t stream) {
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
   const int64_t blocks = std::min<int64_t>((num_tokens + 7) / 8, static_cast<int64_t>(info->sm_count) * 8);
-  gated_join_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, stream>>>(
-      static_cast<const uint4*>(dx_rows), gate_partial, copy_row, static_cast<uint4*>(dx), dgate, gate_dtype, num_tokens, k,
-      d_model / 8, ffn_dim / 128);
-  return check_launch("gated_join");
+  return launch_small(gated_join_kernel, blocks, kSmallThreads, stream, "moe_gated_backward (join)",
+                      static_cast<const uint4*>(dx_rows), copy_row, static_cast<uint4*>(dx), dgate, gate_dtype, num_tokens, k,
+                      d_model / 8);
 }
 
 bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
@@ -932,10 +900,10 @@ struct GatedBuffers {
   int32_t row_blocks, ffn_blocks;
   // state (keep) or scratch: the layout's arrays, then the blocks
   int64_t tokens_per_expert, padded_offsets, row_token, copy_row, row_block_expert, row_offsets, col_indices, error, work;
-  int64_t h, g, u, y;
+  int64_t x_rows, h, g, u, y;
   int64_t state_bytes, scratch_bytes;
   // scratch of the backward pass
-  int64_t x_rows, grad_rows, row_gate, gate_partial, dg, du, backward_bytes;
+  int64_t grad_rows, dg, du, backward_bytes;
 };
 
 int gated_buffers(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int keep,
@@ -971,6 +939,8 @@ int gated_buffers(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_di
   b->row_offsets = take((row_blocks + 1) * 4);
   b->col_indices = take(row_blocks * ffn_blocks * 4);
   b->error = take(4);
+  b->x_rows = take(rows * d_model * 2);
+  b->y = take(rows * d_model * 2);
   b->h = take(rows * ffn_dim * 2);
   if (keep) {
     b->g = take(rows * ffn_dim * 2);
@@ -978,14 +948,10 @@ int gated_buffers(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_di
     b->state_bytes = at;
     at = 0;
   }
-  b->work = take(static_cast<int64_t>(sb_route_workspace_bytes(n, num_experts)));
-  b->y = take(rows * d_model * 2);
+  b->work = take(std::max<int64_t>(4, static_cast<int64_t>(sb_route_workspace_bytes(n, num_experts))));  // never NULL
   b->scratch_bytes = at;
   at = 0;
-  b->x_rows = take(rows * d_model * 2);
   b->grad_rows = take(rows * d_model * 2);
-  b->row_gate = take(rows * 4);
-  b->gate_partial = take(rows * ffn_blocks * 4);
   b->dg = take(rows * ffn_dim * 2);
   b->du = take(rows * ffn_dim * 2);
   b->backward_bytes = at;
@@ -1057,13 +1023,21 @@ int forward_small(const GatedBuffers& b, const void* x, const void* expert_idx, 
 using namespace sb;
 
 extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
-                            const int32_t* row_block_expert, const int32_t* row_offsets, void* h_blocks, void* g_blocks,
-                            void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
-                            int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
-                            sb_stream_t stream) {
+                            const int32_t* row_block_expert, const int32_t* row_offsets, const int32_t* padded_offsets,
+                            void* x_rows, void* h_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim,
+                            int32_t num_experts, int32_t num_row_blocks, int32_t activation, int skip_padding_rows,
+                            int32_t* dev_status, sb_stream_t stream) {
   clear_error();
-  return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, row_offsets, h_blocks, g_blocks, u_blocks, num_tokens,
-                   d_model, ffn_dim, num_experts, num_row_blocks, activation, skip_padding_rows, dev_status, as_stream(stream));
+  if (int rc = check_gated("sdd_gated", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
+  if (num_row_blocks == 0) return SB_OK;
+  if (any_null({x, w_gate, w_up, row_token, row_block_expert, row_offsets, padded_offsets, x_rows, h_blocks}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: NULL buffer");
+  if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: T must be positive");
+  if (any_misaligned({x, w_gate, w_up, x_rows, h_blocks}))
+    return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: x, the weights, the rows and the blocks must be 16-byte aligned");
+  return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, row_offsets, padded_offsets + num_experts, x_rows, h_blocks,
+                   nullptr, nullptr, d_model, ffn_dim, num_experts, num_row_blocks, activation, skip_padding_rows, dev_status,
+                   as_stream(stream));
 }
 
 extern "C" int sb_moe_gated_bytes(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
@@ -1106,18 +1080,19 @@ extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int i
                         ints(b.tokens_per_expert), ints(b.padded_offsets), ints(b.row_token), ints(b.copy_row),
                         ints(b.row_block_expert), ints(b.row_offsets), ints(b.col_indices), ints(b.error), temp + b.work, stream))
     return rc;
-  if (int rc = sdd_gated(x, w_gate, w_up, ints(b.row_token), ints(b.row_block_expert), ints(b.row_offsets), base + b.h,
-                         keep ? base + b.g : nullptr, keep ? base + b.u : nullptr, num_tokens, d_model, ffn_dim, num_experts,
-                         b.row_blocks, activation, 1, dev_status, as_stream(stream)))
+  if (int rc = sdd_gated(x, w_gate, w_up, ints(b.row_token), ints(b.row_block_expert), ints(b.row_offsets),
+                         ints(b.padded_offsets) + num_experts, base + b.x_rows, base + b.h, keep ? base + b.g : nullptr,
+                         keep ? base + b.u : nullptr, d_model, ffn_dim, num_experts, b.row_blocks, activation, 1, dev_status,
+                         as_stream(stream)))
     return rc;
   if (int rc = sb_dsd(base + b.h, static_cast<int64_t>(b.row_blocks) * b.ffn_blocks, w_down,
                       static_cast<int64_t>(num_experts) * ffn_dim, d_model, ints(b.row_offsets), ints(b.col_indices),
-                      b.row_blocks, 128, 0, ints(b.row_token), temp + b.y, ints(b.padded_offsets), num_experts, dev_status, stream))
+                      b.row_blocks, 128, 0, ints(b.row_token), base + b.y, ints(b.padded_offsets), num_experts, dev_status, stream))
     return rc;
-  return sb_combine(temp + b.y, ints(b.copy_row), gate, gate_dtype, out, num_tokens, k, d_model, stream);
+  return sb_combine(base + b.y, ints(b.copy_row), gate, gate_dtype, out, num_tokens, k, d_model, stream);
 }
 
-extern "C" int sb_moe_gated_backward(const void* grad_out, const void* x, const void* gate, int gate_dtype,
+extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int gate_dtype,
                                      const void* w_gate, const void* w_up, const void* w_down, const void* state,
                                      int64_t state_bytes, void* dx, void* dgate, void* dw_gate, void* dw_up, void* dw_down,
                                      int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
@@ -1126,10 +1101,13 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* x, const 
   clear_error();
   GatedBuffers b;
   if (int rc = gated_buffers(num_tokens, k, d_model, ffn_dim, num_experts, 1, &b)) return rc;
-  if (any_null({grad_out, x, gate, w_gate, w_up, w_down, state, dx, dgate, dw_gate, dw_up, dw_down, scratch}))
+  if (int rc = check_gated("moe_gated_backward", d_model, ffn_dim, num_experts, b.row_blocks, activation)) return rc;
+  if (gate_dtype != 0 && gate_dtype != 1)
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: gate_dtype must be 0 (bf16) or 1 (fp32)");
+  if (any_null({grad_out, gate, w_gate, w_up, w_down, state, dx, dgate, dw_gate, dw_up, dw_down, scratch}))
     return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: NULL buffer");
-  if (!aligned256(state) || !aligned256(scratch))
-    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: state and scratch must be 256-byte aligned");
+  if (any_misaligned({grad_out, w_gate, w_up, w_down, dx, dw_gate, dw_up, dw_down}) || !aligned256(state) || !aligned256(scratch))
+    return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: buffers must be 16-byte aligned, state and scratch 256-byte aligned");
   if (state_bytes < b.state_bytes || scratch_bytes < b.backward_bytes)
     return fail(SB_ERR_INVALID_ARGUMENT, "moe_gated_backward: the buffers have %lld and %lld bytes, %lld and %lld are needed",
                 (long long)state_bytes, (long long)scratch_bytes, (long long)b.state_bytes, (long long)b.backward_bytes);
@@ -1138,22 +1116,20 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* x, const 
   const cudaStream_t st = as_stream(stream);
   auto ints = [base](int64_t at) { return reinterpret_cast<const int32_t*>(base + at); };
   const int32_t* row_token = ints(b.row_token);
-  float* row_gate = reinterpret_cast<float*>(temp + b.row_gate);
-  float* gate_partial = reinterpret_cast<float*>(temp + b.gate_partial);
-  if (int rc = gated_gather(x, grad_out, gate, gate_dtype, row_token, ints(b.copy_row), ints(b.padded_offsets), num_experts,
-                            temp + b.x_rows, temp + b.grad_rows, row_gate, num_tokens, k, d_model, b.row_blocks, st))
+  if (int rc = gated_grad_rows_of(grad_out, base + b.y, gate, gate_dtype, row_token, ints(b.copy_row),
+                                  ints(b.padded_offsets) + num_experts, temp + b.grad_rows, dgate, k, d_model, b.row_blocks, st))
     return rc;
-  if (int rc = gated_grad_hidden(grad_out, w_down, base + b.g, base + b.u, row_gate, row_token, ints(b.row_block_expert),
-                                 ints(b.row_offsets), temp + b.dg, temp + b.du, gate_partial, num_tokens, d_model, ffn_dim,
-                                 num_experts, b.row_blocks, activation, dev_status, st))
+  if (int rc = gated_grad_hidden(temp + b.grad_rows, w_down, base + b.g, base + b.u, row_token, ints(b.row_block_expert),
+                                 ints(b.row_offsets), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
+                                 activation, dev_status, st))
     return rc;
-  if (int rc = gated_grad_weights(temp + b.x_rows, temp + b.grad_rows, base + b.h, temp + b.dg, temp + b.du,
-                                  ints(b.padded_offsets), ints(b.tokens_per_expert), ints(b.row_offsets), dw_gate, dw_up,
-                                  dw_down, d_model, ffn_dim, num_experts, b.row_blocks, dev_status, st))
+  if (int rc = gated_grad_weights(base + b.x_rows, temp + b.grad_rows, base + b.h, temp + b.dg, temp + b.du,
+                                  ints(b.padded_offsets), ints(b.tokens_per_expert), dw_gate, dw_up, dw_down, d_model,
+                                  ffn_dim, num_experts, b.row_blocks, dev_status, st))
     return rc;
-  // The rows of dx take the place of the gathered rows of x, which the weight gradients were the last to read.
-  if (int rc = gated_grad_rows(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert),
-                               ints(b.row_offsets), temp + b.x_rows, d_model, ffn_dim, num_experts, b.row_blocks, dev_status, st))
+  // The rows of dx take the place of grad_rows, which the weight gradients were the last to read.
+  if (int rc = gated_grad_x(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert), ints(b.row_offsets),
+                            temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks, dev_status, st))
     return rc;
-  return gated_join(temp + b.x_rows, gate_partial, ints(b.copy_row), dx, dgate, gate_dtype, num_tokens, k, d_model, ffn_dim, st);
+  return gated_join(temp + b.grad_rows, ints(b.copy_row), dx, dgate, gate_dtype, num_tokens, k, d_model, st);
 }

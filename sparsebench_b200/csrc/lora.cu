@@ -140,7 +140,7 @@ struct LoraShrink {
   struct Early { int32_t slot; };
   static constexpr int kStages = 4, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = true, kExtension = false, kGather = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.row_tiles * p.groups * p.splits; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -249,7 +249,7 @@ struct LoraExpand {
   struct Early { int32_t loner; };  // this row's adapter when its B is not finite, else -1
   static constexpr int kStages = 4, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = true, kExtension = true, kGather = false, kAMnMajor = false, kBMnMajor = true;
+  static constexpr bool kVariable = true, kExtension = true, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {

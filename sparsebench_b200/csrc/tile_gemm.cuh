@@ -3,7 +3,7 @@
 //
 // One output tile = 128 rows x 256 columns, accumulated in fp32 in TMEM (two accumulators, so the epilogue of one
 // tile runs while the tensor cores fill the other). K steps of 64. Warp roles, with nothing but mbarriers between
-// them: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue, warps 10-13 row gather (policies that gather).
+// them: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue, warps 10-13 extension rows of A (policies that have them).
 //
 // A stage of the shared-memory ring holds A (16 KB) and B (32 KB) with the 128-byte swizzle, each in one of two forms:
 //   K-major   rows of the M (N) dimension, 64 K elements = 128 bytes per row
@@ -103,9 +103,8 @@ struct BandOrder {
 
 // A policy Op has
 //   Params, Tile (with int32_t k_steps: 0 = nothing to multiply; bool live: the epilogue has something to do)
-//   static constexpr bool kGather, kAMnMajor, kBMnMajor
+//   static constexpr bool kAMnMajor, kBMnMajor
 //   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar), tx_bytes
-//   gather_row(p, tile, row) -> source row of A or nullptr (zeros), for kGather; any_row(p): a readable address
 //   static constexpr int kStages (of the ring), kBuffers (staging tiles per epilogue warp)
 //   With kExtension: Tile has base_steps; A of the K steps behind them is written by four warps from registers:
 //   Rows rows(p, tile, row0) once per tile, extension_chunk(p, tile, rows, j, row, ks, chunk) = the 16 bytes of chunk
@@ -113,10 +112,9 @@ struct BandOrder {
 //   With kVariable: columns(p) <= 256 (a multiple of 16) accumulator columns in use, tx_bytes(p, tile, ks) per stage
 template <class Op>
 struct TileConfig {
-  static constexpr int kGatherWarps = Op::kGather || Op::kExtension ? 4 : 0;
-  static constexpr int kFirstGatherWarp = 2 + TileSmem::kEpilogueWarps;
-  static constexpr int kThreads = 32 * (kFirstGatherWarp + kGatherWarps);
-  static constexpr uint32_t kFullArrivals = Op::kGather ? 1 + 32 * kGatherWarps : 1;
+  static constexpr int kExtensionWarps = Op::kExtension ? 4 : 0;
+  static constexpr int kFirstExtensionWarp = 2 + TileSmem::kEpilogueWarps;
+  static constexpr int kThreads = 32 * (kFirstExtensionWarp + kExtensionWarps);
   static constexpr int kSmemBytes = 1024 + Op::kStages * (TileSmem::kABytes + TileSmem::kBBytes) +
                                     TileSmem::kEpilogueWarps * Op::kBuffers * TileSmem::kStagingBytes + TileSmem::kBarrierBytes;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
@@ -149,11 +147,11 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Op::kStages; ++s) {
-      ptx::mbar_init(full_bar + 8 * s, Cfg::kFullArrivals);
+      ptx::mbar_init(full_bar + 8 * s, 1);
       ptx::mbar_init(empty_bar + 8 * s, 1);
       if (Op::kExtension) {
         ptx::mbar_init(go_bar + 8 * s, 1);
-        ptx::mbar_init(ready_bar + 8 * s, Cfg::kGatherWarps);
+        ptx::mbar_init(ready_bar + 8 * s, Cfg::kExtensionWarps);
       }
     }
     for (int a = 0; a < 2; ++a) {
@@ -205,7 +203,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
             if (ks >= tile.base_steps) ptx::mbar_arrive(go_bar + 8 * stage);
           }
           if constexpr (Op::kVariable) ptx::mbar_arrive_expect_tx(bar, Op::tx_bytes(p, tile, ks));
-          else ptx::mbar_arrive_expect_tx(bar, S::kBBytes + (Op::kGather ? 0 : S::kABytes));
+          else ptx::mbar_arrive_expect_tx(bar, S::kBBytes + S::kABytes);
           Op::load(maps, p, tile, ks, a_base + stage * S::kABytes, b_base + stage * S::kBBytes, bar);
           if (++stage == Op::kStages) { stage = 0; phase ^= 1u; }
         }
@@ -248,7 +246,6 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
             }
             ready_phases ^= 1u << stage;
           }
-          if (Op::kGather) ptx::fence_proxy_async_shared();  // rows written by cp.async, read by the tensor core
           ptx::tcgen05_fence_after_sync();
           const uint32_t a_addr = a_base + stage * S::kABytes;
           const uint32_t b_addr = b_base + stage * S::kBBytes;
@@ -269,7 +266,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
         if (acc == 0) acc_phase ^= 1u;
       }
     }
-  } else if (warp < Cfg::kFirstGatherWarp) {
+  } else if (warp < Cfg::kFirstExtensionWarp) {
     // ---------------------------------------------------------------- epilogue
     EpilogueWarp w;
     w.quarter = warp & 3;
@@ -278,13 +275,17 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     w.staging = staging_base + static_cast<uint32_t>(warp - 2) * (Op::kBuffers * S::kStagingBytes);
     w.buffer = 0;
     uint32_t acc = 0, acc_phase = 0;
+    typename Op::Tile next{};
+    if (static_cast<int32_t>(blockIdx.x) < total) next = Op::tile(p, blockIdx.x);
     for (int32_t index = blockIdx.x; index < total; index += step) {
-      const typename Op::Tile tile = Op::tile(p, index);
-      if constexpr (Op::kAhead) {
-        if (index + step < total) Op::ahead(p, Op::tile(p, index + step), w);
+      const typename Op::Tile tile = next;
+      typename Op::Early early{};
+      if (tile.live) early = Op::prefetch(p, tile, w);
+      if (index + step < total) {
+        next = Op::tile(p, index + step);
+        if constexpr (Op::kAhead) Op::ahead(p, next, w);
       }
       if (!tile.live) continue;
-      const typename Op::Early early = Op::prefetch(p, tile, w);
       if (tile.k_steps > 0) {
         if (!ptx::mbar_wait_bounded(acc_full_bar + 8 * acc, acc_phase, abort_word)) {
           give_up(SB_DEV_TIMEOUT_EPILOGUE);
@@ -303,54 +304,11 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     }
     if (lane == 0) ptx::bulk_wait_all();
   } else {
-    // ---------------------------------------------------------------- row gather
-    if constexpr (Op::kGather) {
-      // Eight lanes share a row (its 128 bytes of the K step), a warp instruction moves four rows; warp gw covers
-      // rows j * 16 + gw * 4 + lane / 8. Rows without a source use the zero-fill form, which reads nothing.
-      const int gw = warp - Cfg::kFirstGatherWarp;
-      const int row0 = gw * 4 + (lane >> 3);
-      const uint32_t chunk = static_cast<uint32_t>(lane & 7);
-      const uint32_t dst_off = static_cast<uint32_t>(row0) * 128u + ((chunk ^ static_cast<uint32_t>(row0 & 7)) << 4);
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      int32_t index = blockIdx.x;
-      typename Op::Tile next{};
-      const __nv_bfloat16* next_src[8];
-      auto fetch = [&](int32_t at) {
-        next = Op::tile(p, at);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) next_src[j] = next.k_steps > 0 ? Op::gather_row(p, next, row0 + j * 16) : nullptr;
-      };
-      if (index < total) fetch(index);
-      for (; ok && index < total; index += step) {
-        const int32_t k_steps = next.k_steps;
-        const __nv_bfloat16* src[8];
-        bool real[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          real[j] = next_src[j] != nullptr;
-          src[j] = (real[j] ? next_src[j] : Op::any_row(p)) + chunk * 8;  // padding still passes a valid address
-        }
-        if (index + step < total) fetch(index + step);
-        for (int32_t ks = 0; ks < k_steps; ++ks) {
-          if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
-            give_up(SB_DEV_TIMEOUT_PRODUCER);
-            ok = false;
-            break;
-          }
-          const uint32_t dst = a_base + stage * S::kABytes + dst_off;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ptx::cp_async_16_zfill(dst + j * 2048, src[j] + ks * kTileStep, real[j]);
-          ptx::cp_async_mbar_arrive_noinc(full_bar + 8 * stage);
-          if (++stage == Op::kStages) { stage = 0; phase ^= 1u; }
-        }
-      }
-      ptx::cp_async_wait_all();
-    }
+    // ---------------------------------------------------------------- extension rows of A
     if constexpr (Op::kExtension) {
-      // The same rows and chunks, for the steps behind the base steps only. The producer says when a stage is free
+      // Eight lanes share a row's 128 bytes of the K step; rows j * 16 + warp * 4 + lane / 8. The producer says when a stage is free
       // (its own wait on empty_bar passed), so that these warps need not follow the ring through the base steps.
-      const int row0 = (warp - Cfg::kFirstGatherWarp) * 4 + (lane >> 3);
+      const int row0 = (warp - Cfg::kFirstExtensionWarp) * 4 + (lane >> 3);
       const int chunk = lane & 7;
       const uint32_t dst_off = static_cast<uint32_t>(row0) * 128u + (static_cast<uint32_t>(chunk ^ (row0 & 7)) << 4);
       uint32_t stage = 0, go_phases = 0;

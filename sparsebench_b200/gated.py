@@ -19,9 +19,9 @@ from sparsebench_b200 import _C
 
 @dataclass(frozen=True)
 class GatedSaved:
-    """What moe_forward_gated_saved keeps for moe_backward_gated: the inputs by reference (they must still hold the
-    same values then) and the layout with the blocks of H, G and U (3 * rows * F bf16). state is None for an empty
-    batch."""
+    """What moe_forward_gated_saved keeps for moe_backward_gated: the inputs by reference (the gates and
+    weights must still hold the same values then) and, in one buffer, the layout, x and Y in its order and the blocks of
+    H, G and U (rows * (2 D + 3 F) bf16). state is None for an empty batch."""
 
     x: torch.Tensor
     expert_weight: torch.Tensor
