@@ -70,15 +70,43 @@ __device__ __forceinline__ bool half_has_rows(const int32_t* row_token, int32_t 
   return __ldg(row_token + static_cast<int64_t>(row_block) * kTileRows + (quarter & 2) * 32) >= 0;
 }
 
+// Tile order of the products over (row block, column slice): expert by expert, in an expert bands of up to kBand row
+// blocks, in a band the row block changes fastest. The thread blocks that run at the same time then work on few column
+// slices of one expert's weights for all of its row blocks: a weight tile comes from memory once and from L2 for the
+// other row blocks. (Bands of a fixed height over all row blocks straddled the experts: about twice the weight traffic
+// with nine row blocks per expert.) Every row block of an expert has `slices` tiles, so the tiles of an expert are
+// consecutive, and tile / slices is one of its row blocks: no search.
+struct ExpertOrder {
+  const int32_t* row_block_expert;
+  const int32_t* padded_offsets;
+  int32_t num_row_blocks, slices;
+  static constexpr int32_t kBand = 16;
+  __device__ __forceinline__ int32_t tiles() const { return num_row_blocks * slices; }
+  // False: past the last real row block.
+  __device__ __forceinline__ bool at(int32_t tile, int32_t* row_block, int32_t* slice, int32_t* expert) const {
+    const int32_t e = __ldg(row_block_expert + tile / slices);
+    if (e < 0) return false;
+    const int32_t begin = __ldg(padded_offsets + e) / kTileRows;
+    const int32_t end = __ldg(padded_offsets + e + 1) / kTileRows;
+    int32_t inside = tile - begin * slices;
+    const int32_t band = inside / (kBand * slices);
+    inside -= band * (kBand * slices);
+    const int32_t first = begin + band * kBand;
+    const int32_t height = min(kBand, end - first);
+    *slice = inside / height;
+    *row_block = first + inside - *slice * height;
+    *expert = e;
+    return true;
+  }
+};
+
 // ---- forward: both projections, the activation and the product ----------------------------------------------------
 // The tile's 256 accumulator columns are 128 columns of G next to the same 128 of U, so a thread that drains column c
 // finds its partner 128 columns on and H leaves the chip as the only result (plus G and U for training).
 struct GatedUp {
   struct Params {
-    BandOrder order;
-    const int32_t* row_offsets;
+    ExpertOrder order;
     const int32_t* row_token;
-    const int32_t* row_block_expert;
     int32_t d_model;
     int32_t activation;
     int32_t skip_padding;  // 32-row groups of padding are not stored
@@ -93,16 +121,15 @@ struct GatedUp {
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = true;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
-    Tile t;
+    Tile t{};
     int32_t slice;
-    p.order.at(index, &t.row_block, &slice);
+    t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
+    if (!t.live) return t;
     t.n0 = slice * 128;
-    t.first_block = __ldg(p.row_offsets + t.row_block);
-    t.live = __ldg(p.row_offsets + t.row_block + 1) != t.first_block;
-    t.k_steps = t.live ? p.d_model / kTileStep : 0;
-    t.expert = __ldg(p.row_block_expert + t.row_block);
+    t.first_block = t.row_block * p.order.slices;  // of the layout's blocks, F / 128 per row block
+    t.k_steps = p.d_model / kTileStep;
     return t;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
@@ -160,10 +187,8 @@ struct GatedUp {
 // results for TMA stores instead made the warps wait for their 4 KB tile at every step.
 struct GradHidden {
   struct Params {
-    BandOrder order;
-    const int32_t* row_offsets;
+    ExpertOrder order;
     const int32_t* row_token;
-    const int32_t* row_block_expert;
     const __nv_bfloat16* g;
     const __nv_bfloat16* u;
     __nv_bfloat16* dg;
@@ -187,16 +212,15 @@ struct GradHidden {
   static constexpr bool kAhead = true;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
-    Tile t;
+    Tile t{};
     int32_t slice;
-    p.order.at(index, &t.row_block, &slice);
+    t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
+    if (!t.live) return t;
     t.n0 = slice * kTileCols;
-    t.first_block = __ldg(p.row_offsets + t.row_block);
-    t.live = __ldg(p.row_offsets + t.row_block + 1) != t.first_block;
-    t.k_steps = t.live ? p.d_model / kTileStep : 0;
-    t.expert = __ldg(p.row_block_expert + t.row_block);
+    t.first_block = t.row_block * (p.ffn_dim >> 7);
+    t.k_steps = p.d_model / kTileStep;
     return t;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
@@ -280,10 +304,8 @@ struct GradHidden {
 // dG Wg^T + dU Wu^T as one product with 2 F inner columns. Wg and Wu [D, F] are K-major operands as they lie.
 struct GradRows {
   struct Params {
-    BandOrder order;
-    const int32_t* row_offsets;
+    ExpertOrder order;
     const int32_t* row_token;
-    const int32_t* row_block_expert;
     int32_t d_model, ffn_dim;
   };
   struct Tile {
@@ -295,16 +317,15 @@ struct GradRows {
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
-    Tile t;
+    Tile t{};
     int32_t slice;
-    p.order.at(index, &t.row_block, &slice);
+    t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
+    if (!t.live) return t;
     t.n0 = slice * kTileCols;
-    t.first_block = __ldg(p.row_offsets + t.row_block);
-    t.live = __ldg(p.row_offsets + t.row_block + 1) != t.first_block;
-    t.k_steps = t.live ? 2 * (p.ffn_dim / kTileStep) : 0;
-    t.expert = __ldg(p.row_block_expert + t.row_block);
+    t.first_block = t.row_block * (p.ffn_dim >> 7);
+    t.k_steps = 2 * (p.ffn_dim / kTileStep);
     return t;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
@@ -718,11 +739,6 @@ int check_gated(const char* what, int32_t d_model, int32_t ffn_dim, int32_t num_
   return SB_OK;
 }
 
-// Row blocks per band of the tile walk, for products that stream an expert's weights in column slices.
-int32_t band_for(int32_t num_row_blocks, int32_t num_experts) {
-  return num_row_blocks >= 4 * static_cast<int64_t>(num_experts) ? 8 : 1;
-}
-
 bool any_misaligned(std::initializer_list<const void*> ptrs) {
   for (const void* p : ptrs)
     if (!aligned16(p)) return true;
@@ -751,9 +767,9 @@ int launch_small(void (*kernel)(Params...), int64_t blocks, int threads, cudaStr
   return SB_OK;
 }
 
-// x_rows, then H (and G, U) on the layout; num_rows: the real row count on the device.
+// x_rows, then H (and G, U) on the layout.
 int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token, const int32_t* row_block_expert,
-              const int32_t* row_offsets, const int32_t* num_rows, void* x_rows, void* h_blocks, void* g_blocks,
+              const int32_t* padded_offsets, void* x_rows, void* h_blocks, void* g_blocks,
               void* u_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
               int32_t activation, int skip_padding_rows, int32_t* dev_status, cudaStream_t stream) {
   const DeviceInfo* info = current_device_info();
@@ -771,13 +787,11 @@ int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t
   if (int rc = encode_2d_map(&maps.m[5], x_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, "sdd_gated (rows)")) return rc;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
   if (int rc = launch_small(gated_rows_kernel, blocks, kSmallThreads, stream, "sdd_gated (rows)", static_cast<const uint4*>(x),
-                            row_token, num_rows, static_cast<uint4*>(x_rows), d_model / 8))
+                            row_token, padded_offsets + num_experts, static_cast<uint4*>(x_rows), d_model / 8))
     return rc;
   GatedUp::Params p{};
-  p.order = {num_row_blocks, ffn_dim / 128, band_for(num_row_blocks, num_experts)};
-  p.row_offsets = row_offsets;
+  p.order = {row_block_expert, padded_offsets, num_row_blocks, ffn_dim / 128};
   p.row_token = row_token;
-  p.row_block_expert = row_block_expert;
   p.d_model = d_model;
   p.activation = activation;
   p.skip_padding = skip_padding_rows ? 1 : 0;
@@ -798,7 +812,7 @@ int gated_grad_rows_of(const void* grad_out, const void* y_rows, const void* gat
 }
 
 int gated_grad_hidden(const void* grad_rows, const void* w_down, const void* g_blocks, const void* u_blocks,
-                      const int32_t* row_token, const int32_t* row_block_expert, const int32_t* row_offsets, void* dg_blocks,
+                      const int32_t* row_token, const int32_t* row_block_expert, const int32_t* padded_offsets, void* dg_blocks,
                       void* du_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
                       int32_t activation, int32_t* dev_status, cudaStream_t stream) {
   const char* what = "moe_gated_backward (hidden)";
@@ -807,10 +821,8 @@ int gated_grad_hidden(const void* grad_rows, const void* w_down, const void* g_b
   if (int rc = encode_2d_map(&maps.m[1], grad_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, what)) return rc;
   GradHidden::Params p{};
   const int32_t slices = (ffn_dim + kTileCols - 1) / kTileCols;
-  p.order = {num_row_blocks, slices, band_for(num_row_blocks, num_experts)};
-  p.row_offsets = row_offsets;
+  p.order = {row_block_expert, padded_offsets, num_row_blocks, slices};
   p.row_token = row_token;
-  p.row_block_expert = row_block_expert;
   p.g = static_cast<const __nv_bfloat16*>(g_blocks);
   p.u = static_cast<const __nv_bfloat16*>(u_blocks);
   p.dg = static_cast<__nv_bfloat16*>(dg_blocks);
@@ -854,7 +866,7 @@ int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_
 }
 
 int gated_grad_x(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up, const int32_t* row_token,
-                 const int32_t* row_block_expert, const int32_t* row_offsets, void* dx_rows, int32_t d_model,
+                 const int32_t* row_block_expert, const int32_t* padded_offsets, void* dx_rows, int32_t d_model,
                  int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
   const char* what = "moe_gated_backward (x)";
   const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
@@ -867,10 +879,8 @@ int gated_grad_x(const void* dg_blocks, const void* du_blocks, const void* w_gat
   if (int rc = encode_2d_map(&maps.m[4], dx_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, what)) return rc;
   GradRows::Params p{};
   const int32_t slices = (d_model + kTileCols - 1) / kTileCols;
-  p.order = {num_row_blocks, slices, 1};
-  p.row_offsets = row_offsets;
+  p.order = {row_block_expert, padded_offsets, num_row_blocks, slices};
   p.row_token = row_token;
-  p.row_block_expert = row_block_expert;
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
   return launch_tile_gemm<GradRows>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
@@ -1023,19 +1033,18 @@ int forward_small(const GatedBuffers& b, const void* x, const void* expert_idx, 
 using namespace sb;
 
 extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
-                            const int32_t* row_block_expert, const int32_t* row_offsets, const int32_t* padded_offsets,
-                            void* x_rows, void* h_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim,
+                            const int32_t* row_block_expert, const int32_t* padded_offsets, void* x_rows, void* h_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim,
                             int32_t num_experts, int32_t num_row_blocks, int32_t activation, int skip_padding_rows,
                             int32_t* dev_status, sb_stream_t stream) {
   clear_error();
   if (int rc = check_gated("sdd_gated", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
   if (num_row_blocks == 0) return SB_OK;
-  if (any_null({x, w_gate, w_up, row_token, row_block_expert, row_offsets, padded_offsets, x_rows, h_blocks}))
+  if (any_null({x, w_gate, w_up, row_token, row_block_expert, padded_offsets, x_rows, h_blocks}))
     return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: NULL buffer");
   if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: T must be positive");
   if (any_misaligned({x, w_gate, w_up, x_rows, h_blocks}))
     return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: x, the weights, the rows and the blocks must be 16-byte aligned");
-  return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, row_offsets, padded_offsets + num_experts, x_rows, h_blocks,
+  return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, padded_offsets, x_rows, h_blocks,
                    nullptr, nullptr, d_model, ffn_dim, num_experts, num_row_blocks, activation, skip_padding_rows, dev_status,
                    as_stream(stream));
 }
@@ -1080,8 +1089,8 @@ extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int i
                         ints(b.tokens_per_expert), ints(b.padded_offsets), ints(b.row_token), ints(b.copy_row),
                         ints(b.row_block_expert), ints(b.row_offsets), ints(b.col_indices), ints(b.error), temp + b.work, stream))
     return rc;
-  if (int rc = sdd_gated(x, w_gate, w_up, ints(b.row_token), ints(b.row_block_expert), ints(b.row_offsets),
-                         ints(b.padded_offsets) + num_experts, base + b.x_rows, base + b.h, keep ? base + b.g : nullptr,
+  if (int rc = sdd_gated(x, w_gate, w_up, ints(b.row_token), ints(b.row_block_expert), ints(b.padded_offsets),
+                         base + b.x_rows, base + b.h, keep ? base + b.g : nullptr,
                          keep ? base + b.u : nullptr, d_model, ffn_dim, num_experts, b.row_blocks, activation, 1, dev_status,
                          as_stream(stream)))
     return rc;
@@ -1120,7 +1129,7 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int
                                   ints(b.padded_offsets) + num_experts, temp + b.grad_rows, dgate, k, d_model, b.row_blocks, st))
     return rc;
   if (int rc = gated_grad_hidden(temp + b.grad_rows, w_down, base + b.g, base + b.u, row_token, ints(b.row_block_expert),
-                                 ints(b.row_offsets), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
+                                 ints(b.padded_offsets), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
                                  activation, dev_status, st))
     return rc;
   if (int rc = gated_grad_weights(base + b.x_rows, temp + b.grad_rows, base + b.h, temp + b.dg, temp + b.du,
@@ -1128,7 +1137,7 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int
                                   ffn_dim, num_experts, b.row_blocks, dev_status, st))
     return rc;
   // The rows of dx take the place of grad_rows, which the weight gradients were the last to read.
-  if (int rc = gated_grad_x(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert), ints(b.row_offsets),
+  if (int rc = gated_grad_x(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert), ints(b.padded_offsets),
                             temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks, dev_status, st))
     return rc;
   return gated_join(temp + b.grad_rows, ints(b.copy_row), dx, dgate, gate_dtype, num_tokens, k, d_model, st);
