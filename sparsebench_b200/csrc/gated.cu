@@ -117,7 +117,7 @@ struct GatedUp {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = true;
 
@@ -163,9 +163,9 @@ struct GatedUp {
   static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
     if (!early.store) return;
-    const int32_t col = w.half * 64;
+    const int32_t col = w.part * 64;
     const int32_t row = (t.first_block + (t.n0 >> 7)) * kTileRows + w.quarter * 32;
-    const uint32_t gate = w.taddr + w.half * 64;
+    const uint32_t gate = w.taddr + w.part * 64;
     const uint32_t up = gate + 128;
     uint32_t packed[32];
     if (p.keep) {
@@ -180,11 +180,12 @@ struct GatedUp {
   }
 };
 
-// ---- backward: gradients of G, U and of the gates -----------------------------------------------------------------
-// S = dO Wd^T over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. In the epilogue a lane has a row
-// to itself: it reads G and U and writes dG and dU a sector (16 columns) at a time, two sectors ahead of the one it works
-// on, and leaves per row and 128 columns its share of dgate, summed in a fixed order by the join kernel. Staging the
-// results for TMA stores instead made the warps wait for their 4 KB tile at every step.
+// ---- backward: gradients of G and U -----------------------------------------------------------------
+// dH = (w dO) Wd^T over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. In the epilogue a lane has a row
+// to itself: it reads G and U and writes dG and dU a sector (16 columns) at a time, the next sector on its way while it
+// works on one. What bounds it is the latency of those reads, so sixteen warps share the tile (8: 226 us, 16: 201 us at
+// T = 4096, D = 1024, F = 4096, E = 64). Staging the results for TMA stores costs a stage of the ring and is slower (1000
+// against 850 us on the Mixtral-like layer).
 struct GradHidden {
   struct Params {
     ExpertOrder order;
@@ -196,19 +197,20 @@ struct GradHidden {
     int32_t d_model, ffn_dim;
     int32_t activation;
   };
-  static constexpr int kPart = 16;  // columns at a time: 32 bytes of a row, one sector
+  static constexpr int kPart = 16;       // columns at a time: 32 bytes of a row, one sector
+  static constexpr int kWarpCols = 64;  // of the tile's 256 per epilogue warp
   struct Tile {
     int32_t k_steps, row_block, n0, expert, first_block;
     bool live;
   };
   struct Early {
     bool store;
-    const __nv_bfloat16* g;  // this row's 128 columns, as U's and the results' are
+    const __nv_bfloat16* g;  // this row's 64 columns, as U's and the results' are
     const __nv_bfloat16* u;
     int64_t at;
-    uint32_t first[2][2][8];  // G and U of the first two parts
+    uint32_t first[2][8];  // G and U of the first part
   };
-  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 16, kBuffers = 0;
   static constexpr bool kAhead = true;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
@@ -232,24 +234,21 @@ struct GradHidden {
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
     Early e;
-    const int32_t n = t.n0 + w.half * 128;
+    const int32_t n = t.n0 + w.part * kWarpCols;
     e.store = n < p.ffn_dim && half_has_rows(p.row_token, t.row_block, w.quarter);
     if (!e.store) return e;
-    e.at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128;
+    e.at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128 + (n & 127);
     e.g = p.g + e.at;
     e.u = p.u + e.at;
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      ptx::ld_global_v8(e.g + part * kPart, e.first[part][0]);
-      ptx::ld_global_v8(e.u + part * kPart, e.first[part][1]);
-    }
+    ptx::ld_global_v8(e.g, e.first[0]);
+    ptx::ld_global_v8(e.u, e.first[1]);
     return e;
   }
-  // The warp's 32 rows of a block are 8 KB in one piece: the next tile's are asked into L2 before this one is worked on,
+  // 32 rows of a block are 8 KB in one piece: the next tile's are asked into L2 before this one is worked on,
   // because what a warp can hold in flight in registers does not cover the way to memory.
   static __device__ __forceinline__ void ahead(const Params& p, const Tile& next, const EpilogueWarp& w) {
-    const int32_t n = next.n0 + w.half * 128;
-    if (!next.live || n >= p.ffn_dim || w.lane != 0 || !half_has_rows(p.row_token, next.row_block, w.quarter)) return;
+    const int32_t n = next.n0 + w.part * kWarpCols;
+    if ((w.part & 1) != 0 || !next.live || n >= p.ffn_dim || w.lane != 0 || !half_has_rows(p.row_token, next.row_block, w.quarter)) return;
     const int64_t at = ((static_cast<int64_t>(next.first_block) + (n >> 7)) * kTileRows + w.quarter * 32) * 128;
     ptx::bulk_prefetch_l2(p.g + at, 32 * 256);
     ptx::bulk_prefetch_l2(p.u + at, 32 * 256);
@@ -257,35 +256,33 @@ struct GradHidden {
   static __device__ __forceinline__ void epilogue(const TileMaps&, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
     if (!early.store) return;
-    if (p.activation == SB_ACT_SILU) work<SB_ACT_SILU>(p, t, w, early);
-    else work<SB_ACT_GELU>(p, t, w, early);
+    if (p.activation == SB_ACT_SILU) work<SB_ACT_SILU>(p, w, early);
+    else work<SB_ACT_GELU>(p, w, early);
   }
   template <int kActivation>
-  static __device__ __forceinline__ void work(const Params& p, const Tile& t, const EpilogueWarp& w, const Early& early) {
+  static __device__ __forceinline__ void work(const Params& p, const EpilogueWarp& w, const Early& early) {
     __nv_bfloat16* dg_row = p.dg + early.at;
     __nv_bfloat16* du_row = p.du + early.at;
-    uint32_t held[3][2][8];  // G and U of this part and the next two
+    uint32_t held[2][2][8];  // G and U of this part and the next
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      held[0][0][q] = early.first[0][0][q];
-      held[0][1][q] = early.first[0][1][q];
-      held[1][0][q] = early.first[1][0][q];
-      held[1][1][q] = early.first[1][1][q];
+      held[0][0][q] = early.first[0][q];
+      held[0][1][q] = early.first[1][q];
     }
 #pragma unroll
-    for (int part = 0; part < 128 / kPart; ++part) {
+    for (int part = 0; part < kWarpCols / kPart; ++part) {
       uint32_t s[16];
-      ptx::tmem_ld_32x32b_x16(w.taddr + w.half * 128 + part * kPart, s);
-      if (part + 2 < 128 / kPart) {
-        ptx::ld_global_v8(early.g + (part + 2) * kPart, held[(part + 2) % 3][0]);
-        ptx::ld_global_v8(early.u + (part + 2) * kPart, held[(part + 2) % 3][1]);
+      ptx::tmem_ld_32x32b_x16(w.taddr + w.part * kWarpCols + part * kPart, s);
+      if (part + 1 < kWarpCols / kPart) {
+        ptx::ld_global_v8(early.g + (part + 1) * kPart, held[(part + 1) & 1][0]);
+        ptx::ld_global_v8(early.u + (part + 1) * kPart, held[(part + 1) & 1][1]);
       }
       ptx::tmem_ld_wait();
       uint32_t dg[8], du[8];
 #pragma unroll
       for (int h = 0; h < 8; ++h) {
-        const float2 gf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[part % 3][0][h]));
-        const float2 uf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[part % 3][1][h]));
+        const float2 gf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[part & 1][0][h]));
+        const float2 uf = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&held[part & 1][1][h]));
         float a0, a1, d0, d1;
         act_and_slope<kActivation>(gf.x, &a0, &d0);
         act_and_slope<kActivation>(gf.y, &a1, &d1);
@@ -313,7 +310,7 @@ struct GradRows {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
@@ -345,10 +342,10 @@ struct GradRows {
     if (!early.store) return;
 #pragma unroll 1
     for (int g = 0; g < 2; ++g) {
-      const int32_t col = t.n0 + w.half * 128 + g * 64;
+      const int32_t col = t.n0 + w.part * 128 + g * 64;
       if (col >= p.d_model) break;
       uint32_t packed[32];
-      load_packed_x64(w.taddr + w.half * 128 + g * 64, packed);
+      load_packed_x64(w.taddr + w.part * 128 + g * 64, packed);
       store_rows_128b<kBuffers>(w, &maps.m[4], packed, col, t.row_block * kTileRows + w.quarter * 32);
     }
   }
@@ -356,8 +353,10 @@ struct GradRows {
 
 // ---- backward: the three weight gradients -------------------------------------------------------------------------
 // The rows of an expert are the inner dimension, so both operands are MN-major: X, w dO, H, dG and dU as they lie.
-// An expert's rows end inside a step of 64; the rest of that step is zero rows in X and w dO (written by the gather
-// kernel) against finite ones (zeros) in H, dG and dU. An expert without rows gets zeros.
+// An expert's rows end inside a step of 64; the rest of that step is zero rows in X and w dO against finite ones (zeros) in
+// H, dG and dU. An expert without rows gets zeros. Bound by writing: with two or three K steps per tile the kernel moves
+// 5.1 TB/s (T = 4096, D = 1024, F = 4096, E = 64: 362 us). Tried and slower: two staging tiles per warp or sixteen warps for
+// a stage of the ring (385 us), stores from registers (444 us); no gain: fetching only the real rows of the last step.
 struct GradWeights {
   struct Params {
     const int32_t* padded_offsets;
@@ -371,7 +370,7 @@ struct GradWeights {
     bool live;
   };
   struct Early {};
-  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = true, kBMnMajor = true;
 
@@ -430,11 +429,11 @@ struct GradWeights {
     const int32_t row = t.expert * (t.which == 0 ? p.ffn_dim : p.d_model) + t.m0 + w.quarter * 32;
 #pragma unroll 1
     for (int g = 0; g < 2; ++g) {
-      const int32_t col = t.n0 + w.half * 128 + g * 64;
+      const int32_t col = t.n0 + w.part * 128 + g * 64;
       if (col >= width) break;
       uint32_t packed[32];
       if (t.k_steps > 0) {
-        load_packed_x64(w.taddr + w.half * 128 + g * 64, packed);
+        load_packed_x64(w.taddr + w.part * 128 + g * 64, packed);
       } else {
 #pragma unroll
         for (int h = 0; h < 32; ++h) packed[h] = 0u;
@@ -840,14 +839,14 @@ int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_
   const char* what = "moe_gated_backward (weights)";
   const uint64_t rows = static_cast<uint64_t>(num_row_blocks) * kTileRows;
   const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
-  const uint64_t up_rows = static_cast<uint64_t>(num_experts) * d_model;
-  const uint64_t down_rows = static_cast<uint64_t>(num_experts) * ffn_dim;
   TileMaps maps{};
   if (int rc = encode_2d_map(&maps.m[0], x_rows, rows, d_model, 64, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[1], grad_rows, rows, d_model, 64, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[2], h_blocks, b_rows, 128, 64, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[3], dg_blocks, b_rows, 128, 64, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[4], du_blocks, b_rows, 128, 64, 64, 2, what)) return rc;
+  const uint64_t up_rows = static_cast<uint64_t>(num_experts) * d_model;
+  const uint64_t down_rows = static_cast<uint64_t>(num_experts) * ffn_dim;
   if (int rc = encode_2d_map(&maps.m[5], dw_down, down_rows, d_model, 32, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[6], dw_gate, up_rows, ffn_dim, 32, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[7], dw_up, up_rows, ffn_dim, 32, 64, 2, what)) return rc;

@@ -138,7 +138,7 @@ struct LoraShrink {
     bool live;
   };
   struct Early { int32_t slot; };
-  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
@@ -177,7 +177,7 @@ struct LoraShrink {
                                                   const Early& early) {
     const int32_t token = t.row_tile * kTileRows + w.quarter * 32 + w.lane;
     float* dst = p.partial + (static_cast<int64_t>(t.split) * p.num_tokens + token) * p.rank;
-    for (int32_t s = w.half; s < t.slots; s += 2) {  // the two warps of a quarter share the slots
+    for (int32_t s = w.part; s < t.slots; s += 2) {  // the two warps of a quarter share the slots
       const bool mine = early.slot == t.first_slot + s;
       if (__ballot_sync(0xffffffffu, mine) == 0u) continue;
       for (int32_t j = 0; j < p.rank; j += 8) {
@@ -247,7 +247,7 @@ struct LoraExpand {
   };
   struct Rows { int32_t slot[8]; };
   struct Early { int32_t loner; };  // this row's adapter when its B is not finite, else -1
-  static constexpr int kStages = 4, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = true, kAMnMajor = false, kBMnMajor = true;
 
@@ -321,9 +321,9 @@ struct LoraExpand {
     const int32_t row = t.row_tile * kTileRows + w.quarter * 32;
     if (row >= p.num_tokens) return;
     const bool loners = __ballot_sync(0xffffffffu, early.loner >= 0) != 0u;
-    const int32_t end = min(t.n0 + (p.cols > 128 ? (w.half + 1) * 128 : (w.half == 0 ? 128 : 0)), p.width);
+    const int32_t end = min(t.n0 + (p.cols > 128 ? (w.part + 1) * 128 : (w.part == 0 ? 128 : 0)), p.width);
 #pragma unroll 1
-    for (int32_t col = t.n0 + w.half * 128; col < end; col += 64) {
+    for (int32_t col = t.n0 + w.part * 128; col < end; col += 64) {
       uint32_t packed[32];
 #pragma unroll
       for (int part = 0; part < 2; ++part) {

@@ -3,7 +3,7 @@
 //
 // One output tile = 128 rows x 256 columns, accumulated in fp32 in TMEM (two accumulators, so the epilogue of one
 // tile runs while the tensor cores fill the other). K steps of 64. Warp roles, with nothing but mbarriers between
-// them: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue, warps 10-13 extension rows of A (policies that have them).
+// them: warp 0 TMA producer, warp 1 MMA issuer, 8 or 16 epilogue warps, 4 warps for rows of A (policies that have them).
 //
 // A stage of the shared-memory ring holds A (16 KB) and B (32 KB) with the 128-byte swizzle, each in one of two forms:
 //   K-major   rows of the M (N) dimension, 64 K elements = 128 bytes per row
@@ -30,7 +30,6 @@ struct TileSmem {
   static constexpr int kABytes = kTileRows * kTileStep * 2;
   static constexpr int kBBytes = kTileCols * kTileStep * 2;
   static constexpr int kSlabBytes = kTileStep * 128;
-  static constexpr int kEpilogueWarps = 8;
   static constexpr int kStagingBytes = 32 * 128;  // one staging tile of an epilogue warp: 32 rows x 128 bytes
   static constexpr int kBarrierBytes = 256;
 };
@@ -38,7 +37,7 @@ struct TileSmem {
 // What an epilogue warp works with.
 struct EpilogueWarp {
   int quarter;       // rows quarter * 32 .. + 31 of the tile (TMEM lanes this warp may read)
-  int half;          // 0 or 1: which half of the tile's columns is this warp's
+  int part;          // which of the kEpilogueWarps / 4 parts of the tile's columns is this warp's
   int lane;
   uint32_t staging;  // this warp's staging tiles in shared memory, 4 KB each
   uint32_t buffer;   // the one to use next
@@ -105,7 +104,7 @@ struct BandOrder {
 //   Params, Tile (with int32_t k_steps: 0 = nothing to multiply; bool live: the epilogue has something to do)
 //   static constexpr bool kAMnMajor, kBMnMajor
 //   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar), tx_bytes
-//   static constexpr int kStages (of the ring), kBuffers (staging tiles per epilogue warp)
+//   static constexpr int kStages (of the ring), kEpilogueWarps, kBuffers (staging tiles of each, may be 0)
 //   With kExtension: Tile has base_steps; A of the K steps behind them is written by four warps from registers:
 //   Rows rows(p, tile, row0) once per tile, extension_chunk(p, tile, rows, j, row, ks, chunk) = the 16 bytes of chunk
 //   `chunk` of row `row` = row0 + 16 j.
@@ -113,10 +112,10 @@ struct BandOrder {
 template <class Op>
 struct TileConfig {
   static constexpr int kExtensionWarps = Op::kExtension ? 4 : 0;
-  static constexpr int kFirstExtensionWarp = 2 + TileSmem::kEpilogueWarps;
+  static constexpr int kFirstExtensionWarp = 2 + Op::kEpilogueWarps;
   static constexpr int kThreads = 32 * (kFirstExtensionWarp + kExtensionWarps);
   static constexpr int kSmemBytes = 1024 + Op::kStages * (TileSmem::kABytes + TileSmem::kBBytes) +
-                                    TileSmem::kEpilogueWarps * Op::kBuffers * TileSmem::kStagingBytes + TileSmem::kBarrierBytes;
+                                    Op::kEpilogueWarps * Op::kBuffers * TileSmem::kStagingBytes + TileSmem::kBarrierBytes;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -130,7 +129,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
   const uint32_t a_base = smem_base;
   const uint32_t b_base = a_base + Op::kStages * S::kABytes;
   const uint32_t staging_base = b_base + Op::kStages * S::kBBytes;
-  const uint32_t full_bar = staging_base + S::kEpilogueWarps * Op::kBuffers * S::kStagingBytes;  // [kStages]
+  const uint32_t full_bar = staging_base + Op::kEpilogueWarps * Op::kBuffers * S::kStagingBytes;  // [kStages]
   const uint32_t empty_bar = full_bar + 8 * Op::kStages;                          // [kStages]
   const uint32_t acc_full_bar = empty_bar + 8 * Op::kStages;                      // [2]
   const uint32_t acc_empty_bar = acc_full_bar + 16;                               // [2]
@@ -156,7 +155,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(acc_full_bar + 8 * a, 1);
-      ptx::mbar_init(acc_empty_bar + 8 * a, 32 * S::kEpilogueWarps);
+      ptx::mbar_init(acc_empty_bar + 8 * a, 32 * Op::kEpilogueWarps);
     }
     *abort_word = 0u;
     ptx::fence_barrier_init();
@@ -270,7 +269,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     // ---------------------------------------------------------------- epilogue
     EpilogueWarp w;
     w.quarter = warp & 3;
-    w.half = (warp - 2) >> 2;
+    w.part = (warp - 2) >> 2;
     w.lane = lane;
     w.staging = staging_base + static_cast<uint32_t>(warp - 2) * (Op::kBuffers * S::kStagingBytes);
     w.buffer = 0;
