@@ -1,10 +1,10 @@
 // The gated expert block of the MoE layer and its backward pass, on the block-sparse layout of sb_route.
 //
-//   forward    G = X Wg[e], U = X Wu[e], H = act(G) * U            (GatedUp; Y = H Wd[e] is sb_dsd)
+//   forward    G = X Wg[e], U = X Wu[e], H = act(G) * U            (GatedUp), Y = H Wd[e] (RowsProduct)
 //   backward   with dO = grad_out of the row's token and w the gate of its copy:
 //              dgate = dO . Y, dH = (w dO) Wd[e]^T, dU = dH act(G), dG = dH U act'(G)     (grad rows kernel, GradHidden)
 //              dWd = H^T (w dO), dWg = X^T dG, dWu = X^T dU                               (GradWeights)
-//              dx[t] = sum over the token's copies of dG Wg^T + dU Wu^T                   (GradRows, join)
+//              dx[t] = sum over the token's copies of dG Wg^T + dU Wu^T                   (RowsProduct, join)
 //
 // The forward keeps X (rows in layout order), G, U, H and Y. Everything that is an operand of a product is bf16, as the
 // weights are: G, U, H, Y, w dO, dG, dU and the rows of dx are each rounded once; sums, the activation and its derivative
@@ -186,6 +186,7 @@ struct GatedUp {
 // works on one. What bounds it is the latency of those reads, so sixteen warps share the tile (8: 226 us, 16: 201 us at
 // T = 4096, D = 1024, F = 4096, E = 64). Staging the results for TMA stores costs a stage of the ring and is slower (1000
 // against 850 us on the Mixtral-like layer).
+template <int kCols>
 struct GradHidden {
   struct Params {
     ExpertOrder order;
@@ -197,22 +198,22 @@ struct GradHidden {
     int32_t d_model, ffn_dim;
     int32_t activation;
   };
-  static constexpr int kPart = 16;       // columns at a time: 32 bytes of a row, one sector
-  static constexpr int kWarpCols = 64;  // of the tile's 256 per epilogue warp
+  static constexpr int kPart = 16;                // columns at a time: 32 bytes of a row, one sector
+  static constexpr int kWarpCols = kCols / 4;     // of the tile's, per epilogue warp
   struct Tile {
     int32_t k_steps, row_block, n0, expert, first_block;
     bool live;
   };
   struct Early {
     bool store;
-    const __nv_bfloat16* g;  // this row's 64 columns, as U's and the results' are
+    const __nv_bfloat16* g;  // this row's columns, as U's and the results' are
     const __nv_bfloat16* u;
     int64_t at;
     uint32_t first[2][8];  // G and U of the first part
   };
   static constexpr int kStages = 4, kEpilogueWarps = 16, kBuffers = 0;
   static constexpr bool kAhead = true;
-  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -220,10 +221,14 @@ struct GradHidden {
     int32_t slice;
     t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
     if (!t.live) return t;
-    t.n0 = slice * kTileCols;
+    t.n0 = slice * kCols;
     t.first_block = t.row_block * (p.ffn_dim >> 7);
     t.k_steps = p.d_model / kTileStep;
     return t;
+  }
+  static __device__ __forceinline__ int columns(const Params&) { return kCols; }
+  static __device__ __forceinline__ uint32_t tx_bytes(const Params&, const Tile&, int32_t) {
+    return TileSmem::kABytes + kCols * 128u;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
@@ -248,7 +253,7 @@ struct GradHidden {
   // because what a warp can hold in flight in registers does not cover the way to memory.
   static __device__ __forceinline__ void ahead(const Params& p, const Tile& next, const EpilogueWarp& w) {
     const int32_t n = next.n0 + w.part * kWarpCols;
-    if ((w.part & 1) != 0 || !next.live || n >= p.ffn_dim || w.lane != 0 || !half_has_rows(p.row_token, next.row_block, w.quarter)) return;
+    if ((w.part != 0 && (n & 127) != 0) || !next.live || n >= p.ffn_dim || w.lane != 0 || !half_has_rows(p.row_token, next.row_block, w.quarter)) return;
     const int64_t at = ((static_cast<int64_t>(next.first_block) + (n >> 7)) * kTileRows + w.quarter * 32) * 128;
     ptx::bulk_prefetch_l2(p.g + at, 32 * 256);
     ptx::bulk_prefetch_l2(p.u + at, 32 * 256);
@@ -297,13 +302,15 @@ struct GradHidden {
   }
 };
 
-// ---- backward: the rows of dx -------------------------------------------------------------------------------------
-// dG Wg^T + dU Wu^T as one product with 2 F inner columns. Wg and Wu [D, F] are K-major operands as they lie.
-struct GradRows {
+// ---- the products that give rows: the down projection, and the backward pass's rows of dx ---------------------------
+// Down (kBack false): Y = H Wd, Wd [F, D] an MN-major operand. Back: dG Wg^T + dU Wu^T as one product with 2 F inner
+// columns, Wg and Wu [D, F] K-major operands. Either way the weights lie as the tensor cores read them.
+template <bool kBack>
+struct RowsProduct {
   struct Params {
     ExpertOrder order;
     const int32_t* row_token;
-    int32_t d_model, ffn_dim;
+    int32_t d_model, ffn_dim, cols;
   };
   struct Tile {
     int32_t k_steps, row_block, n0, expert, first_block;
@@ -312,7 +319,7 @@ struct GradRows {
   struct Early { bool store; };
   static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = false;
+  static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = !kBack;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -320,19 +327,28 @@ struct GradRows {
     int32_t slice;
     t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
     if (!t.live) return t;
-    t.n0 = slice * kTileCols;
+    t.n0 = slice * p.cols;
     t.first_block = t.row_block * (p.ffn_dim >> 7);
-    t.k_steps = 2 * (p.ffn_dim / kTileStep);
+    t.k_steps = (kBack ? 2 : 1) * (p.ffn_dim / kTileStep);
     return t;
+  }
+  static __device__ __forceinline__ int columns(const Params& p) { return p.cols; }
+  static __device__ __forceinline__ uint32_t tx_bytes(const Params& p, const Tile&, int32_t) {
+    return TileSmem::kABytes + static_cast<uint32_t>(p.cols) * 128u;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
     const uint64_t once = ptx::policy_evict_first();
     const int32_t steps = p.ffn_dim / kTileStep;
-    const int which = ks < steps ? 0 : 1;
+    const int which = kBack && ks >= steps ? 1 : 0;
     const int32_t k = (ks - which * steps) * kTileStep;
     ptx::tma_load_2d_hint(a, &maps.m[which], k & 127, (t.first_block + (k >> 7)) * kTileRows, bar, once);
-    ptx::tma_load_2d_hint(b, &maps.m[2 + which], k, t.expert * p.d_model + t.n0, bar, once);
+    if (kBack) {
+      ptx::tma_load_2d_hint(b, &maps.m[2 + which], k, t.expert * p.d_model + t.n0, bar, once);
+    } else {
+      for (int32_t j = 0; j < p.cols / 64; ++j)
+        ptx::tma_load_2d_hint(b + j * TileSmem::kSlabBytes, &maps.m[2], t.n0 + j * 64, t.expert * p.ffn_dim + k, bar, once);
+    }
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
     return {__ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32) >= 0};
@@ -341,12 +357,11 @@ struct GradRows {
                                                   const Early& early) {
     if (!early.store) return;
 #pragma unroll 1
-    for (int g = 0; g < 2; ++g) {
-      const int32_t col = t.n0 + w.part * 128 + g * 64;
-      if (col >= p.d_model) break;
+    for (int32_t c = w.part * 64; c < p.cols; c += 128) {
+      if (t.n0 + c >= p.d_model) break;
       uint32_t packed[32];
-      load_packed_x64(w.taddr + w.part * 128 + g * 64, packed);
-      store_rows_128b<kBuffers>(w, &maps.m[4], packed, col, t.row_block * kTileRows + w.quarter * 32);
+      load_packed_x64(w.taddr + c, packed);
+      store_rows_128b<kBuffers>(w, &maps.m[4], packed, t.n0 + c, t.row_block * kTileRows + w.quarter * 32);
     }
   }
 };
@@ -810,16 +825,25 @@ int gated_grad_rows_of(const void* grad_out, const void* y_rows, const void* gat
   return check_launch("moe_gated_backward (rows)");
 }
 
+// Columns of a tile: 256, and fewer where that leaves SMs without a tile. A tile of 128 (64) columns moves 1.3 (2) times
+// the operand bytes per result, so only then.
+int32_t tile_cols(int64_t num_row_blocks, int32_t width, int sm_count) {
+  int32_t cols = kTileCols;
+  while (cols > 64 && num_row_blocks * ((width + cols - 1) / cols) < sm_count) cols /= 2;
+  return cols;
+}
+
+template <int kCols>
 int gated_grad_hidden(const void* grad_rows, const void* w_down, const void* g_blocks, const void* u_blocks,
                       const int32_t* row_token, const int32_t* row_block_expert, const int32_t* padded_offsets, void* dg_blocks,
                       void* du_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
                       int32_t activation, int32_t* dev_status, cudaStream_t stream) {
   const char* what = "moe_gated_backward (hidden)";
   TileMaps maps{};
-  if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, 256, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, kCols, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[1], grad_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, what)) return rc;
-  GradHidden::Params p{};
-  const int32_t slices = (ffn_dim + kTileCols - 1) / kTileCols;
+  typename GradHidden<kCols>::Params p{};
+  const int32_t slices = (ffn_dim + kCols - 1) / kCols;
   p.order = {row_block_expert, padded_offsets, num_row_blocks, slices};
   p.row_token = row_token;
   p.g = static_cast<const __nv_bfloat16*>(g_blocks);
@@ -829,7 +853,7 @@ int gated_grad_hidden(const void* grad_rows, const void* w_down, const void* g_b
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
   p.activation = activation;
-  return launch_tile_gemm<GradHidden>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
+  return launch_tile_gemm<GradHidden<kCols>>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
 }
 
 int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_blocks, const void* dg_blocks,
@@ -864,25 +888,35 @@ int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_
   return launch_tile_gemm<GradWeights>(maps, p, tiles, dev_status, stream, what);
 }
 
-int gated_grad_x(const void* dg_blocks, const void* du_blocks, const void* w_gate, const void* w_up, const int32_t* row_token,
-                 const int32_t* row_block_expert, const int32_t* padded_offsets, void* dx_rows, int32_t d_model,
-                 int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
-  const char* what = "moe_gated_backward (x)";
+// Y = H Wd (back: false; a0 = H, w0 = Wd), or the rows of dx = dG Wg^T + dU Wu^T (a0, a1, w0, w1).
+template <bool kBack>
+int rows_product(const void* a0, const void* a1, const void* w0, const void* w1, const int32_t* row_token,
+                 const int32_t* row_block_expert, const int32_t* padded_offsets, void* rows, int32_t d_model, int32_t ffn_dim,
+                 int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
+  const char* what = kBack ? "moe_gated_backward (x)" : "moe_gated (down)";
+  const DeviceInfo* info = current_device_info();
+  if (info == nullptr) return SB_ERR_CUDA;
+  const int32_t cols = tile_cols(num_row_blocks, d_model, info->sm_count);
   const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
-  const uint64_t w_rows = static_cast<uint64_t>(num_experts) * d_model;
   TileMaps maps{};
-  if (int rc = encode_2d_map(&maps.m[0], dg_blocks, b_rows, 128, 128, 64, 2, what)) return rc;
-  if (int rc = encode_2d_map(&maps.m[1], du_blocks, b_rows, 128, 128, 64, 2, what)) return rc;
-  if (int rc = encode_2d_map(&maps.m[2], w_gate, w_rows, ffn_dim, 256, 64, 2, what)) return rc;
-  if (int rc = encode_2d_map(&maps.m[3], w_up, w_rows, ffn_dim, 256, 64, 2, what)) return rc;
-  if (int rc = encode_2d_map(&maps.m[4], dx_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, what)) return rc;
-  GradRows::Params p{};
-  const int32_t slices = (d_model + kTileCols - 1) / kTileCols;
+  if (int rc = encode_2d_map(&maps.m[0], a0, b_rows, 128, 128, 64, 2, what)) return rc;
+  if (kBack) {
+    const uint64_t w_rows = static_cast<uint64_t>(num_experts) * d_model;
+    if (int rc = encode_2d_map(&maps.m[1], a1, b_rows, 128, 128, 64, 2, what)) return rc;
+    if (int rc = encode_2d_map(&maps.m[2], w0, w_rows, ffn_dim, cols, 64, 2, what)) return rc;
+    if (int rc = encode_2d_map(&maps.m[3], w1, w_rows, ffn_dim, cols, 64, 2, what)) return rc;
+  } else {
+    if (int rc = encode_2d_map(&maps.m[2], w0, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, 64, 64, 2, what)) return rc;
+  }
+  if (int rc = encode_2d_map(&maps.m[4], rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, what)) return rc;
+  typename RowsProduct<kBack>::Params p{};
+  const int32_t slices = (d_model + cols - 1) / cols;
   p.order = {row_block_expert, padded_offsets, num_row_blocks, slices};
   p.row_token = row_token;
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
-  return launch_tile_gemm<GradRows>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
+  p.cols = cols;
+  return launch_tile_gemm<RowsProduct<kBack>>(maps, p, static_cast<int64_t>(num_row_blocks) * slices, dev_status, stream, what);
 }
 
 int gated_join(const void* dx_rows, const int32_t* copy_row, void* dx, void* dgate, int gate_dtype, int64_t num_tokens,
@@ -1093,9 +1127,9 @@ extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int i
                          keep ? base + b.u : nullptr, d_model, ffn_dim, num_experts, b.row_blocks, activation, 1, dev_status,
                          as_stream(stream)))
     return rc;
-  if (int rc = sb_dsd(base + b.h, static_cast<int64_t>(b.row_blocks) * b.ffn_blocks, w_down,
-                      static_cast<int64_t>(num_experts) * ffn_dim, d_model, ints(b.row_offsets), ints(b.col_indices),
-                      b.row_blocks, 128, 0, ints(b.row_token), base + b.y, ints(b.padded_offsets), num_experts, dev_status, stream))
+  if (int rc = rows_product<false>(base + b.h, nullptr, w_down, nullptr, ints(b.row_token), ints(b.row_block_expert),
+                                   ints(b.padded_offsets), base + b.y, d_model, ffn_dim, num_experts, b.row_blocks, dev_status,
+                                   as_stream(stream)))
     return rc;
   return sb_combine(base + b.y, ints(b.copy_row), gate, gate_dtype, out, num_tokens, k, d_model, stream);
 }
@@ -1127,17 +1161,21 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int
   if (int rc = gated_grad_rows_of(grad_out, base + b.y, gate, gate_dtype, row_token, ints(b.copy_row),
                                   ints(b.padded_offsets) + num_experts, temp + b.grad_rows, dgate, k, d_model, b.row_blocks, st))
     return rc;
-  if (int rc = gated_grad_hidden(temp + b.grad_rows, w_down, base + b.g, base + b.u, row_token, ints(b.row_block_expert),
-                                 ints(b.padded_offsets), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
-                                 activation, dev_status, st))
+  const DeviceInfo* info = current_device_info();
+  if (info == nullptr) return SB_ERR_CUDA;
+  const auto grad_hidden = tile_cols(b.row_blocks, ffn_dim, info->sm_count) == kTileCols ? gated_grad_hidden<kTileCols> : gated_grad_hidden<64>;
+  if (int rc = grad_hidden(temp + b.grad_rows, w_down, base + b.g, base + b.u, row_token, ints(b.row_block_expert),
+                           ints(b.padded_offsets), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
+                           activation, dev_status, st))
     return rc;
   if (int rc = gated_grad_weights(base + b.x_rows, temp + b.grad_rows, base + b.h, temp + b.dg, temp + b.du,
                                   ints(b.padded_offsets), ints(b.tokens_per_expert), dw_gate, dw_up, dw_down, d_model,
                                   ffn_dim, num_experts, b.row_blocks, dev_status, st))
     return rc;
   // The rows of dx take the place of grad_rows, which the weight gradients were the last to read.
-  if (int rc = gated_grad_x(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert), ints(b.padded_offsets),
-                            temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks, dev_status, st))
+  if (int rc = rows_product<true>(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert),
+                                  ints(b.padded_offsets), temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks,
+                                  dev_status, st))
     return rc;
   return gated_join(temp + b.grad_rows, ints(b.copy_row), dx, dgate, gate_dtype, num_tokens, k, d_model, st);
 }
