@@ -5,9 +5,8 @@
 // The products run on tiles of 128 consecutive tokens. A tile's distinct adapters are its slots, in order of first
 // appearance (a batch is its requests' tokens one after another, so a tile has few). Per call:
 //
-//   plan     slots of every tile; which of the used adapters have a B that is not finite
-//   shrink   V = x A[a]^T: the rows of all slots' A side by side are the columns of one product, of which each token
-//            keeps its own slot's; split over D, joined in a fixed order with the scale
+//   shrink   the slots of every tile; V = x A[a]^T: the rows of all slots' A side by side are the columns of one product,
+//            of which each token keeps its own slot's; split over D within a cluster, joined there with the scale
 //   expand   y = [x | V in its slot's columns, zeros elsewhere] [W ; B of the slots]: the second term is a few more K
 //            steps of the projection itself, so y is written once and never read back
 //
@@ -18,8 +17,8 @@
 // against the same rows of B), 2^-17 of V off.
 //
 // There a zero of V meets B of other requests' adapters: an infinity or NaN in one adapter would reach its neighbours'
-// rows. So an adapter whose B is not finite stays out of the product (plan finds it, reading B once, on its way into
-// L2) and its own rows get their term from the epilogue, number by number.
+// rows. So an adapter whose B is not finite stays out of the product (shrink finds it, reading B beside its own loads and
+// on its way into L2) and its own rows get their term from the epilogue, number by number.
 
 #include <algorithm>
 #include <initializer_list>
@@ -31,43 +30,116 @@ namespace sb {
 namespace {
 
 constexpr int kMaxSlots = kTileRows;
-// Per tile: the slot count, the adapter of each slot, the slot of each row (-1: none), and again the adapter of each slot,
-// or -1 where its B is not finite.
-constexpr int kSlotAdapter = 1, kRowSlot = kSlotAdapter + kMaxSlots, kSlotShared = kRowSlot + kTileRows;
-constexpr int kTableInts = kSlotShared + kMaxSlots;
-constexpr int kPlanThreads = 256;
+// Per tile: the slot count, the adapter of each slot, the slot of each row (-1: none).
+constexpr int kSlotAdapter = 1, kRowSlot = kSlotAdapter + kMaxSlots;
+constexpr int kTableInts = kRowSlot + kTileRows;
+constexpr int kMaxSplits = 8;  // thread blocks of a cluster; also the bytes per adapter that say whether its B is finite
 
-// ---- plan ---------------------------------------------------------------------------------------------------------
+// Every block of the shrink kernel looks through its part of the adapter's B and sets its byte.
+__device__ __forceinline__ bool adapter_finite(const uint8_t* not_finite, int32_t adapter, int32_t splits) {
+  const unsigned long long f = __ldg(reinterpret_cast<const unsigned long long*>(not_finite) + adapter);
+  return (splits < kMaxSplits ? f & ((1ull << (8 * splits)) - 1ull) : f) == 0ull;
+}
 
-// Block (tile, part): the tile's slots; part 0 writes them down, and every part looks through its part of the B of those
-// of the tile's adapters that the tile before does not have (they are being looked through there, or further up). For a
-// batch of whole requests that is once per request; in any order it is at most what expand reads of B anyway. Tiles that
-// share an adapter write the same answer.
-template <typename index_t>
-__global__ void __launch_bounds__(kPlanThreads)
-lora_plan_kernel(const index_t* __restrict__ adapter_idx, const uint4* __restrict__ b, int32_t* __restrict__ tables,
-                 uint8_t* __restrict__ not_finite, int32_t num_tokens, int32_t num_adapters, int32_t vecs_per_adapter) {
-  __shared__ alignas(16) int32_t id[kTileRows];
-  __shared__ int32_t slot_adapter[kMaxSlots];
-  __shared__ int32_t slot_of_first[kTileRows];
-  __shared__ int32_t warp_count[4];
-  __shared__ int32_t seen[kMaxSlots];
+// ---- shrink -------------------------------------------------------------------------------------------------------
+// A cluster per tile of 128 tokens, each block a part of D. Per group of slots (as many as fit 128 columns) one product:
+// x tile (K-major) times the slots' rows of A (K-major, 8 to 128 rows by TMA per slot and step). Row i of the tile takes
+// the columns of its slot from TMEM into shared memory; after the last group the blocks of the cluster add their parts up
+// over distributed shared memory, in rank order, each for its share of the rows.
+//
+// Meanwhile twelve more warps look for infinities and NaN in B: of those of the tile's adapters that the tile before
+// does not have (they are being looked through there, or further up). For a batch of whole requests that is once per
+// request; in any order it is at most what expand reads of B anyway. Tiles that share an adapter write the same answer.
+constexpr int kScanThreads = 384;
+constexpr int kShrinkThreads = 192 + kScanThreads;  // warp 0 TMA, warp 1 MMA, warps 2-5 workers (a row of the tile each), scan
+constexpr int kShrinkCols = 128;
+constexpr int kShrinkStageBytes = (kTileRows + kShrinkCols) * 128;
+
+struct ShrinkMaps {
+  CUtensorMap x, a;
+};
+struct ShrinkParams {
+  const void* adapter_idx;
+  const uint4* b;
+  const float* scale;
+  int32_t* tables;
+  uint8_t* not_finite;
+  __nv_bfloat16* v;  // [T, rank * parts]: the values, with parts = 2 then what rounding took from them
+  int32_t idx_is_i64, num_tokens, num_adapters, rank, parts, splits, steps, total_steps, stages;
+  int32_t b_vecs;  // 16-byte pieces of an adapter's B
+};
+constexpr int kShrinkHeadBytes = 512 + 4 * (4 * kTileRows + 8);  // barriers, ids, slots, first rows, seen, counts
+
+inline int shrink_smem_bytes(int stages, int rank) { return 1024 + kShrinkHeadBytes + stages * kShrinkStageBytes + kTileRows * rank * 4; }
+
+__device__ __forceinline__ int32_t adapter_of(const ShrinkParams& p, int32_t token) {
+  if (token < 0 || token >= p.num_tokens) return -1;
+  const int64_t a = p.idx_is_i64 ? __ldg(static_cast<const long long*>(p.adapter_idx) + token)
+                                 : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.adapter_idx) + token));
+  return a >= 0 && a < p.num_adapters ? static_cast<int32_t>(a) : -1;
+}
+
+__global__ void __launch_bounds__(kShrinkThreads, 1)
+lora_shrink_kernel(const __grid_constant__ ShrinkMaps maps, const __grid_constant__ ShrinkParams p, int32_t* dev_status) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_aligned = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
+  const uint32_t red_base = smem_base + static_cast<uint32_t>(p.stages) * kShrinkStageBytes;  // red[rank][128] fp32
+  const uint32_t head = red_base + static_cast<uint32_t>(kTileRows * p.rank) * 4u;
+  const uint32_t full_bar = head;             // [stages], at most 8
+  const uint32_t empty_bar = head + 64;       // [stages]
+  const uint32_t acc_full_bar = head + 128;   // [2]
+  const uint32_t acc_empty_bar = head + 144;  // [2]
+  const uint32_t tmem_slot = head + 160;
+  const uint32_t abort_slot = head + 164;
+  volatile uint32_t* tmem_word = reinterpret_cast<volatile uint32_t*>(smem_aligned + (tmem_slot - smem_base));
+  volatile uint32_t* abort_word = reinterpret_cast<volatile uint32_t*>(smem_aligned + (abort_slot - smem_base));
+  int32_t* id = reinterpret_cast<int32_t*>(smem_aligned + (head + 512 - smem_base));
+  int32_t* slot_adapter = id + kTileRows;
+  int32_t* work = slot_adapter + kTileRows;  // slot of the first row of an adapter; then: slot of each row
+  int32_t* seen = work + kTileRows;          // the slot's adapter is in the tile before, too
+  int32_t* count = seen + kTileRows;         // [4] per worker warp
+  float* red = reinterpret_cast<float*>(smem_aligned + (red_base - smem_base));
+
+  const int warp = static_cast<int>(threadIdx.x >> 5);
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int row = static_cast<int>(threadIdx.x) - 64;  // of the workers
+  const bool worker = row >= 0 && row < kTileRows;
+  const int32_t rank = static_cast<int32_t>(blockIdx.x) % p.splits;
+  const int32_t tile = static_cast<int32_t>(blockIdx.x) / p.splits;
+  const int32_t first_token = tile * kTileRows;
+
   ptx::grid_launch_dependents();
-  const int i = static_cast<int>(threadIdx.x);
-  const int32_t first_token = static_cast<int32_t>(blockIdx.x) * kTileRows;
-  int32_t mine = -1;
-  if (i < kTileRows) {
-    if (first_token + i < num_tokens) {
-      const int64_t a = static_cast<int64_t>(__ldg(adapter_idx + first_token + i));
-      if (a >= 0 && a < num_adapters) mine = static_cast<int32_t>(a);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      ptx::mbar_init(full_bar + 8 * s, 1);
+      ptx::mbar_init(empty_bar + 8 * s, 1);
     }
-    id[i] = mine;
-    seen[i] = 0;
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(acc_full_bar + 8 * a, 1);
+      ptx::mbar_init(acc_empty_bar + 8 * a, kTileRows);
+    }
+    *abort_word = 0u;
+    ptx::fence_barrier_init();
   }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, 2 * kShrinkCols);
+    ptx::tmem_relinquish();
+  }
+  int32_t mine = -1;
+  if (worker) {
+    mine = adapter_of(p, first_token + row);
+    id[row] = mine;
+    seen[row] = 0;
+  }
+  ptx::tcgen05_fence_before_sync();
   __syncthreads();
-  int first = i;
-  if (i < kTileRows && mine >= 0) {
-    for (int j = 0; j < i; j += 4) {
+  ptx::tcgen05_fence_after_sync();
+  const uint32_t tmem_base = *tmem_word;
+  // Slots. first never lies behind the row: its own id matches.
+  int first = row;
+  if (mine >= 0) {
+    for (int j = 0; j < row; j += 4) {
       const int4 four = *reinterpret_cast<const int4*>(id + j);
       if (four.x == mine) { first = j; break; }
       if (four.y == mine) { first = j + 1; break; }
@@ -75,160 +147,203 @@ lora_plan_kernel(const index_t* __restrict__ adapter_idx, const uint4* __restric
       if (four.w == mine) { first = j + 3; break; }
     }
   }
-  const bool leads = i < kTileRows && mine >= 0 && first == i;  // first never lies behind i: id[i] itself matches
-  const unsigned ballot = __ballot_sync(0xffffffffu, leads);
-  if (i < kTileRows && (i & 31) == 0) warp_count[i >> 5] = __popc(ballot);
+  const bool leads = mine >= 0 && first == row;
+  const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+  if (worker && lane == 0) count[warp - 2] = __popc(leaders);
   __syncthreads();
-  int32_t slots = 0, slot = __popc(ballot & ((1u << (i & 31)) - 1u));
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < (i >> 5)) slot += warp_count[w];
-    slots += warp_count[w];
-  }
+  const int32_t slots = count[0] + count[1] + count[2] + count[3];
   if (leads) {
+    int32_t slot = __popc(leaders & ((1u << lane) - 1u));
+    for (int w = 0; w < warp - 2; ++w) slot += count[w];
     slot_adapter[slot] = mine;
-    slot_of_first[i] = slot;
+    work[row] = slot;
   }
   __syncthreads();
-  if (blockIdx.y == 0) {
-    int32_t* table = tables + static_cast<int64_t>(blockIdx.x) * kTableInts;
-    if (i == 0) table[0] = slots;
-    if (i < slots) table[kSlotAdapter + i] = slot_adapter[i];
-    if (i < kTileRows) table[kRowSlot + i] = mine >= 0 ? slot_of_first[first] : -1;
+  const int32_t my_slot = mine >= 0 ? work[first] : -1;
+  if (worker && rank == 0) {
+    int32_t* table = p.tables + static_cast<int64_t>(tile) * kTableInts;
+    if (row == 0) table[0] = slots;
+    if (row < slots) table[kSlotAdapter + row] = slot_adapter[row];
+    table[kRowSlot + row] = my_slot;
   }
-  if (i < kTileRows && first_token > 0) {
-    const int64_t a = static_cast<int64_t>(__ldg(adapter_idx + first_token - kTileRows + i));
-    for (int32_t s = 0; s < slots; ++s)
-      if (slot_adapter[s] == a) seen[s] = 1;
-  }
-  __syncthreads();
-  const int32_t parts = static_cast<int32_t>(gridDim.y);
-  const int32_t per_part = (vecs_per_adapter + parts - 1) / parts;
-  const int32_t begin = static_cast<int32_t>(blockIdx.y) * per_part;
-  const int32_t end = min(vecs_per_adapter, begin + per_part);
-  for (int32_t s = 0; s < slots; ++s) {
-    if (seen[s] != 0) continue;
-    const int32_t a = slot_adapter[s];
-    const uint4* rows = b + static_cast<int64_t>(a) * vecs_per_adapter;
-    bool bad = false;
-#pragma unroll 4
-    for (int32_t v = begin + i; v < end; v += kPlanThreads) {
-      const uint4 raw = __ldg(rows + v);
-      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int q = 0; q < 4; ++q)  // bf16: all eight exponent bits set
-        bad |= (words[q] & 0x7f80u) == 0x7f80u || (words[q] & 0x7f800000u) == 0x7f800000u;
-    }
-    const int any = __syncthreads_or(bad);
-    if (i == 0) not_finite[static_cast<int64_t>(a) * parts + blockIdx.y] = any ? 1 : 0;
-  }
-}
-
-// ---- shrink -------------------------------------------------------------------------------------------------------
-// One tile = 128 tokens x the slots of one group (as many as fit 256 columns) x one part of D.
-struct LoraShrink {
-  struct Params {
-    const int32_t* tables;
-    float* partial;  // [splits, T, r]
-    int32_t num_tokens, rank, row_tiles, groups, group_slots, splits, steps, total_steps;  // steps: per split
+  const int32_t group_slots = kShrinkCols / p.rank;
+  const int32_t groups = (slots + group_slots - 1) / group_slots;
+  const int32_t k0 = rank * p.steps;
+  const int32_t steps = max(0, min(p.steps, p.total_steps - k0));
+  auto give_up = [&](int bit) {
+    *abort_word = 1u;
+    if (dev_status != nullptr) atomicOr(dev_status, bit);
   };
-  struct Tile {
-    int32_t k_steps, row_tile, first_slot, slots, step0, split;
-    const int32_t* adapters;
-    bool live;
-  };
-  struct Early { int32_t slot; };
-  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
-  static constexpr bool kAhead = false;
-  static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.row_tiles * p.groups * p.splits; }
-  static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
-    Tile t;
-    // Groups past a tile's slots are dead: the group is the slowest index, so the live tiles come first.
-    const int32_t group = index / (p.row_tiles * p.splits);
-    const int32_t rest = index - group * (p.row_tiles * p.splits);
-    t.row_tile = rest / p.splits;
-    t.split = rest - t.row_tile * p.splits;
-    const int32_t* table = p.tables + static_cast<int64_t>(t.row_tile) * kTableInts;
-    t.first_slot = group * p.group_slots;
-    t.slots = min(p.group_slots, __ldg(table) - t.first_slot);
-    t.adapters = table + kSlotAdapter + t.first_slot;
-    t.step0 = t.split * p.steps;
-    t.live = t.slots > 0;
-    t.k_steps = t.live ? min(p.steps, p.total_steps - t.step0) : 0;
-    return t;
-  }
-  static __device__ __forceinline__ int columns(const Params& p) { return (p.group_slots * p.rank + 15) & ~15; }
-  static __device__ __forceinline__ uint32_t tx_bytes(const Params& p, const Tile& t, int32_t) {
-    return TileSmem::kABytes + static_cast<uint32_t>(t.slots * p.rank) * 128u;
-  }
-  static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
-                                              uint32_t b, uint32_t bar) {
-    const int32_t k = (t.step0 + ks) * kTileStep;
-    ptx::tma_load_2d(a, &maps.m[0], k, t.row_tile * kTileRows, bar);
-    for (int32_t s = 0; s < t.slots; ++s)
-      ptx::tma_load_2d(b + static_cast<uint32_t>(s * p.rank) * 128u, &maps.m[1], k, __ldg(t.adapters + s) * p.rank, bar);
-  }
-  static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
-    return {__ldg(p.tables + static_cast<int64_t>(t.row_tile) * kTableInts + kRowSlot + w.quarter * 32 + w.lane)};
-  }
-  static __device__ __forceinline__ void epilogue(const TileMaps&, const Params& p, const Tile& t, EpilogueWarp& w,
-                                                  const Early& early) {
-    const int32_t token = t.row_tile * kTileRows + w.quarter * 32 + w.lane;
-    float* dst = p.partial + (static_cast<int64_t>(t.split) * p.num_tokens + token) * p.rank;
-    for (int32_t s = w.part; s < t.slots; s += 2) {  // the two warps of a quarter share the slots
-      const bool mine = early.slot == t.first_slot + s;
-      if (__ballot_sync(0xffffffffu, mine) == 0u) continue;
-      for (int32_t j = 0; j < p.rank; j += 8) {
-        uint32_t v[8];
-        ptx::tmem_ld_32x32b_x8(w.taddr + s * p.rank + j, v);
-        ptx::tmem_ld_wait();
-        if (mine) {
-          *reinterpret_cast<uint4*>(dst + j) = make_uint4(v[0], v[1], v[2], v[3]);
-          *reinterpret_cast<uint4*>(dst + j + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int32_t g = 0; ok && g < groups; ++g) {
+        const int32_t n = min(group_slots, slots - g * group_slots);
+        for (int32_t ks = 0; ks < steps; ++ks) {
+          if (!ptx::mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort_word)) {
+            give_up(SB_DEV_TIMEOUT_PRODUCER);
+            ok = false;
+            break;
+          }
+          const uint32_t bar = full_bar + 8 * stage;
+          const uint32_t a = smem_base + stage * kShrinkStageBytes;
+          const int32_t k = (k0 + ks) * kTileStep;
+          ptx::mbar_arrive_expect_tx(bar, kTileRows * 128u + static_cast<uint32_t>(n * p.rank) * 128u);
+          ptx::tma_load_2d(a, &maps.x, k, first_token, bar);
+          for (int32_t s = 0; s < n; ++s)
+            ptx::tma_load_2d(a + (kTileRows + s * p.rank) * 128u, &maps.a, k, slot_adapter[g * group_slots + s] * p.rank, bar);
+          if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
         }
       }
     }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && steps > 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int32_t g = 0; ok && g < groups; ++g) {
+        const uint32_t acc = static_cast<uint32_t>(g) & 1u;
+        const uint32_t acc_phase = (static_cast<uint32_t>(g) >> 1) & 1u;
+        if (!ptx::mbar_wait_bounded(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_word)) {
+          give_up(SB_DEV_TIMEOUT_MMA);
+          break;
+        }
+        ptx::tcgen05_fence_after_sync();
+        const int n = (min(group_slots, slots - g * group_slots) * p.rank + 15) & ~15;
+        const uint32_t idesc = ptx::make_idesc_bf16(kTileRows, n, false);
+        for (int32_t ks = 0; ks < steps; ++ks) {
+          if (!ptx::mbar_wait_bounded(full_bar + 8 * stage, phase, abort_word)) {
+            give_up(SB_DEV_TIMEOUT_MMA);
+            ok = false;
+            break;
+          }
+          ptx::tcgen05_fence_after_sync();
+          const uint32_t a = smem_base + stage * kShrinkStageBytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            ptx::umma_bf16(tmem_base + acc * kShrinkCols, ptx::make_smem_desc(a + kk * 32, 16, 1024),
+                           ptx::make_smem_desc(a + kTileRows * 128 + kk * 32, 16, 1024), idesc, (ks | kk) != 0);
+          ptx::umma_commit(empty_bar + 8 * stage);
+          if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) ptx::umma_commit(acc_full_bar + 8 * acc);
+      }
+    }
+    __syncwarp();
+  } else if (!worker) {
+    // ---- B of the adapters that are new in this tile
+    const int i = static_cast<int>(threadIdx.x) - 192;
+    if (i < kTileRows && first_token > 0) {
+      const int32_t before = adapter_of(p, first_token - kTileRows + i);
+      if (before >= 0)
+        for (int32_t s = 0; s < slots; ++s)
+          if (slot_adapter[s] == before) seen[s] = 1;
+    }
+    named_barrier(2, kScanThreads);
+    const int32_t per_part = (p.b_vecs + p.splits - 1) / p.splits;
+    const int32_t end = min(p.b_vecs, (rank + 1) * per_part);
+    for (int32_t s = 0; s < slots; ++s) {
+      if (seen[s] != 0) continue;
+      const int32_t a = slot_adapter[s];
+      const uint4* from = p.b + static_cast<int64_t>(a) * p.b_vecs;
+      bool bad = false;
+      for (int32_t v0 = rank * per_part + i; v0 < end; v0 += 16 * kScanThreads) {
+        uint4 raw[16];  // all on their way at once: what bounds this is the latency of the loads
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+          raw[u] = v0 + u * kScanThreads < end ? __ldg(from + v0 + u * kScanThreads) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const uint32_t words[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)  // bf16: all eight exponent bits set
+            bad |= (words[q] & 0x7f80u) == 0x7f80u || (words[q] & 0x7f800000u) == 0x7f800000u;
+        }
+      }
+      const bool any = named_barrier_or(2, kScanThreads, bad);
+      if (i == 0) p.not_finite[static_cast<int64_t>(a) * kMaxSplits + rank] = any ? 1 : 0;
+    }
+  } else {
+    // ---- this block's part of V: TMEM lane = row
+    const int quarter = warp & 3;
+    const int lane_row = quarter * 32 + lane;
+    // The row a thread drains is its TMEM lane, which is another row than the one it found the slot of.
+    named_barrier(1, kTileRows);  // every worker has its slot: `work` may be used again
+    work[row] = my_slot;
+    named_barrier(1, kTileRows);
+    const int32_t slot_here = work[lane_row];
+    if (steps == 0 && slot_here >= 0)
+      for (int32_t j = 0; j < p.rank; ++j) red[j * kTileRows + lane_row] = 0.0f;
+    for (int32_t g = 0; steps > 0 && g < groups; ++g) {
+      const uint32_t acc = static_cast<uint32_t>(g) & 1u;
+      if (!ptx::mbar_wait_bounded(acc_full_bar + 8 * acc, (static_cast<uint32_t>(g) >> 1) & 1u, abort_word)) {
+        give_up(SB_DEV_TIMEOUT_EPILOGUE);
+        break;
+      }
+      ptx::tcgen05_fence_after_sync();
+      const int32_t n = min(group_slots, slots - g * group_slots);
+      for (int32_t s = 0; s < n; ++s) {
+        const bool take = slot_here == g * group_slots + s;
+        if (__ballot_sync(0xffffffffu, take) == 0u) continue;
+        for (int32_t j = 0; j < p.rank; j += 8) {
+          uint32_t v[8];
+          ptx::tmem_ld_32x32b_x8(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kShrinkCols + s * p.rank + j, v);
+          ptx::tmem_ld_wait();
+          if (take) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) red[(j + q) * kTileRows + lane_row] = __uint_as_float(v[q]);
+          }
+        }
+      }
+      ptx::tcgen05_fence_before_sync();
+      ptx::mbar_arrive(acc_empty_bar + 8 * acc);
+    }
   }
-};
-
-// V[t] = scale * sum over the parts, in order, as one bf16 (parts = 1) or as a pair (parts = 2: r values, then r
-// remainders). Tokens without an adapter are not read later and not written. Also the last column of the tables.
-template <typename index_t>
-__global__ void __launch_bounds__(256)
-lora_join_kernel(const float* __restrict__ partial, const index_t* __restrict__ adapter_idx, const float* __restrict__ scale,
-                 __nv_bfloat16* __restrict__ v, int32_t num_tokens, int32_t num_adapters, int32_t rank, int32_t splits,
-                 int32_t parts, int32_t* __restrict__ tables, const uint8_t* __restrict__ not_finite, int32_t row_tiles,
-                 int32_t scan_parts) {
-  ptx::grid_launch_dependents();
-  ptx::grid_dependency_wait();
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t start = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  for (int64_t i = start; i < static_cast<int64_t>(row_tiles) * kMaxSlots; i += stride) {
-    int32_t* table = tables + i / kMaxSlots * kTableInts;
-    const int32_t s = static_cast<int32_t>(i % kMaxSlots);
-    if (s >= __ldcg(table)) continue;
-    int32_t a = __ldcg(table + kSlotAdapter + s);
-    const uint8_t* flags = not_finite + static_cast<int64_t>(a) * scan_parts;
-    unsigned bad = 0;
-    for (int32_t q = 0; q < scan_parts; ++q) bad |= __ldcg(flags + q);
-    table[kSlotShared + s] = bad != 0 ? -1 : a;
+  if (*abort_word != 0u) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the shared memory is handed back
   }
-  const int64_t total = static_cast<int64_t>(num_tokens) * rank;
-  for (int64_t i = start; i < total; i += stride) {
-    const int32_t t = static_cast<int32_t>(i / rank);
-    const int32_t j = static_cast<int32_t>(i - static_cast<int64_t>(t) * rank);
-    const int64_t a = static_cast<int64_t>(__ldg(adapter_idx + t));
-    if (a < 0 || a >= num_adapters) continue;
-    float sum = 0.0f;
-    for (int32_t s = 0; s < splits; ++s) sum += __ldcg(partial + s * total + i);
-    if (scale != nullptr) sum *= __ldg(scale + a);
-    const __nv_bfloat16 high = __float2bfloat16_rn(sum);
-    __nv_bfloat16* row = v + static_cast<int64_t>(t) * rank * parts;
-    row[j] = high;
-    if (parts == 2) row[rank + j] = __float2bfloat16_rn(isfinite(__bfloat162float(high)) ? sum - __bfloat162float(high) : 0.0f);
+  __syncwarp();
+  ptx::tcgen05_fence_before_sync();
+  if (p.splits > 1) ptx::cluster_sync_all();
+  else __syncthreads();
+  if (warp == 1) {
+    ptx::tcgen05_fence_after_sync();
+    ptx::tmem_dealloc(tmem_base, 2 * kShrinkCols);
   }
+  if (worker && *abort_word == 0u) {
+    // Eight values of a row per thread; the block's share of the rows is every splits-th.
+    const int32_t pieces = p.rank / 8;
+    const int32_t rows = (kTileRows - rank + p.splits - 1) / p.splits;
+    for (int32_t i = row; i < rows * pieces; i += kTileRows) {
+      const int32_t r = rank + (i % rows) * p.splits;
+      const int32_t j0 = i / rows * 8;
+      const int32_t a = id[r];
+      if (a < 0) continue;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+      for (int32_t part = 0; part < p.splits; ++part) {
+        const uint32_t from = ptx::map_to_cta(red_base + static_cast<uint32_t>(j0 * kTileRows + r) * 4u, static_cast<uint32_t>(part));
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] += ptx::ld_cluster_f32(from + q * kTileRows * 4u);
+      }
+      const float factor = p.scale != nullptr ? __ldg(p.scale + a) : 1.0f;
+      uint32_t high[4], low[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float v0 = v[2 * q] * factor, v1 = v[2 * q + 1] * factor;
+        high[q] = pack_bf16(v0, v1);
+        const float2 h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&high[q]));
+        low[q] = pack_bf16(isfinite(h.x) ? v0 - h.x : 0.0f, isfinite(h.y) ? v1 - h.y : 0.0f);
+      }
+      __nv_bfloat16* dst = p.v + static_cast<int64_t>(first_token + r) * p.rank * p.parts + j0;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(high[0], high[1], high[2], high[3]);
+      if (p.parts == 2) *reinterpret_cast<uint4*>(dst + p.rank) = make_uint4(low[0], low[1], low[2], low[3]);
+    }
+  }
+  if (p.splits > 1) ptx::cluster_sync_all();  // nobody's shared memory is read any more
 }
 
 // ---- expand -------------------------------------------------------------------------------------------------------
@@ -236,9 +351,10 @@ struct LoraExpand {
   struct Params {
     BandOrder order;
     const int32_t* tables;
+    const uint8_t* not_finite;
     const __nv_bfloat16* v;
     const __nv_bfloat16* b;
-    int32_t num_tokens, width, rank, v_cols, base_steps, adapter_rows, cols, out_fp32;  // v_cols = rank * parts
+    int32_t num_tokens, width, rank, v_cols, base_steps, adapter_rows, cols, out_fp32, splits;  // v_cols = rank * parts
   };
   struct Tile {
     int32_t k_steps, base_steps, row_tile, n0, slots;
@@ -271,35 +387,33 @@ struct LoraExpand {
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
+    ptx::tma_load_2d(a, &maps.m[3], ks * kTileStep, t.row_tile * kTileRows, bar);
     const int n = slabs(p);
-    if (ks < t.base_steps) {
-      ptx::tma_load_2d(a, &maps.m[3], ks * kTileStep, t.row_tile * kTileRows, bar);
-      for (int j = 0; j < n; ++j)
-        ptx::tma_load_2d(b + j * TileSmem::kSlabBytes, &maps.m[0], t.n0 + j * 64, ks * kTileStep, bar);
-      return;
-    }
-    // Eight K rows at a time: rows of one adapter's B, or of none (past the end, or not finite: zeros).
-    int32_t row[8];
-#pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const int32_t q = (ks - t.base_steps) * kTileStep + g * 8;
-      const int32_t slot = q / p.v_cols;
-      const int32_t a_id = slot < t.slots ? __ldg(t.table + kSlotShared + slot) : -1;
-      int32_t j = q - slot * p.v_cols;
-      if (j >= p.rank) j -= p.rank;
-      row[g] = a_id >= 0 ? a_id * p.rank + j : p.adapter_rows;
-    }
-#pragma unroll
-    for (int g = 0; g < 8; ++g)
-      for (int j = 0; j < n; ++j)
-        ptx::tma_load_2d(b + j * TileSmem::kSlabBytes + g * 1024, &maps.m[1], t.n0 + j * 64, row[g], bar);
+    for (int j = 0; j < n; ++j)
+      ptx::tma_load_2d(b + j * TileSmem::kSlabBytes, &maps.m[0], t.n0 + j * 64, ks * kTileStep, bar);
   }
-  static __device__ __forceinline__ Rows rows(const Params&, const Tile& t, int row0) {
+  // Eight K rows at a time: rows of one adapter's B, or of none (past the end, or not finite: zeros).
+  static __device__ __forceinline__ int32_t extension_row(const Params& p, const Tile& t, int32_t ks, int piece) {
+    const int32_t q = (ks - t.base_steps) * kTileStep + piece * 8;
+    const int32_t slot = q / p.v_cols;
+    if (slot >= t.slots) return p.adapter_rows;
+    const int32_t a = __ldg(t.table + kSlotAdapter + slot);
+    if (!adapter_finite(p.not_finite, a, p.splits)) return p.adapter_rows;
+    const int32_t j = q - slot * p.v_cols;
+    return a * p.rank + (j >= p.rank ? j - p.rank : j);
+  }
+  static __device__ __forceinline__ void extension_load(const TileMaps& maps, const Params& p, const Tile& t, int piece,
+                                                        int32_t row, uint32_t b, uint32_t bar) {
+    const int n = slabs(p);
+    for (int j = 0; j < n; ++j)
+      ptx::tma_load_2d(b + j * TileSmem::kSlabBytes + piece * 1024, &maps.m[1], t.n0 + j * 64, row, bar);
+  }
+  static __device__ __forceinline__ Rows rows(const Params& p, const Tile& t, int row0) {
     Rows r;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       r.slot[j] = __ldg(t.table + kRowSlot + row0 + j * 16);
-      if (r.slot[j] >= 0 && __ldg(t.table + kSlotShared + r.slot[j]) < 0) r.slot[j] = -1;
+      if (r.slot[j] >= 0 && !adapter_finite(p.not_finite, __ldg(t.table + kSlotAdapter + r.slot[j]), p.splits)) r.slot[j] = -1;
     }
     return r;
   }
@@ -313,8 +427,9 @@ struct LoraExpand {
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
     const int32_t slot = __ldg(t.table + kRowSlot + w.quarter * 32 + w.lane);
-    if (slot < 0 || __ldg(t.table + kSlotShared + slot) >= 0) return {-1};
-    return {__ldg(t.table + kSlotAdapter + slot)};
+    if (slot < 0) return {-1};
+    const int32_t a = __ldg(t.table + kSlotAdapter + slot);
+    return {adapter_finite(p.not_finite, a, p.splits) ? -1 : a};
   }
   static __device__ __forceinline__ void epilogue(const TileMaps& maps, const Params& p, const Tile& t, EpilogueWarp& w,
                                                   const Early& early) {
@@ -533,13 +648,13 @@ int lora_small(const void* x, const void* weight, const void* lora_a, const void
 }
 
 struct LoraSizes {
-  int64_t row_tiles, tables, not_finite, partial, v, total;  // bytes of each part, 256-byte aligned, then all
-  int32_t splits, steps, total_steps, parts, scan_parts;
+  int64_t row_tiles, tables, not_finite, v, total;  // bytes of each part, 256-byte aligned, then all
+  int32_t splits, steps, total_steps, parts;
 };
 
 int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
-LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t width, int32_t rank, int32_t num_adapters, int out_fp32, int sm_count) {
+LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t rank, int32_t num_adapters, int out_fp32, int sm_count) {
   LoraSizes s{};
   if (num_tokens <= kSkinnyMaxRows) {
     s.v = align256(num_tokens * rank * 4);
@@ -549,19 +664,14 @@ LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t width, int32_t
   s.row_tiles = (num_tokens + kTileRows - 1) / kTileRows;
   s.parts = out_fp32 ? 2 : 1;
   s.total_steps = (d_model + kTileStep - 1) / kTileStep;
-  // Parts of D for few row tiles: enough to fill the GPU, each of at least 8 K steps.
-  const int64_t want = std::max<int64_t>(1, sm_count / std::max<int64_t>(1, s.row_tiles));
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(want, s.total_steps / 8));
-  s.steps = static_cast<int32_t>((s.total_steps + parts - 1) / parts);
-  s.splits = (s.total_steps + s.steps - 1) / s.steps;
+  // Parts of D for few row tiles: up to a block per SM, each of at least 4 K steps.
+  s.splits = 1;
+  while (s.splits < kMaxSplits && s.row_tiles * s.splits * 2 <= sm_count && s.total_steps >= 8 * s.splits) s.splits *= 2;
+  s.steps = (s.total_steps + s.splits - 1) / s.splits;
   s.tables = align256(s.row_tiles * kTableInts * 4);
-  // Thread blocks that look through one adapter's B: about four per SM over all tiles, each for 8 KB at least.
-  const int64_t b_bytes = static_cast<int64_t>(rank) * width * 2;
-  s.scan_parts = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({64, 4 * sm_count / s.row_tiles, b_bytes / 8192})));
-  s.not_finite = align256(static_cast<int64_t>(num_adapters) * s.scan_parts);
-  s.partial = align256(static_cast<int64_t>(s.splits) * num_tokens * rank * 4);
+  s.not_finite = align256(static_cast<int64_t>(num_adapters) * kMaxSplits);
   s.v = align256(num_tokens * rank * s.parts * 2);
-  s.total = s.tables + s.not_finite + s.partial + s.v;
+  s.total = s.tables + s.not_finite + s.v;
   return s;
 }
 
@@ -587,7 +697,7 @@ extern "C" int64_t sb_lora_workspace_bytes(int64_t num_tokens, int32_t d_model, 
   if (check_lora(num_tokens, d_model, width, rank, num_adapters) != SB_OK) return -1;
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return -1;
-  return lora_sizes(num_tokens, d_model, width, rank, num_adapters, out_fp32, info->sm_count).total;
+  return lora_sizes(num_tokens, d_model, rank, num_adapters, out_fp32, info->sm_count).total;
 }
 
 extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lora_a, const void* lora_b,
@@ -603,7 +713,7 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
     if (!aligned16(q)) return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: buffers must be 16-byte aligned");
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
-  const LoraSizes s = lora_sizes(num_tokens, d_model, width, rank, num_adapters, out_fp32, info->sm_count);
+  const LoraSizes s = lora_sizes(num_tokens, d_model, rank, num_adapters, out_fp32, info->sm_count);
   if (workspace_bytes < s.total)
     return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: the workspace has %lld bytes, %lld are needed",
                 (long long)workspace_bytes, (long long)s.total);
@@ -613,59 +723,53 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
                       d_model, width, rank, num_adapters, reinterpret_cast<float*>(ws), info, dev_status, as_stream(stream));
   int32_t* tables = reinterpret_cast<int32_t*>(ws);
   uint8_t* not_finite = ws + s.tables;
-  float* partial = reinterpret_cast<float*>(not_finite + s.not_finite);
-  __nv_bfloat16* v = reinterpret_cast<__nv_bfloat16*>(not_finite + s.not_finite + s.partial);
+  __nv_bfloat16* v = reinterpret_cast<__nv_bfloat16*>(not_finite + s.not_finite);
   const cudaStream_t st = as_stream(stream);
   const int32_t tokens = static_cast<int32_t>(num_tokens);
   const int32_t row_tiles = static_cast<int32_t>(s.row_tiles);
-
-  const dim3 plan_grid(static_cast<unsigned>(row_tiles), static_cast<unsigned>(s.scan_parts));
-  const int32_t b_vecs = rank * (width / 8);
-  if (idx_is_i64)
-    lora_plan_kernel<int64_t><<<plan_grid, kPlanThreads, 0, st>>>(static_cast<const int64_t*>(adapter_idx),
-        static_cast<const uint4*>(lora_b), tables, not_finite, tokens, num_adapters, b_vecs);
-  else
-    lora_plan_kernel<int32_t><<<plan_grid, kPlanThreads, 0, st>>>(static_cast<const int32_t*>(adapter_idx),
-        static_cast<const uint4*>(lora_b), tables, not_finite, tokens, num_adapters, b_vecs);
-  if (int rc = check_launch("lora_linear (plan)")) return rc;
-
   {
-    TileMaps maps{};
-    if (int rc = encode_2d_map(&maps.m[0], x, num_tokens, d_model, kTileRows, 64, 2, "lora_linear (x)")) return rc;
-    if (int rc = encode_2d_map(&maps.m[1], lora_a, static_cast<uint64_t>(num_adapters) * rank, d_model, rank, 64, 2, "lora_linear (A)")) return rc;
-    LoraShrink::Params p{};
+    ShrinkMaps maps{};
+    if (int rc = encode_2d_map(&maps.x, x, num_tokens, d_model, kTileRows, 64, 2, "lora_linear (x)")) return rc;
+    if (int rc = encode_2d_map(&maps.a, lora_a, static_cast<uint64_t>(num_adapters) * rank, d_model, rank, 64, 2, "lora_linear (A)")) return rc;
+    ShrinkParams p{};
+    p.adapter_idx = adapter_idx;
+    p.b = static_cast<const uint4*>(lora_b);
+    p.scale = scale;
     p.tables = tables;
-    p.partial = partial;
+    p.not_finite = not_finite;
+    p.v = v;
+    p.idx_is_i64 = idx_is_i64;
     p.num_tokens = tokens;
+    p.num_adapters = num_adapters;
     p.rank = rank;
-    p.row_tiles = row_tiles;
-    const int32_t most = static_cast<int32_t>(std::min<int64_t>({kMaxSlots, num_adapters, num_tokens}));
-    p.group_slots = std::min(kTileCols / rank, most);
-    p.groups = (most + p.group_slots - 1) / p.group_slots;
+    p.parts = s.parts;
     p.splits = s.splits;
     p.steps = s.steps;
     p.total_steps = s.total_steps;
-    if (int rc = launch_tile_gemm<LoraShrink>(maps, p, static_cast<int64_t>(row_tiles) * p.groups * p.splits, dev_status, st, "lora_linear (shrink)")) return rc;
-  }
-  {
-    const int64_t values = std::max<int64_t>(num_tokens * rank, static_cast<int64_t>(row_tiles) * kMaxSlots);
+    p.b_vecs = rank * (width / 8);
+    p.stages = std::min(6, (225 * 1024 - 1024 - kShrinkHeadBytes - kTileRows * rank * 4) / kShrinkStageBytes);
+    int device = 0;
+    if (current_device_info(&device) == nullptr) return SB_ERR_CUDA;
+    static std::atomic<bool> done[kMaxDevices] = {};
+    if (!done[device].load(std::memory_order_acquire)) {
+      const cudaError_t err = cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
+      if (err != cudaSuccess) return fail(SB_ERR_CUDA, "lora_linear: shared memory opt-in: %s", cudaGetErrorString(err));
+      done[device].store(true, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((values + 255) / 256, static_cast<int64_t>(info->sm_count) * 8)));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(static_cast<unsigned>(row_tiles * s.splits));
+    cfg.blockDim = dim3(kShrinkThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(shrink_smem_bytes(p.stages, rank));
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(s.splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const float* parts = partial;
-    const uint8_t* flags = not_finite;
-    const cudaError_t err =
-        idx_is_i64 ? cudaLaunchKernelEx(&cfg, lora_join_kernel<int64_t>, parts, static_cast<const int64_t*>(adapter_idx), scale, v, tokens,
-                                        num_adapters, rank, s.splits, s.parts, tables, flags, row_tiles, s.scan_parts)
-                   : cudaLaunchKernelEx(&cfg, lora_join_kernel<int32_t>, parts, static_cast<const int32_t*>(adapter_idx), scale, v, tokens,
-                                        num_adapters, rank, s.splits, s.parts, tables, flags, row_tiles, s.scan_parts);
-    if (err != cudaSuccess) return fail(SB_ERR_CUDA, "lora_linear (join): %s", cudaGetErrorString(err));
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, lora_shrink_kernel, maps, p, dev_status);
+    if (err != cudaSuccess) return fail(SB_ERR_CUDA, "lora_linear (shrink): %s", cudaGetErrorString(err));
   }
 
   TileMaps maps{};
@@ -677,6 +781,8 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
   const int32_t slices = (width + kTileCols - 1) / kTileCols;
   p.order = {row_tiles, slices, 8};
   p.tables = tables;
+  p.not_finite = not_finite;
+  p.splits = s.splits;
   p.v = v;
   p.b = static_cast<const __nv_bfloat16*>(lora_b);
   p.num_tokens = tokens;

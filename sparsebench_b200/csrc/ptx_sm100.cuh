@@ -317,6 +317,11 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
   return out;
 }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 // Arrivals on a barrier given by its shared::cluster address (this CTA's or the peer's). Default semantics
 // (release at CTA scope), as for a local arrive: asking for a cluster-scope release here made every arrive of
 // the TMA producer cost about a memory round trip (the producer, not the tensor core, then set the pace:

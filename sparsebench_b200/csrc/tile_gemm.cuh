@@ -105,9 +105,10 @@ struct BandOrder {
 //   static constexpr bool kAMnMajor, kBMnMajor
 //   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar), tx_bytes
 //   static constexpr int kStages (of the ring), kEpilogueWarps, kBuffers (staging tiles of each, may be 0)
-//   With kExtension: Tile has base_steps; A of the K steps behind them is written by four warps from registers:
+//   With kExtension: Tile has base_steps; four warps fill the stages of the K steps behind them. A from registers:
 //   Rows rows(p, tile, row0) once per tile, extension_chunk(p, tile, rows, j, row, ks, chunk) = the 16 bytes of chunk
-//   `chunk` of row `row` = row0 + 16 j.
+//   `chunk` of row `row` = row0 + 16 j. B (MN-major) eight K rows at a time: extension_row(p, tile, ks, i) says where
+//   piece i comes from, ahead of time, extension_load(maps, p, tile, i, row, b, bar) issues its loads.
 //   With kVariable: columns(p) <= 256 (a multiple of 16) accumulator columns in use, tx_bytes(p, tile, ks) per stage
 template <class Op>
 struct TileConfig {
@@ -198,12 +199,15 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
             break;
           }
           const uint32_t bar = full_bar + 8 * stage;
-          if constexpr (Op::kExtension) {
-            if (ks >= tile.base_steps) ptx::mbar_arrive(go_bar + 8 * stage);
+          bool extension = false;
+          if constexpr (Op::kExtension) extension = ks >= tile.base_steps;
+          if (extension) {
+            ptx::mbar_arrive(go_bar + 8 * stage);  // the extension warps fill this stage
+          } else {
+            if constexpr (Op::kVariable) ptx::mbar_arrive_expect_tx(bar, Op::tx_bytes(p, tile, ks));
+            else ptx::mbar_arrive_expect_tx(bar, S::kBBytes + S::kABytes);
+            Op::load(maps, p, tile, ks, a_base + stage * S::kABytes, b_base + stage * S::kBBytes, bar);
           }
-          if constexpr (Op::kVariable) ptx::mbar_arrive_expect_tx(bar, Op::tx_bytes(p, tile, ks));
-          else ptx::mbar_arrive_expect_tx(bar, S::kBBytes + S::kABytes);
-          Op::load(maps, p, tile, ks, a_base + stage * S::kABytes, b_base + stage * S::kBBytes, bar);
           if (++stage == Op::kStages) { stage = 0; phase ^= 1u; }
         }
       }
@@ -321,12 +325,19 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
           uint4 chunks[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) chunks[j] = Op::extension_chunk(p, tile, rows, j, row0 + j * 16, ks, chunk);
+          const bool loads = warp == Cfg::kFirstExtensionWarp && lane < 8;
+          const int32_t b_row = loads ? Op::extension_row(p, tile, ks, lane) : 0;
           if (!ptx::mbar_wait_bounded(go_bar + 8 * stage, (go_phases >> stage) & 1u, abort_word)) {
             give_up(SB_DEV_TIMEOUT_PRODUCER);
             ok = false;
             break;
           }
           go_phases ^= 1u << stage;
+          if (warp == Cfg::kFirstExtensionWarp) {
+            if (lane == 0) ptx::mbar_arrive_expect_tx(full_bar + 8 * stage, Op::tx_bytes(p, tile, ks));
+            __syncwarp();
+            if (loads) Op::extension_load(maps, p, tile, lane, b_row, b_base + stage * S::kBBytes, full_bar + 8 * stage);
+          }
           const uint32_t dst = a_base + stage * S::kABytes + dst_off;
 #pragma unroll
           for (int j = 0; j < 8; ++j) ptx::st_shared_v4(dst + j * 2048, chunks[j].x, chunks[j].y, chunks[j].z, chunks[j].w);
