@@ -83,9 +83,9 @@ def gated_reference(x, expert_idx, gate, w_gate, w_up, w_down, act: str = "silu"
         do = go[t]
         val["dgate"][t, j] = (do * y).sum(1)
         bnd["dgate"][t, j] = (do.abs() * y_b + d_model * HALF_FP32 * (do * y).abs()).sum(1)
-        wdo = w * do  # held as bf16
+        wdo = w * do  # held as bf16 for dw_down; dh takes the unscaled rows and w in fp32
         dh = wdo @ wd.T
-        dh_b = (HALF_BF16 + d_model * HALF_FP32) * (wdo.abs() @ wd.abs().T)
+        dh_b = (d_model + 1) * HALF_FP32 * (wdo.abs() @ wd.abs().T)
         du, dg = dh * a, dh * u * s
         du_b = dh_b * a.abs() + dh.abs() * a_b + HALF_BF16 * du.abs()
         dg_b = dh_b * (u * s).abs() + dh.abs() * (u_b * s.abs() + u.abs() * s_b) + HALF_BF16 * dg.abs()

@@ -2,7 +2,7 @@
 //
 //   forward    G = X Wg[e], U = X Wu[e], H = act(G) * U            (GatedUp), Y = H Wd[e] (RowsProduct)
 //   backward   with dO = grad_out of the row's token and w the gate of its copy:
-//              dgate = dO . Y, dH = (w dO) Wd[e]^T, dU = dH act(G), dG = dH U act'(G)     (grad rows kernel, GradHidden)
+//              dgate = dO . Y, dH = w (dO Wd[e]^T), dU = dH act(G), dG = dH U act'(G)     (grad rows kernel, GradHidden)
 //              dWd = H^T (w dO), dWg = X^T dG, dWu = X^T dU                               (GradWeights)
 //              dx[t] = sum over the token's copies of dG Wg^T + dU Wu^T                   (RowsProduct, join)
 //
@@ -181,7 +181,7 @@ struct GatedUp {
 };
 
 // ---- backward: gradients of G and U -----------------------------------------------------------------
-// dH = (w dO) Wd^T over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. In the epilogue a lane has a row
+// dH = w (dO Wd^T) over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. In the epilogue a lane has a row
 // to itself: it reads G and U and writes dG and dU a sector (16 columns) at a time, the next sector on its way while it
 // works on one. What bounds it is the latency of those reads, so sixteen warps share the tile (8: 226 us, 16: 201 us at
 // T = 4096, D = 1024, F = 4096, E = 64). Staging the results for TMA stores costs a stage of the ring and is slower (1000
@@ -191,6 +191,7 @@ struct GradHidden {
   struct Params {
     ExpertOrder order;
     const int32_t* row_token;
+    const float* row_gate;
     const __nv_bfloat16* g;
     const __nv_bfloat16* u;
     __nv_bfloat16* dg;
@@ -206,6 +207,7 @@ struct GradHidden {
   };
   struct Early {
     bool store;
+    float gate;
     const __nv_bfloat16* g;  // this row's columns, as U's and the results' are
     const __nv_bfloat16* u;
     int64_t at;
@@ -242,6 +244,7 @@ struct GradHidden {
     const int32_t n = t.n0 + w.part * kWarpCols;
     e.store = n < p.ffn_dim && half_has_rows(p.row_token, t.row_block, w.quarter);
     if (!e.store) return e;
+    e.gate = __ldg(p.row_gate + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane);
     e.at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128 + (n & 127);
     e.g = p.g + e.at;
     e.u = p.u + e.at;
@@ -291,8 +294,8 @@ struct GradHidden {
         float a0, a1, d0, d1;
         act_and_slope<kActivation>(gf.x, &a0, &d0);
         act_and_slope<kActivation>(gf.y, &a1, &d1);
-        const float s0 = __uint_as_float(s[2 * h]);
-        const float s1 = __uint_as_float(s[2 * h + 1]);
+        const float s0 = __uint_as_float(s[2 * h]) * early.gate;
+        const float s1 = __uint_as_float(s[2 * h + 1]) * early.gate;
         dg[h] = pack_bf16(s0 * uf.x * d0, s1 * uf.y * d1);
         du[h] = pack_bf16(s0 * a0, s1 * a1);
       }
@@ -636,22 +639,25 @@ gated_rows_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ row_t
   }
 }
 
-// One warp per row of the layout, for the copy that it is: grad_rows[r] = w grad_out[token], rounded to bf16 (an operand
-// of both gradient products), zeros for padding, and dgate = grad_out[token] . Y[r] in fp32.
+// One warp per row of the layout, for the copy that it is: grad_rows[r] = grad_out[token], scaled_rows[r] = w times that,
+// rounded to bf16 (what dWd is summed from; dH takes the unscaled rows and w in fp32, one rounding less), row_gate[r] = w,
+// zeros for padding; and dgate = grad_out[token] . Y[r] in fp32.
 __global__ void __launch_bounds__(kSmallThreads)
 gated_grad_rows_kernel(const uint4* __restrict__ grad_out, const uint4* __restrict__ y_rows, const void* __restrict__ gate,
                        int gate_dtype, const int32_t* __restrict__ row_token, const int32_t* __restrict__ copy_row,
-                       const int32_t* __restrict__ num_rows, uint4* __restrict__ grad_rows, void* __restrict__ dgate,
-                       int32_t k, int32_t vecs) {
+                       const int32_t* __restrict__ num_rows, uint4* __restrict__ grad_rows, uint4* __restrict__ scaled_rows,
+                       float* __restrict__ row_gate, void* __restrict__ dgate, int32_t k, int32_t vecs) {
   ptx::grid_launch_dependents();
   const int lane = static_cast<int>(threadIdx.x & 31);
   const int32_t rows = __ldg(num_rows);
   const int32_t warps = static_cast<int32_t>(gridDim.x * (kSmallThreads / 32));
   for (int32_t r = static_cast<int32_t>(blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)); r < rows; r += warps) {
     const int32_t token = __ldg(row_token + r);
-    uint4* dst = grad_rows + static_cast<int64_t>(r) * vecs;
+    uint4* plain = grad_rows + static_cast<int64_t>(r) * vecs;
+    uint4* scaled = scaled_rows + static_cast<int64_t>(r) * vecs;
     if (token < 0) {
-      for (int32_t v = lane; v < vecs; v += 32) dst[v] = make_uint4(0u, 0u, 0u, 0u);
+      for (int32_t v = lane; v < vecs; v += 32) plain[v] = scaled[v] = make_uint4(0u, 0u, 0u, 0u);
+      if (lane == 0) row_gate[r] = 0.0f;
       continue;
     }
     // The copy of the token that this row is: the one whose row it is (rows are unique).
@@ -684,8 +690,10 @@ gated_grad_rows_kernel(const uint4* __restrict__ grad_out, const uint4* __restri
         dot = fmaf(f.y, y.y, dot);
         q[c] = pack_bf16(f.x * w, f.y * w);
       }
-      dst[v] = make_uint4(q[0], q[1], q[2], q[3]);
+      plain[v] = raw;
+      scaled[v] = make_uint4(q[0], q[1], q[2], q[3]);
     }
+    if (lane == 0) row_gate[r] = w;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
     if (lane == 0) {
@@ -814,14 +822,14 @@ int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t
 }
 
 int gated_grad_rows_of(const void* grad_out, const void* y_rows, const void* gate, int gate_dtype, const int32_t* row_token,
-                       const int32_t* copy_row, const int32_t* num_rows, void* grad_rows, void* dgate, int32_t k,
-                       int32_t d_model, int32_t num_row_blocks, cudaStream_t stream) {
+                       const int32_t* copy_row, const int32_t* num_rows, void* grad_rows, void* scaled_rows, float* row_gate,
+                       void* dgate, int32_t k, int32_t d_model, int32_t num_row_blocks, cudaStream_t stream) {
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
   gated_grad_rows_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, stream>>>(
       static_cast<const uint4*>(grad_out), static_cast<const uint4*>(y_rows), gate, gate_dtype, row_token, copy_row, num_rows,
-      static_cast<uint4*>(grad_rows), dgate, k, d_model / 8);
+      static_cast<uint4*>(grad_rows), static_cast<uint4*>(scaled_rows), row_gate, dgate, k, d_model / 8);
   return check_launch("moe_gated_backward (rows)");
 }
 
@@ -834,7 +842,7 @@ int32_t tile_cols(int64_t num_row_blocks, int32_t width, int sm_count) {
 }
 
 template <int kCols>
-int gated_grad_hidden(const void* grad_rows, const void* w_down, const void* g_blocks, const void* u_blocks,
+int gated_grad_hidden(const void* grad_rows, const float* row_gate, const void* w_down, const void* g_blocks, const void* u_blocks,
                       const int32_t* row_token, const int32_t* row_block_expert, const int32_t* padded_offsets, void* dg_blocks,
                       void* du_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
                       int32_t activation, int32_t* dev_status, cudaStream_t stream) {
@@ -843,6 +851,7 @@ int gated_grad_hidden(const void* grad_rows, const void* w_down, const void* g_b
   if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, kCols, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[1], grad_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, what)) return rc;
   typename GradHidden<kCols>::Params p{};
+  p.row_gate = row_gate;
   const int32_t slices = (ffn_dim + kCols - 1) / kCols;
   p.order = {row_block_expert, padded_offsets, num_row_blocks, slices};
   p.row_token = row_token;
@@ -946,7 +955,7 @@ struct GatedBuffers {
   int64_t x_rows, h, g, u, y;
   int64_t state_bytes, scratch_bytes;
   // scratch of the backward pass
-  int64_t grad_rows, dg, du, backward_bytes;
+  int64_t grad_rows, scaled_rows, row_gate, dg, du, backward_bytes;
 };
 
 int gated_buffers(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int keep,
@@ -995,6 +1004,8 @@ int gated_buffers(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_di
   b->scratch_bytes = at;
   at = 0;
   b->grad_rows = take(rows * d_model * 2);
+  b->scaled_rows = take(rows * d_model * 2);
+  b->row_gate = take(rows * 4);
   b->dg = take(rows * ffn_dim * 2);
   b->du = take(rows * ffn_dim * 2);
   b->backward_bytes = at;
@@ -1158,21 +1169,23 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int
   const cudaStream_t st = as_stream(stream);
   auto ints = [base](int64_t at) { return reinterpret_cast<const int32_t*>(base + at); };
   const int32_t* row_token = ints(b.row_token);
+  float* row_gate = reinterpret_cast<float*>(temp + b.row_gate);
   if (int rc = gated_grad_rows_of(grad_out, base + b.y, gate, gate_dtype, row_token, ints(b.copy_row),
-                                  ints(b.padded_offsets) + num_experts, temp + b.grad_rows, dgate, k, d_model, b.row_blocks, st))
+                                  ints(b.padded_offsets) + num_experts, temp + b.grad_rows, temp + b.scaled_rows, row_gate, dgate, k,
+                                  d_model, b.row_blocks, st))
     return rc;
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
   const auto grad_hidden = tile_cols(b.row_blocks, ffn_dim, info->sm_count) == kTileCols ? gated_grad_hidden<kTileCols> : gated_grad_hidden<64>;
-  if (int rc = grad_hidden(temp + b.grad_rows, w_down, base + b.g, base + b.u, row_token, ints(b.row_block_expert),
+  if (int rc = grad_hidden(temp + b.grad_rows, row_gate, w_down, base + b.g, base + b.u, row_token, ints(b.row_block_expert),
                            ints(b.padded_offsets), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
                            activation, dev_status, st))
     return rc;
-  if (int rc = gated_grad_weights(base + b.x_rows, temp + b.grad_rows, base + b.h, temp + b.dg, temp + b.du,
+  if (int rc = gated_grad_weights(base + b.x_rows, temp + b.scaled_rows, base + b.h, temp + b.dg, temp + b.du,
                                   ints(b.padded_offsets), ints(b.tokens_per_expert), dw_gate, dw_up, dw_down, d_model,
                                   ffn_dim, num_experts, b.row_blocks, dev_status, st))
     return rc;
-  // The rows of dx take the place of grad_rows, which the weight gradients were the last to read.
+  // The rows of dx take the place of grad_rows, which the hidden gradients were the last to read.
   if (int rc = rows_product<true>(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert),
                                   ints(b.padded_offsets), temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks,
                                   dev_status, st))
