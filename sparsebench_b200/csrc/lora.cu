@@ -11,10 +11,10 @@
 //            steps of the projection itself, so y is written once and never read back
 //
 // Up to 64 tokens (a decoding step) the weights are streamed by the kernel of skinny.cuh and the second term is plain
-// fp32 arithmetic on each token's own rows of A and B (lora_rows_kernel, SkinnyLora): no plan, no pairing of tokens.
+// fp32 arithmetic on each token's own rows of A and B (lora_rows_kernel, SkinnyLora).
 //
-// In the products V is rounded to bf16 for y in bf16; for y in fp32 it travels as a pair of bf16 (V and what rounding took from it,
-// against the same rows of B), 2^-17 of V off.
+// In the products V is rounded to bf16 for y in bf16; for y in fp32 it travels as a pair of bf16 (V and what rounding took
+// from it, against the same rows of B), at most 2^-16 of V off.
 //
 // There a zero of V meets B of other requests' adapters: an infinity or NaN in one adapter would reach its neighbours'
 // rows. So an adapter whose B is not finite stays out of the product (shrink finds it, reading B beside its own loads and
@@ -46,6 +46,9 @@ __device__ __forceinline__ bool adapter_finite(const uint8_t* not_finite, int32_
 // x tile (K-major) times the slots' rows of A (K-major, 8 to 128 rows by TMA per slot and step). Row i of the tile takes
 // the columns of its slot from TMEM into shared memory; after the last group the blocks of the cluster add their parts up
 // over distributed shared memory, in rank order, each for its share of the rows.
+//
+// Latency sets the time: 11 us at T = 4096, D = 1024, rank 8 (most of it start, slots and join), 40 us cold and about half of
+// that behind a warm L2 at T = 8191, D = 4096, rank 64, where the tiles with most slots finish last.
 //
 // Meanwhile twelve more warps look for infinities and NaN in B: of those of the tile's adapters that the tile before
 // does not have (they are being looked through there, or further up). For a batch of whole requests that is once per
@@ -347,9 +350,17 @@ lora_shrink_kernel(const __grid_constant__ ShrinkMaps maps, const __grid_constan
 }
 
 // ---- expand -------------------------------------------------------------------------------------------------------
+// y on tiles of 128 tokens x 256 columns. The K steps behind D hold V in the columns of its slot: eight K rows at a time
+// belong to one adapter, so slots of any rank that is a multiple of 8 share a step, and a tile of few slots has few steps
+// (1 of 65 for one adapter of rank 64 at D = 4096). Bound by the tensor cores: T = 8191, 4096 x 4096, rank 64: 211 us,
+// 1330 TFLOP/s, 82 % of the measured burst peak and of the issue rate at the clock it ran at. With x gathered by cp.async
+// instead of TMA it was 290 us.
+// Tiles are walked in bands of 8 row tiles, in a band the row tile changes fastest: 148 tiles in flight are then 8 row
+// tiles x 18 column slices, whose x and W are small against L2 (bands of 2 to 16: the same 211 us, 64: 219).
 struct LoraExpand {
+  static constexpr int32_t kBand = 8;
   struct Params {
-    BandOrder order;
+    int32_t row_tiles, slices;
     const int32_t* tables;
     const uint8_t* not_finite;
     const __nv_bfloat16* v;
@@ -367,11 +378,14 @@ struct LoraExpand {
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = true, kAMnMajor = false, kBMnMajor = true;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.num_row_blocks * p.order.num_slices; }
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.row_tiles * p.slices; }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
     Tile t;
-    int32_t slice;
-    p.order.at(index, &t.row_tile, &slice);
+    const int32_t band = index / (kBand * p.slices);
+    const int32_t inside = index - band * (kBand * p.slices);
+    const int32_t height = min(kBand, p.row_tiles - band * kBand);
+    const int32_t slice = inside / height;
+    t.row_tile = band * kBand + inside - slice * height;
     t.n0 = slice * kTileCols;
     t.table = p.tables + static_cast<int64_t>(t.row_tile) * kTableInts;
     t.slots = __ldg(t.table);
@@ -779,7 +793,8 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
   if (int rc = encode_2d_map(&maps.m[3], x, num_tokens, d_model, kTileRows, 64, 2, "lora_linear (x)")) return rc;
   LoraExpand::Params p{};
   const int32_t slices = (width + kTileCols - 1) / kTileCols;
-  p.order = {row_tiles, slices, 8};
+  p.row_tiles = row_tiles;
+  p.slices = slices;
   p.tables = tables;
   p.not_finite = not_finite;
   p.splits = s.splits;

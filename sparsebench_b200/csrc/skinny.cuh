@@ -10,6 +10,11 @@
 // Two blocks fit an SM, so that one's start and end hide behind the other's stream. The kernels of a chain are launched
 // with programmatic dependence: a kernel's weights are on their way before the rows it waits for are written.
 //
+// Bound by the weights' way from memory; with little of it, by the latency of start, first loads and join (about 5 us).
+// Measured as replayed graphs: gated layer, D = 4096, F = 14336, E = 8: one token (two experts, 0.70 GB) 119 us, 5.9 TB/s;
+// 16 tokens 413 us, 6.8 TB/s. D = 1024, F = 4096, E = 64: one token (50 MB) 16.5 us, 16 tokens 111 us (5.8 TB/s).
+// Projection with adapters, 4096 x 4096: one token 12 us; 4096 x 14336, 64 tokens with 32 adapters: 31 us (4.5 TB/s).
+//
 // Waits are bounded as in tile_gemm.cuh; a block that gave up still takes part in the cluster's barriers.
 #pragma once
 

@@ -84,22 +84,6 @@ __device__ __forceinline__ void load_packed_x64(uint32_t taddr, uint32_t (&packe
   }
 }
 
-// Tile order over (row block, column slice): bands of `band` row blocks, inside a band the row block changes fastest.
-// A band of 1 is row-block-major. Taller bands let the row blocks of one expert that run at the same time share a
-// weight tile through L2 where an expert has many row blocks.
-struct BandOrder {
-  int32_t num_row_blocks, num_slices, band;
-  __device__ __forceinline__ void at(int32_t tile, int32_t* row_block, int32_t* slice) const {
-    const int32_t per_band = band * num_slices;
-    const int32_t b = tile / per_band;
-    const int32_t first = b * band;
-    const int32_t height = min(band, num_row_blocks - first);
-    const int32_t inside = tile - b * per_band;
-    *slice = inside / height;
-    *row_block = first + inside - *slice * height;
-  }
-};
-
 // A policy Op has
 //   Params, Tile (with int32_t k_steps: 0 = nothing to multiply; bool live: the epilogue has something to do)
 //   static constexpr bool kAMnMajor, kBMnMajor

@@ -131,4 +131,6 @@ def moe_gated(
 ) -> torch.Tensor:
     """moe_forward_gated for torch.autograd: differentiable in x, expert_weight and the three weights (once). Its
     backward pass refuses to run under CUDA graph capture: capture the two explicit calls instead."""
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, expert_weight, w_gate, w_up, w_down)):
+        return moe_forward_gated(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)  # nothing to keep
     return _GatedMoE.apply(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)

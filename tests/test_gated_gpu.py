@@ -263,6 +263,74 @@ def test_autograd_form():
         assert torch.equal(leaf.grad, ones[n]), n
 
 
+def test_autograd_form_without_gradients_and_on_an_empty_batch():
+    from sparsebench_b200 import moe_forward_gated, moe_gated
+
+    x, idx, gate, wg, wu, wd, go = make(30, 128, 256, 4, 2)
+    leaf = x.clone().requires_grad_()
+    with torch.no_grad():
+        out = moe_gated(leaf, idx, gate, wg, wu, wd)
+    assert not out.requires_grad and torch.equal(out, moe_forward_gated(x, idx, gate, wg, wu, wd))
+    assert not moe_gated(x, idx, gate, wg, wu, wd).requires_grad
+    weight = wg.clone().requires_grad_()  # one leaf alone
+    moe_gated(x, idx, gate, weight, wu, wd).backward(go)
+    assert torch.equal(weight.grad, step(x, idx, gate, wg, wu, wd, go, "silu")["dw_gate"])
+    empty = x[:0].clone().requires_grad_()
+    moe_gated(empty, idx[:0], gate[:0], weight, wu, wd).sum().backward()
+    assert empty.grad.shape == (0, 128)
+
+
+def test_backward_twice_and_two_forwards_at_once():
+    from sparsebench_b200 import moe_backward_gated, moe_forward_gated_saved
+
+    a, b = make(140, 256, 384, 8, 2, seed=1), make(77, 256, 384, 8, 2, seed=2)
+    want = [step(*args, "silu") for args in (a, b)]
+    _, first = moe_forward_gated_saved(*a[:6])
+    _, second = moe_forward_gated_saved(*b[:6])
+    for _ in range(2):
+        for saved, args, ref in ((first, a, want[0]), (second, b, want[1])):
+            for n, g in zip(NAMES, moe_backward_gated(args[6], saved)):
+                assert torch.equal(g, ref[n]), n
+
+
+def test_views_with_an_offset_and_misaligned_ones():
+    from sparsebench_b200 import moe_forward_gated
+
+    x, idx, gate, wg, wu, wd, _ = make(100, 128, 256, 4, 2)
+    for num_tokens in (10, 90):
+        want = moe_forward_gated(x[:num_tokens].clone(), idx[:num_tokens].clone(), gate[:num_tokens].clone(), wg, wu, wd)
+        stack = torch.stack([wg, wg])  # a layer's weights as a slice of all layers'
+        got = moe_forward_gated(x[:num_tokens], idx[:num_tokens], gate[:num_tokens], stack[1], wu, wd)
+        assert torch.equal(got, want)
+        odd = torch.empty(num_tokens * 128 + 8, dtype=torch.bfloat16, device="cuda")[1:num_tokens * 128 + 1].view(num_tokens, 128)
+        odd.copy_(x[:num_tokens])
+        with pytest.raises(RuntimeError, match="aligned"):
+            moe_forward_gated(odd, idx[:num_tokens], gate[:num_tokens], wg, wu, wd)
+
+
+def test_two_streams_at_once():
+    from sparsebench_b200 import lora_linear, moe_forward_gated
+
+    args = [make(t, 256, 512, 8, 2, seed=t) for t in (4, 300)]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = (torch.randn(256, 264, generator=g, device="cuda") / 16).bfloat16()
+    la = (torch.randn(3, 16, 256, generator=g, device="cuda") / 16).bfloat16()
+    lb = torch.randn(3, 16, 264, generator=g, device="cuda").bfloat16()
+    ids = [torch.arange(t, device="cuda") % 4 - 1 for t in (4, 300)]
+    run = lambda i: (moe_forward_gated(*args[i][:6]), lora_linear(args[i][0], w, la, lb, ids[i]))  # noqa: E731
+    want = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for round_ in range(20):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((n % 2, run(n % 2)))
+    torch.cuda.synchronize()
+    for i, (out, y) in got:
+        assert torch.equal(out, want[i][0]) and torch.equal(y, want[i][1])
+
+
 def test_sdd_gated_alone():
     from sparsebench_b200 import route_device, sdd_gated
 

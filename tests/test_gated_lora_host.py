@@ -1,0 +1,148 @@
+"""What of the gated layer and the projection with adapters needs no GPU: their refusals, before anything is launched,
+and their oracles against each other."""
+
+import ctypes
+
+import pytest
+import torch
+
+from oracle.gated import activation, gated_layer, gated_reference, slope
+from oracle.lora import lora_reference
+from sparsebench_b200 import _build, _lib
+
+
+@pytest.fixture(scope="module")
+def lib() -> ctypes.CDLL:
+    _build.build()
+    return _lib.load()
+
+
+@pytest.mark.parametrize(("args", "text"), [
+    ((0, 2, 128, 128, 4, 0), b"must be positive"),
+    ((4, 0, 128, 128, 4, 0), b"must be positive"),
+    ((4, 2, 64, 128, 4, 0), b"D (64) must be a positive multiple of 128"),
+    ((4, 2, 128, 192, 4, 1), b"F (192) must be a positive multiple of 128"),
+    ((4, 2, 128, 128, 0, 0), b""),
+    ((4, 2, 128, 128, 1025, 0), b"num_experts"),
+    ((2**31, 2, 128, 128, 4, 0), b"too large"),
+    ((2**24, 8, 128, 2**20, 4, 1), b"too large"),
+])
+def test_gated_sizes_are_refused(lib, args, text) -> None:
+    sizes = (ctypes.c_int64 * 3)()
+    assert lib.sb_moe_gated_bytes(*args, sizes) == 1
+    assert text in lib.sb_last_error()
+
+
+def test_gated_sizes(lib) -> None:
+    sizes = (ctypes.c_int64 * 3)()
+    assert lib.sb_moe_gated_bytes(4096, 2, 1024, 4096, 64, 1, sizes) == 0
+    rows = (8192 + 64 * 127) // 128 * 128
+    blocks = rows * 4096 * 2
+    assert sizes[0] > 3 * blocks + 2 * rows * 1024 * 2 and sizes[2] > 2 * blocks  # H, G, U, x and Y; dG, dU
+    kept = list(sizes)
+    assert lib.sb_moe_gated_bytes(4096, 2, 1024, 4096, 64, 0, sizes) == 0
+    assert sizes[0] == 0 and blocks < sizes[1] < kept[0] and sizes[2] == 0
+    assert lib.sb_moe_gated_bytes(32, 2, 1024, 4096, 64, 0, sizes) == 0  # a decoding step: H and Y of 64 copies
+    assert sizes[1] == 64 * 4096 * 2 + 64 * 1024 * 4
+    assert lib.sb_moe_gated_bytes(32, 2, 1024, 4096, 64, 0, None) == 1
+
+
+def test_gated_calls_are_refused_before_any_launch(lib) -> None:
+    one, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)  # never dereferenced
+    big = 1 << 40
+
+    def forward(x=one, ids=one, gate_dtype=0, state=one, scratch=one, act=0, state_bytes=big, scratch_bytes=big, d=128):
+        return lib.sb_moe_gated_forward(x, ids, 1, one, gate_dtype, one, one, one, one, 100, 2, d, 128, 4, act, state,
+                                        state_bytes, scratch, scratch_bytes, None, None)
+
+    def backward(grad=one, gate_dtype=0, state=one, scratch=one, act=0, state_bytes=big, scratch_bytes=big):
+        return lib.sb_moe_gated_backward(grad, one, gate_dtype, one, one, one, state, state_bytes, one, one, one, one, one,
+                                         100, 2, 128, 128, 4, act, scratch, scratch_bytes, None, None)
+
+    for call, text in [
+        (lambda: forward(x=None), b"NULL"), (lambda: forward(ids=None), b"NULL"), (lambda: forward(scratch=None), b"NULL"),
+        (lambda: forward(x=odd), b"aligned"), (lambda: forward(state=odd), b"aligned"), (lambda: forward(gate_dtype=2), b"gate_dtype"),
+        (lambda: forward(act=2), b"activation"), (lambda: forward(d=130), b"multiple of 128"),
+        (lambda: forward(state_bytes=1000), b"are needed"), (lambda: forward(scratch_bytes=0), b"are needed"),
+        (lambda: backward(grad=None), b"NULL"), (lambda: backward(state=None), b"NULL"), (lambda: backward(grad=odd), b"aligned"),
+        (lambda: backward(scratch=odd), b"aligned"), (lambda: backward(gate_dtype=-1), b"gate_dtype"), (lambda: backward(act=-1), b"activation"),
+        (lambda: backward(state_bytes=1000), b"are needed"), (lambda: backward(scratch_bytes=1000), b"are needed"),
+    ]:
+        assert call() == 1 and text in lib.sb_last_error(), text
+    args = [one] * 8
+    assert lib.sb_sdd_gated(*args, 10, 128, 128, 4, 3, 5, 0, None, None) == 1 and b"activation" in lib.sb_last_error()
+    assert lib.sb_sdd_gated(*args, 10, 100, 128, 4, 3, 0, 0, None, None) == 1 and b"multiple of 128" in lib.sb_last_error()
+    assert lib.sb_sdd_gated(*args[:7], None, 10, 128, 128, 4, 3, 0, 0, None, None) == 1 and b"NULL" in lib.sb_last_error()
+    assert lib.sb_sdd_gated(*args, 10, 128, 128, 4, 0, 0, 0, None, None) == 0  # no row blocks: nothing to do
+
+
+@pytest.mark.parametrize(("sizes", "text"), [
+    ((-1, 64, 64, 8, 2), b"31 bits"),
+    ((10, 60, 64, 8, 2), b"D (60)"),
+    ((10, 64, 60, 8, 2), b"N (60)"),
+    ((10, 64, 64, 4, 2), b"rank (4)"),
+    ((10, 64, 64, 136, 2), b"rank (136)"),
+    ((10, 64, 64, 8, 0), b"adapters (0)"),
+    ((10, 64, 64, 128, 2**25), b"31 bits"),
+])
+def test_lora_sizes_are_refused(lib, sizes, text) -> None:
+    assert lib.sb_lora_workspace_bytes(*sizes, 0) == -1 and text in lib.sb_last_error()
+    one = ctypes.c_void_p(1 << 20)
+    assert lib.sb_lora_linear(one, one, one, one, one, 1, None, one, 0, *sizes, one, 1 << 40, None, None) == 1
+    assert text in lib.sb_last_error()
+
+
+def test_lora_calls_are_refused_before_any_launch(lib) -> None:
+    one, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)
+    assert lib.sb_lora_linear(one, one, one, one, None, 1, None, one, 0, 10, 64, 64, 8, 2, one, 1 << 40, None, None) == 1
+    assert b"NULL" in lib.sb_last_error()
+    assert lib.sb_lora_linear(odd, one, one, one, one, 1, None, one, 0, 10, 64, 64, 8, 2, one, 1 << 40, None, None) == 1
+    assert b"aligned" in lib.sb_last_error()
+    assert lib.sb_lora_linear(one, one, one, one, one, 1, None, one, 0, 0, 64, 64, 8, 2, one, 0, None, None) == 0  # no tokens
+
+
+def test_tensors_on_the_cpu_are_refused() -> None:
+    from sparsebench_b200 import lora_linear, moe_forward_gated
+
+    x, w = torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(2, 128, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        moe_forward_gated(x, torch.zeros(4, 1, dtype=torch.int64), torch.ones(4, 1), w, w, w)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        lora_linear(x, w[0], torch.zeros(1, 8, 128, dtype=torch.bfloat16), torch.zeros(1, 8, 128, dtype=torch.bfloat16),
+                    torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="w_down must be"):
+        moe_forward_gated(x, torch.zeros(4, 1, dtype=torch.int64), torch.ones(4, 1), w, w, w[:1])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gated_oracle_against_autograd(act) -> None:
+    g = torch.Generator().manual_seed(1)
+    leaves = [torch.randn(*s, generator=g, dtype=torch.float64).requires_grad_()
+              for s in ((9, 6), (9, 2), (4, 6, 5), (4, 6, 5), (4, 5, 6))]
+    idx = torch.randint(-1, 5, (9, 2), generator=g)
+    go = torch.randn(9, 6, generator=g, dtype=torch.float64)
+    out = gated_layer(leaves[0], idx, *leaves[1:], act)
+    grads = torch.autograd.grad(out, leaves, go)
+    got = gated_reference(leaves[0].detach(), idx, *(t.detach() for t in leaves[1:]), act, go)
+    torch.testing.assert_close(got["out"][0], out.detach(), rtol=1e-12, atol=1e-12)
+    for name, want in zip(("dx", "dgate", "dw_gate", "dw_up", "dw_down"), grads):
+        torch.testing.assert_close(got[name][0], want, rtol=1e-12, atol=1e-12)
+        assert bool((got[name][1] >= 0).all())
+    v = torch.linspace(-12, 12, 4001, dtype=torch.float64, requires_grad=True)
+    (d,) = torch.autograd.grad(activation(v, act).sum(), v)
+    torch.testing.assert_close(slope(v.detach(), act), d, rtol=1e-12, atol=1e-12)
+    assert float(d.abs().max()) < 1.13  # what the error bounds take for the steepest slope
+
+
+def test_lora_oracle_row_by_row() -> None:
+    g = torch.Generator().manual_seed(2)
+    x, w, a, b = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((7, 6), (6, 5), (3, 2, 6), (3, 2, 5)))
+    idx = torch.tensor([0, 2, -1, 1, 3, 2, 0])
+    scale = torch.tensor([0.5, 2.0, 1.5])
+    got, bound = lora_reference(x, w, a, b, idx, scale)
+    for t, i in enumerate(idx.tolist()):
+        want = x[t] @ w
+        if 0 <= i < 3:
+            want = want + float(scale[i]) * ((a[i] @ x[t]) @ b[i])
+        torch.testing.assert_close(got[t], want, rtol=1e-12, atol=1e-12)
+    assert bool((bound > 0).all())
