@@ -419,8 +419,8 @@ int sb_ep_sdd_dispatch(const void* recv_rows, const void* w1, const int32_t* row
  */
 enum sb_activation { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* erf form */ };
 int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
-                 const int32_t* row_block_expert, const int32_t* padded_offsets, void* x_rows, void* h_blocks,
-                 int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
+                 const int32_t* row_block_expert, const int32_t* padded_offsets, const int32_t* tokens_per_expert,
+                 void* x_rows, void* h_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts,
                  int32_t num_row_blocks, int32_t activation, int skip_padding_rows, int32_t* dev_status,
                  sb_stream_t stream);
 int sb_moe_gated_bytes(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int keep,

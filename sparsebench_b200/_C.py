@@ -370,19 +370,21 @@ def _check_gated_weights(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
 
 
 def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, row_token: torch.Tensor,
-                   row_block_expert: torch.Tensor, padded_offsets: torch.Tensor, num_nnz: int, activation: str,
-                   skip_padding_rows: bool = False) -> torch.Tensor:
+                   row_block_expert: torch.Tensor, padded_offsets: torch.Tensor, tokens_per_expert: torch.Tensor,
+                   num_nnz: int, activation: str, skip_padding_rows: bool = False) -> torch.Tensor:
     """Blocks [num_nnz, 128, 128] = act(x[row_token] @ w_gate[expert]) * (x[row_token] @ w_up[expert]) on the layout's
     blocks. Dead row blocks are left unwritten, with skip_padding_rows 32-row groups of padding too."""
     lib = _lib.load()
     _check_gated_weights(x, w_gate, w_up)
     code = _check_activation(activation)
-    for t, name in ((row_token, "row_token"), (row_block_expert, "row_block_expert"), (padded_offsets, "padded_offsets")):
+    for t, name in ((row_token, "row_token"), (row_block_expert, "row_block_expert"), (padded_offsets, "padded_offsets"),
+                    (tokens_per_expert, "tokens_per_expert")):
         _check_index(t, name)
         _check(t.device == x.device, f"{name} must be on x's GPU")
     num_experts, d_model, ffn_dim = w_gate.shape
     num_row_blocks = row_block_expert.numel()
-    _check(row_token.numel() == num_row_blocks * BLOCK and padded_offsets.numel() == num_experts + 1, "the layout does not match block size 128 and the number of experts")
+    _check(row_token.numel() == num_row_blocks * BLOCK and padded_offsets.numel() == num_experts + 1 and
+           tokens_per_expert.numel() == num_experts, "the layout does not match block size 128 and the number of experts")
     _check(num_nnz == num_row_blocks * (ffn_dim // BLOCK),
            f"expected {num_row_blocks * (ffn_dim // BLOCK)} blocks (row blocks x F/128), got {num_nnz}")
     with torch.cuda.device(x.device):
@@ -390,8 +392,8 @@ def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, ro
         if num_row_blocks > 0:
             rows = torch.empty((num_row_blocks * BLOCK, d_model), dtype=torch.bfloat16, device=x.device)
             _lib.check(lib.sb_sdd_gated(_ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(row_token), _ptr(row_block_expert),
-                                        _ptr(padded_offsets), _ptr(rows), _ptr(h), x.shape[0], d_model, ffn_dim,
-                                        num_experts, num_row_blocks, code, int(bool(skip_padding_rows)),
+                                        _ptr(padded_offsets), _ptr(tokens_per_expert), _ptr(rows), _ptr(h), x.shape[0],
+                                        d_model, ffn_dim, num_experts, num_row_blocks, code, int(bool(skip_padding_rows)),
                                         _ptr(device_status(x.device)), _stream()))
     return h
 

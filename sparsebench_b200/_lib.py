@@ -56,7 +56,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                    c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P]),
     "sb_ep_dsd_push": (c_int, [_P, c_int64, _P, c_int64, c_int32, _P, _P, c_int32, _P, _P, c_int32, c_int32, c_int32,
                                _P, _P]),
-    "sb_sdd_gated": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+    "sb_sdd_gated": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
                              c_int, _P, _P]),
     "sb_moe_gated_bytes": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int, _P]),
     "sb_moe_gated_forward": (c_int, [_P, _P, c_int, _P, c_int, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32,

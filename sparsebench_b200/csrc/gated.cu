@@ -79,15 +79,18 @@ __device__ __forceinline__ bool half_has_rows(const int32_t* row_token, int32_t 
 struct ExpertOrder {
   const int32_t* row_block_expert;
   const int32_t* padded_offsets;
-  int32_t num_row_blocks, slices;
+  const int32_t* tokens_per_expert;
+  int32_t num_experts, slices;
   static constexpr int32_t kBand = 16;
-  __device__ __forceinline__ int32_t tiles() const { return num_row_blocks * slices; }
-  // False: past the last real row block.
-  __device__ __forceinline__ bool at(int32_t tile, int32_t* row_block, int32_t* slice, int32_t* expert) const {
+  __device__ __forceinline__ int32_t live_tiles() const { return __ldg(padded_offsets + num_experts) / kTileRows * slices; }
+  // False: not a row block of any expert.
+  // groups: how many of the row block's four groups of 32 rows hold real rows (padding sits at the end).
+  __device__ __forceinline__ bool at(int32_t tile, int32_t* row_block, int32_t* slice, int32_t* expert, int32_t* groups) const {
     const int32_t e = __ldg(row_block_expert + tile / slices);
     if (e < 0) return false;
     const int32_t begin = __ldg(padded_offsets + e) / kTileRows;
     const int32_t end = __ldg(padded_offsets + e + 1) / kTileRows;
+    const int32_t count = __ldg(tokens_per_expert + e);
     int32_t inside = tile - begin * slices;
     const int32_t band = inside / (kBand * slices);
     inside -= band * (kBand * slices);
@@ -96,9 +99,24 @@ struct ExpertOrder {
     *slice = inside / height;
     *row_block = first + inside - *slice * height;
     *expert = e;
+    *groups = max(1, min(4, (count - (*row_block - begin) * kTileRows + 31) / 32));
     return true;
   }
 };
+
+// 64 inner columns of the first `groups` x 32 rows of a row block. The rest of the stage keeps what it held, and the
+// accumulator rows that come of it are never stored. With a row or two per expert (a small batch) the full 128 rows would
+// be a third of all bytes.
+template <bool kOnce>  // read once: first out of L2
+__device__ __forceinline__ void load_rows(uint32_t a, const CUtensorMap* all, const CUtensorMap* rows32, int32_t col, int32_t row,
+                                          int32_t groups, uint32_t bar) {
+  const CUtensorMap* map = groups == 4 ? all : rows32;
+  const int32_t boxes = groups == 4 ? 1 : groups;
+  for (int32_t g = 0; g < boxes; ++g) {
+    if (kOnce) ptx::tma_load_2d_hint(a + g * 4096, map, col, row + g * 32, bar, ptx::policy_evict_first());
+    else ptx::tma_load_2d(a + g * 4096, map, col, row + g * 32, bar);
+  }
+}
 
 // ---- forward: both projections, the activation and the product ----------------------------------------------------
 // The tile's 256 accumulator columns are 128 columns of G next to the same 128 of U, so a thread that drains column c
@@ -116,29 +134,36 @@ struct GatedUp {
     int32_t keep;          // G and U are stored too, and every row that the backward pass reads
   };
   struct Tile {
-    int32_t k_steps, row_block, n0, expert, first_block;
+    int32_t k_steps, row_block, n0, expert, first_block, groups;
     bool live;
   };
   struct Early { bool store; };
   static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = true;
+  static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = true;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.live_tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
     Tile t{};
     int32_t slice;
-    t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
+    t.live = p.order.at(index, &t.row_block, &slice, &t.expert, &t.groups);
     if (!t.live) return t;
     t.n0 = slice * 128;
+    // Padding rows that are stored have to be multiplied, as the zeros they are: whole halves for training, or all.
+    if (p.keep) t.groups = (t.groups + 1) & ~1;
+    else if (!p.skip_padding) t.groups = 4;
     t.first_block = t.row_block * p.order.slices;  // of the layout's blocks, F / 128 per row block
     t.k_steps = p.d_model / kTileStep;
     return t;
   }
+  static __device__ __forceinline__ int columns(const Params&, const Tile&) { return kTileCols; }
+  static __device__ __forceinline__ uint32_t tx_bytes(const Params&, const Tile& t, int32_t) {
+    return TileSmem::kBBytes + static_cast<uint32_t>(t.groups) * 4096u;
+  }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
     const uint64_t once = ptx::policy_evict_first();
-    ptx::tma_load_2d(a, &maps.m[5], ks * kTileStep, t.row_block * kTileRows, bar);
+    load_rows<false>(a, &maps.m[5], &maps.m[6], ks * kTileStep, t.row_block * kTileRows, t.groups, bar);
     const int32_t row = t.expert * p.d_model + ks * kTileStep;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -205,7 +230,7 @@ struct GradHidden {
   static constexpr int kPart = 16;                // columns at a time: 32 bytes of a row, one sector
   static constexpr int kWarpCols = kCols / 4;     // of the tile's, per epilogue warp
   struct Tile {
-    int32_t k_steps, row_block, n0, expert, first_block;
+    int32_t k_steps, row_block, n0, expert, first_block, groups;
     bool live;
   };
   struct Early {
@@ -220,24 +245,25 @@ struct GradHidden {
   static constexpr bool kAhead = true;
   static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.live_tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
     Tile t{};
     int32_t slice;
-    t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
+    t.live = p.order.at(index, &t.row_block, &slice, &t.expert, &t.groups);
     if (!t.live) return t;
     t.n0 = slice * kCols;
+    t.groups = (t.groups + 1) & ~1;  // whole halves: their padding rows are stored, as zeros
     t.first_block = t.row_block * (p.ffn_dim >> 7);
     t.k_steps = p.d_model / kTileStep;
     return t;
   }
-  static __device__ __forceinline__ int columns(const Params&) { return kCols; }
-  static __device__ __forceinline__ uint32_t tx_bytes(const Params&, const Tile&, int32_t) {
-    return TileSmem::kABytes + kCols * 128u;
+  static __device__ __forceinline__ int columns(const Params&, const Tile&) { return kCols; }
+  static __device__ __forceinline__ uint32_t tx_bytes(const Params&, const Tile& t, int32_t) {
+    return static_cast<uint32_t>(t.groups) * 4096u + kCols * 128u;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
-    ptx::tma_load_2d(a, &maps.m[1], ks * kTileStep, t.row_block * kTileRows, bar);
+    load_rows<false>(a, &maps.m[1], &maps.m[2], ks * kTileStep, t.row_block * kTileRows, t.groups, bar);
     // With F an odd multiple of 128 the last tile's upper 128 columns are rows of the next expert (or zeros past the
     // end): computed, never stored.
     ptx::tma_load_2d_hint(b, &maps.m[0], ks * kTileStep, t.expert * p.ffn_dim + t.n0, bar, ptx::policy_evict_first());
@@ -322,7 +348,7 @@ struct RowsProduct {
     int32_t d_model, ffn_dim, cols;
   };
   struct Tile {
-    int32_t k_steps, row_block, n0, expert, first_block;
+    int32_t k_steps, row_block, n0, cols, expert, first_block, groups;
     bool live;
   };
   struct Early { bool store; };
@@ -330,20 +356,44 @@ struct RowsProduct {
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = !kBack;
 
-  static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.tiles(); }
+  // Down: the tiles of the last wave, where they would leave half of the thread blocks or more without one, are cut into
+  // two or four by columns (not below 64); `whole` tiles come before them. (176 tiles of a batch of 37 tokens: 76 -> 72 us.
+  // Back reads its weights in boxes as tall as the tile is wide, one TMA load per step; cutting those cost 3 %.)
+  static __device__ __forceinline__ void waves(const Params& p, int32_t* whole, int32_t* rest, int32_t* cut) {
+    const int32_t total = p.order.live_tiles();
+    const int32_t blocks = static_cast<int32_t>(gridDim.x);
+    *rest = total % blocks;
+    *whole = total - *rest;
+    *cut = 1;
+    while (!kBack && *rest > 0 && *rest * *cut * 2 <= blocks && p.cols / (*cut * 2) >= 64) *cut *= 2;
+  }
+  static __device__ __forceinline__ int32_t total_tiles(const Params& p) {
+    int32_t whole, rest, cut;
+    waves(p, &whole, &rest, &cut);
+    return whole + rest * cut;
+  }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
     Tile t{};
-    int32_t slice;
-    t.live = p.order.at(index, &t.row_block, &slice, &t.expert);
+    int32_t whole, rest, cut, slice, piece = 0;
+    waves(p, &whole, &rest, &cut);
+    t.cols = p.cols;
+    if (index >= whole) {
+      piece = (index - whole) % cut;
+      index = whole + (index - whole) / cut;
+      t.cols /= cut;
+    }
+    t.live = p.order.at(index, &t.row_block, &slice, &t.expert, &t.groups);
     if (!t.live) return t;
-    t.n0 = slice * p.cols;
+    t.n0 = slice * p.cols + piece * t.cols;
     t.first_block = t.row_block * (p.ffn_dim >> 7);
-    t.k_steps = (kBack ? 2 : 1) * (p.ffn_dim / kTileStep);
+    // A piece that lies behind D (an odd multiple of 128) has nothing to do.
+    t.live = t.n0 < p.d_model;
+    t.k_steps = t.live ? (kBack ? 2 : 1) * (p.ffn_dim / kTileStep) : 0;
     return t;
   }
-  static __device__ __forceinline__ int columns(const Params& p) { return p.cols; }
-  static __device__ __forceinline__ uint32_t tx_bytes(const Params& p, const Tile&, int32_t) {
-    return TileSmem::kABytes + static_cast<uint32_t>(p.cols) * 128u;
+  static __device__ __forceinline__ int columns(const Params&, const Tile& t) { return t.cols; }
+  static __device__ __forceinline__ uint32_t tx_bytes(const Params&, const Tile& t, int32_t) {
+    return static_cast<uint32_t>(t.groups) * 4096u + static_cast<uint32_t>(t.cols) * 128u;
   }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
@@ -351,11 +401,11 @@ struct RowsProduct {
     const int32_t steps = p.ffn_dim / kTileStep;
     const int which = kBack && ks >= steps ? 1 : 0;
     const int32_t k = (ks - which * steps) * kTileStep;
-    ptx::tma_load_2d_hint(a, &maps.m[which], k & 127, (t.first_block + (k >> 7)) * kTileRows, bar, once);
+    load_rows<true>(a, &maps.m[which], &maps.m[5 + which], k & 127, (t.first_block + (k >> 7)) * kTileRows, t.groups, bar);
     if (kBack) {
       ptx::tma_load_2d_hint(b, &maps.m[2 + which], k, t.expert * p.d_model + t.n0, bar, once);
     } else {
-      for (int32_t j = 0; j < p.cols / 64; ++j)
+      for (int32_t j = 0; j < t.cols / 64; ++j)
         ptx::tma_load_2d_hint(b + j * TileSmem::kSlabBytes, &maps.m[2], t.n0 + j * 64, t.expert * p.ffn_dim + k, bar, once);
     }
   }
@@ -366,7 +416,7 @@ struct RowsProduct {
                                                   const Early& early) {
     if (!early.store) return;
 #pragma unroll 1
-    for (int32_t c = w.part * 64; c < p.cols; c += 128) {
+    for (int32_t c = w.part * 64; c < t.cols; c += 128) {
       if (t.n0 + c >= p.d_model) break;
       uint32_t packed[32];
       load_packed_x64(w.taddr + c, packed);
@@ -797,7 +847,7 @@ int launch_small(void (*kernel)(Params...), int64_t blocks, int threads, cudaStr
 
 // x_rows, then H (and G, U) on the layout.
 int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token, const int32_t* row_block_expert,
-              const int32_t* padded_offsets, void* x_rows, void* h_blocks, void* g_blocks,
+              const int32_t* padded_offsets, const int32_t* tokens_per_expert, void* x_rows, void* h_blocks, void* g_blocks,
               void* u_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
               int32_t activation, int skip_padding_rows, int32_t* dev_status, cudaStream_t stream) {
   const DeviceInfo* info = current_device_info();
@@ -813,12 +863,13 @@ int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t
     if (int rc = encode_2d_map(&maps.m[4], u_blocks, b_rows, 128, 32, 64, 2, "sdd_gated (kept up)")) return rc;
   }
   if (int rc = encode_2d_map(&maps.m[5], x_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, "sdd_gated (rows)")) return rc;
+  if (int rc = encode_2d_map(&maps.m[6], x_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, "sdd_gated (rows)")) return rc;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
   if (int rc = launch_small(gated_rows_kernel, blocks, kSmallThreads, stream, "sdd_gated (rows)", static_cast<const uint4*>(x),
                             row_token, padded_offsets + num_experts, static_cast<uint4*>(x_rows), d_model / 8))
     return rc;
   GatedUp::Params p{};
-  p.order = {row_block_expert, padded_offsets, num_row_blocks, ffn_dim / 128};
+  p.order = {row_block_expert, padded_offsets, tokens_per_expert, num_experts, ffn_dim / 128};
   p.row_token = row_token;
   p.d_model = d_model;
   p.activation = activation;
@@ -849,17 +900,19 @@ int32_t tile_cols(int64_t num_row_blocks, int32_t width, int sm_count) {
 
 template <int kCols>
 int gated_grad_hidden(const void* grad_rows, const float* row_gate, const void* w_down, const void* g_blocks, const void* u_blocks,
-                      const int32_t* row_token, const int32_t* row_block_expert, const int32_t* padded_offsets, void* dg_blocks,
+                      const int32_t* row_token, const int32_t* row_block_expert, const int32_t* padded_offsets,
+                      const int32_t* tokens_per_expert, void* dg_blocks,
                       void* du_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
                       int32_t activation, int32_t* dev_status, cudaStream_t stream) {
   const char* what = "moe_gated_backward (hidden)";
   TileMaps maps{};
   if (int rc = encode_2d_map(&maps.m[0], w_down, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, kCols, 64, 2, what)) return rc;
   if (int rc = encode_2d_map(&maps.m[1], grad_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[2], grad_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, what)) return rc;
   typename GradHidden<kCols>::Params p{};
   p.row_gate = row_gate;
   const int32_t slices = (ffn_dim + kCols - 1) / kCols;
-  p.order = {row_block_expert, padded_offsets, num_row_blocks, slices};
+  p.order = {row_block_expert, padded_offsets, tokens_per_expert, num_experts, slices};
   p.row_token = row_token;
   p.g = static_cast<const __nv_bfloat16*>(g_blocks);
   p.u = static_cast<const __nv_bfloat16*>(u_blocks);
@@ -906,7 +959,8 @@ int gated_grad_weights(const void* x_rows, const void* grad_rows, const void* h_
 // Y = H Wd (back: false; a0 = H, w0 = Wd), or the rows of dx = dG Wg^T + dU Wu^T (a0, a1, w0, w1).
 template <bool kBack>
 int rows_product(const void* a0, const void* a1, const void* w0, const void* w1, const int32_t* row_token,
-                 const int32_t* row_block_expert, const int32_t* padded_offsets, void* rows, int32_t d_model, int32_t ffn_dim,
+                 const int32_t* row_block_expert, const int32_t* padded_offsets, const int32_t* tokens_per_expert, void* rows,
+                 int32_t d_model, int32_t ffn_dim,
                  int32_t num_experts, int32_t num_row_blocks, int32_t* dev_status, cudaStream_t stream) {
   const char* what = kBack ? "moe_gated_backward (x)" : "moe_gated (down)";
   const DeviceInfo* info = current_device_info();
@@ -915,9 +969,11 @@ int rows_product(const void* a0, const void* a1, const void* w0, const void* w1,
   const uint64_t b_rows = static_cast<uint64_t>(num_row_blocks) * ffn_dim;
   TileMaps maps{};
   if (int rc = encode_2d_map(&maps.m[0], a0, b_rows, 128, 128, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[5], a0, b_rows, 128, 32, 64, 2, what)) return rc;
   if (kBack) {
     const uint64_t w_rows = static_cast<uint64_t>(num_experts) * d_model;
     if (int rc = encode_2d_map(&maps.m[1], a1, b_rows, 128, 128, 64, 2, what)) return rc;
+    if (int rc = encode_2d_map(&maps.m[6], a1, b_rows, 128, 32, 64, 2, what)) return rc;
     if (int rc = encode_2d_map(&maps.m[2], w0, w_rows, ffn_dim, cols, 64, 2, what)) return rc;
     if (int rc = encode_2d_map(&maps.m[3], w1, w_rows, ffn_dim, cols, 64, 2, what)) return rc;
   } else {
@@ -926,7 +982,7 @@ int rows_product(const void* a0, const void* a1, const void* w0, const void* w1,
   if (int rc = encode_2d_map(&maps.m[4], rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, what)) return rc;
   typename RowsProduct<kBack>::Params p{};
   const int32_t slices = (d_model + cols - 1) / cols;
-  p.order = {row_block_expert, padded_offsets, num_row_blocks, slices};
+  p.order = {row_block_expert, padded_offsets, tokens_per_expert, num_experts, slices};
   p.row_token = row_token;
   p.d_model = d_model;
   p.ffn_dim = ffn_dim;
@@ -1083,18 +1139,18 @@ int forward_small(const GatedBuffers& b, const void* x, const void* expert_idx, 
 using namespace sb;
 
 extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token,
-                            const int32_t* row_block_expert, const int32_t* padded_offsets, void* x_rows, void* h_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim,
+                            const int32_t* row_block_expert, const int32_t* padded_offsets, const int32_t* tokens_per_expert, void* x_rows, void* h_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim,
                             int32_t num_experts, int32_t num_row_blocks, int32_t activation, int skip_padding_rows,
                             int32_t* dev_status, sb_stream_t stream) {
   clear_error();
   if (int rc = check_gated("sdd_gated", d_model, ffn_dim, num_experts, num_row_blocks, activation)) return rc;
   if (num_row_blocks == 0) return SB_OK;
-  if (any_null({x, w_gate, w_up, row_token, row_block_expert, padded_offsets, x_rows, h_blocks}))
+  if (any_null({x, w_gate, w_up, row_token, row_block_expert, padded_offsets, tokens_per_expert, x_rows, h_blocks}))
     return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: NULL buffer");
   if (num_tokens <= 0) return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: T must be positive");
   if (any_misaligned({x, w_gate, w_up, x_rows, h_blocks}))
     return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: x, the weights, the rows and the blocks must be 16-byte aligned");
-  return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, padded_offsets, x_rows, h_blocks,
+  return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, padded_offsets, tokens_per_expert, x_rows, h_blocks,
                    nullptr, nullptr, d_model, ffn_dim, num_experts, num_row_blocks, activation, skip_padding_rows, dev_status,
                    as_stream(stream));
 }
@@ -1140,12 +1196,12 @@ extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int i
                         ints(b.row_block_expert), ints(b.row_offsets), ints(b.col_indices), ints(b.error), temp + b.work, stream))
     return rc;
   if (int rc = sdd_gated(x, w_gate, w_up, ints(b.row_token), ints(b.row_block_expert), ints(b.padded_offsets),
-                         base + b.x_rows, base + b.h, keep ? base + b.g : nullptr,
+                         ints(b.tokens_per_expert), base + b.x_rows, base + b.h, keep ? base + b.g : nullptr,
                          keep ? base + b.u : nullptr, d_model, ffn_dim, num_experts, b.row_blocks, activation, 1, dev_status,
                          as_stream(stream)))
     return rc;
   if (int rc = rows_product<false>(base + b.h, nullptr, w_down, nullptr, ints(b.row_token), ints(b.row_block_expert),
-                                   ints(b.padded_offsets), base + b.y, d_model, ffn_dim, num_experts, b.row_blocks, dev_status,
+                                   ints(b.padded_offsets), ints(b.tokens_per_expert), base + b.y, d_model, ffn_dim, num_experts, b.row_blocks, dev_status,
                                    as_stream(stream)))
     return rc;
   return sb_combine(base + b.y, ints(b.copy_row), gate, gate_dtype, out, num_tokens, k, d_model, stream);
@@ -1184,7 +1240,7 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int
   if (info == nullptr) return SB_ERR_CUDA;
   const auto grad_hidden = tile_cols(b.row_blocks, ffn_dim, info->sm_count) == kTileCols ? gated_grad_hidden<kTileCols> : gated_grad_hidden<64>;
   if (int rc = grad_hidden(temp + b.grad_rows, row_gate, w_down, base + b.g, base + b.u, row_token, ints(b.row_block_expert),
-                           ints(b.padded_offsets), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
+                           ints(b.padded_offsets), ints(b.tokens_per_expert), temp + b.dg, temp + b.du, d_model, ffn_dim, num_experts, b.row_blocks,
                            activation, dev_status, st))
     return rc;
   if (int rc = gated_grad_weights(base + b.x_rows, temp + b.scaled_rows, base + b.h, temp + b.dg, temp + b.du,
@@ -1193,7 +1249,7 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int
     return rc;
   // The rows of dx take the place of grad_rows, which the hidden gradients were the last to read.
   if (int rc = rows_product<true>(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert),
-                                  ints(b.padded_offsets), temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks,
+                                  ints(b.padded_offsets), ints(b.tokens_per_expert), temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks,
                                   dev_status, st))
     return rc;
   return gated_join(temp + b.grad_rows, ints(b.copy_row), dx, dgate, gate_dtype, num_tokens, k, d_model, st);

@@ -394,7 +394,7 @@ struct LoraExpand {
     t.live = true;
     return t;
   }
-  static __device__ __forceinline__ int columns(const Params& p) { return p.cols; }
+  static __device__ __forceinline__ int columns(const Params& p, const Tile&) { return p.cols; }
   static __device__ __forceinline__ int slabs(const Params& p) { return (p.cols + 63) >> 6; }
   static __device__ __forceinline__ uint32_t tx_bytes(const Params& p, const Tile& t, int32_t ks) {
     return static_cast<uint32_t>(slabs(p)) * TileSmem::kSlabBytes + (ks < t.base_steps ? TileSmem::kABytes : 0);

@@ -93,7 +93,7 @@ __device__ __forceinline__ void load_packed_x64(uint32_t taddr, uint32_t (&packe
 //   Rows rows(p, tile, row0) once per tile, extension_chunk(p, tile, rows, j, row, ks, chunk) = the 16 bytes of chunk
 //   `chunk` of row `row` = row0 + 16 j. B (MN-major) eight K rows at a time: extension_row(p, tile, ks, i) says where
 //   piece i comes from, ahead of time, extension_load(maps, p, tile, i, row, b, bar) issues its loads.
-//   With kVariable: columns(p) <= 256 (a multiple of 16) accumulator columns in use, tx_bytes(p, tile, ks) per stage
+//   With kVariable: columns(p, tile) <= 256 (a multiple of 16) accumulator columns in use, tx_bytes(p, tile, ks) per stage
 template <class Op>
 struct TileConfig {
   static constexpr int kExtensionWarps = Op::kExtension ? 4 : 0;
@@ -200,8 +200,6 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
       uint32_t idesc = ptx::make_idesc_bf16(kTileRows, kTileCols, Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
-      if constexpr (Op::kVariable)
-        idesc = ptx::make_idesc_bf16(kTileRows, Op::columns(p), Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, ready_phases = 0;
       bool ok = true;
       int32_t index = blockIdx.x;
@@ -211,6 +209,8 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
         const int32_t k_steps = next.k_steps;
         int32_t base_steps = k_steps;
         if constexpr (Op::kExtension) base_steps = next.base_steps;
+        if constexpr (Op::kVariable)
+          idesc = ptx::make_idesc_bf16(kTileRows, Op::columns(p, next), Op::kBMnMajor) | (Op::kAMnMajor ? 1u << 15 : 0u);
         if (index + step < total) next = Op::tile(p, index + step);
         if (k_steps == 0) continue;
         if (!ptx::mbar_wait_bounded(acc_empty_bar + 8 * acc, acc_phase ^ 1u, abort_word)) {

@@ -63,7 +63,7 @@ def sdd_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, topo: T
     if topo.block_size != 128:
         raise ValueError(f"sdd_gated needs block size 128, got {topo.block_size}")
     return _C.sdd_gated_cuda(x, w_gate, w_up, topo.row_token, topo.row_block_expert, topo.padded_offsets,
-                             topo.col_indices.numel(), activation, skip_padding_rows)
+                             topo.tokens_per_expert, topo.col_indices.numel(), activation, skip_padding_rows)
 
 
 def combine(y: torch.Tensor, expert_weight: torch.Tensor, topo: Topology | DeviceTopology) -> torch.Tensor:

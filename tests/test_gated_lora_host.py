@@ -69,10 +69,10 @@ def test_gated_calls_are_refused_before_any_launch(lib) -> None:
         (lambda: backward(state_bytes=1000), b"are needed"), (lambda: backward(scratch_bytes=1000), b"are needed"),
     ]:
         assert call() == 1 and text in lib.sb_last_error(), text
-    args = [one] * 8
+    args = [one] * 9
     assert lib.sb_sdd_gated(*args, 10, 128, 128, 4, 3, 5, 0, None, None) == 1 and b"activation" in lib.sb_last_error()
     assert lib.sb_sdd_gated(*args, 10, 100, 128, 4, 3, 0, 0, None, None) == 1 and b"multiple of 128" in lib.sb_last_error()
-    assert lib.sb_sdd_gated(*args[:7], None, 10, 128, 128, 4, 3, 0, 0, None, None) == 1 and b"NULL" in lib.sb_last_error()
+    assert lib.sb_sdd_gated(*args[:8], None, 10, 128, 128, 4, 3, 0, 0, None, None) == 1 and b"NULL" in lib.sb_last_error()
     assert lib.sb_sdd_gated(*args, 10, 128, 128, 4, 0, 0, 0, None, None) == 0  # no row blocks: nothing to do
 
 
