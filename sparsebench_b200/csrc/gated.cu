@@ -121,6 +121,8 @@ __device__ __forceinline__ void load_rows(uint32_t a, const CUtensorMap* all, co
 // ---- forward: both projections, the activation and the product ----------------------------------------------------
 // The tile's 256 accumulator columns are 128 columns of G next to the same 128 of U, so a thread that drains column c
 // finds its partner 128 columns on and H leaves the chip as the only result (plus G and U for training).
+// Padding rows of x are loaded as the zeros they are: multiplying zeros takes less of the power limit, which sets the clock
+// of a longer run, than what a stage happens to hold (395 against 406 us a pass of the layer below, one after another).
 // Bound by the weights' way from memory where experts have few rows (T = 4096, D = 1024, F = 4096, E = 64: 1.07 GB of
 // weights in 194 us, 5.5 TB/s of a measured 6.56 copy peak; 238 us with G and U kept) and by the tensor cores where they
 // have many (T = 4096, D = 4096, F = 14336, E = 8: 1.45 ms, 1490 TFLOP/s executed, at the clock that the power limit leaves).
@@ -140,7 +142,7 @@ struct GatedUp {
   struct Early { bool store; };
   static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
-  static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = true;
+  static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.live_tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
@@ -149,21 +151,14 @@ struct GatedUp {
     t.live = p.order.at(index, &t.row_block, &slice, &t.expert, &t.groups);
     if (!t.live) return t;
     t.n0 = slice * 128;
-    // Padding rows that are stored have to be multiplied, as the zeros they are: whole halves for training, or all.
-    if (p.keep) t.groups = (t.groups + 1) & ~1;
-    else if (!p.skip_padding) t.groups = 4;
     t.first_block = t.row_block * p.order.slices;  // of the layout's blocks, F / 128 per row block
     t.k_steps = p.d_model / kTileStep;
     return t;
   }
-  static __device__ __forceinline__ int columns(const Params&, const Tile&) { return kTileCols; }
-  static __device__ __forceinline__ uint32_t tx_bytes(const Params&, const Tile& t, int32_t) {
-    return TileSmem::kBBytes + static_cast<uint32_t>(t.groups) * 4096u;
-  }
   static __device__ __forceinline__ void load(const TileMaps& maps, const Params& p, const Tile& t, int32_t ks, uint32_t a,
                                               uint32_t b, uint32_t bar) {
     const uint64_t once = ptx::policy_evict_first();
-    load_rows<false>(a, &maps.m[5], &maps.m[6], ks * kTileStep, t.row_block * kTileRows, t.groups, bar);
+    ptx::tma_load_2d(a, &maps.m[5], ks * kTileStep, t.row_block * kTileRows, bar);
     const int32_t row = t.expert * p.d_model + ks * kTileStep;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -863,7 +858,6 @@ int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t
     if (int rc = encode_2d_map(&maps.m[4], u_blocks, b_rows, 128, 32, 64, 2, "sdd_gated (kept up)")) return rc;
   }
   if (int rc = encode_2d_map(&maps.m[5], x_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, "sdd_gated (rows)")) return rc;
-  if (int rc = encode_2d_map(&maps.m[6], x_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, "sdd_gated (rows)")) return rc;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
   if (int rc = launch_small(gated_rows_kernel, blocks, kSmallThreads, stream, "sdd_gated (rows)", static_cast<const uint4*>(x),
                             row_token, padded_offsets + num_experts, static_cast<uint4*>(x_rows), d_model / 8))
