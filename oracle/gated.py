@@ -71,9 +71,9 @@ def gated_reference(x, expert_idx, gate, w_gate, w_up, w_down, act: str = "silu"
         a_b = 1.13 * g_b + ACT_ERROR * g.abs()  # |act'| <= 1.13
         h_b = a_b * u.abs() + a.abs() * u_b + HALF_BF16 * h.abs()
         y = h @ wd
-        y_b = h_b @ wd.abs() + ffn_dim * HALF_FP32 * (h.abs() @ wd.abs()) + HALF_BF16 * y.abs()
+        y_b = h_b @ wd.abs() + ffn_dim * HALF_FP32 * (h.abs() @ wd.abs())
         out.index_add_(0, t, w * y)
-        out_b.index_add_(0, t, w.abs() * y_b)
+        out_b.index_add_(0, t, w.abs() * (y_b + 4 * HALF_FP32 * y.abs()))
         if grad_out is None:
             continue
         # G and U are read back as bf16.
@@ -96,10 +96,10 @@ def gated_reference(x, expert_idx, gate, w_gate, w_up, w_down, act: str = "silu"
             val[name][e] = xs.T @ d
             bnd[name][e] = xs.abs().T @ d_b + n * HALF_FP32 * (xs.abs().T @ d.abs())
         row = dg @ wg.T + du @ wu.T
-        row_b = (dg_b @ wg.abs().T + du_b @ wu.abs().T + HALF_BF16 * row.abs()
+        row_b = (dg_b @ wg.abs().T + du_b @ wu.abs().T
                  + 2 * ffn_dim * HALF_FP32 * (dg.abs() @ wg.abs().T + du.abs() @ wu.abs().T))
         val["dx"].index_add_(0, t, row)
-        bnd["dx"].index_add_(0, t, row_b)
+        bnd["dx"].index_add_(0, t, row_b + 4 * HALF_FP32 * row.abs())
     result = {"out": (out, out_b)}
     if grad_out is not None:
         result.update({n: (val[n], bnd[n]) for n in val})

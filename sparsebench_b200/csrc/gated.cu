@@ -6,9 +6,9 @@
 //              dWd = H^T (w dO), dWg = X^T dG, dWu = X^T dU                               (GradWeights)
 //              dx[t] = sum over the token's copies of dG Wg^T + dU Wu^T                   (RowsProduct, join)
 //
-// The forward keeps X (rows in layout order), G, U, H and Y. Everything that is an operand of a product is bf16, as the
-// weights are: G, U, H, Y, w dO, dG, dU and the rows of dx are each rounded once; sums, the activation and its derivative
-// are in fp32. dgate takes Y, not H dH / w, which a gate of 0 would spoil.
+// The forward keeps X (rows in layout order), G, U, H and Y. What is an operand of a product is bf16, as the weights are:
+// H, w dO, dG and dU are each rounded once, and so are G and U, which the backward pass reads back (in fp32 they would be
+// most of its traffic). Y, the rows of dx, all sums, the activation and its derivative are in fp32. dgate takes Y, not H dH / w, which a gate of 0 would spoil.
 //
 // A decoding step (at most 64 copies, nothing kept) takes another way: no layout, the weights of the picked experts
 // streamed by the kernels of skinny.cuh (SkinnyUp, SkinnyDown, gated_small_combine_kernel).
@@ -331,7 +331,8 @@ struct GradHidden {
 
 // ---- the products that give rows: the down projection, and the backward pass's rows of dx ---------------------------
 // Down (kBack false): Y = H Wd, Wd [F, D] an MN-major operand. Back: dG Wg^T + dU Wu^T as one product with 2 F inner
-// columns, Wg and Wu [D, F] K-major operands. Either way the weights lie as the tensor cores read them.
+// columns, Wg and Wu [D, F] K-major operands. Either way the weights lie as the tensor cores read them. The rows stay in
+// fp32: each token's rows are summed, and rounded once, behind this.
 // At T = 4096, D = 1024, F = 4096, E = 64: 105 us (0.54 GB of weights, 5.1 TB/s) and 220 us (4.9 TB/s); what is left is the
 // last wave, 368 tiles of 256 columns on 148 SMs. Tiles of 128 columns fill it but keep fewer bytes in flight: 141 and
 // 285 us. On the Mixtral-like layer (T = 4096, D = 4096, F = 14336, E = 8) 745 us and 1.50 ms, 1450 TFLOP/s executed.
@@ -411,11 +412,12 @@ struct RowsProduct {
                                                   const Early& early) {
     if (!early.store) return;
 #pragma unroll 1
-    for (int32_t c = w.part * 64; c < t.cols; c += 128) {
+    for (int32_t c = w.part * 32; c < t.cols; c += 64) {
       if (t.n0 + c >= p.d_model) break;
-      uint32_t packed[32];
-      load_packed_x64(w.taddr + c, packed);
-      store_rows_128b<kBuffers>(w, &maps.m[4], packed, t.n0 + c, t.row_block * kTileRows + w.quarter * 32);
+      uint32_t v[32];
+      ptx::tmem_ld_32x32b_x32(w.taddr + c, v);
+      ptx::tmem_ld_wait();
+      store_rows_128b<kBuffers>(w, &maps.m[4], v, t.n0 + c, t.row_block * kTileRows + w.quarter * 32);
     }
   }
 };
@@ -671,6 +673,31 @@ gated_small_combine_kernel(const float4* __restrict__ y, const void* __restrict_
   out[static_cast<int64_t>(t) * quads + v] = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
 }
 
+// The same from the fp32 rows of the layout: out[t] = sum over the picks j, in order, of gate[t, j] * Y[copy_row[t, j]].
+__global__ void __launch_bounds__(kSmallThreads)
+gated_combine_kernel(const float4* __restrict__ y, const int32_t* __restrict__ copy_row, const void* __restrict__ gate,
+                     int gate_dtype, uint2* __restrict__ out, int64_t num_tokens, int32_t k, int32_t quads) {
+  ptx::grid_dependency_wait();
+  const int64_t total = num_tokens * quads;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kSmallThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kSmallThreads + threadIdx.x; i < total; i += stride) {
+    const int64_t t = i / quads;
+    const int32_t v = static_cast<int32_t>(i - t * quads);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int32_t j = 0; j < k; ++j) {
+      const int32_t row = __ldg(copy_row + t * k + j);
+      if (row < 0) continue;
+      const float w = gate_at(gate, gate_dtype, t * k + j);
+      const float4 r = __ldcg(y + static_cast<int64_t>(row) * quads + v);
+      acc.x = fmaf(w, r.x, acc.x);
+      acc.y = fmaf(w, r.y, acc.y);
+      acc.z = fmaf(w, r.z, acc.z);
+      acc.w = fmaf(w, r.w, acc.w);
+    }
+    out[i] = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
+  }
+}
+
 // One warp per row of the layout: x_rows[r] = x[token], zeros for padding (the rows that the products' TMA loads want side
 // by side; gathering them inside the products with cp.async took a quarter of their time instead).
 __global__ void __launch_bounds__(kSmallThreads)
@@ -694,7 +721,7 @@ gated_rows_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ row_t
 // rounded to bf16 (what dWd is summed from; dH takes the unscaled rows and w in fp32, one rounding less), row_gate[r] = w,
 // zeros for padding; and dgate = grad_out[token] . Y[r] in fp32.
 __global__ void __launch_bounds__(kSmallThreads)
-gated_grad_rows_kernel(const uint4* __restrict__ grad_out, const uint4* __restrict__ y_rows, const void* __restrict__ gate,
+gated_grad_rows_kernel(const uint4* __restrict__ grad_out, const float4* __restrict__ y_rows, const void* __restrict__ gate,
                        int gate_dtype, const int32_t* __restrict__ row_token, const int32_t* __restrict__ copy_row,
                        const int32_t* __restrict__ num_rows, uint4* __restrict__ grad_rows, uint4* __restrict__ scaled_rows,
                        float* __restrict__ row_gate, void* __restrict__ dgate, int32_t k, int32_t vecs) {
@@ -724,21 +751,20 @@ gated_grad_rows_kernel(const uint4* __restrict__ grad_out, const uint4* __restri
     }
     const float w = gate_at(gate, gate_dtype, copy);
     const uint4* gs = grad_out + static_cast<int64_t>(token) * vecs;
-    const uint4* ys = y_rows + static_cast<int64_t>(r) * vecs;
+    const float4* ys = y_rows + static_cast<int64_t>(r) * vecs * 2;
     float dot = 0.0f;
 #pragma unroll 2
     for (int32_t v = lane; v < vecs; v += 32) {
       const uint4 raw = __ldg(gs + v);
-      const uint4 yraw = __ldg(ys + v);
+      const float4 y0 = __ldg(ys + 2 * v), y1 = __ldg(ys + 2 * v + 1);
       const uint32_t gq[4] = {raw.x, raw.y, raw.z, raw.w};
-      const uint32_t yq[4] = {yraw.x, yraw.y, yraw.z, yraw.w};
+      const float yq[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
       uint32_t q[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&gq[c]));
-        const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&yq[c]));
-        dot = fmaf(f.x, y.x, dot);
-        dot = fmaf(f.y, y.y, dot);
+        dot = fmaf(f.x, yq[2 * c], dot);
+        dot = fmaf(f.y, yq[2 * c + 1], dot);
         q[c] = pack_bf16(f.x * w, f.y * w);
       }
       plain[v] = raw;
@@ -757,8 +783,8 @@ gated_grad_rows_kernel(const uint4* __restrict__ grad_out, const uint4* __restri
 // dx[t] = sum over the token's copies of their rows, in copy order in fp32, one warp per token; and zeros into the dgate
 // of copies that have no row.
 __global__ void __launch_bounds__(kSmallThreads)
-gated_join_kernel(const uint4* __restrict__ dx_rows, const int32_t* __restrict__ copy_row, uint4* __restrict__ dx,
-                  void* __restrict__ dgate, int gate_dtype, int64_t num_tokens, int32_t k, int32_t vecs) {
+gated_join_kernel(const float4* __restrict__ dx_rows, const int32_t* __restrict__ copy_row, uint2* __restrict__ dx,
+                  void* __restrict__ dgate, int gate_dtype, int64_t num_tokens, int32_t k, int32_t quads) {
   ptx::grid_dependency_wait();
   const int lane = static_cast<int>(threadIdx.x & 31);
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kSmallThreads / 32);
@@ -769,27 +795,18 @@ gated_join_kernel(const uint4* __restrict__ dx_rows, const int32_t* __restrict__
       else static_cast<__nv_bfloat16*>(dgate)[t * k + j] = __float2bfloat16_rn(0.0f);
     }
 #pragma unroll 2
-    for (int32_t v = lane; v < vecs; v += 32) {
-      float acc[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
+    for (int32_t v = lane; v < quads; v += 32) {
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int32_t j = 0; j < k; ++j) {
         const int32_t row = __ldg(copy_row + t * k + j);
         if (row < 0) continue;
-        const uint4 raw = __ldcg(dx_rows + static_cast<int64_t>(row) * vecs + v);
-        const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float2 f = __bfloat1622float2(pairs[q]);
-          acc[2 * q] += f.x;
-          acc[2 * q + 1] += f.y;
-        }
+        const float4 r = __ldcg(dx_rows + static_cast<int64_t>(row) * quads + v);
+        acc.x += r.x;
+        acc.y += r.y;
+        acc.z += r.z;
+        acc.w += r.w;
       }
-      uint4 packed;
-      uint32_t* o = reinterpret_cast<uint32_t*>(&packed);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = pack_bf16(acc[2 * q], acc[2 * q + 1]);
-      dx[t * vecs + v] = packed;
+      dx[t * quads + v] = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
     }
   }
 }
@@ -879,7 +896,7 @@ int gated_grad_rows_of(const void* grad_out, const void* y_rows, const void* gat
   if (info == nullptr) return SB_ERR_CUDA;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
   gated_grad_rows_kernel<<<static_cast<unsigned>(blocks), kSmallThreads, 0, stream>>>(
-      static_cast<const uint4*>(grad_out), static_cast<const uint4*>(y_rows), gate, gate_dtype, row_token, copy_row, num_rows,
+      static_cast<const uint4*>(grad_out), static_cast<const float4*>(y_rows), gate, gate_dtype, row_token, copy_row, num_rows,
       static_cast<uint4*>(grad_rows), static_cast<uint4*>(scaled_rows), row_gate, dgate, k, d_model / 8);
   return check_launch("moe_gated_backward (rows)");
 }
@@ -973,7 +990,7 @@ int rows_product(const void* a0, const void* a1, const void* w0, const void* w1,
   } else {
     if (int rc = encode_2d_map(&maps.m[2], w0, static_cast<uint64_t>(num_experts) * ffn_dim, d_model, 64, 64, 2, what)) return rc;
   }
-  if (int rc = encode_2d_map(&maps.m[4], rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 64, 2, what)) return rc;
+  if (int rc = encode_2d_map(&maps.m[4], rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 32, 32, 4, what)) return rc;
   typename RowsProduct<kBack>::Params p{};
   const int32_t slices = (d_model + cols - 1) / cols;
   p.order = {row_block_expert, padded_offsets, tokens_per_expert, num_experts, slices};
@@ -990,8 +1007,8 @@ int gated_join(const void* dx_rows, const int32_t* copy_row, void* dx, void* dga
   if (info == nullptr) return SB_ERR_CUDA;
   const int64_t blocks = std::min<int64_t>((num_tokens + 7) / 8, static_cast<int64_t>(info->sm_count) * 8);
   return launch_small(gated_join_kernel, blocks, kSmallThreads, stream, "moe_gated_backward (join)",
-                      static_cast<const uint4*>(dx_rows), copy_row, static_cast<uint4*>(dx), dgate, gate_dtype, num_tokens, k,
-                      d_model / 8);
+                      static_cast<const float4*>(dx_rows), copy_row, static_cast<uint2*>(dx), dgate, gate_dtype, num_tokens, k,
+                      d_model / 4);
 }
 
 bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
@@ -1048,7 +1065,7 @@ int gated_buffers(int64_t num_tokens, int32_t k, int32_t d_model, int32_t ffn_di
   b->col_indices = take(row_blocks * ffn_blocks * 4);
   b->error = take(4);
   b->x_rows = take(rows * d_model * 2);
-  b->y = take(rows * d_model * 2);
+  b->y = take(rows * d_model * 4);
   b->h = take(rows * ffn_dim * 2);
   if (keep) {
     b->g = take(rows * ffn_dim * 2);
@@ -1198,7 +1215,12 @@ extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int i
                                    ints(b.padded_offsets), ints(b.tokens_per_expert), base + b.y, d_model, ffn_dim, num_experts, b.row_blocks, dev_status,
                                    as_stream(stream)))
     return rc;
-  return sb_combine(base + b.y, ints(b.copy_row), gate, gate_dtype, out, num_tokens, k, d_model, stream);
+  const DeviceInfo* info = current_device_info();
+  if (info == nullptr) return SB_ERR_CUDA;
+  const int64_t blocks = std::min<int64_t>((num_tokens * (d_model / 4) + kSmallThreads - 1) / kSmallThreads, info->sm_count * 16);
+  return launch_small(gated_combine_kernel, blocks, kSmallThreads, as_stream(stream), "moe_gated (combine)",
+                      reinterpret_cast<const float4*>(base + b.y), ints(b.copy_row), gate, gate_dtype, static_cast<uint2*>(out),
+                      num_tokens, k, d_model / 4);
 }
 
 extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int gate_dtype,
@@ -1241,7 +1263,8 @@ extern "C" int sb_moe_gated_backward(const void* grad_out, const void* gate, int
                                   ints(b.padded_offsets), ints(b.tokens_per_expert), dw_gate, dw_up, dw_down, d_model,
                                   ffn_dim, num_experts, b.row_blocks, dev_status, st))
     return rc;
-  // The rows of dx take the place of grad_rows, which the hidden gradients were the last to read.
+  // The rows of dx (fp32) take the place of grad_rows and scaled_rows (bf16, one behind the other), which the hidden
+  // and the weight gradients were the last to read.
   if (int rc = rows_product<true>(temp + b.dg, temp + b.du, w_gate, w_up, row_token, ints(b.row_block_expert),
                                   ints(b.padded_offsets), ints(b.tokens_per_expert), temp + b.grad_rows, d_model, ffn_dim, num_experts, b.row_blocks,
                                   dev_status, st))

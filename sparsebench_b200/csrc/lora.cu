@@ -13,8 +13,8 @@
 // Up to 64 tokens (a decoding step) the weights are streamed by the kernel of skinny.cuh and the second term is plain
 // fp32 arithmetic on each token's own rows of A and B (lora_rows_kernel, SkinnyLora).
 //
-// In the products V is rounded to bf16 for y in bf16; for y in fp32 it travels as a pair of bf16 (V and what rounding took
-// from it, against the same rows of B), at most 2^-16 of V off.
+// In the products V is rounded to bf16 for y in bf16; for y in fp32 it travels as three bf16 (V, what rounding took from it,
+// and what that left, against the same rows of B): the 24 bits of an fp32.
 //
 // There a zero of V meets B of other requests' adapters: an infinity or NaN in one adapter would reach its neighbours'
 // rows. So an adapter whose B is not finite stays out of the product (shrink finds it, reading B beside its own loads and
@@ -67,7 +67,7 @@ struct ShrinkParams {
   const float* scale;
   int32_t* tables;
   uint8_t* not_finite;
-  __nv_bfloat16* v;  // [T, rank * parts]: the values, with parts = 2 then what rounding took from them
+  __nv_bfloat16* v;  // [T, rank * parts]: the values, with parts = 3 then what rounding took from them, twice
   int32_t idx_is_i64, num_tokens, num_adapters, rank, parts, splits, steps, total_steps, stages;
   int32_t b_vecs;  // 16-byte pieces of an adapter's B
 };
@@ -333,17 +333,20 @@ lora_shrink_kernel(const __grid_constant__ ShrinkMaps maps, const __grid_constan
         for (int q = 0; q < 8; ++q) v[q] += ptx::ld_cluster_f32(from + q * kTileRows * 4u);
       }
       const float factor = p.scale != nullptr ? __ldg(p.scale + a) : 1.0f;
-      uint32_t high[4], low[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float v0 = v[2 * q] * factor, v1 = v[2 * q + 1] * factor;
-        high[q] = pack_bf16(v0, v1);
-        const float2 h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&high[q]));
-        low[q] = pack_bf16(isfinite(h.x) ? v0 - h.x : 0.0f, isfinite(h.y) ? v1 - h.y : 0.0f);
-      }
+      for (int q = 0; q < 8; ++q) v[q] *= factor;
       __nv_bfloat16* dst = p.v + static_cast<int64_t>(first_token + r) * p.rank * p.parts + j0;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(high[0], high[1], high[2], high[3]);
-      if (p.parts == 2) *reinterpret_cast<uint4*>(dst + p.rank) = make_uint4(low[0], low[1], low[2], low[3]);
+      for (int32_t part = 0; part < p.parts; ++part) {
+        uint32_t packed[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          packed[q] = pack_bf16(v[2 * q], v[2 * q + 1]);
+          const float2 held = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&packed[q]));
+          v[2 * q] = isfinite(held.x) ? v[2 * q] - held.x : 0.0f;
+          v[2 * q + 1] = isfinite(held.y) ? v[2 * q + 1] - held.y : 0.0f;
+        }
+        *reinterpret_cast<uint4*>(dst + part * p.rank) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+      }
     }
   }
   if (p.splits > 1) ptx::cluster_sync_all();  // nobody's shared memory is read any more
@@ -413,8 +416,7 @@ struct LoraExpand {
     if (slot >= t.slots) return p.adapter_rows;
     const int32_t a = __ldg(t.table + kSlotAdapter + slot);
     if (!adapter_finite(p.not_finite, a, p.splits)) return p.adapter_rows;
-    const int32_t j = q - slot * p.v_cols;
-    return a * p.rank + (j >= p.rank ? j - p.rank : j);
+    return a * p.rank + (q - slot * p.v_cols) % p.rank;
   }
   static __device__ __forceinline__ void extension_load(const TileMaps& maps, const Params& p, const Tile& t, int piece,
                                                         int32_t row, uint32_t b, uint32_t bar) {
@@ -463,7 +465,7 @@ struct LoraExpand {
           const __nv_bfloat16* vr = p.v + static_cast<int64_t>(row + w.lane) * p.v_cols;
           for (int32_t q = 0; q < p.v_cols; ++q) {
             const float f = __bfloat162float(__ldg(vr + q));
-            const __nv_bfloat16* br = p.b + (static_cast<int64_t>(early.loner) * p.rank + (q >= p.rank ? q - p.rank : q)) * p.width;
+            const __nv_bfloat16* br = p.b + (static_cast<int64_t>(early.loner) * p.rank + q % p.rank) * p.width;
 #pragma unroll
             for (int h = 0; h < 32; ++h) {
               const int32_t c = col + part * 32 + h;
@@ -676,7 +678,7 @@ LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t rank, int32_t 
     return s;
   }
   s.row_tiles = (num_tokens + kTileRows - 1) / kTileRows;
-  s.parts = out_fp32 ? 2 : 1;
+  s.parts = out_fp32 ? 3 : 1;
   s.total_steps = (d_model + kTileStep - 1) / kTileStep;
   // Parts of D for few row tiles: up to a block per SM, each of at least 4 K steps.
   s.splits = 1;

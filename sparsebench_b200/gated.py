@@ -21,7 +21,7 @@ from sparsebench_b200 import _C
 class GatedSaved:
     """What moe_forward_gated_saved keeps for moe_backward_gated: the inputs by reference (the gates and
     weights must still hold the same values then) and, in one buffer, the layout, x and Y in its order and the blocks of
-    H, G and U (rows * (2 D + 3 F) bf16). state is None for an empty batch."""
+    H, G and U (rows * (6 D + 6 F) bytes). state is None for an empty batch."""
 
     x: torch.Tensor
     expert_weight: torch.Tensor
@@ -72,7 +72,8 @@ def moe_forward_gated(
 ) -> torch.Tensor:
     """x [T, D], expert_idx / expert_weight [T, k], w_gate and w_up [E, D, F], w_down [E, F, D] -> [T, D]; bf16 (gates
     bf16 or fp32), fp32 accumulation inside the kernels, D and F multiples of 128. activation: "silu" (SwiGLU experts)
-    or "gelu" (erf form). An expert id outside [0, E) is skipped, as in moe_forward."""
+    or "gelu" (erf form). An expert id outside [0, E) is skipped, as in moe_forward. Keeps
+    nothing for a gradient: see moe_gated."""
     return _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, False)[0]
 
 
