@@ -8,7 +8,8 @@
 //
 // The forward keeps X (rows in layout order), G, U, H and Y. What is an operand of a product is bf16, as the weights are:
 // H, w dO, dG and dU are each rounded once, and so are G and U, which the backward pass reads back (in fp32 they would be
-// most of its traffic). Y, the rows of dx, all sums, the activation and its derivative are in fp32. dgate takes Y, not H dH / w, which a gate of 0 would spoil.
+// most of its traffic). Y, the rows of dx, all sums, the activation and its derivative are in fp32. dgate takes Y, not
+// H dH / w, which a gate of 0 would spoil.
 //
 // A decoding step (at most 64 copies, nothing kept) takes another way: no layout, the weights of the picked experts
 // streamed by the kernels of skinny.cuh (SkinnyUp, SkinnyDown, gated_small_combine_kernel).
@@ -124,7 +125,7 @@ __device__ __forceinline__ void load_rows(uint32_t a, const CUtensorMap* all, co
 // Padding rows of x are loaded as the zeros they are: multiplying zeros takes less of the power limit, which sets the clock
 // of a longer run, than what a stage happens to hold (395 against 406 us a pass of the layer below, one after another).
 // Bound by the weights' way from memory where experts have few rows (T = 4096, D = 1024, F = 4096, E = 64: 1.07 GB of
-// weights in 194 us, 5.5 TB/s of a measured 6.56 copy peak; 238 us with G and U kept) and by the tensor cores where they
+// weights in 196 us, 5.5 TB/s of a measured 6.56 copy peak; 234 us with G and U kept) and by the tensor cores where they
 // have many (T = 4096, D = 4096, F = 14336, E = 8: 1.45 ms, 1490 TFLOP/s executed, at the clock that the power limit leaves).
 struct GatedUp {
   struct Params {
@@ -813,7 +814,7 @@ gated_join_kernel(const float4* __restrict__ dx_rows, const int32_t* __restrict_
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-// Size rules all the products of the gated layer share. Sets *ffn_blocks.
+// Size rules all the products of the gated layer share.
 int check_gated(const char* what, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
                 int32_t activation) {
   if (d_model <= 0 || d_model % 128 != 0) return fail(SB_ERR_INVALID_ARGUMENT, "%s: D (%d) must be a positive multiple of 128", what, d_model);

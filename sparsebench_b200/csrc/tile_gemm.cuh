@@ -1,5 +1,6 @@
 // A persistent tcgen05 matmul kernel whose tiles, operand loads and epilogue come from a policy class; the matmuls
-// of the gated expert layer and of its backward pass (gated.cu) are policies of it.
+// of the gated expert layer and of its backward pass (gated.cu) and of the projection with adapters (lora.cu) are
+// policies of it.
 //
 // One output tile = 128 rows x 256 columns, accumulated in fp32 in TMEM (two accumulators, so the epilogue of one
 // tile runs while the tensor cores fill the other). K steps of 64. Warp roles, with nothing but mbarriers between
@@ -86,8 +87,10 @@ __device__ __forceinline__ void load_packed_x64(uint32_t taddr, uint32_t (&packe
 
 // A policy Op has
 //   Params, Tile (with int32_t k_steps: 0 = nothing to multiply; bool live: the epilogue has something to do)
-//   static constexpr bool kAMnMajor, kBMnMajor
-//   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar), tx_bytes
+//   static constexpr bool kAMnMajor, kBMnMajor, kAhead, kVariable, kExtension
+//   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar)
+//   prefetch(p, tile, w) -> Early: global loads that can start before the accumulator is ready; then
+//   epilogue(maps, p, tile, w, early). With kAhead: ahead(p, next tile, w) between the two.
 //   static constexpr int kStages (of the ring), kEpilogueWarps, kBuffers (staging tiles of each, may be 0)
 //   With kExtension: Tile has base_steps; four warps fill the stages of the K steps behind them. A from registers:
 //   Rows rows(p, tile, row0) once per tile, extension_chunk(p, tile, rows, j, row, ks, chunk) = the 16 bytes of chunk
