@@ -11,7 +11,7 @@
 // most of its traffic). Y, the rows of dx, all sums, the activation and its derivative are in fp32. dgate takes Y, not
 // H dH / w, which a gate of 0 would spoil.
 //
-// A decoding step (at most 64 copies, nothing kept) takes another way: no layout, the weights of the picked experts
+// A decoding step (at most 128 copies, nothing kept) takes another way: no layout, the weights of the picked experts
 // streamed by the kernels of skinny.cuh (SkinnyUp, SkinnyDown, gated_small_combine_kernel).
 //
 // act is SiLU, v / (1 + exp(-v)), or the erf form of GELU.
@@ -524,7 +524,8 @@ struct ExpertItem { int32_t expert, tile, rows; };
 // False: fewer distinct experts than block items. list: the expert's copies, ascending.
 __device__ __forceinline__ bool find_expert(const void* expert_idx, int idx_is_i64, int32_t copies, int32_t num_experts,
                                             int32_t which, ExpertItem& item, int32_t* ids, int32_t* list) {
-  __shared__ int32_t count[4];
+  constexpr int kWarps = kSkinnyMaxRows / 32;
+  __shared__ int32_t lead_count[kWarps], match_count[kWarps];
   __shared__ int32_t found;
   const int c = static_cast<int>(threadIdx.x);
   int32_t mine = -1;
@@ -536,21 +537,39 @@ __device__ __forceinline__ bool find_expert(const void* expert_idx, int idx_is_i
   if (c < kSkinnyMaxRows) ids[c] = mine;
   __syncthreads();
   bool leads = mine >= 0;
-  for (int j = 0; leads && j < c; ++j) leads = ids[j] != mine;
-  const unsigned lead_mask = __ballot_sync(0xffffffffu, leads);
-  if (c < kSkinnyMaxRows && (c & 31) == 0) count[c >> 5] = __popc(lead_mask);
-  __syncthreads();
+  int j = 0;
+  for (; leads && j + 4 <= c; j += 4) {
+    const int4 four = *reinterpret_cast<const int4*>(ids + j);
+    leads = four.x != mine && four.y != mine && four.z != mine && four.w != mine;
+  }
+  for (; leads && j < c; ++j) leads = ids[j] != mine;
+  const int warp = c >> 5;
   const unsigned below = (1u << (c & 31)) - 1u;
-  if (leads && __popc(lead_mask & below) + (c >= 32 ? count[0] : 0) == which) found = mine;
-  if (which >= count[0] + count[1]) return false;
+  const unsigned lead_mask = __ballot_sync(0xffffffffu, leads);
+  if (warp < kWarps && (c & 31) == 0) lead_count[warp] = __popc(lead_mask);
+  __syncthreads();
+  int32_t distinct = 0, before = __popc(lead_mask & below);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += lead_count[w];
+    distinct += lead_count[w];
+  }
+  if (leads && before == which) found = mine;
+  if (which >= distinct) return false;
   __syncthreads();
   item.expert = found;
   const bool match = c < kSkinnyMaxRows && mine == item.expert;
   const unsigned match_mask = __ballot_sync(0xffffffffu, match);
-  if (c < kSkinnyMaxRows && (c & 31) == 0) count[2 + (c >> 5)] = __popc(match_mask);
+  if (warp < kWarps && (c & 31) == 0) match_count[warp] = __popc(match_mask);
   __syncthreads();
-  if (match) list[__popc(match_mask & below) + (c >= 32 ? count[2] : 0)] = c;
-  item.rows = count[2] + count[3];
+  int32_t place = __popc(match_mask & below);
+  item.rows = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) place += match_count[w];
+    item.rows += match_count[w];
+  }
+  if (match) list[place] = c;
   return true;  // the caller's next barrier publishes the list
 }
 
@@ -1016,9 +1035,9 @@ bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) 
 int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
 // The two ways of the forward pass. The decoding way needs no layout and splits K over clusters; it starts a block per
-// 64 (128) weight columns of every picked expert. From 65 copies on (and wherever the backward pass needs the layout's
+// 64 (128) weight columns of every picked expert. From 129 copies on (and wherever the backward pass needs the layout's
 // blocks) the persistent kernels of the layout are at least as fast.
-constexpr int64_t kSmallCopies = 64;
+constexpr int64_t kSmallCopies = 128;
 
 // Parts of the buffers, in bytes from their start.
 struct GatedBuffers {

@@ -29,6 +29,10 @@
 namespace sb {
 namespace {
 
+// Up to here a batch is a decoding step.
+constexpr int64_t kSmallTokens = 64;
+static_assert(kSmallTokens <= kSkinnyMaxRows, "rows of the skinny kernel");
+
 constexpr int kMaxSlots = kTileRows;
 // Per tile: the slot count, the adapter of each slot, the slot of each row (-1: none).
 constexpr int kSlotAdapter = 1, kRowSlot = kSlotAdapter + kMaxSlots;
@@ -672,7 +676,7 @@ int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
 LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t rank, int32_t num_adapters, int out_fp32, int sm_count) {
   LoraSizes s{};
-  if (num_tokens <= kSkinnyMaxRows) {
+  if (num_tokens <= kSmallTokens) {
     s.v = align256(num_tokens * rank * 4);
     s.total = s.v;
     return s;
@@ -734,7 +738,7 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
     return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: the workspace has %lld bytes, %lld are needed",
                 (long long)workspace_bytes, (long long)s.total);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (num_tokens <= kSkinnyMaxRows)
+  if (num_tokens <= kSmallTokens)
     return lora_small(x, weight, lora_a, lora_b, adapter_idx, idx_is_i64, scale, out, out_fp32, static_cast<int32_t>(num_tokens),
                       d_model, width, rank, num_adapters, reinterpret_cast<float*>(ws), info, dev_status, as_stream(stream));
   int32_t* tables = reinterpret_cast<int32_t*>(ws);

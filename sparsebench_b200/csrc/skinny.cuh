@@ -2,7 +2,7 @@
 // projection with adapters (lora.cu).
 //
 // With few rows the weights are all that moves, so they take the 128-row side of the tensor-core tile: M = 128 weight
-// columns, N = the rows (16 to 64, in steps of 16), K = 64 per stage. A weight tile [64 k x 128 columns] is the MN-major
+// columns, N = the rows (16 to 128, in steps of 16), K = 64 per stage. A weight tile [64 k x 128 columns] is the MN-major
 // operand it is in memory, the rows are the K-major one. One thread block per 128 columns would leave most SMs without
 // work, so K is split over the thread blocks of a cluster: each leaves its sums in its shared memory and the blocks add
 // them up over distributed shared memory in rank order, each for its share of the rows. No atomics, no workspace.
@@ -29,7 +29,7 @@ constexpr int kSkinnyWorkers = 128;   // threads of warps 2-5
 constexpr int kSkinnyCols = 128;
 constexpr int kSkinnyStep = 64;
 constexpr int kSkinnyWBytes = kSkinnyCols * kSkinnyStep * 2;
-constexpr int kSkinnyMaxRows = 64;
+constexpr int kSkinnyMaxRows = 128;
 
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");

@@ -2,7 +2,7 @@
 
     out[t] = sum over the token's picks of gate * (act(x w_gate[e]) * (x w_up[e])) w_down[e]
 
-Routing, the gated SDD, DSD and the combine as in moe_forward; a decoding step (at most 64 token copies) streams the picked
+Routing, the gated SDD, DSD and the combine as in moe_forward; a decoding step (at most 128 token copies) streams the picked
 experts' weights without a layout. The backward pass is a call of its own (moe_backward_gated), so that a training step can
 be captured into a CUDA graph as it is; moe_gated() wraps the two for torch.autograd. No host sync anywhere.
 """
