@@ -330,12 +330,10 @@ ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
 def _check_activation(activation: str) -> int:
-    _check(activation in ACTIVATIONS, f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    return ACTIVATIONS[activation]
-
-
-def _bf16_on(index: int, t: torch.Tensor) -> bool:
-    return t.dtype is torch.bfloat16 and t.get_device() == index and t.is_contiguous()
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise RuntimeError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    return code
 
 
 def _check_bf16(device: torch.device, **tensors: torch.Tensor) -> None:
@@ -353,6 +351,17 @@ _same_device = contextlib.nullcontext()
 def _on(index: int):
     """torch.cuda.device(index), which costs microseconds, only where another device is current."""
     return _same_device if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _status_ptr(index: int) -> int:
+    """Address of the device's status word; 0 (none) for a first call under graph capture, whose allocations are the
+    graph's."""
+    status = _dev_status.get(index)
+    if status is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        status = device_status(torch.device("cuda", index))
+    return status.data_ptr()
 
 
 def _raw_stream(index: int) -> int:
@@ -401,8 +410,11 @@ def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, ro
 def _check_gated_layer(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
                        w_up: torch.Tensor, w_down: torch.Tensor, activation: str) -> int:
     index = x.get_device()
-    if not (index >= 0 and _bf16_on(index, x) and _bf16_on(index, w_gate) and _bf16_on(index, w_up)
-            and _bf16_on(index, w_down)):
+    bf16 = torch.bfloat16
+    if not (index >= 0 and x.dtype is bf16 and x.is_contiguous()
+            and w_gate.dtype is bf16 and w_gate.get_device() == index and w_gate.is_contiguous()
+            and w_up.dtype is bf16 and w_up.get_device() == index and w_up.is_contiguous()
+            and w_down.dtype is bf16 and w_down.get_device() == index and w_down.is_contiguous()):
         _check(x.is_cuda, "x must be a CUDA tensor")
         _check_bf16(x.device, x=x, w_gate=w_gate, w_up=w_up, w_down=w_down)
     for name, t, dtypes, text in (("expert_idx", expert_idx, (torch.int64, torch.int32), "int32 or int64"),
@@ -421,21 +433,24 @@ def moe_gated_forward_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_wei
     Shapes are the caller's to check; T * k must be positive."""
     lib = _lib.load()
     code = _check_gated_layer(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
-    device = x.device
-    index = device.index
+    index = x.get_device()
     num_tokens, k = expert_idx.shape
     num_experts, d_model, ffn_dim = w_gate.shape
     with _on(index):
         sizes = (ctypes.c_int64 * 3)()
-        _lib.check(lib.sb_moe_gated_bytes(num_tokens, k, d_model, ffn_dim, num_experts, int(keep), sizes))
+        status = lib.sb_moe_gated_bytes(num_tokens, k, d_model, ffn_dim, num_experts, keep, sizes)
+        if status != 0:
+            _lib.check(status)
         out = torch.empty_like(x)
-        state = torch.empty(sizes[0], dtype=torch.uint8, device=device) if keep else None
-        scratch = torch.empty(sizes[1], dtype=torch.uint8, device=device)
-        _lib.check(lib.sb_moe_gated_forward(
-            x.data_ptr(), expert_idx.data_ptr(), int(expert_idx.dtype == torch.int64), expert_weight.data_ptr(),
-            int(expert_weight.dtype == torch.float32), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+        state = x.new_empty(sizes[0], dtype=torch.uint8) if keep else None
+        scratch = x.new_empty(sizes[1] // 2)
+        status = lib.sb_moe_gated_forward(
+            x.data_ptr(), expert_idx.data_ptr(), expert_idx.dtype is torch.int64, expert_weight.data_ptr(),
+            expert_weight.dtype is torch.float32, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
             out.data_ptr(), num_tokens, k, d_model, ffn_dim, num_experts, code, state.data_ptr() if keep else None,
-            sizes[0], scratch.data_ptr(), sizes[1], device_status(device).data_ptr(), _raw_stream(index)))
+            sizes[0], scratch.data_ptr(), sizes[1], _status_ptr(index), _raw_stream(index))
+        if status != 0:
+            _lib.check(status)
     return out, state
 
 
@@ -459,7 +474,7 @@ def moe_gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weig
             grad_out.data_ptr(), expert_weight.data_ptr(), int(expert_weight.dtype == torch.float32),
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), state.data_ptr(), state.numel(),
             *(g.data_ptr() for g in grads), num_tokens, k, d_model, ffn_dim, num_experts, code, scratch.data_ptr(), sizes[2],
-            device_status(device).data_ptr(), _raw_stream(index)))
+            _status_ptr(index), _raw_stream(index)))
     return grads
 
 
@@ -470,8 +485,11 @@ def lora_linear_cuda(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor
     """out [T, N] = x @ weight + scale[a] * (x @ lora_a[a]^T) @ lora_b[a] with a = adapter_idx[t] per token."""
     lib = _lib.load()
     index = x.get_device()
-    if not (index >= 0 and _bf16_on(index, x) and _bf16_on(index, weight) and _bf16_on(index, lora_a)
-            and _bf16_on(index, lora_b)):
+    bf16 = torch.bfloat16
+    if not (index >= 0 and x.dtype is bf16 and x.is_contiguous()
+            and weight.dtype is bf16 and weight.get_device() == index and weight.is_contiguous()
+            and lora_a.dtype is bf16 and lora_a.get_device() == index and lora_a.is_contiguous()
+            and lora_b.dtype is bf16 and lora_b.get_device() == index and lora_b.is_contiguous()):
         _check(x.is_cuda, "x must be a CUDA tensor")
         _check_bf16(x.device, x=x, weight=weight, lora_a=lora_a, lora_b=lora_b)
     x_shape, w_shape, a_shape, b_shape = x.shape, weight.shape, lora_a.shape, lora_b.shape
@@ -490,20 +508,20 @@ def lora_linear_cuda(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor
         _check(scale.get_device() == index and scale.dtype is torch.float32 and scale.dim() == 1 and
                scale.numel() == num_adapters and scale.is_contiguous(),
                "scale must be a contiguous float32 [L] tensor on x's GPU")
-    _check(out_dtype is torch.bfloat16 or out_dtype is torch.float32, f"out_dtype must be bfloat16 or float32, got {out_dtype}")
-    fp32 = int(out_dtype is torch.float32)
-    device = x.device
+    _check(out_dtype is torch.bfloat16 or out_dtype is torch.float32, "out_dtype must be bfloat16 or float32")
+    fp32 = out_dtype is torch.float32
     with _on(index):
         nbytes = lib.sb_lora_workspace_bytes(num_tokens, d_model, width, rank, num_adapters, fp32)
         if nbytes < 0:
             _lib.check(1)
-        out = torch.empty((num_tokens, width), dtype=out_dtype, device=device)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        out = x.new_empty((num_tokens, width), dtype=out_dtype) if fp32 else x.new_empty((num_tokens, width))
+        work = x.new_empty(nbytes // 2)
         status = lib.sb_lora_linear(x.data_ptr(), weight.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(),
-                                    adapter_idx.data_ptr(), int(wide), None if scale is None else scale.data_ptr(),
+                                    adapter_idx.data_ptr(), wide, None if scale is None else scale.data_ptr(),
                                     out.data_ptr(), fp32, num_tokens, d_model, width, rank, num_adapters, work.data_ptr(),
-                                    nbytes, device_status(device).data_ptr(), _raw_stream(index))
-        _lib.check(status)
+                                    nbytes, _status_ptr(index), _raw_stream(index))
+        if status != 0:
+            _lib.check(status)
     return out
 
 
