@@ -75,7 +75,7 @@ struct ShrinkParams {
   int32_t idx_is_i64, num_tokens, num_adapters, rank, parts, splits, steps, total_steps, stages;
   int32_t b_vecs;  // 16-byte pieces of an adapter's B
 };
-constexpr int kShrinkHeadBytes = 512 + 4 * (4 * kTileRows + 8);  // barriers, ids, slots, first rows, seen, counts
+constexpr int kShrinkHeadBytes = 512 + 4 * (5 * kTileRows + 8);  // barriers, ids, slots, first rows, seen, new slots, counts
 
 inline int shrink_smem_bytes(int stages, int rank) { return 1024 + kShrinkHeadBytes + stages * kShrinkStageBytes + kTileRows * rank * 4; }
 
@@ -105,7 +105,8 @@ lora_shrink_kernel(const __grid_constant__ ShrinkMaps maps, const __grid_constan
   int32_t* slot_adapter = id + kTileRows;
   int32_t* work = slot_adapter + kTileRows;  // slot of the first row of an adapter; then: slot of each row
   int32_t* seen = work + kTileRows;          // the slot's adapter is in the tile before, too
-  int32_t* count = seen + kTileRows;         // [4] per worker warp
+  int32_t* fresh_slot = seen + kTileRows;    // the slots whose adapter is not
+  int32_t* count = fresh_slot + kTileRows;   // [4] per worker warp
   float* red = reinterpret_cast<float*>(smem_aligned + (red_base - smem_base));
 
   const int warp = static_cast<int>(threadIdx.x >> 5);
@@ -249,18 +250,33 @@ lora_shrink_kernel(const __grid_constant__ ShrinkMaps maps, const __grid_constan
           if (slot_adapter[s] == before) seen[s] = 1;
     }
     named_barrier(2, kScanThreads);
+    // The slots that are new, in slot order, and the flag of each: both in `seen`, whose entry of a slot in front has been
+    // read by everybody before it is written again.
+    int32_t fresh = 0, nth = -1;
+    for (int32_t s = 0; s < slots; ++s) {
+      if (s == i && seen[s] == 0) nth = fresh;
+      fresh += seen[s] == 0 ? 1 : 0;
+    }
+    named_barrier(2, kScanThreads);
+    if (nth >= 0) fresh_slot[nth] = i;
+    if (i < kTileRows) seen[i] = 0;
+    named_barrier(2, kScanThreads);
+    // The warps are shared out over the new slots: several to one slot where there are few, one after another where many.
+    constexpr int kScanWarps = kScanThreads / 32;
     const int32_t per_part = (p.b_vecs + p.splits - 1) / p.splits;
     const int32_t end = min(p.b_vecs, (rank + 1) * per_part);
-    for (int32_t s = 0; s < slots; ++s) {
-      if (seen[s] != 0) continue;
-      const int32_t a = slot_adapter[s];
-      const uint4* from = p.b + static_cast<int64_t>(a) * p.b_vecs;
+    const int32_t team = max(1, kScanWarps / max(1, fresh));  // warps of a slot
+    const int32_t teams = kScanWarps / team;
+    const int32_t me = (i >> 5) % team, threads = team * 32;
+    for (int32_t f = (i >> 5) / team; f < fresh; f += teams) {
+      if ((i >> 5) >= team * teams) break;  // warps left over
+      const uint4* from = p.b + static_cast<int64_t>(slot_adapter[fresh_slot[f]]) * p.b_vecs;
       bool bad = false;
-      for (int32_t v0 = rank * per_part + i; v0 < end; v0 += 16 * kScanThreads) {
+      for (int32_t v0 = rank * per_part + me * 32 + lane; v0 < end; v0 += 16 * threads) {
         uint4 raw[16];  // all on their way at once: what bounds this is the latency of the loads
 #pragma unroll
         for (int u = 0; u < 16; ++u)
-          raw[u] = v0 + u * kScanThreads < end ? __ldg(from + v0 + u * kScanThreads) : make_uint4(0u, 0u, 0u, 0u);
+          raw[u] = v0 + u * threads < end ? __ldg(from + v0 + u * threads) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
           const uint32_t words[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
@@ -269,9 +285,10 @@ lora_shrink_kernel(const __grid_constant__ ShrinkMaps maps, const __grid_constan
             bad |= (words[q] & 0x7f80u) == 0x7f80u || (words[q] & 0x7f800000u) == 0x7f800000u;
         }
       }
-      const bool any = named_barrier_or(2, kScanThreads, bad);
-      if (i == 0) p.not_finite[static_cast<int64_t>(a) * kMaxSplits + rank] = any ? 1 : 0;
+      if (bad) seen[f] = 1;
     }
+    named_barrier(2, kScanThreads);
+    if (i < fresh) p.not_finite[static_cast<int64_t>(slot_adapter[fresh_slot[i]]) * kMaxSplits + rank] = seen[i] != 0 ? 1 : 0;
   } else {
     // ---- this block's part of V: TMEM lane = row
     const int quarter = warp & 3;
