@@ -410,7 +410,7 @@ struct LoraExpand {
     const int32_t height = min(kBand, p.row_tiles - band * kBand);
     const int32_t slice = inside / height;
     t.row_tile = band * kBand + inside - slice * height;
-    t.n0 = slice * kTileCols;
+    t.n0 = slice * p.cols;
     t.table = p.tables + static_cast<int64_t>(t.row_tile) * kTableInts;
     t.slots = __ldg(t.table);
     t.base_steps = p.base_steps;
@@ -473,9 +473,9 @@ struct LoraExpand {
     const int32_t row = t.row_tile * kTileRows + w.quarter * 32;
     if (row >= p.num_tokens) return;
     const bool loners = __ballot_sync(0xffffffffu, early.loner >= 0) != 0u;
-    const int32_t end = min(t.n0 + (p.cols > 128 ? (w.part + 1) * 128 : (w.part == 0 ? 128 : 0)), p.width);
+    const int32_t end = min(t.n0 + p.cols, p.width);
 #pragma unroll 1
-    for (int32_t col = t.n0 + w.part * 128; col < end; col += 64) {
+    for (int32_t col = t.n0 + w.part * 64; col < end; col += 128) {
       uint32_t packed[32];
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
@@ -815,7 +815,12 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
   if (int rc = encode_2d_map(&maps.m[2], out, num_tokens, width, 32, out_fp32 ? 32 : 64, out_fp32 ? 4 : 2, "lora_linear (out)")) return rc;
   if (int rc = encode_2d_map(&maps.m[3], x, num_tokens, d_model, kTileRows, 64, 2, "lora_linear (x)")) return rc;
   LoraExpand::Params p{};
-  const int32_t slices = (width + kTileCols - 1) / kTileCols;
+  // Columns of a tile: 256, and fewer where not even a quarter of the SMs has one: a step's bytes come sooner (with four
+  // adapters of rank 16, T = 128, D = N = 4096: 38.9 -> 34.9 us; T = 342, D = 2336, N = 264, 17 adapters: 47.1 -> 35.0 us).
+  // With more tiles than that the rows of x, read once more per tile, cost more (T = 512, D = N = 4096: 41.0 -> 56.8 us).
+  int32_t cols = kTileCols;
+  while (cols > 64 && 4 * s.row_tiles * ((width + cols - 1) / cols) <= info->sm_count) cols /= 2;
+  const int32_t slices = (width + cols - 1) / cols;
   p.row_tiles = row_tiles;
   p.slices = slices;
   p.tables = tables;
@@ -829,7 +834,7 @@ extern "C" int sb_lora_linear(const void* x, const void* weight, const void* lor
   p.v_cols = rank * s.parts;
   p.base_steps = s.total_steps;
   p.adapter_rows = num_adapters * rank;
-  p.cols = width >= kTileCols ? kTileCols : (width + 15) & ~15;
+  p.cols = width >= cols ? cols : (width + 15) & ~15;
   p.out_fp32 = out_fp32 ? 1 : 0;
   return launch_tile_gemm<LoraExpand>(maps, p, static_cast<int64_t>(row_tiles) * slices, dev_status, st, "lora_linear (expand)");
 }

@@ -68,6 +68,25 @@ def test_no_adapter_and_one_for_all(num_tokens, order):
         assert torch.equal(check(x, w, a, b, idx.int(), None), out)
 
 
+@pytest.mark.parametrize("fp32", [False, True], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("width", [648, 2568, 5128])
+def test_columns_of_a_tile(width, fp32):
+    # Two row tiles: few columns have tiles of 64, more have 128, then 256. One adapter's B is not finite in two columns.
+    from sparsebench_b200 import lora_linear
+
+    x, w, a, b, idx, scale = make(130, 72, width, 16, 20, "any", seed=width)
+    want = check(x, w, a, b, idx, scale, fp32)
+    idx[:3] = 4
+    b[4, 2, width - 1] = math.inf
+    b[4, 0, 70] = math.nan
+    got = lora_linear(x, w, a, b, idx, scale, torch.float32 if fp32 else torch.bfloat16)
+    others = idx != 4
+    assert torch.equal(got[others], want[others])
+    bad = torch.zeros(width, dtype=torch.bool, device="cuda")
+    bad[[70, width - 1]] = True
+    assert torch.equal(torch.isfinite(got), others[:, None] | ~bad)
+
+
 @pytest.mark.parametrize("num_tokens", [5, 300])
 def test_more_adapters_in_a_tile_than_one_product_holds(num_tokens):
     # 128 tokens of 128 different adapters of rank 128: 64 groups of two adapters each.
