@@ -920,11 +920,13 @@ int gated_grad_rows_of(const void* grad_out, const void* y_rows, const void* gat
   return check_launch("moe_gated_backward (rows)");
 }
 
-// Columns of a tile: 256, and fewer where that leaves SMs without a tile. A tile of 128 (64) columns moves 1.3 (2) times
-// the operand bytes per result, so only then.
+// Columns of a tile: 256, and fewer where that leaves every second SM without a tile. A tile of 128 (64) columns moves 1.3
+// (2) times the operand bytes per result: halving as soon as one SM has no tile took longer (forward and backward at T = 100,
+// D = 4096, F = 2048, E = 4: 195 against 172 us; T = 179, D = 2688, F = 1536, E = 10: 214 against 200), and so did waiting
+// for three quarters without one (T = 1000, D = F = 1024, E = 4: 90 against 84.5).
 int32_t tile_cols(int64_t num_row_blocks, int32_t width, int sm_count) {
   int32_t cols = kTileCols;
-  while (cols > 64 && num_row_blocks * ((width + cols - 1) / cols) < sm_count) cols /= 2;
+  while (cols > 64 && 2 * num_row_blocks * ((width + cols - 1) / cols) < sm_count) cols /= 2;
   return cols;
 }
 
