@@ -484,9 +484,11 @@ struct LoraExpand {
         ptx::tmem_ld_wait();
         if (loners && early.loner >= 0) {
           const __nv_bfloat16* vr = p.v + static_cast<int64_t>(row + w.lane) * p.v_cols;
-          for (int32_t q = 0; q < p.v_cols; ++q) {
-            const float f = __bfloat162float(__ldg(vr + q));
-            const __nv_bfloat16* br = p.b + (static_cast<int64_t>(early.loner) * p.rank + q % p.rank) * p.width;
+          for (int32_t j = 0; j < p.rank; ++j) {
+            // The parts of V add up to V before they meet B: a part of 0 or of the other sign times infinity is not V's.
+            float f = 0.0f;
+            for (int32_t q = p.v_cols - p.rank + j; q >= 0; q -= p.rank) f += __bfloat162float(__ldg(vr + q));
+            const __nv_bfloat16* br = p.b + (static_cast<int64_t>(early.loner) * p.rank + j) * p.width;
 #pragma unroll
             for (int h = 0; h < 32; ++h) {
               const int32_t c = col + part * 32 + h;

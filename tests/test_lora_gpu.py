@@ -131,6 +131,30 @@ def test_what_is_not_finite_stays_with_its_request(num_tokens, where, bad, fp32)
         assert not torch.isfinite(got[theirs]).any()
 
 
+@pytest.mark.parametrize("fp32", [False, True], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("num_tokens", [3, 50, 260])
+def test_infinities_of_an_adapter_come_out_as_the_definition_has_them(num_tokens, fp32):
+    # An infinite number of B makes the adapter's rows infinite with the sign of x A^T there, whatever the batch size; two
+    # of them with opposite terms, and a NaN, make them NaN. x A^T of these rows is far enough from 0 to have its sign.
+    from sparsebench_b200 import lora_linear
+
+    x, w, a, b, idx, scale = make(num_tokens, 192, 328, 16, 5, "any", seed=2)
+    idx[0] = 3
+    rows = idx == 3
+    v = x[rows].double() @ a[3].double().T
+    v_abs = x[rows].double().abs() @ a[3].double().abs().T
+    b[3, 5, 7] = math.inf
+    b[3, 6, 70] = -math.inf
+    b[3, 5, 200], b[3, 9, 200] = math.inf, -math.inf
+    b[3, 2, 327] = math.nan
+    assert bool((v.abs() > 4 * 192 * 2.0**-24 * v_abs)[:, [2, 5, 6, 9]].all())
+    value, _ = lora_reference(x, w, a, b, idx, scale, fp32)
+    got = lora_linear(x, w, a, b, idx, scale, torch.float32 if fp32 else torch.bfloat16)
+    assert int(torch.isinf(value).sum()) >= 2 * int(rows.sum())
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(got), kind(value)), kind.__name__
+
+
 def test_rows_behind_the_batch_stay_as_they_were():
     import ctypes
 
