@@ -71,6 +71,12 @@ __device__ __forceinline__ bool half_has_rows(const int32_t* row_token, int32_t 
   return __ldg(row_token + static_cast<int64_t>(row_block) * kTileRows + (quarter & 2) * 32) >= 0;
 }
 
+// A lane's row of the tile is no padding. Rows of padding are zeros in X and w dO, and an infinite weight makes NaN of them in
+// H, dG and dU (0 * inf), which the weight gradients would sum up with the rest: they are stored as zeros, whatever came out.
+__device__ __forceinline__ bool row_is_real(const int32_t* row_token, int32_t row_block, const EpilogueWarp& w) {
+  return __ldg(row_token + static_cast<int64_t>(row_block) * kTileRows + w.quarter * 32 + w.lane) >= 0;
+}
+
 // Tile order of the products over (row block, column slice): expert by expert, in an expert bands of up to kBand row
 // blocks, in a band the row block changes fastest. The thread blocks that run at the same time then work on few column
 // slices of one expert's weights for all of its row blocks: a weight tile comes from memory once and from L2 for the
@@ -140,7 +146,10 @@ struct GatedUp {
     int32_t k_steps, row_block, n0, expert, first_block, groups;
     bool live;
   };
-  struct Early { bool store; };
+  struct Early {
+    bool store;
+    bool real;  // this lane's row is no padding
+  };
   static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = true;
@@ -166,8 +175,9 @@ struct GatedUp {
       ptx::tma_load_2d_hint(b + j * TileSmem::kSlabBytes, &maps.m[j >> 1], t.n0 + (j & 1) * 64, row, bar, once);
   }
   static __device__ __forceinline__ Early prefetch(const Params& p, const Tile& t, const EpilogueWarp& w) {
-    if (p.keep) return {half_has_rows(p.row_token, t.row_block, w.quarter)};
-    return {!p.skip_padding || __ldg(p.row_token + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32) >= 0};
+    const bool real = row_is_real(p.row_token, t.row_block, w);
+    if (p.keep) return {half_has_rows(p.row_token, t.row_block, w.quarter), real};
+    return {!p.skip_padding || __any_sync(0xffffffffu, real), real};
   }
   template <int kActivation>
   static __device__ __forceinline__ void product(uint32_t gate, uint32_t up, uint32_t (&packed)[32]) {
@@ -200,6 +210,8 @@ struct GatedUp {
     }
     if (p.activation == SB_ACT_SILU) product<SB_ACT_SILU>(gate, up, packed);
     else product<SB_ACT_GELU>(gate, up, packed);
+#pragma unroll
+    for (int h = 0; h < 32; ++h) packed[h] = early.real ? packed[h] : 0u;
     store_rows_128b<kBuffers>(w, &maps.m[2], packed, col, row);
   }
 };
@@ -226,15 +238,14 @@ struct GradHidden {
   static constexpr int kPart = 16;                // columns at a time: 32 bytes of a row, one sector
   static constexpr int kWarpCols = kCols / 4;     // of the tile's, per epilogue warp
   struct Tile {
-    int32_t k_steps, row_block, n0, expert, first_block, groups;
+    int32_t k_steps, row_block, n0, expert, groups;
     bool live;
   };
   struct Early {
     bool store;
+    bool real;  // no padding
     float gate;
-    const __nv_bfloat16* g;  // this row's columns, as U's and the results' are
-    const __nv_bfloat16* u;
-    int64_t at;
+    int64_t at;  // of this row's columns in G and U, and in the results
     uint32_t first[2][8];  // G and U of the first part
   };
   static constexpr int kStages = 4, kEpilogueWarps = 16, kBuffers = 0;
@@ -249,7 +260,6 @@ struct GradHidden {
     if (!t.live) return t;
     t.n0 = slice * kCols;
     t.groups = (t.groups + 1) & ~1;  // whole halves: their padding rows are stored, as zeros
-    t.first_block = t.row_block * (p.ffn_dim >> 7);
     t.k_steps = p.d_model / kTileStep;
     return t;
   }
@@ -269,12 +279,11 @@ struct GradHidden {
     const int32_t n = t.n0 + w.part * kWarpCols;
     e.store = n < p.ffn_dim && half_has_rows(p.row_token, t.row_block, w.quarter);
     if (!e.store) return e;
+    e.real = row_is_real(p.row_token, t.row_block, w);
     e.gate = __ldg(p.row_gate + static_cast<int64_t>(t.row_block) * kTileRows + w.quarter * 32 + w.lane);
-    e.at = ((static_cast<int64_t>(t.first_block) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128 + (n & 127);
-    e.g = p.g + e.at;
-    e.u = p.u + e.at;
-    ptx::ld_global_v8(e.g, e.first[0]);
-    ptx::ld_global_v8(e.u, e.first[1]);
+    e.at = ((static_cast<int64_t>(t.row_block) * (p.ffn_dim >> 7) + (n >> 7)) * kTileRows + w.quarter * 32 + w.lane) * 128 + (n & 127);
+    ptx::ld_global_v8(p.g + e.at, e.first[0]);
+    ptx::ld_global_v8(p.u + e.at, e.first[1]);
     return e;
   }
   // 32 rows of a block are 8 KB in one piece: the next tile's are asked into L2 before this one is worked on,
@@ -282,7 +291,7 @@ struct GradHidden {
   static __device__ __forceinline__ void ahead(const Params& p, const Tile& next, const EpilogueWarp& w) {
     const int32_t n = next.n0 + w.part * kWarpCols;
     if ((w.part != 0 && (n & 127) != 0) || !next.live || n >= p.ffn_dim || w.lane != 0 || !half_has_rows(p.row_token, next.row_block, w.quarter)) return;
-    const int64_t at = ((static_cast<int64_t>(next.first_block) + (n >> 7)) * kTileRows + w.quarter * 32) * 128;
+    const int64_t at = ((static_cast<int64_t>(next.row_block) * (p.ffn_dim >> 7) + (n >> 7)) * kTileRows + w.quarter * 32) * 128;
     ptx::bulk_prefetch_l2(p.g + at, 32 * 256);
     ptx::bulk_prefetch_l2(p.u + at, 32 * 256);
   }
@@ -294,8 +303,6 @@ struct GradHidden {
   }
   template <int kActivation>
   static __device__ __forceinline__ void work(const Params& p, const EpilogueWarp& w, const Early& early) {
-    __nv_bfloat16* dg_row = p.dg + early.at;
-    __nv_bfloat16* du_row = p.du + early.at;
     uint32_t held[2][2][8];  // G and U of this part and the next
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -307,8 +314,8 @@ struct GradHidden {
       uint32_t s[16];
       ptx::tmem_ld_32x32b_x16(w.taddr + w.part * kWarpCols + part * kPart, s);
       if (part + 1 < kWarpCols / kPart) {
-        ptx::ld_global_v8(early.g + (part + 1) * kPart, held[(part + 1) & 1][0]);
-        ptx::ld_global_v8(early.u + (part + 1) * kPart, held[(part + 1) & 1][1]);
+        ptx::ld_global_v8(p.g + early.at + (part + 1) * kPart, held[(part + 1) & 1][0]);
+        ptx::ld_global_v8(p.u + early.at + (part + 1) * kPart, held[(part + 1) & 1][1]);
       }
       ptx::tmem_ld_wait();
       uint32_t dg[8], du[8];
@@ -321,11 +328,11 @@ struct GradHidden {
         act_and_slope<kActivation>(gf.y, &a1, &d1);
         const float s0 = __uint_as_float(s[2 * h]) * early.gate;
         const float s1 = __uint_as_float(s[2 * h + 1]) * early.gate;
-        dg[h] = pack_bf16(s0 * uf.x * d0, s1 * uf.y * d1);
-        du[h] = pack_bf16(s0 * a0, s1 * a1);
+        dg[h] = early.real ? pack_bf16(s0 * uf.x * d0, s1 * uf.y * d1) : 0u;
+        du[h] = early.real ? pack_bf16(s0 * a0, s1 * a1) : 0u;
       }
-      ptx::st_global_v8(dg_row + part * kPart, dg);
-      ptx::st_global_v8(du_row + part * kPart, du);
+      ptx::st_global_v8(p.dg + early.at + part * kPart, dg);
+      ptx::st_global_v8(p.du + early.at + part * kPart, du);
     }
   }
 };

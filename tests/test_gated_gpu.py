@@ -210,6 +210,23 @@ def test_a_token_with_nan_or_inf_stays_alone():
             assert torch.equal(got[n][untouched], want[n][untouched]), n
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("which", ["w_gate", "w_up", "w_down"])
+@pytest.mark.parametrize(("num_tokens", "d_model", "ffn_dim"), [(140, 128, 256), (70, 384, 640)])
+def test_an_infinite_weight_comes_out_as_the_definition_has_it(num_tokens, d_model, ffn_dim, which, act):
+    # Everything is positive, so no two infinities meet with opposite signs: what the definition makes infinite or NaN has
+    # to be that, and all else finite. The rows of padding (0 times infinity) must not show.
+    x, idx, gate, wg, wu, wd, go = (t if t.dtype == torch.int64 else t.abs() + 0.01 for t in make(num_tokens, d_model, ffn_dim, 4, 2))
+    weights = {"w_gate": wg / 16, "w_up": wu / 16, "w_down": wd / 16}
+    weights[which][1, 5, 9] = math.inf
+    want = gated_reference(x, idx, gate, *weights.values(), act, go)
+    got = step(x, idx, gate, *weights.values(), go, act)
+    assert any(bool(torch.isinf(want[n][0][1]).any()) for n in ("dw_gate", "dw_up", "dw_down"))
+    for name, (value, _) in want.items():
+        for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(kind(got[name]), kind(value)), (name, kind.__name__)
+
+
 def test_memory_left_by_others_does_not_show():
     # Every buffer of the step is torch.empty: with the allocator's memory full of NaN the results are the same.
     args = make(210, 256, 384, 8, 2)
