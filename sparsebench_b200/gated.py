@@ -13,6 +13,7 @@ from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from sparsebench_b200 import _C
 
@@ -130,8 +131,12 @@ def moe_gated(
     w_down: torch.Tensor,
     activation: str = "silu",
 ) -> torch.Tensor:
-    """moe_forward_gated for torch.autograd: differentiable in x, expert_weight and the three weights (once). Its
-    backward pass refuses to run under CUDA graph capture: capture the two explicit calls instead."""
-    if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, expert_weight, w_gate, w_up, w_down)):
+    """moe_forward_gated for torch.autograd: differentiable in x, expert_weight and the three weights (once, and by
+    backward passes: an input that carries a forward-mode tangent is refused). Its backward pass refuses to run under CUDA graph capture: capture the two explicit calls instead."""
+    leaves = (x, expert_weight, w_gate, w_up, w_down)
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in leaves):  # of any dual level; requires_grad is not set there
+        raise NotImplementedError("moe_gated has no forward-mode derivative (make_dual, func.jvp): it is differentiable by "
+                                  "backward passes only")
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in leaves):
         return moe_forward_gated(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)  # nothing to keep
     return _GatedMoE.apply(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)

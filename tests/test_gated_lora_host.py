@@ -2,6 +2,7 @@
 and their oracles against each other."""
 
 import ctypes
+import weakref
 
 import pytest
 import torch
@@ -146,3 +147,55 @@ def test_lora_oracle_row_by_row() -> None:
             want = want + float(scale[i]) * ((a[i] @ x[t]) @ b[i])
         torch.testing.assert_close(got[t], want, rtol=1e-12, atol=1e-12)
     assert bool((bound > 0).all())
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    """The gated layer on the CPU with stand-ins for its two C calls: what Python does around them. Returns the list of
+    (keep, weak reference to the state) of every forward call."""
+    from sparsebench_b200 import _C
+
+    calls = []
+
+    def forward(x, idx, gate, w_gate, w_up, w_down, activation, keep):
+        out = torch.empty_like(x)  # written by a kernel: nothing that autograd could follow
+        out.detach().fill_(1)
+        state = torch.zeros(1000, dtype=torch.uint8) if keep else None
+        calls.append((keep, None if state is None else weakref.ref(state)))
+        return out.detach(), state
+
+    def backward(grad_out, x, gate, w_gate, w_up, w_down, state, activation):
+        assert state.dtype == torch.uint8 and state.numel() == 1000
+        return tuple(torch.ones_like(t) for t in (x, gate, w_gate, w_up, w_down))
+
+    monkeypatch.setattr(_C, "moe_gated_forward_cuda", forward)
+    monkeypatch.setattr(_C, "moe_gated_backward_cuda", backward)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return calls
+
+
+def gated_inputs() -> list[torch.Tensor]:
+    w = torch.zeros(2, 128, 128, dtype=torch.bfloat16)
+    return [torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(4, 1, dtype=torch.int64),
+            torch.ones(4, 1, dtype=torch.bfloat16), w, w, w]
+
+
+@pytest.mark.parametrize("which", [0, 2, 3, 4, 5])
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_derivatives_are_refused(stand_in, which, leaf) -> None:
+    from torch.autograd import forward_ad
+
+    from sparsebench_b200 import moe_gated
+
+    args = gated_inputs()
+    with forward_ad.dual_level():
+        dual = list(args)
+        dual[which] = forward_ad.make_dual(args[which].clone().requires_grad_(leaf), torch.ones_like(args[which]))
+        for mode in (torch.enable_grad, torch.no_grad):  # tangents do not ask for the gradient mode
+            with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                moe_gated(*dual)
+        assert not moe_gated(*args).requires_grad  # others in the same level: as ever
+    primal = args[which]
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: moe_gated(*args[:which], t, *args[which + 1:]), (primal,), (torch.ones_like(primal),))
+    assert [keep for keep, _ in stand_in] == [False]  # nothing was launched for the refused ones
