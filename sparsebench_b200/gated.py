@@ -108,8 +108,10 @@ class _GatedMoE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, expert_idx, expert_weight, w_gate, w_up, w_down, activation):
         out, saved = moe_forward_gated_saved(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
-        ctx.save_for_backward(x, expert_weight, w_gate, w_up, w_down)  # autograd checks them for in-place changes
-        ctx.rest = (activation, saved.state)
+        # Autograd checks the inputs for in-place changes; the state, most of the layer's memory, goes with them: freed
+        # by the backward pass, and in the hands of saved_tensors_hooks (offloading, checkpointing).
+        ctx.save_for_backward(x, expert_weight, w_gate, w_up, w_down, saved.state)
+        ctx.activation = activation
         return out
 
     @staticmethod
@@ -118,7 +120,8 @@ class _GatedMoE(torch.autograd.Function):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the autograd form of the gated layer cannot be captured into a CUDA graph: "
                                "capture moe_forward_gated_saved and moe_backward_gated")
-        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*ctx.saved_tensors, *ctx.rest))
+        *inputs, state = ctx.saved_tensors
+        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*inputs, ctx.activation, state))
         return grads.x, None, grads.expert_weight, grads.w_gate, grads.w_up, grads.w_down, None
 
 

@@ -298,6 +298,29 @@ def test_autograd_form_without_gradients_and_on_an_empty_batch():
     assert empty.grad.shape == (0, 128)
 
 
+def test_autograd_form_offloaded_and_checkpointed():
+    from torch.utils.checkpoint import checkpoint
+
+    from sparsebench_b200 import moe_gated
+
+    x, idx, gate, wg, wu, wd, go = make(140, 256, 384, 4, 2)
+    want = step(x, idx, gate, wg, wu, wd, go, "silu")
+    leaves = [t.clone().requires_grad_() for t in (x, gate, wg, wu, wd)]
+    call = lambda: moe_gated(leaves[0], idx, *leaves[1:])  # noqa: E731
+    with torch.autograd.graph.save_on_cpu():
+        offloaded = call()
+    for out in (offloaded, checkpoint(call, use_reentrant=False)):
+        assert torch.equal(out, want["out"])
+        for n, g in zip(NAMES, torch.autograd.grad(out, leaves, go)):
+            assert torch.equal(g, want[n]), n
+    before = torch.cuda.memory_allocated()
+    out = call()
+    state = torch.cuda.memory_allocated() - before - out.numel() * 2
+    grads = torch.autograd.grad(out, leaves, go)
+    left = torch.cuda.memory_allocated() - before - out.numel() * 2 - sum(g.numel() * 2 for g in grads)
+    assert state > 6 * 128 * 4 * (256 + 384) and left < state / 4  # rows * (6 D + 6 F) bytes, freed while `out` is alive
+
+
 def test_backward_twice_and_two_forwards_at_once():
     from sparsebench_b200 import moe_backward_gated, moe_forward_gated_saved
 

@@ -199,3 +199,31 @@ def test_forward_mode_derivatives_are_refused(stand_in, which, leaf) -> None:
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: moe_gated(*args[:which], t, *args[which + 1:]), (primal,), (torch.ones_like(primal),))
     assert [keep for keep, _ in stand_in] == [False]  # nothing was launched for the refused ones
+
+
+def test_state_is_a_saved_tensor_of_autograd(stand_in) -> None:
+    from torch.utils.checkpoint import checkpoint
+
+    from sparsebench_b200 import moe_gated
+
+    args = gated_inputs()
+    args[0].requires_grad_()
+    out = moe_gated(*args)
+    keep, state = stand_in[-1]
+    assert keep and state() is not None
+    torch.autograd.grad(out, args[0], torch.ones_like(out), retain_graph=True)
+    assert state() is not None
+    out.backward(torch.ones_like(out))
+    assert state() is None  # freed with the other saved tensors, though `out` and its graph are still here
+
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (packed.append(t.dtype), t.clone())[1], lambda t: t):
+        out = moe_gated(*args)
+    assert packed.count(torch.uint8) == 1 and stand_in[-1][1]() is None  # only what the hook made of it is left
+    out.backward(torch.ones_like(out))
+
+    before = len(stand_in)
+    out = checkpoint(moe_gated, *args, use_reentrant=False)
+    assert stand_in[-1][1]() is None  # nothing of the layer is kept until the backward pass runs the forward again
+    out.backward(torch.ones_like(out))
+    assert len(stand_in) == before + 2
