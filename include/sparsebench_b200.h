@@ -61,6 +61,13 @@ const char* sb_version(void);
 int sb_arch_probe(int32_t* out, int64_t n, sb_stream_t stream);
 
 /*
+ * *word = the current device's status word, an int32 in device memory that is 0 when the library is loaded and lasts as
+ * long as the process: what to pass as dev_status below, unless a caller has a word of its own. The same address on every
+ * call. Allocates nothing, enqueues nothing, and may be called while a stream is being captured.
+ */
+int sb_device_status_word(int32_t** word);
+
+/*
  * Worst-case sizes of the routing outputs, computed the way the reference host code does
  * (csrc/routing.cu:213-224): max_row_blocks = (n_copies + num_experts*(block_size-1)) / block_size,
  * max_rows = max_row_blocks * block_size. Returns SB_ERR_INVALID_ARGUMENT where the reference

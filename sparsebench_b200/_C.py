@@ -36,12 +36,24 @@ def _ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None or t.numel() == 0 else t.data_ptr())
 
 
+class _DeviceWord:
+    """An int32 at a fixed address of device memory, for torch.as_tensor."""
+
+    def __init__(self, address: int) -> None:
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "strides": None,
+                                         "version": 3}
+
+
 def device_status(device: torch.device) -> torch.Tensor:
     """int32[1] on `device` that the matmul kernels OR a non-zero code into if one of their bounded
-    device-side waits ever expires. Allocated zeroed on first use; reading it syncs."""
+    device-side waits ever expires. The library's own word, 0 when it is loaded: no memory of torch's
+    allocator, so a first call under graph capture knows it too. Reading it syncs."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     if index not in _dev_status:
-        _dev_status[index] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        word = ctypes.c_void_p()
+        with torch.cuda.device(index):
+            _lib.check(_lib.load().sb_device_status_word(ctypes.byref(word)))
+            _dev_status[index] = torch.as_tensor(_DeviceWord(word.value), device=torch.device("cuda", index))
     return _dev_status[index]
 
 
@@ -354,14 +366,9 @@ def _on(index: int):
 
 
 def _status_ptr(index: int) -> int:
-    """Address of the device's status word; 0 (none) for a first call under graph capture, whose allocations are the
-    graph's."""
+    """Address of the device's status word."""
     status = _dev_status.get(index)
-    if status is None:
-        if torch.cuda.is_current_stream_capturing():
-            return 0
-        status = device_status(torch.device("cuda", index))
-    return status.data_ptr()
+    return (device_status(torch.device("cuda", index)) if status is None else status).data_ptr()
 
 
 def _raw_stream(index: int) -> int:

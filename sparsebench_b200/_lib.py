@@ -22,6 +22,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sb_status_string": (c_char_p, [c_int]),
     "sb_version": (c_char_p, []),
     "sb_arch_probe": (c_int, [_P, c_int64, _P]),
+    "sb_device_status_word": (c_int, [_P]),
     "sb_route_sizes": (c_int, [c_int64, c_int32, c_int64, c_int64, _P, _P, _P]),
     "sb_route_workspace_bytes": (c_size_t, [c_int64, c_int32]),
     "sb_route": (c_int, [_P, c_int, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,

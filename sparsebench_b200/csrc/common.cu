@@ -13,6 +13,9 @@ std::mutex g_device_mutex;
 DeviceInfo g_device_info[kMaxDevices];
 bool g_device_known[kMaxDevices] = {};
 
+// One per device, 0 when the library is loaded there; a part of the module, so that asking for it allocates nothing.
+__device__ int32_t g_status_word;
+
 __global__ void arch_probe_kernel(int32_t* __restrict__ out, int64_t n) {
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += stride) {
@@ -96,6 +99,21 @@ int sb_arch_probe(int32_t* out, int64_t n, sb_stream_t stream) {
   if (blocks > 4096) blocks = 4096;  // grid-stride loop covers the rest
   sb::arch_probe_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, sb::as_stream(stream)>>>(out, n);
   return sb::check_launch("arch_probe");
+}
+
+int sb_device_status_word(int32_t** word) {
+  sb::clear_error();
+  if (word == nullptr) return sb::fail(SB_ERR_INVALID_ARGUMENT, "device_status_word: NULL output");
+  // Looking the address up may load the module, which a stream capture of this thread must not take for a part of it.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t err = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (err == cudaSuccess) {
+    err = cudaGetSymbolAddress(reinterpret_cast<void**>(word), sb::g_status_word);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (err == cudaSuccess) err = back;
+  }
+  if (err != cudaSuccess) return sb::fail(SB_ERR_CUDA, "device_status_word: %s", cudaGetErrorString(err));
+  return SB_OK;
 }
 
 }  // extern "C"

@@ -77,6 +77,10 @@ def test_gated_calls_are_refused_before_any_launch(lib) -> None:
     assert lib.sb_sdd_gated(*args, 10, 128, 128, 4, 0, 0, 0, None, None) == 0  # no row blocks: nothing to do
 
 
+def test_status_word_is_refused_without_a_place_for_it(lib) -> None:
+    assert lib.sb_device_status_word(None) == 1 and b"NULL" in lib.sb_last_error()
+
+
 @pytest.mark.parametrize(("sizes", "text"), [
     ((-1, 64, 64, 8, 2), b"31 bits"),
     ((10, 60, 64, 8, 2), b"D (60)"),
