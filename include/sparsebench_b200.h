@@ -411,7 +411,7 @@ int sb_ep_sdd_dispatch(const void* recv_rows, const void* w1, const int32_t* row
  *
  * sb_sdd_gated: h_blocks = act(x[row_token] . w_gate[e]) * (x[row_token] . w_up[e]) in one matmul kernel, on sb_route's
  * layout at block size 128, laid out like sb_sdd's blocks; the down projection is sb_dsd. x_rows: scratch for
- * [num_row_blocks * 128, D] bf16, x in layout order (padding rows 0). skip_padding_rows works as in sb_sdd.
+ * [num_row_blocks * 128, D] bf16, x in layout order (0 in padding rows and in rows whose token is not in [0, num_tokens)). skip_padding_rows works as in sb_sdd.
  *
  * sb_moe_gated_bytes: bytes[0] of the state, bytes[1] of the forward's scratch, bytes[2] of the backward's; keep = 0: for
  * a forward pass alone (no state). Nothing in these buffers has to be set; they are 256-byte aligned.

@@ -389,7 +389,8 @@ def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, ro
                    row_block_expert: torch.Tensor, padded_offsets: torch.Tensor, tokens_per_expert: torch.Tensor,
                    num_nnz: int, activation: str, skip_padding_rows: bool = False) -> torch.Tensor:
     """Blocks [num_nnz, 128, 128] = act(x[row_token] @ w_gate[expert]) * (x[row_token] @ w_up[expert]) on the layout's
-    blocks. Dead row blocks are left unwritten, with skip_padding_rows 32-row groups of padding too."""
+    blocks. Dead row blocks are left unwritten, with skip_padding_rows 32-row groups of padding too. Rows of tokens that x
+    does not have (a layout of a larger batch) count as rows of zeros."""
     lib = _lib.load()
     _check_gated_weights(x, w_gate, w_up)
     code = _check_activation(activation)

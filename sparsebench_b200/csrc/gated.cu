@@ -725,11 +725,12 @@ gated_combine_kernel(const float4* __restrict__ y, const int32_t* __restrict__ c
   }
 }
 
-// One warp per row of the layout: x_rows[r] = x[token], zeros for padding (the rows that the products' TMA loads want side
-// by side; gathering them inside the products with cp.async took a quarter of their time instead).
+// One warp per row of the layout: x_rows[r] = x[token], zeros for padding and for tokens that x does not have (with the
+// layout of a larger batch nothing is read past x). The products' TMA loads want the rows side by side; gathering them inside
+// the products with cp.async took a quarter of their time instead.
 __global__ void __launch_bounds__(kSmallThreads)
 gated_rows_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ row_token, const int32_t* __restrict__ num_rows,
-                  uint4* __restrict__ x_rows, int32_t vecs) {
+                  uint4* __restrict__ x_rows, int32_t num_tokens, int32_t vecs) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   const int lane = static_cast<int>(threadIdx.x & 31);
@@ -737,10 +738,11 @@ gated_rows_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ row_t
   const int32_t warps = static_cast<int32_t>(gridDim.x * (kSmallThreads / 32));
   for (int32_t r = static_cast<int32_t>(blockIdx.x * (kSmallThreads / 32) + (threadIdx.x >> 5)); r < rows; r += warps) {
     const int32_t token = __ldg(row_token + r);
+    const bool real = token >= 0 && token < num_tokens;
     uint4* dst = x_rows + static_cast<int64_t>(r) * vecs;
-    const uint4* src = x + static_cast<int64_t>(max(token, 0)) * vecs;
+    const uint4* src = x + static_cast<int64_t>(real ? token : 0) * vecs;
 #pragma unroll 4
-    for (int32_t v = lane; v < vecs; v += 32) dst[v] = token >= 0 ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
+    for (int32_t v = lane; v < vecs; v += 32) dst[v] = real ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -886,7 +888,7 @@ int launch_small(void (*kernel)(Params...), int64_t blocks, int threads, cudaStr
 // x_rows, then H (and G, U) on the layout.
 int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t* row_token, const int32_t* row_block_expert,
               const int32_t* padded_offsets, const int32_t* tokens_per_expert, void* x_rows, void* h_blocks, void* g_blocks,
-              void* u_blocks, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
+              void* u_blocks, int64_t num_tokens, int32_t d_model, int32_t ffn_dim, int32_t num_experts, int32_t num_row_blocks,
               int32_t activation, int skip_padding_rows, int32_t* dev_status, cudaStream_t stream) {
   const DeviceInfo* info = current_device_info();
   if (info == nullptr) return SB_ERR_CUDA;
@@ -903,7 +905,8 @@ int sdd_gated(const void* x, const void* w_gate, const void* w_up, const int32_t
   if (int rc = encode_2d_map(&maps.m[5], x_rows, static_cast<uint64_t>(num_row_blocks) * kTileRows, d_model, 128, 64, 2, "sdd_gated (rows)")) return rc;
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(num_row_blocks) * (kTileRows / 8), info->sm_count * 8);
   if (int rc = launch_small(gated_rows_kernel, blocks, kSmallThreads, stream, "sdd_gated (rows)", static_cast<const uint4*>(x),
-                            row_token, padded_offsets + num_experts, static_cast<uint4*>(x_rows), d_model / 8))
+                            row_token, padded_offsets + num_experts, static_cast<uint4*>(x_rows),
+                            static_cast<int32_t>(std::min<int64_t>(num_tokens, INT32_MAX)), d_model / 8))
     return rc;
   GatedUp::Params p{};
   p.order = {row_block_expert, padded_offsets, tokens_per_expert, num_experts, ffn_dim / 128};
@@ -1190,7 +1193,7 @@ extern "C" int sb_sdd_gated(const void* x, const void* w_gate, const void* w_up,
   if (any_misaligned({x, w_gate, w_up, x_rows, h_blocks}))
     return fail(SB_ERR_INVALID_ARGUMENT, "sdd_gated: x, the weights, the rows and the blocks must be 16-byte aligned");
   return sdd_gated(x, w_gate, w_up, row_token, row_block_expert, padded_offsets, tokens_per_expert, x_rows, h_blocks,
-                   nullptr, nullptr, d_model, ffn_dim, num_experts, num_row_blocks, activation, skip_padding_rows, dev_status,
+                   nullptr, nullptr, num_tokens, d_model, ffn_dim, num_experts, num_row_blocks, activation, skip_padding_rows, dev_status,
                    as_stream(stream));
 }
 
@@ -1236,7 +1239,7 @@ extern "C" int sb_moe_gated_forward(const void* x, const void* expert_idx, int i
     return rc;
   if (int rc = sdd_gated(x, w_gate, w_up, ints(b.row_token), ints(b.row_block_expert), ints(b.padded_offsets),
                          ints(b.tokens_per_expert), base + b.x_rows, base + b.h, keep ? base + b.g : nullptr,
-                         keep ? base + b.u : nullptr, d_model, ffn_dim, num_experts, b.row_blocks, activation, 1, dev_status,
+                         keep ? base + b.u : nullptr, num_tokens, d_model, ffn_dim, num_experts, b.row_blocks, activation, 1, dev_status,
                          as_stream(stream)))
     return rc;
   if (int rc = rows_product<false>(base + b.h, nullptr, w_down, nullptr, ints(b.row_token), ints(b.row_block_expert),

@@ -458,6 +458,18 @@ def test_sdd_gated_on_a_trimmed_topology():
         sdd_gated(x, wg, wu, route_device(idx, 4, 256, 64))
 
 
+def test_sdd_gated_with_the_layout_of_a_larger_batch():
+    # x ends where memory that must not be read begins: tokens it does not have are zeros.
+    from sparsebench_b200 import route_device, sdd_gated
+
+    x, idx, gate, wg, wu, wd, go = make(300, 128, 256, 4, 2)
+    topo = route_device(idx, 4, 256, 128)
+    behind = torch.where((torch.arange(300, device="cuda") < 180)[:, None], x, torch.zeros_like(x))
+    want = sdd_gated(behind, wg, wu, topo)
+    live = int(topo.padded_offsets[-1]) // 128 * 2  # blocks of live row blocks
+    assert torch.equal(sdd_gated(x[:180].clone(), wg, wu, topo)[:live], want[:live])
+
+
 def test_sdd_gated_alone():
     from sparsebench_b200 import route_device, sdd_gated
 
