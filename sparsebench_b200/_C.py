@@ -463,9 +463,10 @@ def moe_gated_forward_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_wei
 
 
 def moe_gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
-                            w_up: torch.Tensor, w_down: torch.Tensor, state: torch.Tensor, activation: str
-                            ) -> tuple[torch.Tensor, ...]:
-    """(dx, dexpert_weight, dw_gate, dw_up, dw_down) of moe_gated_forward_cuda, from grad_out [T, D] and its state."""
+                            w_up: torch.Tensor, w_down: torch.Tensor, state: torch.Tensor, activation: str,
+                            state_stream: int | None = None) -> tuple[torch.Tensor, ...]:
+    """(dx, dexpert_weight, dw_gate, dw_up, dw_down) of moe_gated_forward_cuda, from grad_out [T, D] and its state.
+    state_stream: the raw handle of the stream that the state was made on, None if that is not known."""
     lib = _lib.load()
     device = x.device
     _check_bf16(device, grad_out=grad_out)
@@ -483,6 +484,11 @@ def moe_gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weig
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), state.data_ptr(), state.numel(),
             *(g.data_ptr() for g in grads), num_tokens, k, d_model, ffn_dim, num_experts, code, scratch.data_ptr(), sizes[2],
             _status_ptr(index), _raw_stream(index)))
+        if state_stream != _raw_stream(index):
+            # The state is the layer's own buffer: on another stream than the one it was made on, the allocator must not hand
+            # it out again before this call is done, however soon its last reference goes. (The inputs are the caller's to
+            # look after.) Not on every call: it costs 5 us of host time.
+            state.record_stream(torch.cuda.current_stream(index))
     return grads
 
 

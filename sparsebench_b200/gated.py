@@ -22,7 +22,8 @@ from sparsebench_b200 import _C
 class GatedSaved:
     """What moe_forward_gated_saved keeps for moe_backward_gated: the inputs by reference (the gates and
     weights must still hold the same values then) and, in one buffer, the layout, x and Y in its order and the blocks of
-    H, G and U (rows * (6 D + 6 F) bytes). state is None for an empty batch."""
+    H, G and U (rows * (6 D + 6 F) bytes). state is None for an empty batch; stream is the raw handle of the stream that it
+    was made on (None: not known)."""
 
     x: torch.Tensor
     expert_weight: torch.Tensor
@@ -31,6 +32,7 @@ class GatedSaved:
     w_down: torch.Tensor
     activation: str
     state: torch.Tensor | None
+    stream: int | None = None
 
 
 class GatedGrads(NamedTuple):
@@ -89,19 +91,21 @@ def moe_forward_gated_saved(
 ) -> tuple[torch.Tensor, GatedSaved]:
     """moe_forward_gated that also returns what moe_backward_gated needs."""
     out, state = _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, True)
-    return out, GatedSaved(x, expert_weight, w_gate, w_up, w_down, activation, state)
+    stream = None if state is None else _C._raw_stream(x.get_device())
+    return out, GatedSaved(x, expert_weight, w_gate, w_up, w_down, activation, state, stream)
 
 
 def moe_backward_gated(grad_out: torch.Tensor, saved: GatedSaved) -> GatedGrads:
     """The gradients of everything moe_forward_gated_saved took, from the gradient of its output [T, D] (bf16). May be
-    called more than once. Sums over rows are in a fixed order: the same inputs give the same bits."""
+    called more than once, and on another stream than the forward call's after waiting for it. Sums over rows are in a
+    fixed order: the same inputs give the same bits."""
     s = saved
     if grad_out.shape != s.x.shape:
         raise ValueError(f"grad_out must be {tuple(s.x.shape)}, got {tuple(grad_out.shape)}")
     if s.state is None:
         return GatedGrads(*(torch.zeros_like(t) for t in (s.x, s.expert_weight, s.w_gate, s.w_up, s.w_down)))
     return GatedGrads(*_C.moe_gated_backward_cuda(grad_out, s.x, s.expert_weight, s.w_gate, s.w_up, s.w_down, s.state,
-                                                  s.activation))
+                                                  s.activation, s.stream))
 
 
 class _GatedMoE(torch.autograd.Function):
@@ -111,7 +115,7 @@ class _GatedMoE(torch.autograd.Function):
         # Autograd checks the inputs for in-place changes; the state, most of the layer's memory, goes with them: freed
         # by the backward pass, and in the hands of saved_tensors_hooks (offloading, checkpointing).
         ctx.save_for_backward(x, expert_weight, w_gate, w_up, w_down, saved.state)
-        ctx.activation = activation
+        ctx.activation, ctx.stream = activation, saved.stream
         return out
 
     @staticmethod
@@ -121,7 +125,7 @@ class _GatedMoE(torch.autograd.Function):
             raise RuntimeError("the autograd form of the gated layer cannot be captured into a CUDA graph: "
                                "capture moe_forward_gated_saved and moe_backward_gated")
         *inputs, state = ctx.saved_tensors
-        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*inputs, ctx.activation, state))
+        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*inputs, ctx.activation, state, ctx.stream))
         return grads.x, None, grads.expert_weight, grads.w_gate, grads.w_up, grads.w_down, None
 
 

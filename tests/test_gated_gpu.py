@@ -398,6 +398,34 @@ def test_views_with_an_offset_and_misaligned_ones():
             moe_forward_gated(odd, idx[:num_tokens], gate[:num_tokens], wg, wu, wd)
 
 
+def test_state_outlives_a_backward_on_another_stream():
+    # The backward call waits on its stream behind 50 ms of nothing; meanwhile the last reference to the state goes, and the
+    # forward's stream asks for memory of that size. It must not get the state's.
+    from sparsebench_b200 import moe_backward_gated, moe_forward_gated_saved
+
+    x, idx, gate, wg, wu, wd, go = make(400, 256, 512, 4, 2)
+    want = step(x, idx, gate, wg, wu, wd, go, "silu")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        moe_backward_gated(go, moe_forward_gated_saved(x, idx, gate, wg, wu, wd)[1])  # warm: memory of that stream
+    torch.cuda.synchronize()
+    _, saved = moe_forward_gated_saved(x, idx, gate, wg, wu, wd)
+    where, size = saved.state.data_ptr(), saved.state.numel()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        grads = moe_backward_gated(go, saved)
+        done = torch.cuda.Event()
+        done.record()
+    del saved
+    junk = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    assert not done.query()  # else this shows nothing
+    assert all(not where <= t.data_ptr() < where + size for t in junk)
+    torch.cuda.synchronize()
+    for n, g in zip(NAMES, grads):
+        assert torch.equal(g, want[n]), n
+
+
 def test_two_streams_at_once():
     from sparsebench_b200 import lora_linear, moe_forward_gated
 

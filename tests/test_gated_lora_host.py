@@ -168,12 +168,14 @@ def stand_in(monkeypatch):
         calls.append((keep, None if state is None else weakref.ref(state)))
         return out.detach(), state
 
-    def backward(grad_out, x, gate, w_gate, w_up, w_down, state, activation):
+    def backward(grad_out, x, gate, w_gate, w_up, w_down, state, activation, stream):
+        assert stream == 77
         assert state.dtype == torch.uint8 and state.numel() == 1000
         return tuple(torch.ones_like(t) for t in (x, gate, w_gate, w_up, w_down))
 
     monkeypatch.setattr(_C, "moe_gated_forward_cuda", forward)
     monkeypatch.setattr(_C, "moe_gated_backward_cuda", backward)
+    monkeypatch.setattr(_C, "_raw_stream", lambda index: 77)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return calls
 
