@@ -125,7 +125,10 @@ class _GatedMoE(torch.autograd.Function):
             raise RuntimeError("the autograd form of the gated layer cannot be captured into a CUDA graph: "
                                "capture moe_forward_gated_saved and moe_backward_gated")
         *inputs, state = ctx.saved_tensors
-        grads = moe_backward_gated(grad_out.contiguous(), GatedSaved(*inputs, ctx.activation, state, ctx.stream))
+        grad_out = grad_out.contiguous()
+        if grad_out.data_ptr() % 16 != 0:  # a view of a larger gradient, as torch.cat's backward pass hands out
+            grad_out = grad_out.clone()
+        grads = moe_backward_gated(grad_out, GatedSaved(*inputs, ctx.activation, state, ctx.stream))
         return grads.x, None, grads.expert_weight, grads.w_gate, grads.w_up, grads.w_down, None
 
 

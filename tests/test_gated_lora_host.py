@@ -169,7 +169,7 @@ def stand_in(monkeypatch):
         return out.detach(), state
 
     def backward(grad_out, x, gate, w_gate, w_up, w_down, state, activation, stream):
-        assert stream == 77
+        assert stream == 77 and grad_out.is_contiguous() and grad_out.data_ptr() % 16 == 0
         assert state.dtype == torch.uint8 and state.numel() == 1000
         return tuple(torch.ones_like(t) for t in (x, gate, w_gate, w_up, w_down))
 
@@ -233,3 +233,16 @@ def test_state_is_a_saved_tensor_of_autograd(stand_in) -> None:
     assert stand_in[-1][1]() is None  # nothing of the layer is kept until the backward pass runs the forward again
     out.backward(torch.ones_like(out))
     assert len(stand_in) == before + 2
+
+
+def test_gradients_that_are_views_of_others_are_taken(stand_in) -> None:
+    from sparsebench_b200 import moe_gated
+
+    args = gated_inputs()
+    args[0].requires_grad_()
+    for front in (1, 8, 13):  # numbers in front of the layer's output in a larger vector
+        out = moe_gated(*args)
+        torch.cat([torch.zeros(front, dtype=torch.bfloat16), out.flatten()]).backward(torch.ones(front + 512, dtype=torch.bfloat16))
+    moe_gated(*args).sum().backward()  # expanded
+    moe_gated(*args).t().backward(torch.ones(128, 4, dtype=torch.bfloat16))  # transposed
+    assert bool((args[0].grad == 5).all())
