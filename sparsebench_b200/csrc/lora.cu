@@ -718,8 +718,14 @@ int check_lora(int64_t num_tokens, int32_t d_model, int32_t width, int32_t rank,
   if (num_tokens < 0 || num_tokens > INT32_MAX - kTileRows) return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: T must fit 31 bits");
   if (d_model <= 0 || d_model % 8 != 0) return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: D (%d) must be a positive multiple of 8", d_model);
   if (width <= 0 || width % 8 != 0) return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: N (%d) must be a positive multiple of 8", width);
+  // Column and K indexes run up to a tile past the end; an adapter's B is counted in pieces of 16 bytes, up to 16 per thread
+  // of the scan past its end.
+  if (d_model > INT32_MAX - kTileCols || width > INT32_MAX - kTileCols)
+    return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: D (%d) or N (%d) is too large", d_model, width);
   if (rank <= 0 || rank % 8 != 0 || rank > 128)
     return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: the rank (%d) must be a multiple of 8 in [8, 128]", rank);
+  if (num_tokens > kSmallTokens && static_cast<int64_t>(rank) * (width / 8) > INT32_MAX - 16 * kScanThreads)
+    return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: the rank (%d) times N (%d) is too large", rank, width);
   if (num_adapters <= 0 || static_cast<int64_t>(num_adapters) * rank > INT32_MAX - kTileCols)
     return fail(SB_ERR_INVALID_ARGUMENT, "lora_linear: the number of adapters (%d) must be positive, and times the rank fit 31 bits", num_adapters);
   return SB_OK;

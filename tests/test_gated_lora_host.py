@@ -89,6 +89,10 @@ def test_status_word_is_refused_without_a_place_for_it(lib) -> None:
     ((10, 64, 64, 136, 2), b"rank (136)"),
     ((10, 64, 64, 8, 0), b"adapters (0)"),
     ((10, 64, 64, 128, 2**25), b"31 bits"),
+    ((10, 2**31 - 8, 64, 8, 2), b"D (2147483640) or N (64) is too large"),
+    ((10, 64, 2**31 - 136, 8, 2), b"is too large"),
+    ((65, 64, 2**27, 128, 2), b"the rank (128) times N (134217728) is too large"),
+    ((100, 64, 2**28, 64, 2), b"times N"),
 ])
 def test_lora_sizes_are_refused(lib, sizes, text) -> None:
     assert lib.sb_lora_workspace_bytes(*sizes, 0) == -1 and text in lib.sb_last_error()
