@@ -143,22 +143,22 @@ struct GatedUp {
     int32_t keep;          // G and U are stored too, and every row that the backward pass reads
   };
   struct Tile {
-    int32_t k_steps, row_block, n0, expert, first_block, groups;
+    int32_t k_steps, row_block, n0, expert, first_block;
     bool live;
   };
   struct Early {
     bool store;
     bool real;  // this lane's row is no padding
   };
-  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kStaging = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = false, kBMnMajor = true;
 
   static __device__ __forceinline__ int32_t total_tiles(const Params& p) { return p.order.live_tiles(); }
   static __device__ __forceinline__ Tile tile(const Params& p, int32_t index) {
     Tile t{};
-    int32_t slice;
-    t.live = p.order.at(index, &t.row_block, &slice, &t.expert, &t.groups);
+    int32_t slice, groups;  // all rows are loaded, see above
+    t.live = p.order.at(index, &t.row_block, &slice, &t.expert, &groups);
     if (!t.live) return t;
     t.n0 = slice * 128;
     t.first_block = t.row_block * p.order.slices;  // of the layout's blocks, F / 128 per row block
@@ -204,15 +204,15 @@ struct GatedUp {
     uint32_t packed[32];
     if (p.keep) {
       load_packed_x64(gate, packed);
-      store_rows_128b<kBuffers>(w, &maps.m[3], packed, col, row);
+      store_rows_128b(w, &maps.m[3], packed, col, row);
       load_packed_x64(up, packed);
-      store_rows_128b<kBuffers>(w, &maps.m[4], packed, col, row);
+      store_rows_128b(w, &maps.m[4], packed, col, row);
     }
     if (p.activation == SB_ACT_SILU) product<SB_ACT_SILU>(gate, up, packed);
     else product<SB_ACT_GELU>(gate, up, packed);
 #pragma unroll
     for (int h = 0; h < 32; ++h) packed[h] = early.real ? packed[h] : 0u;
-    store_rows_128b<kBuffers>(w, &maps.m[2], packed, col, row);
+    store_rows_128b(w, &maps.m[2], packed, col, row);
   }
 };
 
@@ -248,7 +248,7 @@ struct GradHidden {
     int64_t at;  // of this row's columns in G and U, and in the results
     uint32_t first[2][8];  // G and U of the first part
   };
-  static constexpr int kStages = 4, kEpilogueWarps = 16, kBuffers = 0;
+  static constexpr int kStages = 4, kEpilogueWarps = 16, kStaging = 0;
   static constexpr bool kAhead = true;
   static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = false;
 
@@ -356,7 +356,7 @@ struct RowsProduct {
     bool live;
   };
   struct Early { bool store; };
-  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kStaging = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = false, kAMnMajor = false, kBMnMajor = !kBack;
 
@@ -425,7 +425,7 @@ struct RowsProduct {
       uint32_t v[32];
       ptx::tmem_ld_32x32b_x32(w.taddr + c, v);
       ptx::tmem_ld_wait();
-      store_rows_128b<kBuffers>(w, &maps.m[4], v, t.n0 + c, t.row_block * kTileRows + w.quarter * 32);
+      store_rows_128b(w, &maps.m[4], v, t.n0 + c, t.row_block * kTileRows + w.quarter * 32);
     }
   }
 };
@@ -449,7 +449,7 @@ struct GradWeights {
     bool live;
   };
   struct Early {};
-  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kStaging = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = false, kExtension = false, kAMnMajor = true, kBMnMajor = true;
 
@@ -517,7 +517,7 @@ struct GradWeights {
 #pragma unroll
         for (int h = 0; h < 32; ++h) packed[h] = 0u;
       }
-      store_rows_128b<kBuffers>(w, &maps.m[5 + t.which], packed, col, row);
+      store_rows_128b(w, &maps.m[5 + t.which], packed, col, row);
     }
   }
 };
@@ -1043,7 +1043,6 @@ int gated_join(const void* dx_rows, const int32_t* copy_row, void* dx, void* dga
 }
 
 bool aligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255u) == 0; }
-int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
 // The two ways of the forward pass. The decoding way needs no layout and splits K over clusters; it starts a block per
 // 64 (128) weight columns of every picked expert. From 129 copies on (and wherever the backward pass needs the layout's

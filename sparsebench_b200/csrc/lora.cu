@@ -398,7 +398,7 @@ struct LoraExpand {
   };
   struct Rows { int32_t slot[8]; };
   struct Early { int32_t loner; };  // this row's adapter when its B is not finite, else -1
-  static constexpr int kStages = 4, kEpilogueWarps = 8, kBuffers = 1;
+  static constexpr int kStages = 4, kEpilogueWarps = 8, kStaging = 1;
   static constexpr bool kAhead = false;
   static constexpr bool kVariable = true, kExtension = true, kAMnMajor = false, kBMnMajor = true;
 
@@ -497,14 +497,14 @@ struct LoraExpand {
           }
         }
         if (p.out_fp32) {
-          if (col + part * 32 < p.width) store_rows_128b<kBuffers>(w, &maps.m[2], v, col + part * 32, row);
+          if (col + part * 32 < p.width) store_rows_128b(w, &maps.m[2], v, col + part * 32, row);
         } else {
 #pragma unroll
           for (int h = 0; h < 16; ++h)
             packed[part * 16 + h] = pack_bf16(__uint_as_float(v[2 * h]), __uint_as_float(v[2 * h + 1]));
         }
       }
-      if (!p.out_fp32) store_rows_128b<kBuffers>(w, &maps.m[2], packed, col, row);
+      if (!p.out_fp32) store_rows_128b(w, &maps.m[2], packed, col, row);
     }
   }
 };
@@ -690,8 +690,6 @@ struct LoraSizes {
   int64_t row_tiles, tables, not_finite, v, total;  // bytes of each part, 256-byte aligned, then all
   int32_t splits, steps, total_steps, parts;
 };
-
-int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
 LoraSizes lora_sizes(int64_t num_tokens, int32_t d_model, int32_t rank, int32_t num_adapters, int out_fp32, int sm_count) {
   LoraSizes s{};

@@ -30,6 +30,7 @@ const DeviceInfo* current_device_info(int* device_out = nullptr);
 
 constexpr int kMaxDevices = 64;
 
+inline int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace sb

@@ -38,7 +38,7 @@ int encode_2d_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t co
   const cuuint32_t elem_strides[2] = {1, 1};
   const CUresult rc = encode(map, element_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                              const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                             box_cols * element_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS)
     return fail(SB_ERR_TENSOR_MAP, "%s: cuTensorMapEncodeTiled failed with CUresult %d (rows %llu, cols %llu)", what,

@@ -40,29 +40,25 @@ struct EpilogueWarp {
   int quarter;       // rows quarter * 32 .. + 31 of the tile (TMEM lanes this warp may read)
   int part;          // which of the kEpilogueWarps / 4 parts of the tile's columns is this warp's
   int lane;
-  uint32_t staging;  // this warp's staging tiles in shared memory, 4 KB each
-  uint32_t buffer;   // the one to use next
+  uint32_t staging;  // this warp's staging tile in shared memory, 4 KB (policies that have one)
   uint32_t taddr;    // TMEM address of (lane quarter, column 0) of the finished accumulator
 };
 
 // 128 bytes of this lane's row (64 bf16 columns as pairs, or 32 fp32 columns) -> a staging tile of the warp -> one TMA
-// store of 32 rows. kBuffers staging tiles are used in turn.
-template <int kBuffers>
+// store of 32 rows.
 __device__ __forceinline__ void store_rows_128b(EpilogueWarp& w, const CUtensorMap* map, const uint32_t (&packed)[32],
                                                 int32_t col, int32_t row) {
-  if (w.lane == 0) ptx::bulk_wait_read_but<kBuffers - 1>();  // the tile's last store has read it
+  if (w.lane == 0) ptx::bulk_wait_read();  // the last store has read it
   __syncwarp();
-  const uint32_t tile = w.staging + w.buffer * TileSmem::kStagingBytes;
-  if (kBuffers > 1) w.buffer ^= 1u;
   const uint32_t swz = static_cast<uint32_t>(w.lane & 7);
-  const uint32_t dst = tile + static_cast<uint32_t>(w.lane) * 128u;
+  const uint32_t dst = w.staging + static_cast<uint32_t>(w.lane) * 128u;
 #pragma unroll
   for (uint32_t c = 0; c < 8; ++c)
     ptx::st_shared_v4(dst + ((c ^ swz) << 4), packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
   ptx::fence_proxy_async_shared();
   __syncwarp();
   if (w.lane == 0) {
-    ptx::tma_store_2d(map, tile, col, row);
+    ptx::tma_store_2d(map, w.staging, col, row);
     ptx::bulk_commit();
   }
 }
@@ -91,7 +87,7 @@ __device__ __forceinline__ void load_packed_x64(uint32_t taddr, uint32_t (&packe
 //   total_tiles(p), tile(p, index), load(maps, p, tile, ks, a, b, bar)
 //   prefetch(p, tile, w) -> Early: global loads that can start before the accumulator is ready; then
 //   epilogue(maps, p, tile, w, early). With kAhead: ahead(p, next tile, w) between the two.
-//   static constexpr int kStages (of the ring), kEpilogueWarps, kBuffers (staging tiles of each, may be 0)
+//   static constexpr int kStages (of the ring), kEpilogueWarps, kStaging (staging tiles of each: 1, or 0 where it stores from registers)
 //   With kExtension: Tile has base_steps; four warps fill the stages of the K steps behind them. A from registers:
 //   Rows rows(p, tile, row0) once per tile, extension_chunk(p, tile, rows, j, row, ks, chunk) = the 16 bytes of chunk
 //   `chunk` of row `row` = row0 + 16 j. B (MN-major) eight K rows at a time: extension_row(p, tile, ks, i) says where
@@ -103,7 +99,7 @@ struct TileConfig {
   static constexpr int kFirstExtensionWarp = 2 + Op::kEpilogueWarps;
   static constexpr int kThreads = 32 * (kFirstExtensionWarp + kExtensionWarps);
   static constexpr int kSmemBytes = 1024 + Op::kStages * (TileSmem::kABytes + TileSmem::kBBytes) +
-                                    Op::kEpilogueWarps * Op::kBuffers * TileSmem::kStagingBytes + TileSmem::kBarrierBytes;
+                                    Op::kEpilogueWarps * Op::kStaging * TileSmem::kStagingBytes + TileSmem::kBarrierBytes;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -117,7 +113,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
   const uint32_t a_base = smem_base;
   const uint32_t b_base = a_base + Op::kStages * S::kABytes;
   const uint32_t staging_base = b_base + Op::kStages * S::kBBytes;
-  const uint32_t full_bar = staging_base + Op::kEpilogueWarps * Op::kBuffers * S::kStagingBytes;  // [kStages]
+  const uint32_t full_bar = staging_base + Op::kEpilogueWarps * Op::kStaging * S::kStagingBytes;  // [kStages]
   const uint32_t empty_bar = full_bar + 8 * Op::kStages;                          // [kStages]
   const uint32_t acc_full_bar = empty_bar + 8 * Op::kStages;                      // [2]
   const uint32_t acc_empty_bar = acc_full_bar + 16;                               // [2]
@@ -262,8 +258,7 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
     w.quarter = warp & 3;
     w.part = (warp - 2) >> 2;
     w.lane = lane;
-    w.staging = staging_base + static_cast<uint32_t>(warp - 2) * (Op::kBuffers * S::kStagingBytes);
-    w.buffer = 0;
+    w.staging = staging_base + static_cast<uint32_t>(warp - 2) * (Op::kStaging * S::kStagingBytes);
     uint32_t acc = 0, acc_phase = 0;
     typename Op::Tile next{};
     if (static_cast<int32_t>(blockIdx.x) < total) next = Op::tile(p, blockIdx.x);
@@ -352,8 +347,8 @@ tile_gemm_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ 
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-// A row-major [rows, cols] map of 2-byte (bf16) or 4-byte (fp32) elements whose boxes are 128 bytes wide (128-byte
-// swizzle) or 64 bytes wide (64-byte swizzle).
+// A row-major [rows, cols] map of 2-byte (bf16) or 4-byte (fp32) elements whose boxes are 128 bytes wide, with the
+// 128-byte swizzle.
 int encode_2d_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
                   uint32_t element_bytes, const char* what);
 
