@@ -516,6 +516,64 @@ def test_sdd_gated_alone():
         assert not bool(got[token < 0].any())
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_backward_keeps_what_is_not_finite_in_an_expert_to_itself(which, bad):
+    # D and F are odd multiples of 128: tiles of 256 columns reach into the next expert's weights and the next row block's
+    # hidden gradients, and row blocks of few rows leave the rest of a stage as it was. Expert 4 is neither the first nor last.
+    x, idx, gate, wg, wu, wd, go = make(200, 384, 640, 6, 2)
+    idx[idx[:, 0] == 2, 0] = 4  # expert 4 has more than a row block's half, expert 2 few rows
+    want = step(x, idx, gate, wg, wu, wd, go, "silu")
+    weights = [t.clone() for t in (wg, wu, wd)]
+    weights[which][4] = bad
+    got = step(x, idx, gate, *weights, go, "silu")
+    others = (idx != 4).all(1)
+    assert 20 < int(others.sum()) < 180
+    for n in ("out", "dx"):
+        assert torch.equal(got[n][others], want[n][others]), n
+    assert torch.equal(got["dgate"][idx != 4], want["dgate"][idx != 4])
+    for n in ("dw_gate", "dw_up", "dw_down"):
+        for e in (0, 1, 2, 3, 5):
+            assert torch.equal(got[n][e], want[n][e]), (n, e)
+    assert not torch.isfinite(got["out"][~others]).any()
+    assert not all(bool(torch.isfinite(got[n][4]).all()) for n in ("dw_gate", "dw_up", "dw_down"))
+
+
+@pytest.mark.parametrize("gate_dtype", [torch.bfloat16, torch.float32])
+def test_gates_of_zero_have_gradients(gate_dtype):
+    # dgate = dO . Y does not pass through the gate; everything else of such a copy is exactly 0.
+    x, idx, gate, wg, wu, wd, go = make(150, 256, 384, 5, 2, seed=4, gate_dtype=gate_dtype)
+    gate[::3, 0] = 0
+    gate[1::7] = 0
+    gate[2::9, 1] = -0.0
+    got = check(x, idx, gate, wg, wu, wd, go)
+    assert bool((got["dgate"][gate == 0] != 0).all())
+    gone = (gate == 0).all(1)
+    assert int(gone.sum()) > 10 and not bool(got["dx"][gone].any()) and not bool(got["out"][gone].any())
+    got = check(x, idx, torch.zeros_like(gate), wg, wu, wd, go, "gelu")
+    assert not any(bool(got[n].any()) for n in ("out", "dx", "dw_gate", "dw_up", "dw_down"))
+
+
+@pytest.mark.parametrize("skip", [False, True])
+@pytest.mark.parametrize(("num_tokens", "d_model", "ffn_dim", "num_experts", "k"),
+                         [(1, 256, 128, 3, 2), (150, 256, 640, 4, 2), (700, 512, 256, 9, 3)])
+def test_sdd_gated_then_dsd_then_combine(num_tokens, d_model, ffn_dim, num_experts, k, skip):
+    # The layer from its parts. Between dsd and combine a row is bf16: half a step of every copy's share on top of the bound.
+    from sparsebench_b200 import combine, dsd, route_device, sdd_gated
+
+    x, idx, gate, wg, wu, wd, _ = make(num_tokens, d_model, ffn_dim, num_experts, k, seed=9)
+    topo = route_device(idx, num_experts, ffn_dim, 128)
+    h = sdd_gated(x, wg, wu, topo, activation="gelu", skip_padding_rows=skip)
+    y = dsd(h, wd.reshape(-1, d_model), topo, skip_padding_rows=skip)
+    out = combine(y, gate, topo)
+    want, bound = gated_reference(x, idx, gate, wg, wu, wd, "gelu")["out"]
+    for j in range(k):
+        share, off = gated_reference(x, idx[:, j:j + 1], gate[:, j:j + 1], wg, wu, wd, "gelu")["out"]
+        bound = bound + 2.0**-8 * (share.abs() + off)
+    err = (out.double() - want).abs()
+    assert bool((err <= 1.01 * (bound + 2.0**-8 * (want.abs() + bound)) + 2.0**-133).all())
+
+
 def test_refusals():
     from sparsebench_b200 import moe_backward_gated, moe_forward_gated, moe_forward_gated_saved
 
