@@ -426,6 +426,28 @@ def test_state_outlives_a_backward_on_another_stream():
         assert torch.equal(g, want[n]), n
 
 
+def test_backward_captured_alone():
+    # An eager forward's state read by a graph of the backward call, on the capture's stream; then eager steps again.
+    from sparsebench_b200 import moe_backward_gated, moe_forward_gated_saved
+
+    x, idx, gate, wg, wu, wd, go = make(260, 256, 384, 4, 2)
+    _, saved = moe_forward_gated_saved(x, idx, gate, wg, wu, wd)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = moe_backward_gated(go, saved)
+    for seed in (1, 2):
+        go.copy_(make(260, 256, 384, 4, 2, seed=seed)[6])
+        graph.replay()
+        want = step(x, idx, gate, wg, wu, wd, go, "silu")
+        for n, g in zip(NAMES, grads):
+            assert torch.equal(g, want[n]), n
+    del graph, grads, saved  # the state's memory goes back to the allocator behind the capture's stream
+    torch.cuda.empty_cache()
+    again = step(x, idx, gate, wg, wu, wd, go, "silu")
+    for n in again:
+        assert torch.equal(again[n], want[n]), n
+
+
 def test_two_streams_at_once():
     from sparsebench_b200 import lora_linear, moe_forward_gated
 
