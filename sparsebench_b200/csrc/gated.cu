@@ -14,7 +14,8 @@
 // A decoding step (at most 128 copies, nothing kept) takes another way: no layout, the weights of the picked experts
 // streamed by the kernels of skinny.cuh (SkinnyUp, SkinnyDown, gated_small_combine_kernel).
 //
-// act is SiLU, v / (1 + exp(-v)), or the erf form of GELU.
+// act is SiLU, v / (1 + exp(-v)), or the erf form of GELU. exp and the reciprocal are the hardware's approximations (a few
+// units of 2^-23) and erf is within 1.5e-7: errors of 1e-6 of |v| at most, far below half a step of the bf16 results (2^-8).
 
 #include <algorithm>
 #include <initializer_list>
@@ -131,7 +132,7 @@ __device__ __forceinline__ void load_rows(uint32_t a, const CUtensorMap* all, co
 // Padding rows of x are loaded as the zeros they are: multiplying zeros takes less of the power limit, which sets the clock
 // of a longer run, than what a stage happens to hold (395 against 406 us a pass of the layer below, one after another).
 // Bound by the weights' way from memory where experts have few rows (T = 4096, D = 1024, F = 4096, E = 64: 1.07 GB of
-// weights in 196 us, 5.5 TB/s of a measured 6.56 copy peak; 234 us with G and U kept) and by the tensor cores where they
+// weights in 193 us, 5.6 TB/s of a measured 6.56 copy peak; 235 us with G and U kept) and by the tensor cores where they
 // have many (T = 4096, D = 4096, F = 14336, E = 8: 1.45 ms, 1490 TFLOP/s executed, at the clock that the power limit leaves).
 struct GatedUp {
   struct Params {
@@ -219,8 +220,8 @@ struct GatedUp {
 // ---- backward: gradients of G and U -----------------------------------------------------------------
 // dH = w (dO Wd^T) over 256 hidden columns; Wd [F, D] is read as the K-major operand it is. In the epilogue a lane has a row
 // to itself: it reads G and U and writes dG and dU a sector (16 columns) at a time, the next sector on its way while it
-// works on one. What bounds it is the latency of those reads, so sixteen warps share the tile (8: 226 us, 16: 201 us at
-// T = 4096, D = 1024, F = 4096, E = 64). Staging the results for TMA stores costs a stage of the ring and is slower (1000
+// works on one. What bounds it is the latency of those reads, so sixteen warps share the tile (8: 226 us, 16: 196 us at
+// T = 4096, D = 1024, F = 4096, E = 64; at 96 registers a thread the 256 columns spill 44 bytes). Staging the results for TMA stores costs a stage of the ring and is slower (1000
 // against 850 us on the Mixtral-like layer).
 template <int kCols>
 struct GradHidden {
@@ -341,7 +342,7 @@ struct GradHidden {
 // Down (kBack false): Y = H Wd, Wd [F, D] an MN-major operand. Back: dG Wg^T + dU Wu^T as one product with 2 F inner
 // columns, Wg and Wu [D, F] K-major operands. Either way the weights lie as the tensor cores read them. The rows stay in
 // fp32: each token's rows are summed, and rounded once, behind this.
-// At T = 4096, D = 1024, F = 4096, E = 64: 105 us (0.54 GB of weights, 5.1 TB/s) and 220 us (4.9 TB/s); what is left is the
+// At T = 4096, D = 1024, F = 4096, E = 64: 108 us (0.54 GB of weights, 5.0 TB/s) and 219 us (4.9 TB/s); what is left is the
 // last wave, 368 tiles of 256 columns on 148 SMs. Tiles of 128 columns fill it but keep fewer bytes in flight: 141 and
 // 285 us. On the Mixtral-like layer (T = 4096, D = 4096, F = 14336, E = 8) 745 us and 1.50 ms, 1450 TFLOP/s executed.
 template <bool kBack>
@@ -434,7 +435,7 @@ struct RowsProduct {
 // The rows of an expert are the inner dimension, so both operands are MN-major: X, w dO, H, dG and dU as they lie.
 // An expert's rows end inside a step of 64; the rest of that step is zero rows in X and w dO against finite ones (zeros) in
 // H, dG and dU. An expert without rows gets zeros. Bound by writing: with two or three K steps per tile the kernel moves
-// 5.1 TB/s (T = 4096, D = 1024, F = 4096, E = 64: 362 us). Tried and slower: two staging tiles per warp or sixteen warps for
+// 5.1 TB/s (T = 4096, D = 1024, F = 4096, E = 64: 365 us). Tried and slower: two staging tiles per warp or sixteen warps for
 // a stage of the ring (385 us), stores from registers (444 us); no gain: fetching only the real rows of the last step.
 struct GradWeights {
   struct Params {

@@ -9,7 +9,8 @@
 // A stage of the shared-memory ring holds A (16 KB) and B (32 KB) with the 128-byte swizzle, each in one of two forms:
 //   K-major   rows of the M (N) dimension, 64 K elements = 128 bytes per row
 //   MN-major  slabs of 64 K rows x 64 M (N) elements, 8 KB per slab
-// so weights, activations and their gradients are all consumed as they lie in memory; nothing is transposed or copied.
+// so weights and their gradients are consumed and written as they lie in memory and nothing is transposed. (Which rows of x
+// and of the output's gradient belong together is the policies' business: gated.cu copies them into layout order.)
 //
 // Every wait is bounded; on expiry the role sets a bit in *dev_status, raises the block's abort flag and all roles
 // drain to the common exit, where TMEM is released.
