@@ -415,8 +415,12 @@ def sdd_gated_cuda(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, ro
     return h
 
 
-def _check_gated_layer(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
-                       w_up: torch.Tensor, w_down: torch.Tensor, activation: str) -> int:
+_GATE_TYPES = (torch.bfloat16, torch.float32), "bfloat16 or float32"
+
+
+def _check_gated_layer(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str,
+                       **others: tuple[torch.Tensor, tuple[torch.dtype, ...], str]) -> int:
+    """The activation's code. others: tensor, the types it may have and their names in words."""
     index = x.get_device()
     bf16 = torch.bfloat16
     if not (index >= 0 and x.dtype is bf16 and x.is_contiguous()
@@ -425,13 +429,19 @@ def _check_gated_layer(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight:
             and w_down.dtype is bf16 and w_down.get_device() == index and w_down.is_contiguous()):
         _check(x.is_cuda, "x must be a CUDA tensor")
         _check_bf16(x.device, x=x, w_gate=w_gate, w_up=w_up, w_down=w_down)
-    for name, t, dtypes, text in (("expert_idx", expert_idx, (torch.int64, torch.int32), "int32 or int64"),
-                                  ("expert_weight", expert_weight, (torch.bfloat16, torch.float32), "bfloat16 or float32")):
+    for name, (t, dtypes, text) in others.items():
         if t.get_device() != index or t.dtype not in dtypes or not t.is_contiguous():
             _check(t.device == x.device, f"all inputs must be on the same GPU: {name} is on {t.device}, not {x.device}")
             _check(t.dtype in dtypes, f"{name} must be {text}, got {t.dtype}")
             _check(t.is_contiguous(), f"{name} must be contiguous")
     return _check_activation(activation)
+
+
+def check_gated_inputs(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
+                       w_up: torch.Tensor, w_down: torch.Tensor, activation: str) -> int:
+    return _check_gated_layer(x, w_gate, w_up, w_down, activation,
+                              expert_idx=(expert_idx, (torch.int64, torch.int32), "int32 or int64"),
+                              expert_weight=(expert_weight, *_GATE_TYPES))
 
 
 def moe_gated_forward_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w_gate: torch.Tensor,
@@ -440,7 +450,7 @@ def moe_gated_forward_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_wei
     """(out [T, D], state): the gated layer; state (None unless keep) is what moe_gated_backward_cuda needs of it.
     Shapes are the caller's to check; T * k must be positive."""
     lib = _lib.load()
-    code = _check_gated_layer(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
+    code = check_gated_inputs(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
     index = x.get_device()
     num_tokens, k = expert_idx.shape
     num_experts, d_model, ffn_dim = w_gate.shape
@@ -466,30 +476,30 @@ def moe_gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weig
                             w_up: torch.Tensor, w_down: torch.Tensor, state: torch.Tensor, activation: str,
                             state_stream: int | None = None) -> tuple[torch.Tensor, ...]:
     """(dx, dexpert_weight, dw_gate, dw_up, dw_down) of moe_gated_forward_cuda, from grad_out [T, D] and its state.
-    state_stream: the raw handle of the stream that the state was made on, None if that is not known."""
+    state_stream: the raw handle of the stream that the state was made on, None if that is not known. Shapes are the
+    caller's to check."""
     lib = _lib.load()
-    device = x.device
-    _check_bf16(device, grad_out=grad_out)
-    code = _check_activation(activation)
+    code = _check_gated_layer(x, w_gate, w_up, w_down, activation, grad_out=(grad_out, (torch.bfloat16,), "bfloat16"),
+                              expert_weight=(expert_weight, *_GATE_TYPES), state=(state, (torch.uint8,), "uint8"))
     num_tokens, k = expert_weight.shape
     num_experts, d_model, ffn_dim = w_gate.shape
-    index = device.index
+    index = x.get_device()
     with _on(index):
         sizes = (ctypes.c_int64 * 3)()
         _lib.check(lib.sb_moe_gated_bytes(num_tokens, k, d_model, ffn_dim, num_experts, 1, sizes))
-        scratch = torch.empty(sizes[2], dtype=torch.uint8, device=device)
-        grads = tuple(torch.empty_like(t) for t in (x, expert_weight, w_gate, w_up, w_down))
+        scratch = x.new_empty(sizes[2] // 2)
+        grads = [torch.empty_like(t) for t in (x, expert_weight, w_gate, w_up, w_down)]
         _lib.check(lib.sb_moe_gated_backward(
-            grad_out.data_ptr(), expert_weight.data_ptr(), int(expert_weight.dtype == torch.float32),
+            grad_out.data_ptr(), expert_weight.data_ptr(), expert_weight.dtype is torch.float32,
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), state.data_ptr(), state.numel(),
-            *(g.data_ptr() for g in grads), num_tokens, k, d_model, ffn_dim, num_experts, code, scratch.data_ptr(), sizes[2],
+            *[g.data_ptr() for g in grads], num_tokens, k, d_model, ffn_dim, num_experts, code, scratch.data_ptr(), sizes[2],
             _status_ptr(index), _raw_stream(index)))
         if state_stream != _raw_stream(index):
             # The state is the layer's own buffer: on another stream than the one it was made on, the allocator must not hand
             # it out again before this call is done, however soon its last reference goes. (The inputs are the caller's to
             # look after.) Not on every call: it costs 5 us of host time.
             state.record_stream(torch.cuda.current_stream(index))
-    return grads
+    return tuple(grads)
 
 
 # ---- projections with the low-rank adapters of many requests (no counterpart in the reference) ----------

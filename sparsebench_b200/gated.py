@@ -59,7 +59,7 @@ def _check_shapes(x, expert_idx, expert_weight, w_gate, w_up, w_down) -> None:
 def _forward(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, keep):
     _check_shapes(x, expert_idx, expert_weight, w_gate, w_up, w_down)
     if expert_idx.numel() == 0:  # host-known size: nothing routed anywhere
-        _C._check_gated_layer(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
+        _C.check_gated_inputs(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation)
         return torch.zeros_like(x), None
     return _C.moe_gated_forward_cuda(x, expert_idx, expert_weight, w_gate, w_up, w_down, activation, keep)
 
@@ -100,6 +100,7 @@ def moe_backward_gated(grad_out: torch.Tensor, saved: GatedSaved) -> GatedGrads:
     called more than once, and on another stream than the forward call's after waiting for it. Sums over rows are in a
     fixed order: the same inputs give the same bits."""
     s = saved
+    _check_shapes(s.x, s.expert_weight, s.expert_weight, s.w_gate, s.w_up, s.w_down)
     if grad_out.shape != s.x.shape:
         raise ValueError(f"grad_out must be {tuple(s.x.shape)}, got {tuple(grad_out.shape)}")
     if s.state is None:

@@ -629,6 +629,39 @@ def test_refusals():
         moe_backward_gated(go[:1].expand(20, 128), saved)
 
 
+def test_backward_refuses_what_is_not_what_the_forward_kept():
+    # saved_tensors_hooks and dataclasses.replace can put other tensors there; none of these may reach a kernel.
+    from dataclasses import replace
+
+    from sparsebench_b200 import moe_backward_gated, moe_forward_gated_saved, moe_gated
+
+    x, idx, gate, wg, wu, wd, go = make(20, 128, 256, 4, 2)
+    _, saved = moe_forward_gated_saved(x, idx, gate, wg, wu, wd)
+    for change, error, text in [
+        ({"w_up": wu.cpu()}, RuntimeError, "w_up must be a CUDA tensor"),
+        ({"w_down": wd.float()}, RuntimeError, "w_down must be bfloat16"),
+        ({"w_gate": wg.transpose(1, 2).contiguous().transpose(1, 2)}, RuntimeError, "w_gate must be contiguous"),
+        ({"w_up": wu[:3]}, ValueError, "w_gate and w_up"),
+        ({"w_down": wd[:, :128]}, ValueError, "w_down must be"),
+        ({"expert_weight": gate[:10]}, ValueError, r"\[T, k\]"),
+        ({"expert_weight": gate.cpu()}, RuntimeError, "expert_weight is on cpu"),
+        ({"expert_weight": gate.half()}, RuntimeError, "bfloat16 or float32"),
+        ({"state": saved.state.cpu()}, RuntimeError, "state is on cpu"),
+        ({"state": saved.state[:-256]}, RuntimeError, "are needed"),
+        ({"state": saved.state.float()}, RuntimeError, "uint8"),
+        ({"activation": "relu"}, RuntimeError, "activation"),
+        ({"x": x.cpu()}, RuntimeError, "CUDA|same GPU"),
+    ]:
+        with pytest.raises(error, match=text):
+            moe_backward_gated(go, replace(saved, **change))
+    leaf = x.clone().requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):  # never brought back
+        out = moe_gated(leaf, idx, gate, wg, wu, wd)
+    with pytest.raises(RuntimeError):
+        out.backward(go)
+    assert torch.equal(moe_backward_gated(go, saved).x, step(x, idx, gate, wg, wu, wd, go, "silu")["dx"])
+
+
 def test_autograd_backward_refuses_capture():
     from sparsebench_b200 import moe_gated
 
