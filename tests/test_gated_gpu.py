@@ -166,6 +166,17 @@ def test_ids_out_of_range_and_the_same_expert_twice():
     assert not any(bool(t.any()) for t in got.values())
 
 
+def test_ids_that_differ_in_their_upper_half_only():
+    # 64-bit ids whose lower 32 bits name an expert are out of range all the same.
+    for num_tokens in (20, 200):
+        x, idx, gate, wg, wu, wd, go = make(num_tokens, 128, 256, 6, 2)
+        idx[::5, 0] += 2**32
+        idx[1::5, 1] -= 2**32
+        idx[2::5, 0] += 2**40
+        got = check(x, idx, gate, wg, wu, wd, go)
+        assert not bool(got["dgate"][(idx < 0) | (idx >= 6)].any())
+
+
 def test_int32_ids_and_fp32_gates():
     x, idx, gate, wg, wu, wd, go = make(150, 256, 256, 4, 2, gate_dtype=torch.float32)
     check(x, idx.int(), gate, wg, wu, wd, go)

@@ -68,6 +68,15 @@ def test_no_adapter_and_one_for_all(num_tokens, order):
         assert torch.equal(check(x, w, a, b, idx.int(), None), out)
 
 
+@pytest.mark.parametrize("num_tokens", [1, 40, 200])
+def test_ids_that_differ_in_their_upper_half_only(num_tokens):
+    x, w, a, b, idx, scale = make(num_tokens, 128, 136, 16, 4, "any")
+    idx[::3] = 2**32 + 1
+    idx[1::7] = -(2**32) + 2
+    out = check(x, w, a, b, idx, scale)
+    assert torch.equal(out, check(x, w, a, b, torch.where((idx < 0) | (idx >= 4), -1, idx), scale))
+
+
 @pytest.mark.parametrize("fp32", [False, True], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("width", [648, 2568, 5128])
 def test_columns_of_a_tile(width, fp32):
